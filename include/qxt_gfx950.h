@@ -383,6 +383,127 @@ int qxt_w8a8_linear_noalloc(const float *x, size_t ldx, const void *w, size_t ld
                             const float *bias, float *y, size_t ldy, uint32_t m, uint32_t n, uint32_t k,
                             uint32_t weight_layout, uint32_t flags, void *stream);
 
+/* -------------------------------------------- attention over a paged cache */
+
+/* No counterpart in the reference for anything in this section: its native
+ * runtime stops at the linears and its attention programs know no cache pages. */
+
+/* Element types of the attention operators. */
+#define QXT_TYPE_F32 0u
+#define QXT_TYPE_BF16 1u
+#define QXT_TYPE_F16 2u
+
+/* Keys and values of many sequences in pages.  Row (slot, head) of head_dim
+ * elements lies at keys + page * key_page_stride + offset * key_slot_stride +
+ * head * key_head_stride (bytes; any order of the axes), with page and offset
+ * of a sequence's slot j: block_table[sequence][j / page_size], j % page_size.
+ * A table entry outside [0, pages) names no page: nothing is read or written
+ * through it, and its slots count as zero rows where they would be read.
+ * context_lens: slots in use of each sequence.  Lengths past the table's
+ * width are cut to it. */
+typedef struct qxt_paged_cache {
+    void *keys;
+    size_t key_page_stride, key_slot_stride, key_head_stride;
+    void *values;
+    size_t value_page_stride, value_slot_stride, value_head_stride;
+    const int32_t *block_table; /* [sequences, table_width] */
+    size_t block_table_stride;  /* bytes */
+    const int32_t *context_lens;
+    uint32_t pages, page_size, heads, head_dim, type, table_width, sequences;
+} qxt_paged_cache;
+
+/* Flags of qxt_qk_norm_rope[_cache]. */
+#define QXT_ROPE_INTERLEAVED 1u /* pairs (2i, 2i + 1); without it (i, i + rotary_dim / 2) */
+
+/* Queries [tokens, query_heads, head_dim] and keys [tokens, key_heads,
+ * head_dim] (element strides of rows free, elements dense): each row is
+ * normalised, y = x * rsqrt(mean(x^2) + epsilon) * weight (skipped where the
+ * weight is NULL), then pair i < rotary_dim / 2 of it turns by the angle with
+ * cos/sin[positions[token]][i] (fp32 [table_rows, rotary_dim / 2]); computed in
+ * fp32 and rounded once.  A position outside the table makes the row's rotated
+ * part NaN.  Outputs may be the inputs themselves. */
+int qxt_qk_norm_rope(const void *query, size_t query_token_stride, size_t query_head_stride, const void *key,
+                     size_t key_token_stride, size_t key_head_stride, const float *query_weight,
+                     const float *key_weight, float epsilon, const float *cos, const float *sin,
+                     size_t table_row_stride, uint32_t table_rows, const int32_t *positions, void *query_out,
+                     size_t query_out_token_stride, size_t query_out_head_stride, void *key_out,
+                     size_t key_out_token_stride, size_t key_out_head_stride, uint32_t tokens, uint32_t query_heads,
+                     uint32_t key_heads, uint32_t head_dim, uint32_t rotary_dim, uint32_t input_type,
+                     uint32_t output_type, uint32_t flags, void *stream);
+
+/* As qxt_qk_norm_rope, with keys and (as they are) values stored into slot
+ * slots[token] of the cache, page * page_size + offset, in its type; slots
+ * outside the cache (negative ones: padding) are not stored.  query_out has the
+ * cache's type.  The cache's table and lengths are not read.  Two tokens must
+ * not name one slot. */
+int qxt_qk_norm_rope_cache(const void *query, size_t query_token_stride, size_t query_head_stride, const void *key,
+                           size_t key_token_stride, size_t key_head_stride, const void *value,
+                           size_t value_token_stride, size_t value_head_stride, const float *query_weight,
+                           const float *key_weight, float epsilon, const float *cos, const float *sin,
+                           size_t table_row_stride, uint32_t table_rows, const int32_t *positions,
+                           const int64_t *slots, void *query_out, size_t query_out_token_stride,
+                           size_t query_out_head_stride, const qxt_paged_cache *cache, uint32_t tokens,
+                           uint32_t query_heads, uint32_t rotary_dim, uint32_t input_type, uint32_t flags,
+                           void *stream);
+
+/* Softmax attention of new tokens over the cache.  query: [tokens, query_heads,
+ * head_dim] in the cache's type, 16-byte aligned rows; sequence b owns the
+ * tokens query_starts[b] .. query_starts[b + 1] - 1 (NULL: token b), the newest
+ * of its context_lens[b] slots.  Its token i of n sees slot j when j <
+ * context_lens[b], with `causal` j <= at, with a window j > at - window, at =
+ * context_lens[b] - n + i; query heads share key head h / (query_heads / heads).
+ * out = sum_j p_j v_j / sum_j p_j, p_j = exp(scale * q.k_j), and lse (or NULL) =
+ * log sum_j p_j; a row that sees nothing gets 0 and -inf, whatever unseen slots
+ * hold.  Tokens of no sequence are left alone.  max_query and max_context
+ * (longest chunk and context) only size the launch: larger ones in the device's
+ * arrays are still computed, more slowly.  workspace: 16-byte aligned, of at
+ * least qxt_paged_attention_workspace() bytes for the same sizes, free again
+ * when the stream has passed the call. */
+size_t qxt_paged_attention_workspace(uint32_t query_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t sequences,
+                                     uint32_t tokens, uint32_t max_query, uint32_t max_context);
+int qxt_paged_attention(const void *query, size_t query_token_stride, size_t query_head_stride,
+                        const qxt_paged_cache *cache, const int32_t *query_starts, void *out, size_t out_token_stride,
+                        size_t out_head_stride, uint32_t out_type, float *lse, size_t lse_token_stride, uint32_t tokens,
+                        uint32_t query_heads, float scale, uint32_t causal, uint32_t window, uint32_t max_query,
+                        uint32_t max_context, void *workspace, size_t workspace_bytes, void *stream);
+
+/* scores[b, head, j] = previous[b, head, j] (0 where previous is NULL) + the
+ * sum over sequence b's tokens t and the query heads h of key head `head` of
+ * exp(scale * q.k_j - lse[t, h]), for the slots j that t sees (as
+ * qxt_paged_attention, whose lse this takes: then each row's weights add up to
+ * 1).  Rows with lse = -inf add nothing.  previous and scores: fp32 [sequences,
+ * heads, table_width * page_size], strides in bytes, dense in j; they may be
+ * the same.  Slots at and above a sequence's length keep their previous value.
+ * The order of the sum is fixed by the arguments. */
+size_t qxt_paged_attention_scores_workspace(uint32_t query_heads, uint32_t kv_heads, uint32_t sequences, uint32_t tokens,
+                                            uint32_t slots, uint32_t max_query, uint32_t max_context);
+int qxt_paged_attention_scores(const void *query, size_t query_token_stride, size_t query_head_stride,
+                               const qxt_paged_cache *cache, const int32_t *query_starts, const float *lse,
+                               size_t lse_token_stride, const float *previous, size_t previous_sequence_stride,
+                               size_t previous_head_stride, float *scores, size_t scores_sequence_stride,
+                               size_t scores_head_stride, uint32_t tokens, uint32_t query_heads, float scale,
+                               uint32_t causal, uint32_t window, uint32_t max_query, uint32_t max_context,
+                               void *workspace, size_t workspace_bytes, void *stream);
+
+/* Cut every sequence of more than `budget` slots down to `budget`, head by
+ * head.  Kept are the slots that come first by (recent, score, lower slot);
+ * recent: position > newest - recent, newest the head's largest position in
+ * use; a NaN score is the least.  Kept slots below budget stay; the i-th slot
+ * below it that is given up takes key row, value row, score and position of the
+ * i-th kept slot at or above it.  Slots from budget to the old length get score
+ * 0 and position -1; lens_out[b] = min(length, budget) (not the context_lens
+ * array itself).  scores fp32 and positions int32 [sequences, heads, table_width
+ * * page_size], strides in bytes, dense in the slot; outputs may be the inputs.
+ * No page may belong to two sequences.  workspace (8-byte aligned):
+ * qxt_paged_cache_evict_workspace() bytes. */
+size_t qxt_paged_cache_evict_workspace(uint32_t heads, uint32_t sequences, uint32_t slots, uint32_t budget);
+int qxt_paged_cache_evict(const qxt_paged_cache *cache, const float *scores, size_t scores_sequence_stride,
+                          size_t scores_head_stride, float *scores_out, size_t scores_out_sequence_stride,
+                          size_t scores_out_head_stride, const int32_t *positions, size_t positions_sequence_stride,
+                          size_t positions_head_stride, int32_t *positions_out, size_t positions_out_sequence_stride,
+                          size_t positions_out_head_stride, int32_t *lens_out, uint32_t budget, uint32_t recent,
+                          uint32_t max_context, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

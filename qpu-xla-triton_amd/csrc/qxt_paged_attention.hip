@@ -1,0 +1,628 @@
+// Attention of new tokens over a paged cache: one pass over the visible slots
+// with the running maximum and sum of a softmax.
+//
+// For token t and query head h of a sequence of length L with n new tokens,
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q.k_j - m)
+// over the slots j that the token sees, m the largest logit so far.  The rows
+// of a workgroup are the (token, head) pairs that share one key head (token
+// major), so a key and value row that was fetched serves the whole group of
+// heads; with one new token a sequence the rows are the group alone.
+//
+// WQ x WK waves: wave (wq, wk) computes rows 32 wq .. 32 wq + 31 against the
+// wk-th part of every step's keys.  Logits are taken transposed, S^T = K Q^T
+// (32x32x16 MFMAs): a lane then holds 16 keys of one row, the row's maximum
+// and sum need one exchange between half-waves, and the rounded weights are
+// already the second operand of O^T = V^T P^T: the sum over keys may run in any
+// order, so V^T is read (transposed, from LDS) in the order the lanes hold.
+#include <algorithm>
+
+#include "qxt_paged_attention.h"
+
+namespace qxt {
+namespace {
+
+constexpr float kNone = -__builtin_inff();
+// The running maximum moves only when a logit exceeds it by 2^8: weights stay
+// below 256 (exact in the sums' 32 bits, in range of fp16) and the rescaling of
+// the outputs is rare.
+constexpr float kSlack = 8.0f;
+
+template <typename TO>
+__device__ __forceinline__ void put4(char *p, float a, float b, float c, float d) {
+    typename vec4_of<TO>::type v;
+    v[0] = static_cast<TO>(a);
+    v[1] = static_cast<TO>(b);
+    v[2] = static_cast<TO>(c);
+    v[3] = static_cast<TO>(d);
+    *reinterpret_cast<typename vec4_of<TO>::type *>(p) = v;
+}
+
+__device__ __forceinline__ void put4_as(uint32_t type, char *row, int d, float a, float b, float c, float e) {
+    if (type == QXT_TYPE_BF16)
+        put4<bf16_t>(row + 2 * d, a, b, c, e);
+    else if (type == QXT_TYPE_F16)
+        put4<f16_t>(row + 2 * d, a, b, c, e);
+    else
+        put4<float>(row + 4 * d, a, b, c, e);
+}
+
+// Natural-log sum of a row's exponentials from its maximum (log2 units) and sum.
+__device__ __forceinline__ float lse_of(float top2, float sum) {
+    return sum == 0.0f ? kNone : (top2 + __log2f(sum)) * 0.69314718055994531f;
+}
+
+// One row without matrix instructions, a slot at a time: only the slots that it
+// sees enter.  For the rare waves whose rows see different slots of a step that
+// holds infinite or NaN values.  Lane l gets elements l + 64 k; the slots are
+// [from, to) in parts of `part` every `step`.
+template <typename T, int DP>
+__device__ __forceinline__ float2 attend_alone(const PagedArgs &a, const T *query, const Range &mine, int32_t from,
+                                               int32_t to, int32_t step, int32_t part, const int32_t *table,
+                                               const char *keys, const char *values, float (&out)[DP / 64]) {
+    const int lane = threadIdx.x % 64;
+    float top = kNone, sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < DP / 64; ++k) out[k] = 0.0f;
+    for (int32_t base = from; base < to; base += step) {
+        const int32_t slot = base + lane;
+        const bool seen = lane < part && slot >= mine.low && slot < mine.high;
+        float logit = kNone;
+        int64_t value_at = -1;
+        if (seen) {
+            const uint32_t page = fast_quotient(static_cast<uint32_t>(slot), a.page);
+            const int64_t in_page = static_cast<uint32_t>(slot) - page * a.page.divisor, id = table[page];
+            logit = 0.0f;
+            if (id >= 0 && id < a.pages) {
+                const T *key = reinterpret_cast<const T *>(keys + id * a.keys.page_stride + in_page * a.keys.slot_stride);
+                value_at = id * a.values.page_stride + in_page * a.values.slot_stride;
+                for (uint32_t e = 0; e < a.head_dim; ++e)
+                    logit = fmaf(static_cast<float>(query[e]), static_cast<float>(key[e]), logit);
+            }
+        }
+        float most = logit;
+        for (int off = 32; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
+        const float next = fmaxf(top, most);
+        const float factor = next == kNone ? 1.0f : __builtin_amdgcn_exp2f((top - next) * a.scale2);
+        top = next;
+        const float weight = seen ? __builtin_amdgcn_exp2f(fmaf(logit, a.scale2, top == kNone ? 0.0f : -top * a.scale2)) : 0.0f;
+        float part_sum = weight;
+        for (int off = 32; off > 0; off >>= 1) part_sum += __shfl_xor(part_sum, off, 64);
+        sum = sum * factor + part_sum;
+#pragma unroll
+        for (int k = 0; k < DP / 64; ++k) out[k] *= factor;
+        for (int j = 0; j < part; ++j) {
+            if (!__shfl(static_cast<int>(seen), j, 64)) continue;
+            const float w = __shfl(weight, j, 64);
+            const int64_t at = __shfl(static_cast<long long>(value_at), j, 64);
+            if (at < 0) continue;  // a slot without a page: zero values
+#pragma unroll
+            for (int k = 0; k < DP / 64; ++k) {
+                const uint32_t e = lane + 64 * k;
+                if (e < a.head_dim) out[k] = fmaf(w, static_cast<float>(reinterpret_cast<const T *>(values + at)[e]), out[k]);
+            }
+        }
+    }
+    return make_float2(top == kNone ? kNone : top * a.scale2, sum);
+}
+
+__device__ __forceinline__ void put_as(uint32_t type, char *row, int d, float x) {
+    if (type == QXT_TYPE_BF16)
+        reinterpret_cast<bf16_t *>(row)[d] = static_cast<bf16_t>(x);
+    else if (type == QXT_TYPE_F16)
+        reinterpret_cast<f16_t *>(row)[d] = static_cast<f16_t>(x);
+    else
+        reinterpret_cast<float *>(row)[d] = x;
+}
+
+template <int DP, int WQ, int WK>
+struct Shape {
+    static constexpr int kKeys = DP <= 128 && WQ >= 4 ? 64 : 32;  // keys of one step and key part
+    static constexpr int kStep = kKeys * WK;                      // keys of one step
+    static constexpr int kRows = kKeys / WQ;                      // rows that a wave stages
+    static constexpr int kTileBytes = kKeys * DP * 2;
+    static constexpr int kStageBytes = 2 * kTileBytes * WK;
+    static constexpr int kLds = 2 * kStageBytes;
+    static constexpr int kThreads = 64 * WQ * WK;
+};
+
+// Two waves a SIMD (256 registers each) up to 128 elements of head size, one above.
+template <typename T, int DP, int WQ, int WK>
+__global__ __launch_bounds__(64 * WQ * WK, DP <= 128 ? 2 : 1) void paged_attention_kernel(PagedArgs a) {
+    using S = Shape<DP, WQ, WK>;
+    using TL = Tile<DP>;
+    using M = Mfma<T>;
+    typedef typename M::frag frag;
+    extern __shared__ __align__(16) char lds[];
+    constexpr int kBlocks = S::kKeys / 32, kCols = DP / 32;
+
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int wq = wave % WQ, wk = wave / WQ, col = lane % 32, half = lane / 32;
+    uint32_t id = blockIdx.x;
+    const uint32_t head = id % a.kv_heads;
+    id /= a.kv_heads;
+    const uint32_t first_tile = id % a.tiles;
+    id /= a.tiles;
+    const uint32_t split = id % a.splits, b = id / a.splits;
+    const Sequence seq = sequence_of(a, b);
+    const int32_t group = a.group.divisor, rows = seq.tokens * group;
+    const int32_t tiles = (rows + 32 * WQ - 1) / (32 * WQ);
+
+    Stager<DP, S::kRows> stager;
+    stager.table = a.table + b * a.table_stride;
+    const char *keys = a.keys.data + head * a.keys.head_stride, *values = a.values.data + head * a.values.head_stride;
+    char *const my_keys = lds + 2 * S::kTileBytes * wk;  // this key part's tiles of stage 0
+
+    // Operand addresses within a tile (bytes), without the block's own offset.
+    const int key_at = col * TL::kRowBytes + ((half ^ TL::key_turn(col)) * 16);
+    const int vr = 4 * half + (lane % 16) / 4;
+    const int value_chunk = (2 * ((lane / 16) % 2) + (lane % 4) / 2) ^ TL::value_turn(vr);
+    const int value_at = vr * TL::kRowBytes + value_chunk * 16 + (lane % 2) * 8;
+
+    for (int32_t turn = first_tile; turn < tiles; turn += a.tiles) {
+        // The longest rows first: the last tiles of a causal sequence.
+        const int32_t tile = tiles - 1 - turn;
+        const int32_t row = tile * 32 * WQ + 32 * wq + col, held = min(row, rows - 1);
+        const int32_t token = fast_quotient(held, a.group), in_group = held - token * group;
+        const Range mine = seen_by(a, seq, token);
+        const Range first = seen_by(a, seq, fast_quotient(tile * 32 * WQ, a.group));
+        const Range last = seen_by(a, seq, fast_quotient(min(rows, (tile + 1) * 32 * WQ) - 1, a.group));
+        const int32_t low = first.low, high = last.high;
+        // What this wave's rows see, all of them or any.
+        const int32_t any_low = __builtin_amdgcn_readlane(mine.low, 0), all_low = __builtin_amdgcn_readlane(mine.low, 31);
+        const int32_t all_high = __builtin_amdgcn_readlane(mine.high, 0), any_high = __builtin_amdgcn_readlane(mine.high, 31);
+        const int32_t steps = (high - low + S::kStep - 1) / S::kStep, share = (steps + a.splits - 1) / a.splits;
+        const int32_t from = min<int32_t>(split * share, steps), to = min<int32_t>(from + share, steps);
+
+        const char *query_row = a.query + (seq.start + token) * a.query_token +
+                                static_cast<int64_t>(head * group + in_group) * a.query_head;
+        frag q[DP / 16];
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+            q[s] = frag{};
+            if (16 * s + 8 * half < static_cast<int>(a.head_dim))
+                q[s] = *reinterpret_cast<const frag *>(query_row + (16 * s + 8 * half) * 2);
+        }
+
+        f32x16 acc[kCols];
+#pragma unroll
+        for (int d = 0; d < kCols; ++d) acc[d] = f32x16{};
+        bool special = false;           // unseen values that are no numbers reached acc
+        float top = kNone, sum = 0.0f;  // top in logit units (unscaled), sum over this lane's keys
+
+        // Slot of this lane's staged row in step t.
+        const int stage_row = wq * S::kRows + lane % S::kRows;
+        auto staged_slot = [&](int32_t t) { return low + t * S::kStep + wk * S::kKeys + stage_row; };
+        auto stage = [&](int32_t t) {
+            char *to = my_keys + (t & 1) * S::kStageBytes + wq * S::kRows * TL::kRowBytes;
+            const int32_t slot = staged_slot(t);
+            stager.template load<true>(keys, stager.offset_in(a, a.keys, slot), to, lane, wq * S::kRows, a.head_dim);
+            stager.template load<false>(values, stager.offset_in(a, a.values, slot), to + S::kTileBytes, lane,
+                                        wq * S::kRows, a.head_dim);
+        };
+
+        if (from < to) {
+            stager.look_up(a, staged_slot(from), high);
+            stage(from);
+            stager.look_up(a, staged_slot(from + 1), high);
+        }
+        for (int32_t t = from; t < to; ++t) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's rows of step t have landed
+            if (WQ > 1) __builtin_amdgcn_s_barrier();         // everyone's have, and step t - 1 has been read
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+            if (t + 1 < to) {
+                stage(t + 1);
+                stager.look_up(a, staged_slot(t + 2), high);
+            }
+            const int32_t base = low + t * S::kStep + wk * S::kKeys;
+            if (base >= any_high || base + S::kKeys <= any_low) continue;
+            const char *kt = my_keys + (t & 1) * S::kStageBytes, *vt = kt + S::kTileBytes;
+
+            f32x16 s[kBlocks];
+#pragma unroll
+            for (int kb = 0; kb < kBlocks; ++kb) {
+                s[kb] = f32x16{};
+#pragma unroll
+                for (int c = 0; c < DP / 16; ++c) {
+                    const frag k = *reinterpret_cast<const frag *>(kt + kb * 32 * TL::kRowBytes + (key_at ^ (32 * c)));
+                    s[kb] = M::run(k, q[c], s[kb]);
+                }
+            }
+            const bool partial = base < all_low || base + S::kKeys > all_high;
+            if (partial) {
+#pragma unroll
+                for (int kb = 0; kb < kBlocks; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int32_t slot = base + 32 * kb + 8 * (i / 4) + 4 * half + i % 4;
+                        if (slot < mine.low || slot >= mine.high) s[kb][i] = kNone;
+                    }
+            }
+            float most = s[0][0];
+#pragma unroll
+            for (int kb = 0; kb < kBlocks; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) most = fmaxf(most, s[kb][i]);
+            most = max_halves(most);
+            // A row without a maximum yet takes any; others wait for the slack.
+            if (__any(most * a.scale2 > top * a.scale2 + kSlack)) {
+                const float next = fmaxf(top, most);
+                const float factor = next == kNone ? 1.0f : __builtin_amdgcn_exp2f((top - next) * a.scale2);
+                top = next;
+                sum *= factor;
+#pragma unroll
+                for (int d = 0; d < kCols; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[d][i] *= factor;
+            }
+            const float shift = top == kNone ? 0.0f : top * a.scale2;
+            frag p[kBlocks][2];
+#pragma unroll
+            for (int kb = 0; kb < kBlocks; ++kb) {
+                float part = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float w = __builtin_amdgcn_exp2f(fmaf(s[kb][i], a.scale2, -shift));
+                    part += w;
+                    p[kb][i / 8][i % 8] = static_cast<T>(w);
+                }
+                sum += part;
+            }
+            // Sixteen values of columns 32 d + col, in the order of p[kb][h].
+            auto value_frag = [&](int kb, int h, int d) {
+                const char *at = vt + (32 * kb + 16 * h) * TL::kRowBytes + (value_at ^ (64 * d));
+                const uint2 v0 = read_transposed(at), v1 = read_transposed(at + 8 * TL::kRowBytes);
+                return uint4{v0.x, v0.y, v1.x, v1.y};
+            };
+            // A weight of 0 times an infinite or NaN value is NaN: where this wave's rows see different slots, such
+            // values may belong to slots that a row does not see, and the rows are taken one by one below.
+            if (partial && (any_low != all_low || any_high != all_high)) {
+                uint32_t found = 0;
+#pragma unroll 1
+                for (int x = 0; x < 2 * kBlocks; ++x)
+#pragma unroll
+                    for (int d = 0; d < kCols; ++d) {
+                        const uint4 v = value_frag(x / 2, x % 2, d);
+                        found |= M::special(v.x) | M::special(v.y) | M::special(v.z) | M::special(v.w);
+                    }
+                special = special || __any(found & 0x80008000u);
+            }
+#pragma unroll
+            for (int kb = 0; kb < kBlocks; ++kb)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int d = 0; d < kCols; ++d)
+                        acc[d] = M::run(__builtin_bit_cast(frag, value_frag(kb, h, d)), p[kb][h], acc[d]);
+        }
+        sum = add_halves(sum);
+        // Rows' results: row `row`, elements 32 d + 8 (i / 4) + 4 half + i % 4 in acc[d][i].
+        const int64_t token_index = seq.start + token;
+        const int64_t query_head = static_cast<int64_t>(head) * group + in_group;
+        const int64_t part_row = (static_cast<int64_t>(split) * a.tokens + token_index) * (a.kv_heads * group) + query_head;
+        const float top2 = top == kNone ? kNone : top * a.scale2;
+        // attend_alone for each of this wave's rows; `put` stores (row of the wave, row, its sums, its elements).
+        auto rows_alone = [&](auto put) {
+            for (int r = 0; r < 32; ++r) {
+                const int32_t one = tile * 32 * WQ + 32 * wq + r;
+                if (one >= rows) break;
+                const int32_t t = fast_quotient(one, a.group), h = one - t * group;
+                const T *q_row = reinterpret_cast<const T *>(a.query + (seq.start + t) * a.query_token +
+                                                             static_cast<int64_t>(head * group + h) * a.query_head);
+                float o[DP / 64];
+                const float2 sums = attend_alone<T, DP>(a, q_row, seen_by(a, seq, t), low + from * S::kStep + wk * S::kKeys,
+                                                        low + to * S::kStep, S::kStep, S::kKeys, stager.table, keys, values, o);
+                put(r, static_cast<int64_t>(seq.start + t), static_cast<int64_t>(head) * group + h, sums, o);
+            }
+        };
+        if (WK == 1) {
+            if (special) {
+                rows_alone([&](int, int64_t index, int64_t h, const float2 &sums, const float (&o)[DP / 64]) {
+                    const int64_t at = (static_cast<int64_t>(split) * a.tokens + index) * (a.kv_heads * group) + h;
+                    const bool parts = a.splits > 1;
+                    if (lane == 0 && parts) a.part_sum[at] = sums;
+                    if (lane == 0 && !parts && a.lse != nullptr) a.lse[index * a.lse_token + h] = lse_of(sums.x, sums.y);
+                    const float by = parts ? 1.0f : (sums.y == 0.0f ? 0.0f : 1.0f / sums.y);
+                    for (int k = 0; k < DP / 64; ++k) {
+                        const int e = lane + 64 * k;
+                        if (e >= static_cast<int>(a.head_dim)) continue;
+                        if (parts)
+                            a.part_out[at * a.head_dim + e] = o[k];
+                        else
+                            put_as(a.out_type, a.out + index * a.out_token + h * a.out_head, e, o[k] * by);
+                    }
+                });
+            } else if (row < rows) {
+                if (a.splits > 1) {
+                    if (half == 0) a.part_sum[part_row] = make_float2(top2, sum);
+                } else if (a.lse != nullptr && half == 0) {
+                    a.lse[token_index * a.lse_token + query_head] = lse_of(top2, sum);
+                }
+                const float by = a.splits > 1 ? 1.0f : (sum == 0.0f ? 0.0f : 1.0f / sum);
+                char *out = a.splits > 1 ? reinterpret_cast<char *>(a.part_out + part_row * a.head_dim)
+                                         : a.out + token_index * a.out_token + query_head * a.out_head;
+                const uint32_t type = a.splits > 1 ? QXT_TYPE_F32 : a.out_type;
+                if (a.splits == 1 || sum != 0.0f) {
+#pragma unroll
+                    for (int d = 0; d < kCols; ++d)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int e = 32 * d + 8 * i + 4 * half;
+                            if (e < static_cast<int>(a.head_dim))
+                                put4_as(type, out, e, acc[d][4 * i] * by, acc[d][4 * i + 1] * by, acc[d][4 * i + 2] * by,
+                                        acc[d][4 * i + 3] * by);
+                        }
+                }
+            }
+            if (WQ > 1) __syncthreads();  // before the next tile's staging
+            continue;
+        }
+
+        // Join the key parts: every wave scales to the common maximum and puts
+        // its outputs in LDS, then each wave adds up and stores its share of the elements.
+        constexpr int kPitch = DP + 4;  // floats a row
+        float *joined = reinterpret_cast<float *>(lds);                          // [WK][32 WQ][kPitch]
+        float2 *sums = reinterpret_cast<float2 *>(joined + WK * 32 * WQ * kPitch);  // [WK][32 WQ]
+        __syncthreads();  // staged tiles have been read
+        const int part_at = wk * 32 * WQ + 32 * wq;  // this wave's rows
+        if (special) {
+            rows_alone([&](int r, int64_t, int64_t, const float2 &one, const float (&o)[DP / 64]) {
+                if (lane == 0) sums[part_at + r] = one;
+                for (int k = 0; k < DP / 64; ++k) joined[(part_at + r) * kPitch + lane + 64 * k] = o[k];
+            });
+        } else {
+            if (half == 0) sums[part_at + col] = make_float2(top2, sum);
+#pragma unroll
+            for (int d = 0; d < kCols; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<float4 *>(joined + (part_at + col) * kPitch + 32 * d + 8 * i + 4 * half) =
+                        make_float4(acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]);
+        }
+        __syncthreads();
+        constexpr int kLanes = DP / 4;  // threads a row, four elements each
+        for (int r = threadIdx.x / kLanes; r < 32 * WQ; r += S::kThreads / kLanes) {
+            const int32_t out_row = tile * 32 * WQ + r;
+            if (out_row >= rows) break;
+            const int e = 4 * (threadIdx.x % kLanes);
+            float most = kNone, total = 0.0f;
+            float2 ms[WK];
+#pragma unroll
+            for (int w = 0; w < WK; ++w) {
+                ms[w] = sums[w * 32 * WQ + r];
+                most = fmaxf(most, ms[w].x);
+            }
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < WK; ++w) {
+                if (ms[w].y == 0.0f) continue;  // saw nothing (its maximum is -inf)
+                const float f = __builtin_amdgcn_exp2f(ms[w].x - (most == kNone ? 0.0f : most));
+                const float g = ms[w].x == kNone ? 1.0f : f;
+                const float4 y = *reinterpret_cast<const float4 *>(joined + (w * 32 * WQ + r) * kPitch + e);
+                total += ms[w].y * g;
+                x.x += y.x * g;
+                x.y += y.y * g;
+                x.z += y.z * g;
+                x.w += y.w * g;
+            }
+            const int32_t t = fast_quotient(out_row, a.group);
+            const int64_t index = seq.start + t, h = static_cast<int64_t>(head) * group + (out_row - t * group);
+            if (a.splits > 1) {
+                const int64_t at = (static_cast<int64_t>(split) * a.tokens + index) * (a.kv_heads * group) + h;
+                if (e == 0) a.part_sum[at] = make_float2(most, total);
+                if (total != 0.0f && e < static_cast<int>(a.head_dim))
+                    *reinterpret_cast<float4 *>(a.part_out + at * a.head_dim + e) = x;
+            } else {
+                if (e == 0 && a.lse != nullptr) a.lse[index * a.lse_token + h] = lse_of(most, total);
+                const float by = total == 0.0f ? 0.0f : 1.0f / total;
+                if (e < static_cast<int>(a.head_dim))
+                    put4_as(a.out_type, a.out + index * a.out_token + h * a.out_head, e, x.x * by, x.y * by, x.z * by, x.w * by);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// Join the parts of rows whose slots were split over workgroups: a wave a row,
+// four elements a lane.
+__global__ __launch_bounds__(256) void paged_attention_join_kernel(PagedArgs a) {
+    const uint32_t heads = a.kv_heads * a.group.divisor;
+    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * 4 + threadIdx.x / 64;
+    const uint64_t rows = static_cast<uint64_t>(a.tokens) * heads;
+    if (row >= rows) return;
+    const int64_t token = row / heads, head = row - token * heads;
+    if (a.starts != nullptr && (token < a.starts[0] || token >= a.starts[a.sequences])) return;  // nobody's row
+    const int lane = threadIdx.x % 64;
+    float top = kNone;
+    for (uint32_t s = lane; s < a.splits; s += 64) top = fmaxf(top, a.part_sum[s * rows + row].x);
+    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    float total = 0.0f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int e = 4 * lane;
+    for (uint32_t s = 0; s < a.splits; ++s) {
+        const float2 part = a.part_sum[s * rows + row];
+        if (part.y == 0.0f) continue;
+        const float f = part.x == kNone ? 1.0f : __builtin_amdgcn_exp2f(part.x - top);
+        total += part.y * f;
+        if (e < static_cast<int>(a.head_dim)) {
+            const float4 y = *reinterpret_cast<const float4 *>(a.part_out + (s * rows + row) * a.head_dim + e);
+            x.x += y.x * f;
+            x.y += y.y * f;
+            x.z += y.z * f;
+            x.w += y.w * f;
+        }
+    }
+    if (lane == 0 && a.lse != nullptr) a.lse[token * a.lse_token + head] = lse_of(top, total);
+    const float by = total == 0.0f ? 0.0f : 1.0f / total;
+    if (e < static_cast<int>(a.head_dim))
+        put4_as(a.out_type, a.out + token * a.out_token + head * a.out_head, e, x.x * by, x.y * by, x.z * by, x.w * by);
+}
+
+// ------------------------------------------------------------------ host side
+
+struct Plan {
+    uint32_t wq, wk, tiles, splits;
+};
+
+// Waves by the rows that share a key head (new tokens of the longest chunk
+// times heads of a group), then workgroups until the chip has work: the slots
+// of each row tile are split when tiles, heads and sequences alone are fewer.
+Plan plan_of(uint32_t head_dim, uint32_t group, uint32_t kv_heads, uint32_t sequences, uint32_t tokens,
+             uint32_t max_query, uint32_t max_context) {
+    const uint64_t rows = static_cast<uint64_t>(std::max(1u, std::min(max_query, tokens))) * group;
+    Plan p;
+    const bool wide = head_dim > 128;
+    p.wq = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 || wide ? 4 : 8;
+    p.wk = p.wq == 1 ? (wide ? 2 : 4) : p.wq == 2 ? (wide ? 1 : 2) : 1;
+    p.tiles = static_cast<uint32_t>((rows + 32 * p.wq - 1) / (32 * p.wq));
+    const uint64_t base = static_cast<uint64_t>(p.tiles) * kv_heads * sequences;
+    const uint64_t wanted = 2ull * compute_units();
+    const uint32_t step = (p.wq >= 4 && !wide ? 64 : 32) * p.wk;
+    const uint64_t most = std::max<uint64_t>(1, max_context / (4 * step));  // four steps a split at least
+    p.splits = static_cast<uint32_t>(std::min<uint64_t>({(wanted + base - 1) / base, most, 256}));
+    return p;
+}
+
+size_t workspace_of(const Plan &p, uint64_t tokens, uint64_t heads, uint64_t head_dim) {
+    return p.splits <= 1 ? 0 : p.splits * tokens * heads * (head_dim * 4 + 8);
+}
+
+template <typename T, int DP, int WQ, int WK>
+int launch_attention(const PagedArgs &a, uint32_t grid, hipStream_t stream) {
+    using S = Shape<DP, WQ, WK>;
+    constexpr size_t join = WK > 1 ? WK * 32 * WQ * (DP + 4) * 4 + WK * 32 * WQ * 8 : 0;
+    constexpr size_t lds = join > S::kLds ? join : S::kLds;
+    static_assert(lds <= 160 * 1024, "LDS");
+    return launch("paged_attention_kernel", paged_attention_kernel<T, DP, WQ, WK>, dim3(grid), dim3(S::kThreads), lds,
+                  stream, a);
+}
+
+template <typename T, int DP>
+int launch_attention_shape(const PagedArgs &a, const Plan &p, uint32_t grid, hipStream_t stream) {
+    constexpr bool wide = DP > 128;
+    if (p.wq == 1) return launch_attention<T, DP, 1, wide ? 2 : 4>(a, grid, stream);
+    if (p.wq == 2) return launch_attention<T, DP, 2, wide ? 1 : 2>(a, grid, stream);
+    if (p.wq == 4) return launch_attention<T, DP, 4, 1>(a, grid, stream);
+    if constexpr (!wide) return launch_attention<T, DP, 8, 1>(a, grid, stream);
+    return fail(QXT_INTERNAL_ERROR, "paged attention: no launch for %u waves", p.wq);
+}
+
+template <typename T>
+int launch_attention_dim(const PagedArgs &a, const Plan &p, uint32_t grid, hipStream_t stream) {
+    if (a.head_dim <= 64) return launch_attention_shape<T, 64>(a, p, grid, stream);
+    if (a.head_dim <= 128) return launch_attention_shape<T, 128>(a, p, grid, stream);
+    return launch_attention_shape<T, 256>(a, p, grid, stream);
+}
+
+}  // namespace
+
+int check_paged_cache(const char *name, const qxt_paged_cache *c, bool needs_values) {
+    if (c == nullptr || c->keys == nullptr || (needs_values && c->values == nullptr) || c->block_table == nullptr ||
+        c->context_lens == nullptr)
+        return fail(QXT_INVALID_ARGUMENT, "%s: null pointer", name);
+    if (!half_type(c->type)) return fail(QXT_INVALID_ARGUMENT, "%s: the cache must be bf16 or fp16", name);
+    if (c->page_size == 0 || c->heads == 0 || c->table_width == 0)
+        return fail(QXT_INVALID_ARGUMENT, "%s: page size, heads and table width must be positive", name);
+    if (c->head_dim == 0 || c->head_dim % 8 || c->head_dim > 256)
+        return fail(QXT_INVALID_ARGUMENT, "%s: head size must be a multiple of 8 up to 256", name);
+    if (static_cast<uint64_t>(c->page_size) * c->table_width > INT32_MAX / 2)
+        return fail(QXT_INVALID_ARGUMENT, "%s: a sequence has 2^30 slots or more", name);
+    if (!aligned(c->keys, 16) || !all_multiples(16, {c->key_page_stride, c->key_slot_stride, c->key_head_stride}) ||
+        (needs_values &&
+         (!aligned(c->values, 16) || !all_multiples(16, {c->value_page_stride, c->value_slot_stride, c->value_head_stride}))))
+        return fail(QXT_INVALID_ARGUMENT, "%s: cache rows must be 16-byte aligned", name);
+    if (c->block_table_stride % 4 || !aligned(c->block_table, 4) || !aligned(c->context_lens, 4))
+        return fail(QXT_INVALID_ARGUMENT, "%s: misaligned block table or lengths", name);
+    return QXT_OK;
+}
+
+}  // namespace qxt
+
+extern "C" {
+
+size_t qxt_paged_attention_workspace(uint32_t query_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t sequences,
+                                     uint32_t tokens, uint32_t max_query, uint32_t max_context) {
+    if (kv_heads == 0 || query_heads % kv_heads || query_heads == 0 || sequences == 0 || tokens == 0) return 0;
+    const qxt::Plan p = qxt::plan_of(head_dim, query_heads / kv_heads, kv_heads, sequences, tokens, max_query, max_context);
+    return qxt::workspace_of(p, tokens, query_heads, head_dim);
+}
+
+int qxt_paged_attention(const void *query, size_t query_token_stride, size_t query_head_stride,
+                        const qxt_paged_cache *cache, const int32_t *query_starts, void *out, size_t out_token_stride,
+                        size_t out_head_stride, uint32_t out_type, float *lse, size_t lse_token_stride, uint32_t tokens,
+                        uint32_t query_heads, float scale, uint32_t causal, uint32_t window, uint32_t max_query,
+                        uint32_t max_context, void *workspace, size_t workspace_bytes, void *stream) {
+    using namespace qxt;
+    if (int rc = check_paged_cache("paged attention", cache, true)) return rc;
+    if (tokens == 0 || cache->sequences == 0) return QXT_OK;
+    if (query == nullptr || out == nullptr) return fail(QXT_INVALID_ARGUMENT, "paged attention: null pointer");
+    if (query_heads == 0 || query_heads % cache->heads)
+        return fail(QXT_INVALID_ARGUMENT, "paged attention: query heads must be a multiple of the cache's");
+    if (!known_type(out_type)) return fail(QXT_INVALID_ARGUMENT, "paged attention: unknown element type");
+    if (!(scale > 0.0f) || scale > 3e38f) return fail(QXT_INVALID_ARGUMENT, "paged attention: scale must be positive and finite");
+    if (causal > 1 || window > INT32_MAX) return fail(QXT_INVALID_ARGUMENT, "paged attention: bad causal or window");
+    if (query_starts == nullptr && tokens != cache->sequences)
+        return fail(QXT_INVALID_ARGUMENT, "paged attention: without query starts every sequence has one token");
+    const uint32_t group = query_heads / cache->heads;
+    if (static_cast<uint64_t>(tokens) * query_heads > INT32_MAX / 2)
+        return fail(QXT_INVALID_ARGUMENT, "paged attention: 2^30 rows or more");
+    if (!aligned(query, 16) || !all_multiples(16, {query_token_stride, query_head_stride}))
+        return fail(QXT_INVALID_ARGUMENT, "paged attention: query rows must be 16-byte aligned");
+    const size_t quad = 4 * type_bytes(out_type);
+    if (!aligned(out, quad) || !all_multiples(quad, {out_token_stride, out_head_stride}) || !aligned(lse, 4) || lse_token_stride % 4)
+        return fail(QXT_INVALID_ARGUMENT, "paged attention: misaligned output");
+    if (query_starts == nullptr) max_query = 1;
+    const Plan p = plan_of(cache->head_dim, group, cache->heads, cache->sequences, tokens, max_query, max_context);
+    const size_t needed = workspace_of(p, tokens, query_heads, cache->head_dim);
+    if (needed > 0 && (workspace == nullptr || workspace_bytes < needed || !aligned(workspace, 16)))
+        return fail(QXT_INVALID_ARGUMENT, "paged attention: workspace of %zu bytes needed", needed);
+    const uint64_t grid = static_cast<uint64_t>(p.tiles) * p.splits * cache->heads * cache->sequences;
+    if (grid > INT32_MAX) return fail(QXT_INVALID_ARGUMENT, "paged attention: too many row tiles");
+    if (int rc = injected(QXT_FAIL_SUBMISSION)) return rc;
+
+    PagedArgs a{};
+    a.query = static_cast<const char *>(query);
+    a.query_token = query_token_stride;
+    a.query_head = query_head_stride;
+    a.keys = {static_cast<char *>(cache->keys), static_cast<int64_t>(cache->key_page_stride),
+              static_cast<int64_t>(cache->key_slot_stride), static_cast<int64_t>(cache->key_head_stride)};
+    a.values = {static_cast<char *>(cache->values), static_cast<int64_t>(cache->value_page_stride),
+                static_cast<int64_t>(cache->value_slot_stride), static_cast<int64_t>(cache->value_head_stride)};
+    a.table = cache->block_table;
+    a.table_stride = cache->block_table_stride / 4;
+    a.pages = cache->pages;
+    a.page = fast_div(cache->page_size);
+    a.slots = static_cast<int32_t>(cache->page_size * cache->table_width);
+    a.lens = cache->context_lens;
+    a.starts = query_starts;
+    a.sequences = cache->sequences;
+    a.tokens = tokens;
+    a.kv_heads = cache->heads;
+    a.head_dim = cache->head_dim;
+    a.group = fast_div(group);
+    a.scale = scale;
+    a.scale2 = static_cast<float>(scale * 1.4426950408889634);
+    a.causal = causal;
+    a.window = static_cast<int32_t>(window);
+    a.tiles = p.tiles;
+    a.splits = p.splits;
+    a.out = static_cast<char *>(out);
+    a.out_token = out_token_stride;
+    a.out_head = out_head_stride;
+    a.out_type = out_type;
+    a.lse = lse;
+    a.lse_token = lse_token_stride / 4;
+    if (p.splits > 1) {
+        a.part_out = static_cast<float *>(workspace);
+        a.part_sum = reinterpret_cast<float2 *>(a.part_out + static_cast<size_t>(p.splits) * tokens * query_heads * cache->head_dim);
+    }
+    const int rc = cache->type == QXT_TYPE_BF16
+                       ? launch_attention_dim<bf16_t>(a, p, static_cast<uint32_t>(grid), as_stream(stream))
+                       : launch_attention_dim<f16_t>(a, p, static_cast<uint32_t>(grid), as_stream(stream));
+    if (rc != QXT_OK || p.splits == 1) return rc;
+    const uint64_t rows = static_cast<uint64_t>(tokens) * query_heads;
+    return launch("paged_attention_join_kernel", paged_attention_join_kernel, dim3(static_cast<uint32_t>((rows + 3) / 4)),
+                  dim3(256), 0, as_stream(stream), a);
+}
+
+}  // extern "C"

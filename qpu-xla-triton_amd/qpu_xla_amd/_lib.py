@@ -15,6 +15,7 @@ from ctypes import (
     Structure,
     c_char,
     c_char_p,
+    c_float,
     c_int,
     c_int32,
     c_int64,
@@ -53,6 +54,10 @@ Q4_0_LAYOUT_NATIVE = 0
 Q4_0_LAYOUT_LANES = 1
 WEIGHT_NK = 0
 WEIGHT_K4N = 1
+TYPE_F32 = 0
+TYPE_BF16 = 1
+TYPE_F16 = 2
+ROPE_INTERLEAVED = 1
 
 
 class DeviceInfo(Structure):
@@ -90,6 +95,31 @@ class Q4Task(Structure):
         ("output_column_start", c_uint32),
         ("column_count", c_uint32),
         ("weight_layout", c_uint32),
+    ]
+
+
+class PagedCache(Structure):
+    """``qxt_paged_cache``: keys and values of many sequences in pages."""
+
+    _fields_ = [
+        ("keys", c_void_p),
+        ("key_page_stride", c_size_t),
+        ("key_slot_stride", c_size_t),
+        ("key_head_stride", c_size_t),
+        ("values", c_void_p),
+        ("value_page_stride", c_size_t),
+        ("value_slot_stride", c_size_t),
+        ("value_head_stride", c_size_t),
+        ("block_table", c_void_p),
+        ("block_table_stride", c_size_t),
+        ("context_lens", c_void_p),
+        ("pages", c_uint32),
+        ("page_size", c_uint32),
+        ("heads", c_uint32),
+        ("head_dim", c_uint32),
+        ("type", c_uint32),
+        ("table_width", c_uint32),
+        ("sequences", c_uint32),
     ]
 
 
@@ -182,6 +212,21 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "qxt_w8a8_dequantize": (c_int, [_P, _SZ, _P, _P, _P, _P, _SZ, _U, _U, _P]),
     "qxt_w8a8_linear": (c_int, [_P, _SZ, _P, _SZ, _P, _P, _SZ, _P, _P, _P, _SZ, _U, _U, _U, _U, _U, _P]),
     "qxt_w8a8_linear_noalloc": (c_int, [_P, _SZ, _P, _SZ, _P, _P, _P, _SZ, _U, _U, _U, _U, _U, _P]),
+    "qxt_qk_norm_rope": (
+        c_int, [_P, _SZ, _SZ, _P, _SZ, _SZ, _P, _P, c_float, _P, _P, _SZ, _U, _P, _P, _SZ, _SZ, _P, _SZ, _SZ] + [_U] * 8 + [_P]),
+    "qxt_qk_norm_rope_cache": (
+        c_int, [_P, _SZ, _SZ, _P, _SZ, _SZ, _P, _SZ, _SZ, _P, _P, c_float, _P, _P, _SZ, _U, _P, _P, _P, _SZ, _SZ,
+                POINTER(PagedCache)] + [_U] * 5 + [_P]),
+    "qxt_paged_attention_workspace": (_SZ, [_U] * 7),
+    "qxt_paged_attention": (
+        c_int, [_P, _SZ, _SZ, POINTER(PagedCache), _P, _P, _SZ, _SZ, _U, _P, _SZ, _U, _U, c_float] + [_U] * 4 + [_P, _SZ, _P]),
+    "qxt_paged_attention_scores_workspace": (_SZ, [_U] * 7),
+    "qxt_paged_attention_scores": (
+        c_int, [_P, _SZ, _SZ, POINTER(PagedCache), _P, _P, _SZ, _P, _SZ, _SZ, _P, _SZ, _SZ, _U, _U, c_float] + [_U] * 4
+        + [_P, _SZ, _P]),
+    "qxt_paged_cache_evict_workspace": (_SZ, [_U] * 4),
+    "qxt_paged_cache_evict": (
+        c_int, [POINTER(PagedCache), _P, _SZ, _SZ, _P, _SZ, _SZ, _P, _SZ, _SZ, _P, _SZ, _SZ, _P, _U, _U, _U, _P, _SZ, _P]),
     "qxt_llama_context_create": (c_int, [POINTER(LlamaContextConfig), POINTER(c_void_p)]),
     "qxt_llama_context_destroy": (None, [_P]),
     "qxt_llama_context_last_error": (c_char_p, [_P]),

@@ -44,5 +44,26 @@ from qpu_xla_amd.kernels.ggml_q8_0 import (  # noqa: F401
     ggml_q8_0_q8_0_linear,
     supports_ggml_q8_0_q8_0_linear_m4,
 )
+from qpu_xla_amd.kernels.paged_attention import (  # noqa: F401
+    PAGED_ATTENTION_KERNEL,
+    PAGED_ATTENTION_SCORES_KERNEL,
+    PagedAttentionOptions,
+    paged_attention,
+    paged_attention_grid,
+    paged_attention_scores,
+)
+from qpu_xla_amd.kernels.paged_eviction import (  # noqa: F401
+    PAGED_CACHE_EVICT_KERNEL,
+    PagedEvictionOptions,
+    paged_cache_evict,
+    paged_cache_evict_grid,
+)
+from qpu_xla_amd.kernels.qk_norm_rope import (  # noqa: F401
+    QK_NORM_ROPE_CACHE_KERNEL,
+    QkNormRopeOptions,
+    qk_norm_rope,
+    qk_norm_rope_cache,
+    qk_norm_rope_grid,
+)
 from qpu_xla_amd.kernels.quantize import quantize_q4_0, quantize_q8_0, quantize_rows_int8  # noqa: F401
 from qpu_xla_amd.kernels.w8a8_epilogue import W8A8_DEQUANTIZE_KERNEL, supports_w8a8_dequantize, w8a8_dequantize  # noqa: F401

@@ -1,0 +1,237 @@
+"""Attention of new tokens over a paged cache on gfx950.
+
+* ``paged_attention`` -- queries [T, Hq, D] of one token a sequence, or of chunks, over keys and values in pages.
+* ``paged_attention_scores`` -- the attention weight that each cached slot received, added up per key head.
+
+Caches are [pages, page_size, Hkv, D] (bfloat16 or float16, D a multiple of 8 up to 256, any strides with 16-byte
+aligned rows); ``block_table`` int32 [B, W] names each sequence's pages in order and ``context_lens`` int32 [B] its
+slots in use, the new tokens' included.  ``query_starts`` int32 [B + 1] gives each sequence's tokens
+(``query_starts[b]`` up to ``query_starts[b + 1]``); without it every sequence has one.  Token i of n sees the slots
+``j < L``, with ``causal`` ``j <= L - n + i``, and with a window ``j > L - n + i - window``.  A token that sees none
+gets 0 (and -inf as its log-sum).  Slots that a token does not see do not reach its result, whatever they hold.
+
+``max_query`` and ``max_context`` are the host's bounds of chunk and context lengths; they size the launch (default:
+what the tensors could hold).  The reference's attention programs (``src/qpu_xla/kernels/ggml_flash_attn.py``) take
+one contiguous fp32 sequence; it has no paged cache.
+"""
+
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+from typing import Any
+
+import torch
+
+from qpu_xla_amd import _lib
+from qpu_xla_amd._paged import (
+    TYPES,
+    byte_strides,
+    cache_struct,
+    check_cache,
+    check_head_rows,
+    check_index,
+    check_per_slot,
+    check_size,
+    check_table,
+    dense_last,
+    empty_for,
+)
+from qpu_xla_amd._tensors import ptr, require_gpu, stream_handle
+from qpu_xla_amd.errors import KernelError
+from qpu_xla_amd.kernel import Kernel
+
+
+def _check(name: str, query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor | None,
+           block_table: torch.Tensor, context_lens: torch.Tensor, query_starts: torch.Tensor | None) -> None:
+    check_head_rows(name, "query", query)
+    check_cache(name, key_cache, value_cache)
+    check_table(name, block_table, context_lens)
+    heads, head_dim = key_cache.shape[2:]
+    if query.dtype != key_cache.dtype or query.shape[2] != head_dim:
+        raise ValueError(f"{name}: query must have the cache's type and head size")
+    if query.shape[1] == 0 or query.shape[1] % heads:
+        raise ValueError(f"{name}: query heads must be a multiple of the cache's heads")
+    if head_dim % 8 or head_dim > 256:
+        raise ValueError(f"{name}: head size must be a multiple of 8 up to 256")
+    sequences = block_table.shape[0]
+    if query_starts is not None:
+        check_index(name, "query_starts", query_starts, torch.int32, sequences + 1)
+    elif query.shape[0] != sequences:
+        raise ValueError(f"{name}: without query_starts every sequence has one token")
+
+
+def _check_lse(name: str, query: torch.Tensor, lse: torch.Tensor) -> None:
+    if lse.dtype != torch.float32 or tuple(lse.shape) != tuple(query.shape[:2]) or not dense_last(lse):
+        raise ValueError(f"{name}: lse must be float32 [tokens, heads] with dense rows")
+
+
+def _sizes(name: str, query: torch.Tensor, key_cache: torch.Tensor, block_table: torch.Tensor, scale: float | None,
+           window: int, max_query: int | None, max_context: int | None) -> tuple[float, int, int, int]:
+    scale = 1.0 / math.sqrt(query.shape[2]) if scale is None else float(scale)
+    if not 0.0 < scale < 3e38:
+        raise ValueError(f"{name}: scale must be positive and finite")
+    max_query = query.shape[0] if max_query is None else check_size(name, "max_query", max_query)
+    slots = block_table.shape[1] * key_cache.shape[1]
+    max_context = slots if max_context is None else min(slots, check_size(name, "max_context", max_context))
+    window = int(window)
+    if window < 0:
+        raise ValueError(f"{name}: window must not be negative")
+    return scale, min(window, 2**31 - 1), max_query, max_context
+
+
+def paged_attention(
+    query: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    context_lens: torch.Tensor,
+    query_starts: torch.Tensor | None = None,
+    *,
+    scale: float | None = None,
+    causal: bool = True,
+    window: int = 0,
+    max_query: int | None = None,
+    max_context: int | None = None,
+    out: torch.Tensor | None = None,
+    lse: torch.Tensor | None = None,
+    stream: Any = None,
+) -> torch.Tensor:
+    """Attention outputs [T, Hq, D] (the query's type, or ``out``'s); ``lse`` float32 [T, Hq] receives the log-sums."""
+    name = "paged_attention"
+    _check(name, query, key_cache, value_cache, block_table, context_lens, query_starts)
+    scale, window, max_query, max_context = _sizes(name, query, key_cache, block_table, scale, window, max_query, max_context)
+    tokens, query_heads, head_dim = query.shape
+    if out is None:
+        out = empty_for(stream, tuple(query.shape), query.dtype, query.device)
+    check_head_rows(name, "out", out)
+    if out.shape != query.shape:
+        raise ValueError(f"{name}: out must have the query's shape")
+    if lse is not None:
+        _check_lse(name, query, lse)
+    require_gpu(name, query, key_cache, value_cache, block_table, context_lens, query_starts, out, lse)
+    if tokens == 0 or block_table.shape[0] == 0:
+        return out
+    if query_starts is None:
+        max_query = 1
+    size = (_lib._lib or _lib.load()).qxt_paged_attention_workspace(
+        query_heads, key_cache.shape[2], head_dim, block_table.shape[0], tokens, max_query, max_context)
+    workspace = empty_for(stream, (size,), torch.uint8, query.device) if size else None
+    _lib.call(
+        "qxt_paged_attention", ptr(query), *byte_strides(query, 2),
+        cache_struct(key_cache, value_cache, block_table, context_lens), ptr(query_starts), ptr(out),
+        *byte_strides(out, 2), TYPES[out.dtype], ptr(lse), 0 if lse is None else byte_strides(lse, 1)[0], tokens,
+        query_heads, scale, 1 if causal else 0, window, max_query, max_context, ptr(workspace), size,
+        stream_handle(stream),
+    )
+    return out
+
+
+def paged_attention_scores(
+    query: torch.Tensor,
+    key_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    context_lens: torch.Tensor,
+    lse: torch.Tensor,
+    query_starts: torch.Tensor | None = None,
+    *,
+    scores: torch.Tensor | None = None,
+    scale: float | None = None,
+    causal: bool = True,
+    window: int = 0,
+    max_query: int | None = None,
+    max_context: int | None = None,
+    out: torch.Tensor | None = None,
+    stream: Any = None,
+) -> torch.Tensor:
+    """Weight that each slot received, float32 [B, Hkv, W * page_size], on top of ``scores`` (None: zeros).
+
+    ``lse`` are the log-sums that ``paged_attention`` wrote for the same queries, cache and masks; a row's weights then
+    add up to 1.  ``out`` may be ``scores`` itself.
+    """
+    name = "paged_attention_scores"
+    _check(name, query, key_cache, None, block_table, context_lens, query_starts)
+    scale, window, max_query, max_context = _sizes(name, query, key_cache, block_table, scale, window, max_query, max_context)
+    tokens, query_heads, _ = query.shape
+    _check_lse(name, query, lse)
+    if scores is not None:
+        check_per_slot(name, "scores", scores, torch.float32, key_cache, block_table)
+    sequences, heads, slots = block_table.shape[0], key_cache.shape[2], block_table.shape[1] * key_cache.shape[1]
+    if out is None:
+        out = empty_for(stream, (sequences, heads, slots), torch.float32, query.device)
+    check_per_slot(name, "out", out, torch.float32, key_cache, block_table)
+    require_gpu(name, query, key_cache, block_table, context_lens, lse, query_starts, scores, out)
+    if sequences == 0:
+        return out
+    if query_starts is None:
+        max_query = 1
+    size = (_lib._lib or _lib.load()).qxt_paged_attention_scores_workspace(
+        query_heads, heads, sequences, tokens, slots, max_query, max_context)
+    workspace = empty_for(stream, (size,), torch.uint8, query.device) if size else None
+    before = (0, 0) if scores is None else byte_strides(scores, 2)
+    _lib.call(
+        "qxt_paged_attention_scores", ptr(query), *byte_strides(query, 2),
+        cache_struct(key_cache, None, block_table, context_lens), ptr(query_starts), ptr(lse), byte_strides(lse, 1)[0],
+        ptr(scores), *before, ptr(out), *byte_strides(out, 2), tokens, query_heads, scale, 1 if causal else 0, window,
+        max_query, max_context, ptr(workspace), size, stream_handle(stream),
+    )
+    return out
+
+
+@dataclass(frozen=True, slots=True)
+class PagedAttentionOptions:
+    """Last argument of the ``Kernel`` objects here; the keywords of the functions."""
+
+    scale: float | None = None
+    causal: bool = True
+    window: int = 0
+    max_query: int | None = None
+    max_context: int | None = None
+
+
+def paged_attention_grid(query: torch.Tensor) -> tuple[int, int, int]:
+    """Grid of the ``Kernel`` objects here: (query heads, tokens, 1)."""
+    return (query.shape[1], query.shape[0], 1)
+
+
+def _execute_paged_attention(stream: Any, args: tuple[Any, ...], grid: tuple[int, int, int]) -> None:
+    tensors = args[:5] + args[6:7]
+    if (len(args) != 9 or not all(isinstance(a, torch.Tensor) for a in tensors)
+            or not all(a is None or isinstance(a, torch.Tensor) for a in (args[5], args[7]))
+            or not isinstance(args[8], PagedAttentionOptions)):
+        raise KernelError("paged attention expects (query, key_cache, value_cache, block_table, context_lens, "
+                          "query_starts or None, out, lse or None, PagedAttentionOptions)")
+    if args[0].dim() != 3 or tuple(grid) != paged_attention_grid(args[0]):
+        raise KernelError(f"paged attention grid must be (query heads, tokens, 1), got {tuple(grid)}")
+    o = args[8]
+    paged_attention(*args[:6], scale=o.scale, causal=o.causal, window=o.window, max_query=o.max_query,
+                    max_context=o.max_context, out=args[6], lse=args[7], stream=stream)
+
+
+PAGED_ATTENTION_KERNEL = Kernel("gfx950.paged_attention", _execute_paged_attention)
+
+
+def _execute_paged_attention_scores(stream: Any, args: tuple[Any, ...], grid: tuple[int, int, int]) -> None:
+    tensors = args[:5] + args[7:8]
+    if (len(args) != 9 or not all(isinstance(a, torch.Tensor) for a in tensors)
+            or not all(a is None or isinstance(a, torch.Tensor) for a in (args[5], args[6]))
+            or not isinstance(args[8], PagedAttentionOptions)):
+        raise KernelError("paged attention scores expects (query, key_cache, block_table, context_lens, lse, query_starts or "
+                          "None, scores or None, out, PagedAttentionOptions)")
+    if args[0].dim() != 3 or tuple(grid) != paged_attention_grid(args[0]):
+        raise KernelError(f"paged attention scores grid must be (query heads, tokens, 1), got {tuple(grid)}")
+    o = args[8]
+    paged_attention_scores(*args[:6], scores=args[6], scale=o.scale, causal=o.causal, window=o.window,
+                           max_query=o.max_query, max_context=o.max_context, out=args[7], stream=stream)
+
+
+PAGED_ATTENTION_SCORES_KERNEL = Kernel("gfx950.paged_attention_scores", _execute_paged_attention_scores)
+
+__all__ = [
+    "PAGED_ATTENTION_KERNEL",
+    "PAGED_ATTENTION_SCORES_KERNEL",
+    "PagedAttentionOptions",
+    "paged_attention",
+    "paged_attention_grid",
+    "paged_attention_scores",
+]
