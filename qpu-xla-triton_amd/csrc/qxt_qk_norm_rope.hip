@@ -44,41 +44,42 @@ struct RopeArgs {
 struct RowPlace {
     const char *in;
     char *out;
-    uint32_t kind;  // 0 query, 1 key, 2 value
+    const float *weight;
+    bool turns;  // a query or a key
     uint32_t token;
 };
 
+// (Selections between values, not an index into the argument arrays or a choice between their elements: an
+// address that the compiler does not know sends the whole argument block through scratch memory.)
 __device__ __forceinline__ RowPlace place_row(const RopeArgs &a, uint32_t row) {
     RowPlace p;
     p.token = fast_quotient(row, a.heads);
     uint32_t head = row - p.token * a.heads.divisor;
-    p.kind = 0;
-    if (head >= a.query_heads) {
-        head -= a.query_heads;
-        p.kind = 1;
-        if (head >= a.key_heads) {
-            head -= a.key_heads;
-            p.kind = 2;
+    const bool query = head < a.query_heads;
+    head -= query ? 0 : a.query_heads;
+    const bool key = !query && head < a.key_heads;
+    head -= query || key ? 0 : a.key_heads;
+    p.turns = query || key;
+    const float *const weight0 = a.weight[0], *const weight1 = a.weight[1];
+    p.weight = query ? weight0 : key ? weight1 : nullptr;
+    const char *const in0 = a.in[0], *const in1 = a.in[1], *const in2 = a.in[2];
+    const int64_t token0 = a.in_token[0], token1 = a.in_token[1], token2 = a.in_token[2];
+    const int64_t head0 = a.in_head[0], head1 = a.in_head[1], head2 = a.in_head[2];
+    p.in = (query ? in0 : key ? in1 : in2) + p.token * (query ? token0 : key ? token1 : token2) +
+           head * (query ? head0 : key ? head1 : head2);
+    p.out = a.query_out + p.token * a.query_out_token + head * a.query_out_head;
+    if (!query) {
+        const int64_t slot = a.slots != nullptr ? a.slots[p.token] : p.token;
+        int64_t page = slot, offset = 0;
+        if (a.page_size > 1) {
+            page = a.slot_count <= INT32_MAX ? fast_quotient(static_cast<uint32_t>(slot), a.page) : slot / a.page_size;
+            offset = slot - page * a.page_size;
         }
+        const CacheView keys = a.out[0], values = a.out[1];
+        p.out = (key ? keys.data : values.data) + page * (key ? keys.page_stride : values.page_stride) +
+                offset * (key ? keys.slot_stride : values.slot_stride) + head * (key ? keys.head_stride : values.head_stride);
+        if (slot < 0 || slot >= a.slot_count) p.out = nullptr;  // padding tokens, and nothing outside the cache
     }
-    p.in = a.in[p.kind] + p.token * a.in_token[p.kind] + head * a.in_head[p.kind];
-    if (p.kind == 0) {
-        p.out = a.query_out + p.token * a.query_out_token + head * a.query_out_head;
-        return p;
-    }
-    const int64_t slot = a.slots != nullptr ? a.slots[p.token] : p.token;
-    if (slot < 0 || slot >= a.slot_count) {  // padding tokens, and nothing outside the cache
-        p.out = nullptr;
-        return p;
-    }
-    int64_t page = slot, offset = 0;
-    if (a.page_size > 1) {
-        // (A 64-bit division by every lane took half of the kernel's time.)
-        page = a.slot_count <= INT32_MAX ? fast_quotient(static_cast<uint32_t>(slot), a.page) : slot / a.page_size;
-        offset = slot - page * a.page_size;
-    }
-    const CacheView &c = a.out[p.kind - 1];
-    p.out = c.data + page * c.page_stride + offset * c.slot_stride + head * c.head_stride;
     return p;
 }
 
@@ -134,9 +135,9 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a) {
     float4 x0 = make_float4(0.f, 0.f, 0.f, 0.f), x1 = x0;
     if (has0) x0 = load4(in + 4 * r0);
     if (has1) x1 = load4(in + 4 * r1);
-    if (p.kind < 2) {
+    if (p.turns) {
         const int32_t position = a.positions[p.token];
-        const float *weight = a.weight[p.kind];
+        const float *weight = p.weight;
         if (weight != nullptr) {
             float sum = squares(x0) + squares(x1);
 #pragma unroll
@@ -190,7 +191,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_any_kernel(RopeArgs a) {
     const RowPlace p = place_row(a, row);
     const TI *in = reinterpret_cast<const TI *>(p.in);
     TO *out = reinterpret_cast<TO *>(p.out);
-    const float *weight = p.kind < 2 ? a.weight[p.kind] : nullptr;
+    const float *weight = p.weight;
     float scale = 1.0f;
     if (weight != nullptr) {
         float sum = 0.0f;
@@ -202,9 +203,9 @@ __global__ __launch_bounds__(256) void qk_norm_rope_any_kernel(RopeArgs a) {
         scale = rsqrtf(sum / static_cast<float>(a.head_dim) + a.epsilon);
     }
     if (out == nullptr) return;
-    const int32_t position = p.kind < 2 ? a.positions[p.token] : 0;
+    const int32_t position = p.turns ? a.positions[p.token] : 0;
     const bool known = static_cast<uint32_t>(position) < a.table_rows;
-    const uint32_t half = p.kind < 2 ? a.rotary_dim / 2 : 0, rotated = 2 * half;
+    const uint32_t half = p.turns ? a.rotary_dim / 2 : 0, rotated = 2 * half;
     for (uint32_t i = lane; i < half + (a.head_dim - rotated + 1) / 2; i += 64) {
         const bool turns = i < half;
         const uint32_t e0 = turns && !INTERLEAVED ? i : 2 * i, e1 = turns && !INTERLEAVED ? i + half : 2 * i + 1;
