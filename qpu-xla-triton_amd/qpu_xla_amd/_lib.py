@@ -9,6 +9,7 @@ fallback: when the library is missing every entry point raises
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from ctypes import (
     POINTER,
@@ -98,29 +99,8 @@ class Q4Task(Structure):
     ]
 
 
-class PagedCache(Structure):
-    """``qxt_paged_cache``: keys and values of many sequences in pages."""
-
-    _fields_ = [
-        ("keys", c_void_p),
-        ("key_page_stride", c_size_t),
-        ("key_slot_stride", c_size_t),
-        ("key_head_stride", c_size_t),
-        ("values", c_void_p),
-        ("value_page_stride", c_size_t),
-        ("value_slot_stride", c_size_t),
-        ("value_head_stride", c_size_t),
-        ("block_table", c_void_p),
-        ("block_table_stride", c_size_t),
-        ("context_lens", c_void_p),
-        ("pages", c_uint32),
-        ("page_size", c_uint32),
-        ("heads", c_uint32),
-        ("head_dim", c_uint32),
-        ("type", c_uint32),
-        ("table_width", c_uint32),
-        ("sequences", c_uint32),
-    ]
+# ``qxt_paged_cache`` in C's layout, packed by struct (a ctypes Structure of its 18 fields takes 2 us to fill).
+PAGED_CACHE = struct.Struct("PNNNPNNNPNPIIIIIII0P")
 
 
 class LlamaContextConfig(Structure):
@@ -216,17 +196,17 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
         c_int, [_P, _SZ, _SZ, _P, _SZ, _SZ, _P, _P, c_float, _P, _P, _SZ, _U, _P, _P, _SZ, _SZ, _P, _SZ, _SZ] + [_U] * 8 + [_P]),
     "qxt_qk_norm_rope_cache": (
         c_int, [_P, _SZ, _SZ, _P, _SZ, _SZ, _P, _SZ, _SZ, _P, _P, c_float, _P, _P, _SZ, _U, _P, _P, _P, _SZ, _SZ,
-                POINTER(PagedCache)] + [_U] * 5 + [_P]),
+                _P] + [_U] * 5 + [_P]),
     "qxt_paged_attention_workspace": (_SZ, [_U] * 7),
     "qxt_paged_attention": (
-        c_int, [_P, _SZ, _SZ, POINTER(PagedCache), _P, _P, _SZ, _SZ, _U, _P, _SZ, _U, _U, c_float] + [_U] * 4 + [_P, _SZ, _P]),
+        c_int, [_P, _SZ, _SZ, _P, _P, _P, _SZ, _SZ, _U, _P, _SZ, _U, _U, c_float] + [_U] * 4 + [_P, _SZ, _P]),
     "qxt_paged_attention_scores_workspace": (_SZ, [_U] * 7),
     "qxt_paged_attention_scores": (
-        c_int, [_P, _SZ, _SZ, POINTER(PagedCache), _P, _P, _SZ, _P, _SZ, _SZ, _P, _SZ, _SZ, _U, _U, c_float] + [_U] * 4
+        c_int, [_P, _SZ, _SZ, _P, _P, _P, _SZ, _P, _SZ, _SZ, _P, _SZ, _SZ, _U, _U, c_float] + [_U] * 4
         + [_P, _SZ, _P]),
     "qxt_paged_cache_evict_workspace": (_SZ, [_U] * 4),
     "qxt_paged_cache_evict": (
-        c_int, [POINTER(PagedCache), _P, _SZ, _SZ, _P, _SZ, _SZ, _P, _SZ, _SZ, _P, _SZ, _SZ, _P, _U, _U, _U, _P, _SZ, _P]),
+        c_int, [_P, _P, _SZ, _SZ, _P, _SZ, _SZ, _P, _SZ, _SZ, _P, _SZ, _SZ, _P, _U, _U, _U, _P, _SZ, _P]),
     "qxt_llama_context_create": (c_int, [POINTER(LlamaContextConfig), POINTER(c_void_p)]),
     "qxt_llama_context_destroy": (None, [_P]),
     "qxt_llama_context_last_error": (c_char_p, [_P]),

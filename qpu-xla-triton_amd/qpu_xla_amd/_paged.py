@@ -1,17 +1,19 @@
-"""Checks and C-ABI arguments shared by the attention operators over a paged cache."""
+"""Checks and C-ABI arguments shared by the attention operators over a paged cache.
+
+They run at every call, and a call of few tokens is bound by them: shapes and strides are read once each, devices are
+compared as integers, and the cache description is packed in one go.
+"""
 
 from __future__ import annotations
 
-import ctypes
 from typing import Any
 
 import torch
 
 from qpu_xla_amd import _lib
-from qpu_xla_amd._tensors import ptr, stream_handle
+from qpu_xla_amd._tensors import stream_handle
 
 TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16, torch.float16: _lib.TYPE_F16}
-CACHE_TYPES = (torch.bfloat16, torch.float16)
 UINT32_MAX = 2**32 - 1
 
 
@@ -34,64 +36,89 @@ def empty_for(stream: Any, shape: tuple[int, ...], dtype: torch.dtype, device: t
     return tensor
 
 
-def byte_strides(t: torch.Tensor, dims: int) -> list[int]:
-    """Byte strides of the first ``dims`` dimensions; 0 for those of one entry (torch gives them any)."""
-    size = t.element_size()
-    return [0 if extent == 1 else step * size for extent, step in zip(t.shape[:dims], t.stride()[:dims])]
+def require_one_gpu(name: str, first: torch.Tensor, *others: torch.Tensor | None) -> None:
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            index = -1
+    if index < 0:
+        raise ValueError(f"{name}: all tensors must live on one HIP device (no CPU fallback)")
+
+
+def head_rows(name: str, what: str, t: torch.Tensor) -> tuple[torch.Size, int, int, int]:
+    """Shape, type code and byte strides (token, head; 0 for one of them: torch gives those any) of [T, H, D] rows."""
+    shape = t.shape
+    code = TYPES.get(t.dtype)
+    if code is None or len(shape) != 3:
+        raise ValueError(f"{name}: {what} must be float32, bfloat16 or float16 [tokens, heads, head_dim] with dense rows")
+    tokens, heads, dim = shape
+    token, head, element = t.stride()
+    if element != 1 and dim != 1:
+        raise ValueError(f"{name}: {what} must be float32, bfloat16 or float16 [tokens, heads, head_dim] with dense rows")
+    size = 2 if code else 4
+    return shape, code, 0 if tokens == 1 else token * size, 0 if heads == 1 else head * size
+
+
+def _cache_strides(name: str, what: str, t: torch.Tensor) -> tuple[torch.Size, int, int, int, int]:
+    shape = t.shape
+    code = TYPES.get(t.dtype)
+    if not code or len(shape) != 4:
+        raise ValueError(f"{name}: {what} must be bfloat16 or float16 [pages, page_size, heads, head_dim] with dense rows")
+    pages, page_size, heads, dim = shape
+    page, slot, head, element = t.stride()
+    if element != 1 and dim != 1:
+        raise ValueError(f"{name}: {what} must be bfloat16 or float16 [pages, page_size, heads, head_dim] with dense rows")
+    if not (pages and page_size and heads and dim):
+        raise ValueError(f"{name}: the cache is empty")
+    return shape, code, 0 if pages == 1 else 2 * page, 0 if page_size == 1 else 2 * slot, 0 if heads == 1 else 2 * head
+
+
+def paged_cache(name: str, keys: torch.Tensor, values: torch.Tensor | None, table: torch.Tensor | None = None,
+                lens: torch.Tensor | None = None) -> tuple[torch.Size, int, int, int, bytes]:
+    """(cache shape, type code, sequences, table columns, ``qxt_paged_cache``) of checked tensors."""
+    shape, code, *key_strides = _cache_strides(name, "key_cache", keys)
+    value_at, value_strides = 0, (0, 0, 0)
+    if values is not None:
+        value_shape, value_code, *value_strides = _cache_strides(name, "value_cache", values)
+        if value_shape != shape or value_code != code:
+            raise ValueError(f"{name}: key_cache and value_cache must have one shape and type")
+        value_at = values.data_ptr()
+    sequences = width = table_at = table_stride = lens_at = 0
+    if table is not None:
+        table_shape = table.shape
+        if table.dtype is not torch.int32 or len(table_shape) != 2 or table_shape[1] == 0 or not dense_last(table):
+            raise ValueError(f"{name}: block_table must be int32 [sequences, pages of the longest] with dense rows")
+        sequences, width = table_shape
+        check_index(name, "context_lens", lens, torch.int32, sequences)
+        table_at, lens_at = table.data_ptr(), lens.data_ptr()
+        table_stride = 0 if sequences == 1 else 4 * table.stride(0)
+    packed = _lib.PAGED_CACHE.pack(keys.data_ptr(), *key_strides, value_at, *value_strides, table_at, table_stride, lens_at,
+                                   *shape, code, width, sequences)
+    return shape, code, sequences, width, packed
 
 
 def dense_last(t: torch.Tensor) -> bool:
-    return t.shape[-1] == 1 or t.stride(-1) == 1
-
-
-def check_head_rows(name: str, what: str, t: torch.Tensor) -> None:
-    if t.dim() != 3 or t.dtype not in TYPES or not dense_last(t):
-        raise ValueError(f"{name}: {what} must be float32, bfloat16 or float16 [tokens, heads, head_dim] with dense rows")
-
-
-def check_cache(name: str, keys: torch.Tensor, values: torch.Tensor | None) -> None:
-    for what, t in (("key_cache", keys), ("value_cache", values)):
-        if t is None:
-            continue
-        if t.dim() != 4 or t.dtype not in CACHE_TYPES or not dense_last(t):
-            raise ValueError(f"{name}: {what} must be bfloat16 or float16 [pages, page_size, heads, head_dim] with dense rows")
-    if values is not None and (values.shape != keys.shape or values.dtype != keys.dtype):
-        raise ValueError(f"{name}: key_cache and value_cache must have one shape and type")
-    if min(keys.shape) == 0:
-        raise ValueError(f"{name}: the cache is empty")
-
-
-def check_table(name: str, table: torch.Tensor, lens: torch.Tensor) -> None:
-    if table.dim() != 2 or table.dtype != torch.int32 or not dense_last(table) or table.shape[1] == 0:
-        raise ValueError(f"{name}: block_table must be int32 [sequences, pages of the longest] with dense rows")
-    check_index(name, "context_lens", lens, torch.int32, table.shape[0])
+    return t.stride(-1) == 1 or t.shape[-1] == 1
 
 
 def check_index(name: str, what: str, t: torch.Tensor, dtype: torch.dtype, count: int) -> None:
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != count or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != (count,) or not t.is_contiguous():
         raise ValueError(f"{name}: {what} must be contiguous {str(dtype).removeprefix('torch.')} [{count}]")
 
 
-def cache_struct(keys: torch.Tensor, values: torch.Tensor | None, table: torch.Tensor | None = None,
-                 lens: torch.Tensor | None = None) -> Any:
-    """``qxt_paged_cache`` by reference (the operators that take no values or table leave those out)."""
-    pages, page_size, heads, head_dim = keys.shape
-    value_strides = (0, 0, 0) if values is None else byte_strides(values, 3)
-    sequences, width = (0, 0) if table is None else table.shape
-    return ctypes.byref(_lib.PagedCache(
-        ptr(keys), *byte_strides(keys, 3), ptr(values), *value_strides, ptr(table),
-        0 if table is None or sequences == 1 else table.stride(0) * 4, ptr(lens), pages, page_size, heads, head_dim,
-        TYPES[keys.dtype], width, sequences))
-
-
-def check_per_slot(name: str, what: str, t: torch.Tensor, dtype: torch.dtype, keys: torch.Tensor, table: torch.Tensor) -> None:
-    shape = (table.shape[0], keys.shape[2], table.shape[1] * keys.shape[1])
-    if t.dtype != dtype or tuple(t.shape) != shape or not dense_last(t):
+def per_slot(name: str, what: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple[int, int, int]) -> tuple[int, int]:
+    """Byte strides (sequence, head) of 4-byte values [sequences, heads, slots]."""
+    if t.dtype is not dtype or t.shape != shape:
         raise ValueError(f"{name}: {what} must be {str(dtype).removeprefix('torch.')} [sequences, heads, slots] = {list(shape)} "
                          "with dense rows")
+    sequence, head, slot = t.stride()
+    if slot != 1 and shape[2] != 1:
+        raise ValueError(f"{name}: {what} must be {str(dtype).removeprefix('torch.')} [sequences, heads, slots] = {list(shape)} "
+                         "with dense rows")
+    return 0 if shape[0] == 1 else 4 * sequence, 0 if shape[1] == 1 else 4 * head
 
 
 def check_size(name: str, what: str, value: int) -> int:
-    if not 0 <= int(value) <= UINT32_MAX:
+    if not 0 <= value <= UINT32_MAX:
         raise ValueError(f"{name}: {what} must be non-negative (and below 2^32)")
     return int(value)

@@ -25,59 +25,57 @@ import torch
 
 from qpu_xla_amd import _lib
 from qpu_xla_amd._paged import (
-    TYPES,
-    byte_strides,
-    cache_struct,
-    check_cache,
-    check_head_rows,
     check_index,
-    check_per_slot,
     check_size,
-    check_table,
-    dense_last,
     empty_for,
+    head_rows,
+    paged_cache,
+    per_slot,
+    require_one_gpu,
 )
-from qpu_xla_amd._tensors import ptr, require_gpu, stream_handle
+from qpu_xla_amd._tensors import ptr, stream_handle
 from qpu_xla_amd.errors import KernelError
 from qpu_xla_amd.kernel import Kernel
 
 
 def _check(name: str, query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor | None,
-           block_table: torch.Tensor, context_lens: torch.Tensor, query_starts: torch.Tensor | None) -> None:
-    check_head_rows(name, "query", query)
-    check_cache(name, key_cache, value_cache)
-    check_table(name, block_table, context_lens)
-    heads, head_dim = key_cache.shape[2:]
-    if query.dtype != key_cache.dtype or query.shape[2] != head_dim:
+           block_table: torch.Tensor, context_lens: torch.Tensor, query_starts: torch.Tensor | None) -> tuple:
+    """(query shape, its byte strides, key heads, sequences, slots a sequence, packed cache)."""
+    shape, code, token_stride, head_stride = head_rows(name, "query", query)
+    cache_shape, cache_code, sequences, width, cache = paged_cache(name, key_cache, value_cache, block_table, context_lens)
+    _, page_size, heads, head_dim = cache_shape
+    if code != cache_code or shape[2] != head_dim:
         raise ValueError(f"{name}: query must have the cache's type and head size")
-    if query.shape[1] == 0 or query.shape[1] % heads:
+    if shape[1] == 0 or shape[1] % heads:
         raise ValueError(f"{name}: query heads must be a multiple of the cache's heads")
     if head_dim % 8 or head_dim > 256:
         raise ValueError(f"{name}: head size must be a multiple of 8 up to 256")
-    sequences = block_table.shape[0]
     if query_starts is not None:
         check_index(name, "query_starts", query_starts, torch.int32, sequences + 1)
-    elif query.shape[0] != sequences:
+    elif shape[0] != sequences:
         raise ValueError(f"{name}: without query_starts every sequence has one token")
+    return shape, (token_stride, head_stride), heads, sequences, width * page_size, cache
 
 
-def _check_lse(name: str, query: torch.Tensor, lse: torch.Tensor) -> None:
-    if lse.dtype != torch.float32 or tuple(lse.shape) != tuple(query.shape[:2]) or not dense_last(lse):
+def _lse_stride(name: str, shape: torch.Size, lse: torch.Tensor) -> int:
+    if lse.dtype is not torch.float32 or lse.shape != shape[:2] or not (lse.stride(1) == 1 or shape[1] == 1):
         raise ValueError(f"{name}: lse must be float32 [tokens, heads] with dense rows")
+    return 0 if shape[0] == 1 else 4 * lse.stride(0)
 
 
-def _sizes(name: str, query: torch.Tensor, key_cache: torch.Tensor, block_table: torch.Tensor, scale: float | None,
-           window: int, max_query: int | None, max_context: int | None) -> tuple[float, int, int, int]:
-    scale = 1.0 / math.sqrt(query.shape[2]) if scale is None else float(scale)
+def _sizes(name: str, shape: torch.Size, slots: int, query_starts: torch.Tensor | None, scale: float | None, window: int,
+           max_query: int | None, max_context: int | None) -> tuple[float, int, int, int]:
+    scale = 1.0 / math.sqrt(shape[2]) if scale is None else float(scale)
     if not 0.0 < scale < 3e38:
         raise ValueError(f"{name}: scale must be positive and finite")
-    max_query = query.shape[0] if max_query is None else check_size(name, "max_query", max_query)
-    slots = block_table.shape[1] * key_cache.shape[1]
+    if query_starts is None:
+        max_query = 1
+    else:
+        max_query = shape[0] if max_query is None else check_size(name, "max_query", max_query)
     max_context = slots if max_context is None else min(slots, check_size(name, "max_context", max_context))
-    window = int(window)
     if window < 0:
         raise ValueError(f"{name}: window must not be negative")
-    return scale, min(window, 2**31 - 1), max_query, max_context
+    return scale, min(int(window), 2**31 - 1), max_query, max_context
 
 
 def paged_attention(
@@ -99,30 +97,26 @@ def paged_attention(
 ) -> torch.Tensor:
     """Attention outputs [T, Hq, D] (the query's type, or ``out``'s); ``lse`` float32 [T, Hq] receives the log-sums."""
     name = "paged_attention"
-    _check(name, query, key_cache, value_cache, block_table, context_lens, query_starts)
-    scale, window, max_query, max_context = _sizes(name, query, key_cache, block_table, scale, window, max_query, max_context)
-    tokens, query_heads, head_dim = query.shape
+    shape, strides, heads, sequences, slots, cache = _check(name, query, key_cache, value_cache, block_table, context_lens,
+                                                            query_starts)
+    scale, window, max_query, max_context = _sizes(name, shape, slots, query_starts, scale, window, max_query, max_context)
+    tokens, query_heads, head_dim = shape
     if out is None:
-        out = empty_for(stream, tuple(query.shape), query.dtype, query.device)
-    check_head_rows(name, "out", out)
-    if out.shape != query.shape:
+        out = empty_for(stream, shape, query.dtype, query.device)
+    out_shape, out_code, *out_strides = head_rows(name, "out", out)
+    if out_shape != shape:
         raise ValueError(f"{name}: out must have the query's shape")
-    if lse is not None:
-        _check_lse(name, query, lse)
-    require_gpu(name, query, key_cache, value_cache, block_table, context_lens, query_starts, out, lse)
-    if tokens == 0 or block_table.shape[0] == 0:
+    lse_stride = 0 if lse is None else _lse_stride(name, shape, lse)
+    require_one_gpu(name, query, key_cache, value_cache, block_table, context_lens, query_starts, out, lse)
+    if tokens == 0 or sequences == 0:
         return out
-    if query_starts is None:
-        max_query = 1
-    size = (_lib._lib or _lib.load()).qxt_paged_attention_workspace(
-        query_heads, key_cache.shape[2], head_dim, block_table.shape[0], tokens, max_query, max_context)
+    size = (_lib._lib or _lib.load()).qxt_paged_attention_workspace(query_heads, heads, head_dim, sequences, tokens,
+                                                                    max_query, max_context)
     workspace = empty_for(stream, (size,), torch.uint8, query.device) if size else None
     _lib.call(
-        "qxt_paged_attention", ptr(query), *byte_strides(query, 2),
-        cache_struct(key_cache, value_cache, block_table, context_lens), ptr(query_starts), ptr(out),
-        *byte_strides(out, 2), TYPES[out.dtype], ptr(lse), 0 if lse is None else byte_strides(lse, 1)[0], tokens,
-        query_heads, scale, 1 if causal else 0, window, max_query, max_context, ptr(workspace), size,
-        stream_handle(stream),
+        "qxt_paged_attention", query.data_ptr(), *strides, cache, ptr(query_starts), out.data_ptr(), *out_strides, out_code,
+        ptr(lse), lse_stride, tokens, query_heads, scale, 1 if causal else 0, window, max_query, max_context,
+        ptr(workspace), size, stream_handle(stream),
     )
     return out
 
@@ -150,30 +144,26 @@ def paged_attention_scores(
     add up to 1.  ``out`` may be ``scores`` itself.
     """
     name = "paged_attention_scores"
-    _check(name, query, key_cache, None, block_table, context_lens, query_starts)
-    scale, window, max_query, max_context = _sizes(name, query, key_cache, block_table, scale, window, max_query, max_context)
-    tokens, query_heads, _ = query.shape
-    _check_lse(name, query, lse)
-    if scores is not None:
-        check_per_slot(name, "scores", scores, torch.float32, key_cache, block_table)
-    sequences, heads, slots = block_table.shape[0], key_cache.shape[2], block_table.shape[1] * key_cache.shape[1]
+    shape, strides, heads, sequences, slots, cache = _check(name, query, key_cache, None, block_table, context_lens,
+                                                            query_starts)
+    scale, window, max_query, max_context = _sizes(name, shape, slots, query_starts, scale, window, max_query, max_context)
+    tokens, query_heads, _ = shape
+    lse_stride = _lse_stride(name, shape, lse)
+    scores_shape = (sequences, heads, slots)
+    before = (0, 0) if scores is None else per_slot(name, "scores", scores, torch.float32, scores_shape)
     if out is None:
-        out = empty_for(stream, (sequences, heads, slots), torch.float32, query.device)
-    check_per_slot(name, "out", out, torch.float32, key_cache, block_table)
-    require_gpu(name, query, key_cache, block_table, context_lens, lse, query_starts, scores, out)
+        out = empty_for(stream, scores_shape, torch.float32, query.device)
+    after = per_slot(name, "out", out, torch.float32, scores_shape)
+    require_one_gpu(name, query, key_cache, block_table, context_lens, lse, query_starts, scores, out)
     if sequences == 0:
         return out
-    if query_starts is None:
-        max_query = 1
-    size = (_lib._lib or _lib.load()).qxt_paged_attention_scores_workspace(
-        query_heads, heads, sequences, tokens, slots, max_query, max_context)
+    size = (_lib._lib or _lib.load()).qxt_paged_attention_scores_workspace(query_heads, heads, sequences, tokens, slots,
+                                                                           max_query, max_context)
     workspace = empty_for(stream, (size,), torch.uint8, query.device) if size else None
-    before = (0, 0) if scores is None else byte_strides(scores, 2)
     _lib.call(
-        "qxt_paged_attention_scores", ptr(query), *byte_strides(query, 2),
-        cache_struct(key_cache, None, block_table, context_lens), ptr(query_starts), ptr(lse), byte_strides(lse, 1)[0],
-        ptr(scores), *before, ptr(out), *byte_strides(out, 2), tokens, query_heads, scale, 1 if causal else 0, window,
-        max_query, max_context, ptr(workspace), size, stream_handle(stream),
+        "qxt_paged_attention_scores", query.data_ptr(), *strides, cache, ptr(query_starts), lse.data_ptr(), lse_stride,
+        ptr(scores), *before, out.data_ptr(), *after, tokens, query_heads, scale, 1 if causal else 0, window, max_query,
+        max_context, ptr(workspace), size, stream_handle(stream),
     )
     return out
 

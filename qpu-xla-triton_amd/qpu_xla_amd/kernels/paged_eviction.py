@@ -20,17 +20,8 @@ from typing import Any
 import torch
 
 from qpu_xla_amd import _lib
-from qpu_xla_amd._paged import (
-    byte_strides,
-    cache_struct,
-    check_cache,
-    check_index,
-    check_per_slot,
-    check_size,
-    check_table,
-    empty_for,
-)
-from qpu_xla_amd._tensors import ptr, require_gpu, stream_handle
+from qpu_xla_amd._paged import check_index, check_size, empty_for, paged_cache, per_slot, require_one_gpu
+from qpu_xla_amd._tensors import stream_handle
 from qpu_xla_amd.errors import KernelError
 from qpu_xla_amd.kernel import Kernel
 
@@ -57,36 +48,38 @@ def paged_cache_evict(
     ``max_context`` is the host's bound of the lengths and sizes the launch.
     """
     name = "paged_cache_evict"
-    check_cache(name, key_cache, value_cache)
-    check_table(name, block_table, context_lens)
-    if key_cache.shape[3] % 8 or key_cache.shape[3] > 256:
+    cache_shape, _, sequences, width, cache = paged_cache(name, key_cache, value_cache, block_table, context_lens)
+    _, page_size, heads, head_dim = cache_shape
+    if head_dim % 8 or head_dim > 256:
         raise ValueError(f"{name}: head size must be a multiple of 8 up to 256")
     budget, recent = int(budget), int(recent)
     if not 0 < budget < 2**30 or not 0 <= recent <= budget:
         raise ValueError(f"{name}: budget must be positive (below 2^30) and recent between 0 and the budget")
-    sequences, heads, slots = block_table.shape[0], key_cache.shape[2], block_table.shape[1] * key_cache.shape[1]
+    slots = width * page_size
     max_context = slots if max_context is None else min(slots, check_size(name, "max_context", max_context))
     shape = (sequences, heads, slots)
+    device = key_cache.device
     if scores_out is None:
-        scores_out = empty_for(stream, shape, torch.float32, scores.device)
+        scores_out = empty_for(stream, shape, torch.float32, device)
     if positions_out is None:
-        positions_out = empty_for(stream, shape, torch.int32, positions.device)
+        positions_out = empty_for(stream, shape, torch.int32, device)
     if lens_out is None:
-        lens_out = empty_for(stream, (sequences,), torch.int32, context_lens.device)
-    for what, t, dtype in (("scores", scores, torch.float32), ("scores_out", scores_out, torch.float32),
-                           ("positions", positions, torch.int32), ("positions_out", positions_out, torch.int32)):
-        check_per_slot(name, what, t, dtype, key_cache, block_table)
-    check_index(name, "lens_out", lens_out, torch.int32, sequences)
-    require_gpu(name, key_cache, value_cache, block_table, context_lens, scores, positions, scores_out, positions_out, lens_out)
+        lens_out = empty_for(stream, (sequences,), torch.int32, device)
+    else:
+        check_index(name, "lens_out", lens_out, torch.int32, sequences)
+    strides = [per_slot(name, what, t, dtype, shape)
+               for what, t, dtype in (("scores", scores, torch.float32), ("scores_out", scores_out, torch.float32),
+                                      ("positions", positions, torch.int32), ("positions_out", positions_out, torch.int32))]
+    require_one_gpu(name, key_cache, value_cache, block_table, context_lens, scores, positions, scores_out, positions_out,
+                    lens_out)
     if sequences == 0:
         return lens_out, scores_out, positions_out
     size = (_lib._lib or _lib.load()).qxt_paged_cache_evict_workspace(heads, sequences, slots, budget)
-    workspace = empty_for(stream, (size,), torch.uint8, key_cache.device)
+    workspace = empty_for(stream, (size,), torch.uint8, device)
     _lib.call(
-        "qxt_paged_cache_evict", cache_struct(key_cache, value_cache, block_table, context_lens),
-        ptr(scores), *byte_strides(scores, 2), ptr(scores_out), *byte_strides(scores_out, 2),
-        ptr(positions), *byte_strides(positions, 2), ptr(positions_out), *byte_strides(positions_out, 2), ptr(lens_out),
-        budget, recent, max_context, ptr(workspace), size, stream_handle(stream),
+        "qxt_paged_cache_evict", cache, scores.data_ptr(), *strides[0], scores_out.data_ptr(), *strides[1],
+        positions.data_ptr(), *strides[2], positions_out.data_ptr(), *strides[3], lens_out.data_ptr(), budget, recent,
+        max_context, workspace.data_ptr(), size, stream_handle(stream),
     )
     return lens_out, scores_out, positions_out
 

@@ -22,29 +22,33 @@ from typing import Any
 import torch
 
 from qpu_xla_amd import _lib
-from qpu_xla_amd._paged import TYPES, byte_strides, cache_struct, check_cache, check_head_rows, check_index, empty_for
-from qpu_xla_amd._tensors import ptr, require_gpu, stream_handle
+from qpu_xla_amd._paged import check_index, empty_for, head_rows, paged_cache, require_one_gpu
+from qpu_xla_amd._tensors import ptr, stream_handle
 from qpu_xla_amd.errors import KernelError
 from qpu_xla_amd.kernel import Kernel
 
 
-def _check(name: str, query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
-           positions: torch.Tensor, weights: tuple[torch.Tensor | None, torch.Tensor | None]) -> None:
-    check_head_rows(name, "query", query)
-    check_head_rows(name, "key", key)
-    if query.shape[0] != key.shape[0] or query.shape[2] != key.shape[2] or query.dtype != key.dtype:
-        raise ValueError(f"{name}: query and key must agree in tokens, head size and type")
-    head_dim = query.shape[2]
-    for table in (cos, sin):
-        if table.dtype != torch.float32 or table.dim() != 2 or not table.is_contiguous():
-            raise ValueError(f"{name}: cos and sin must be contiguous float32 [positions, rotary / 2]")
-    if cos.shape != sin.shape or 2 * cos.shape[1] > head_dim:
-        raise ValueError(f"{name}: cos and sin must have one shape, of at most half the head size")
-    check_index(name, "positions", positions, torch.int32, query.shape[0])
+def _check_tables(name: str, tokens: int, head_dim: int, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
+                  *weights: torch.Tensor | None) -> tuple[int, int]:
+    """(positions, half the rotary size) of the tables."""
+    shape = cos.shape
+    if (len(shape) != 2 or sin.shape != shape or cos.dtype is not torch.float32 or sin.dtype is not torch.float32
+            or not cos.is_contiguous() or not sin.is_contiguous()):
+        raise ValueError(f"{name}: cos and sin must be contiguous float32 [positions, rotary / 2] of one shape")
+    if 2 * shape[1] > head_dim:
+        raise ValueError(f"{name}: cos and sin turn more than the head size")
+    check_index(name, "positions", positions, torch.int32, tokens)
     for weight in weights:
-        if weight is not None and (weight.dtype != torch.float32 or tuple(weight.shape) != (head_dim,)
-                                   or not weight.is_contiguous()):
-            raise ValueError(f"{name}: weights must be contiguous float32 [{head_dim}]")
+        if weight is not None:
+            check_index(name, "weights", weight, torch.float32, head_dim)
+    return shape[0], shape[1]
+
+
+def _check_rows(name: str, query: torch.Tensor, key: torch.Tensor) -> tuple[tuple, tuple]:
+    q, k = head_rows(name, "query", query), head_rows(name, "key", key)
+    if q[0][0] != k[0][0] or q[0][2] != k[0][2] or q[1] != k[1]:
+        raise ValueError(f"{name}: query and key must agree in tokens, head size and type")
+    return q, k
 
 
 def qk_norm_rope(
@@ -64,23 +68,24 @@ def qk_norm_rope(
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """Normalised and rotated (query, key), in the inputs' type unless outputs are given (which may be the inputs)."""
     name = "qk_norm_rope"
-    _check(name, query, key, cos, sin, positions, (query_weight, key_weight))
-    tokens, query_heads, head_dim = query.shape
+    (shape, code, *query_strides), (key_shape, _, *key_strides) = _check_rows(name, query, key)
+    tokens, query_heads, head_dim = shape
+    rows, half = _check_tables(name, tokens, head_dim, cos, sin, positions, query_weight, key_weight)
     if query_out is None:
-        query_out = empty_for(stream, tuple(query.shape), query.dtype if key_out is None else key_out.dtype, query.device)
+        query_out = empty_for(stream, shape, query.dtype if key_out is None else key_out.dtype, query.device)
     if key_out is None:
-        key_out = empty_for(stream, tuple(key.shape), query_out.dtype, key.device)
-    check_head_rows(name, "query_out", query_out)
-    check_head_rows(name, "key_out", key_out)
-    if query_out.shape != query.shape or key_out.shape != key.shape or query_out.dtype != key_out.dtype:
+        key_out = empty_for(stream, key_shape, query_out.dtype, query.device)
+    query_out_shape, out_code, *query_out_strides = head_rows(name, "query_out", query_out)
+    key_out_shape, key_code, *key_out_strides = head_rows(name, "key_out", key_out)
+    if query_out_shape != shape or key_out_shape != key_shape or out_code != key_code:
         raise ValueError(f"{name}: outputs must have the inputs' shapes and one type")
-    require_gpu(name, query, key, cos, sin, positions, query_weight, key_weight, query_out, key_out)
+    require_one_gpu(name, query, key, cos, sin, positions, query_weight, key_weight, query_out, key_out)
     _lib.call(
-        "qxt_qk_norm_rope", ptr(query), *byte_strides(query, 2), ptr(key), *byte_strides(key, 2), ptr(query_weight),
-        ptr(key_weight), epsilon, ptr(cos), ptr(sin), cos.shape[1] * 4, cos.shape[0], ptr(positions), ptr(query_out),
-        *byte_strides(query_out, 2), ptr(key_out), *byte_strides(key_out, 2), tokens, query_heads, key.shape[1],
-        head_dim, 2 * cos.shape[1], TYPES[query.dtype], TYPES[query_out.dtype],
-        _lib.ROPE_INTERLEAVED if interleaved else 0, stream_handle(stream),
+        "qxt_qk_norm_rope", query.data_ptr(), *query_strides, key.data_ptr(), *key_strides, ptr(query_weight),
+        ptr(key_weight), epsilon, cos.data_ptr(), sin.data_ptr(), half * 4, rows, positions.data_ptr(),
+        query_out.data_ptr(), *query_out_strides, key_out.data_ptr(), *key_out_strides, tokens, query_heads,
+        key_shape[1], head_dim, 2 * half, code, out_code, _lib.ROPE_INTERLEAVED if interleaved else 0,
+        stream_handle(stream),
     )
     return query_out, key_out
 
@@ -105,27 +110,28 @@ def qk_norm_rope_cache(
 ) -> torch.Tensor:
     """Normalise and rotate, store keys and values at ``slots`` (int64 [T]) of the cache; the queries in its type."""
     name = "qk_norm_rope_cache"
-    _check(name, query, key, cos, sin, positions, (query_weight, key_weight))
-    check_head_rows(name, "value", value)
-    if value.shape != key.shape or value.dtype != key.dtype:
+    (shape, code, *query_strides), (key_shape, _, *key_strides) = _check_rows(name, query, key)
+    value_shape, value_code, *value_strides = head_rows(name, "value", value)
+    if value_shape != key_shape or value_code != code:
         raise ValueError(f"{name}: key and value must have one shape and type")
-    check_cache(name, key_cache, value_cache)
-    if tuple(key_cache.shape[2:]) != tuple(key.shape[1:]):
+    tokens, query_heads, head_dim = shape
+    rows, half = _check_tables(name, tokens, head_dim, cos, sin, positions, query_weight, key_weight)
+    cache_shape, cache_code, _, _, cache = paged_cache(name, key_cache, value_cache)
+    if cache_shape[2:] != key_shape[1:]:
         raise ValueError(f"{name}: the cache must hold the keys' heads and head size")
-    check_index(name, "slots", slots, torch.int64, query.shape[0])
+    check_index(name, "slots", slots, torch.int64, tokens)
     if query_out is None:
-        query_out = empty_for(stream, tuple(query.shape), key_cache.dtype, query.device)
-    check_head_rows(name, "query_out", query_out)
-    if query_out.shape != query.shape or query_out.dtype != key_cache.dtype:
+        query_out = empty_for(stream, shape, key_cache.dtype, query.device)
+    out_shape, out_code, *out_strides = head_rows(name, "query_out", query_out)
+    if out_shape != shape or out_code != cache_code:
         raise ValueError(f"{name}: query_out must have the query's shape and the cache's type")
-    require_gpu(name, query, key, value, cos, sin, positions, slots, key_cache, value_cache, query_weight, key_weight,
-                query_out)
+    require_one_gpu(name, query, key, value, cos, sin, positions, slots, key_cache, value_cache, query_weight, key_weight,
+                    query_out)
     _lib.call(
-        "qxt_qk_norm_rope_cache", ptr(query), *byte_strides(query, 2), ptr(key), *byte_strides(key, 2), ptr(value),
-        *byte_strides(value, 2), ptr(query_weight), ptr(key_weight), epsilon, ptr(cos), ptr(sin), cos.shape[1] * 4,
-        cos.shape[0], ptr(positions), ptr(slots), ptr(query_out), *byte_strides(query_out, 2),
-        cache_struct(key_cache, value_cache), query.shape[0], query.shape[1], 2 * cos.shape[1], TYPES[query.dtype],
-        _lib.ROPE_INTERLEAVED if interleaved else 0, stream_handle(stream),
+        "qxt_qk_norm_rope_cache", query.data_ptr(), *query_strides, key.data_ptr(), *key_strides, value.data_ptr(),
+        *value_strides, ptr(query_weight), ptr(key_weight), epsilon, cos.data_ptr(), sin.data_ptr(), half * 4, rows,
+        positions.data_ptr(), slots.data_ptr(), query_out.data_ptr(), *out_strides, cache, tokens, query_heads, 2 * half,
+        code, _lib.ROPE_INTERLEAVED if interleaved else 0, stream_handle(stream),
     )
     return query_out
 
