@@ -41,7 +41,9 @@ inline FastDiv fast_div(uint32_t d) {
     f.shift = s - 1;
     return f;
 }
-__host__ __device__ __forceinline__ uint32_t fast_quotient(uint32_t n, const FastDiv &f) {
+// (F: FastDiv, in any address space.)
+template <typename F>
+__host__ __device__ __forceinline__ uint32_t fast_quotient(uint32_t n, const F &f) {
     if (f.divisor <= 1) return n;
     return static_cast<uint32_t>((static_cast<uint64_t>(n) * f.magic) >> 32) >> f.shift;
 }

@@ -30,13 +30,32 @@ struct PagedArgs {
     float2 *part_sum;  // [splits, tokens, heads]: (maximum in log2 units, sum)
 };
 
+// A kernel's arguments in the kernarg segment, where they are the first.  The
+// kernels read them there instead of from the parameter: what is only needed
+// before or after the main loop is then loaded there (`late` hides that it is
+// the same memory) and holds no scalar registers over it.  With all arguments
+// live the loop needs more than there are, and the compiler gives up ordering it.
+template <typename A>
+using Kernarg = const __attribute__((address_space(4))) A;
+template <typename A>
+__device__ __forceinline__ Kernarg<A> *kernargs() {
+    return (Kernarg<A> *)__builtin_amdgcn_kernarg_segment_ptr();
+}
+template <typename A>
+__device__ __forceinline__ A *late(A *args) {
+    asm volatile("" : "+s"(args));
+    return args;
+}
+
+// (A: PagedArgs, in any address space.)
 // The tokens and cache length of one sequence; lengths from the device are
 // clamped to what the tensors hold, so no index leaves them.
 struct Sequence {
     int32_t start, tokens, length;
 };
 
-__device__ __forceinline__ Sequence sequence_of(const PagedArgs &a, uint32_t b) {
+template <typename A>
+__device__ __forceinline__ Sequence sequence_of(const A &a, uint32_t b) {
     Sequence s;
     const int32_t most = static_cast<int32_t>(a.tokens);
     int32_t first = b, last = b + 1;
@@ -56,7 +75,8 @@ __device__ __forceinline__ Sequence sequence_of(const PagedArgs &a, uint32_t b) 
 struct Range {
     int32_t low, high;
 };
-__device__ __forceinline__ Range seen_by(const PagedArgs &a, const Sequence &s, int32_t token) {
+template <typename A>
+__device__ __forceinline__ Range seen_by(const A &a, const Sequence &s, int32_t token) {
     const int32_t at = s.length - s.tokens + token;  // its own slot
     Range r;
     r.high = a.causal ? min(s.length, max(at + 1, 0)) : s.length;
@@ -81,47 +101,119 @@ struct Tile {
 
 // Source of rows that are not in the cache: slots past a sequence's end, pages
 // that its table does not name, and the columns from head_dim up to DP.
-__device__ __constant__ const uint4 kZeroRow = {0, 0, 0, 0};
+__device__ __constant__ const uint4 kZeroRow[32] = {};
 
-// One wave's share of staging: rows [0, ROWS) of its part of a tile, one row
-// per lane for the address work (lanes past ROWS repeat).
+// 64 lanes' 16 bytes from `src` (each lane its own) to LDS at `to` + 16 * lane.
+// Inline assembly because the compiler, which cannot tell the buffers of a
+// ring apart, waits for every such load in flight before it reads any of LDS;
+// here the waits are the kernels' own (landed<N>).  There is no register output.
+// (The compiler warns that it may not preserve m0; it has no other use for it in these kernels.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void dma16(const char *src, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(src) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// Wait until all but the wave's N youngest loads are done.
+template <int N>
+__device__ __forceinline__ void landed() {
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+// All of the wave's LDS reads have returned.
+__device__ __forceinline__ void reads_done() {
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+// A workgroup barrier that, unlike __syncthreads, waits for no load in flight.
+__device__ __forceinline__ void meet() {
+    asm volatile("" : : : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" : : : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+__device__ __forceinline__ uint32_t lds_offset(const char *p) {
+    return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(
+        reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char *)p)));
+}
+
+// One wave's share of staging: ROWS consecutive slots of a tile, one row per
+// lane for the address work (lanes past ROWS repeat).  Each lane holds the page
+// id of one of 64 consecutive table entries, refetched when the slots leave
+// them, so that a tile's addresses wait for no load.
 template <int DP, int ROWS>
 struct Stager {
+    using TL = Tile<DP>;
+    static constexpr int kLoads = ROWS / TL::kRowsPerLoad;  // of keys, and as many of values
     const int32_t *table;
-    int32_t page_id;  // of this lane's row of the next tile to stage
+    const char *keys, *values;  // of this head
+    int32_t held, page0;        // page id of entry page0 + lane
 
-    // Fetch the page of slot `slot` (one tile ahead of its use).
-    __device__ __forceinline__ void look_up(const PagedArgs &a, int32_t slot, int32_t high) {
-        page_id = -1;
-        if (slot < high) page_id = table[fast_quotient(static_cast<uint32_t>(slot), a.page)];
+    template <typename A>
+    __device__ __forceinline__ void start(const A &a, uint32_t b, uint32_t head) {
+        table = a.table + b * a.table_stride;
+        keys = a.keys.data + head * a.keys.head_stride;
+        values = a.values.data + head * a.values.head_stride;
+        held = -1;
+        page0 = -64;
     }
 
-    // Byte offset of this lane's row in a cache, or -1.
-    __device__ __forceinline__ int64_t offset_in(const PagedArgs &a, const CacheView &c, int32_t slot) const {
-        const uint32_t page = fast_quotient(static_cast<uint32_t>(slot), a.page);
-        const uint32_t in_page = static_cast<uint32_t>(slot) - page * a.page.divisor;
-        return static_cast<uint32_t>(page_id) < a.pages
-                   ? static_cast<int64_t>(page_id) * c.page_stride + static_cast<int64_t>(in_page) * c.slot_stride
-                   : -1;
-    }
-
-    // DMA this wave's ROWS rows into LDS at `to` (wave-uniform), KEYS choosing the chunk exchange.
-    template <bool KEYS>
-    __device__ __forceinline__ void load(const char *base, int64_t offset, char *to, int lane, int row0,
-                                         uint32_t head_dim) const {
-        using TL = Tile<DP>;
-        const int lo = static_cast<int>(offset), hi = static_cast<int>(offset >> 32);
-#pragma unroll
-        for (int i = 0; i < ROWS / TL::kRowsPerLoad; ++i) {
-            const int r = i * TL::kRowsPerLoad + lane / TL::kChunks;
-            const int64_t off = (static_cast<int64_t>(__shfl(hi, r, 64)) << 32) | static_cast<uint32_t>(__shfl(lo, r, 64));
-            const int turn = KEYS ? TL::key_turn(row0 + r) : TL::value_turn(row0 + r);
-            const int chunk = (lane % TL::kChunks) ^ turn;
-            const char *src = base + off + chunk * 16;
-            if (off < 0 || chunk * 8 >= static_cast<int>(head_dim)) src = reinterpret_cast<const char *>(&kZeroRow);
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
-                                             (__attribute__((address_space(3))) void *)(to + i * 1024), 16, 0, 0);
+    // Page entry and place in the page of this lane's row (slot slot0 + lane % ROWS), or entry -1 from `high` on.
+    struct Row {
+        int32_t id;
+        uint32_t in_page;
+    };
+    template <typename A>
+    __device__ __forceinline__ Row locate(const A &a, int32_t slot0, int32_t high) {
+        const int lane = threadIdx.x % 64;
+        if (slot0 < high) {
+            const int32_t first = fast_quotient(slot0, a.page), last = fast_quotient(min(slot0 + ROWS, high) - 1, a.page);
+            if (first < page0 || last >= page0 + 64) {
+                page0 = first;
+                const int32_t entry = first + lane, end = fast_quotient(high - 1, a.page);
+                held = table[min(entry, end)];
+            }
         }
+        const int32_t slot = slot0 + lane % ROWS;
+        const uint32_t page = fast_quotient(static_cast<uint32_t>(slot), a.page);
+        Row r;
+        r.in_page = static_cast<uint32_t>(slot) - page * a.page.divisor;
+        const int32_t id = __shfl(held, static_cast<int>(page) - page0, 64);
+        r.id = slot < high && static_cast<uint32_t>(id) < a.pages ? id : -1;
+        return r;
+    }
+
+    template <typename V>
+    __device__ __forceinline__ static uint64_t address(const char *base, const V &c, const Row &r) {
+        const char *at = base + static_cast<int64_t>(r.id) * c.page_stride + static_cast<int64_t>(r.in_page) * c.slot_stride;
+        return reinterpret_cast<uint64_t>(r.id < 0 ? reinterpret_cast<const char *>(kZeroRow) : at);
+    }
+
+    // DMA this wave's rows, row0 .. of the tile, to LDS offset `to`.
+    template <bool KEYS>
+    __device__ __forceinline__ static void load(uint64_t row, uint32_t to, int row0, uint32_t head_dim) {
+        const int lane = threadIdx.x % 64;
+        const int lo = static_cast<int>(row), hi = static_cast<int>(row >> 32);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int r = i * TL::kRowsPerLoad + lane / TL::kChunks;
+            const uint64_t at = (static_cast<uint64_t>(static_cast<uint32_t>(__shfl(hi, r, 64))) << 32) |
+                                static_cast<uint32_t>(__shfl(lo, r, 64));
+            const int chunk = (lane % TL::kChunks) ^ (KEYS ? TL::key_turn(row0 + r) : TL::value_turn(row0 + r));
+            const uint64_t src = chunk * 8 < static_cast<int>(head_dim) ? at + chunk * 16 : reinterpret_cast<uint64_t>(kZeroRow);
+            dma16(reinterpret_cast<const char *>(src), to + i * 1024);
+        }
+    }
+
+    // Both tiles' rows; keys at `to`, values at `to_values`.
+    template <typename A>
+    __device__ __forceinline__ void stage(const A &a, int32_t slot0, int32_t high, uint32_t to, uint32_t to_values,
+                                          int row0) {
+        const Row r = locate(a, slot0, high);
+        load<true>(address(keys, a.keys, r), to, row0, a.head_dim);
+        load<false>(address(values, a.values, r), to_values, row0, a.head_dim);
     }
 };
 

@@ -55,8 +55,8 @@ __device__ __forceinline__ float lse_of(float top2, float sum) {
 // sees enter.  For the rare waves whose rows see different slots of a step that
 // holds infinite or NaN values.  Lane l gets elements l + 64 k; the slots are
 // [from, to) in parts of `part` every `step`.
-template <typename T, int DP>
-__device__ __forceinline__ float2 attend_alone(const PagedArgs &a, const T *query, const Range &mine, int32_t from,
+template <typename T, int DP, typename A>
+__device__ __forceinline__ float2 attend_alone(const A &a, const T *query, const Range &mine, int32_t from,
                                                int32_t to, int32_t step, int32_t part, const int32_t *table,
                                                const char *keys, const char *values, float (&out)[DP / 64]) {
     const int lane = threadIdx.x % 64;
@@ -114,6 +114,284 @@ __device__ __forceinline__ void put_as(uint32_t type, char *row, int d, float x)
         reinterpret_cast<float *>(row)[d] = x;
 }
 
+// What one wave does with KB x 32 staged keys and its 32 rows.
+template <typename T, int DP, int KB>
+struct Core {
+    using TL = Tile<DP>;
+    using M = Mfma<T>;
+    typedef typename M::frag frag;
+    static constexpr int kCols = DP / 32, kSteps = DP / 16;
+
+    int32_t key_at, value_at;  // operand addresses within a tile (bytes), without the block's own offset
+    frag q[kSteps];
+    f32x16 acc[kCols];
+    float top, sum;  // running maximum (unscaled logits) of the row, sum over this lane's keys
+    bool special;    // unseen values that are no numbers reached acc
+
+    __device__ __forceinline__ void place(int lane) {
+        const int col = lane % 32, half = lane / 32, vr = 4 * half + (lane % 16) / 4;
+        key_at = col * TL::kRowBytes + ((half ^ TL::key_turn(col)) * 16);
+        const int value_chunk = (2 * ((lane / 16) % 2) + (lane % 4) / 2) ^ TL::value_turn(vr);
+        value_at = vr * TL::kRowBytes + value_chunk * 16 + (lane % 2) * 8;
+    }
+
+    __device__ __forceinline__ void begin(const char *query_row, int half, int head_dim) {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            q[s] = frag{};
+            if (16 * s + 8 * half < head_dim) q[s] = *reinterpret_cast<const frag *>(query_row + (16 * s + 8 * half) * 2);
+        }
+#pragma unroll
+        for (int d = 0; d < kCols; ++d) acc[d] = f32x16{};
+        top = kNone;
+        sum = 0.0f;
+        special = false;
+    }
+
+    // s[kb][i]: logit of this lane's row with key 32 kb + 8 (i / 4) + 4 half + i % 4 of the tile.
+    __device__ __forceinline__ void logits(const char *keys, f32x16 (&s)[KB]) const {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) s[kb] = f32x16{};
+#pragma unroll
+        for (int c = 0; c < kSteps; ++c)
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                const frag k = *reinterpret_cast<const frag *>(keys + kb * 32 * TL::kRowBytes + (key_at ^ (32 * c)));
+                s[kb] = M::run(k, q[c], s[kb]);
+            }
+        ahead<KB * kSteps, 1, kKeysAhead>();
+    }
+
+    __device__ __forceinline__ static void hide(f32x16 (&s)[KB], int32_t base, int half, const Range &mine) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int32_t slot = base + 32 * kb + 8 * (i / 4) + 4 * half + i % 4;
+                if (slot < mine.low || slot >= mine.high) s[kb][i] = kNone;
+            }
+    }
+
+    // Weights of the logits, rounded; the running maximum and sum move on.
+    __device__ __forceinline__ void weigh(const f32x16 (&s)[KB], float scale2, frag (&p)[KB][2]) {
+        float most = s[0][0];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) most = fmaxf(most, s[kb][i]);
+        most = max_halves(most);
+        // A row without a maximum yet takes any; others wait for the slack.
+        if (__any(most * scale2 > top * scale2 + kSlack)) {
+            const float next = fmaxf(top, most);
+            const float factor = next == kNone ? 1.0f : __builtin_amdgcn_exp2f((top - next) * scale2);
+            top = next;
+            sum *= factor;
+#pragma unroll
+            for (int d = 0; d < kCols; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[d][i] *= factor;
+        }
+        const float shift = top == kNone ? 0.0f : top * scale2;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            float part = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float w = __builtin_amdgcn_exp2f(fmaf(s[kb][i], scale2, -shift));
+                part += w;
+                p[kb][i / 8][i % 8] = static_cast<T>(w);
+            }
+            sum += part;
+        }
+    }
+
+    // Sixteen values of columns 32 d + col, in the order of p[kb][h].
+    __device__ __forceinline__ uint4 value_frag(const char *values, int kb, int h, int d) const {
+        const char *at = values + (32 * kb + 16 * h) * TL::kRowBytes + (value_at ^ (64 * d));
+        const uint2 v0 = read_transposed(at), v1 = read_transposed(at + 8 * TL::kRowBytes);
+        return uint4{v0.x, v0.y, v1.x, v1.y};
+    }
+
+    // A weight of 0 times an infinite or NaN value is NaN: where this wave's rows see different slots, such values
+    // may belong to slots that a row does not see, and the wave's rows are taken one by one in the end.
+    __device__ __forceinline__ void inspect(const char *values) {
+        uint32_t found = 0;
+#pragma unroll 1
+        for (int x = 0; x < 2 * KB; ++x)
+#pragma unroll
+            for (int d = 0; d < kCols; ++d) {
+                const uint4 v = value_frag(values, x / 2, x % 2, d);
+                found |= M::special(v.x) | M::special(v.y) | M::special(v.z) | M::special(v.w);
+            }
+        special = special || __any(found & 0x80008000u);
+    }
+
+    __device__ __forceinline__ void add_values(const char *values, const frag (&p)[KB][2]) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int d = 0; d < kCols; ++d)
+                    acc[d] = M::run(__builtin_bit_cast(frag, value_frag(values, kb, h, d)), p[kb][h], acc[d]);
+        ahead<KB * 2 * kCols, 2, kValuesAhead>();
+    }
+
+    // The compiler would wait for every operand read right before its product; this orders the surrounding block's
+    // LDS reads (READS a product) AHEAD products before their use.
+    static constexpr int kKeysAhead = 4, kValuesAhead = 4;
+    template <int PRODUCTS, int READS, int AHEAD>
+    __device__ __forceinline__ static void ahead() {
+        __builtin_amdgcn_sched_group_barrier(0x100, READS * AHEAD, 0);  // LDS reads
+#pragma unroll
+        for (int i = 0; i < PRODUCTS - AHEAD; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix instructions
+            __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+    }
+
+    // Have the queries arrive here: left to their first use, the compiler waits for all loads in flight at every step.
+    __device__ __forceinline__ void hold_queries() {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) asm volatile("" : "+v"(q[s]));
+    }
+};
+
+// The rows of a workgroup's tile and what they see.
+struct RowTile {
+    int32_t row, token, in_group;           // this lane's row (its last one repeated past the end)
+    Range mine;
+    int32_t low, high;                      // any row of the workgroup's
+    int32_t any_low, all_low, all_high, any_high;  // this wave's rows, any of them or all
+    int32_t from, to;                       // steps of this split
+
+    template <typename A>
+    __device__ __forceinline__ RowTile(const A &a, const Sequence &seq, int32_t tile, int tile_rows, int wave_row,
+                                       int32_t rows, uint32_t split, int step) {
+        row = tile * tile_rows + wave_row + threadIdx.x % 32;
+        token = fast_quotient(min(row, rows - 1), a.group);
+        in_group = min(row, rows - 1) - token * a.group.divisor;
+        mine = seen_by(a, seq, token);
+        low = seen_by(a, seq, fast_quotient(tile * tile_rows, a.group)).low;
+        high = seen_by(a, seq, fast_quotient(min(rows, (tile + 1) * tile_rows) - 1, a.group)).high;
+        any_low = __builtin_amdgcn_readlane(mine.low, 0);
+        all_low = __builtin_amdgcn_readlane(mine.low, 31);
+        all_high = __builtin_amdgcn_readlane(mine.high, 0);
+        any_high = __builtin_amdgcn_readlane(mine.high, 31);
+        const int32_t steps = (high - low + step - 1) / step, share = (steps + a.splits - 1) / a.splits;
+        from = min<int32_t>(split * share, steps);
+        to = min<int32_t>(from + share, steps);
+    }
+};
+
+// Where the results of row (token, head) go.
+struct RowOut {
+    int64_t index, head, part;
+
+    template <typename A>
+    __device__ __forceinline__ RowOut(const A &a, const Sequence &seq, uint32_t kv_head, int32_t token, int32_t in_group,
+                                      uint32_t split) {
+        index = seq.start + token;
+        head = static_cast<int64_t>(kv_head) * a.group.divisor + in_group;
+        part = (static_cast<int64_t>(split) * a.tokens + index) * (a.kv_heads * a.group.divisor) + head;
+    }
+    template <typename A>
+    __device__ __forceinline__ void put_sums(const A &a, float top2, float total) const {
+        if (a.splits > 1)
+            a.part_sum[part] = make_float2(top2, total);
+        else if (a.lse != nullptr)
+            a.lse[index * a.lse_token + head] = lse_of(top2, total);
+    }
+    template <typename A>
+    __device__ __forceinline__ char *row(const A &a) const {
+        return a.splits > 1 ? reinterpret_cast<char *>(a.part_out + part * a.head_dim)
+                            : a.out + index * a.out_token + head * a.out_head;
+    }
+};
+
+// acc times `by` to a row: elements 32 d + 8 i + 4 half .. + 3 are acc[d][4 i .. 4 i + 3].
+template <typename TO, int COLS>
+__device__ __forceinline__ void put_row(char *row, const f32x16 (&acc)[COLS], float by, int half, int head_dim) {
+#pragma unroll
+    for (int d = 0; d < COLS; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int e = 32 * d + 8 * i + 4 * half;
+            if (e < head_dim)
+                put4<TO>(row + e * sizeof(TO), acc[d][4 * i] * by, acc[d][4 * i + 1] * by, acc[d][4 * i + 2] * by,
+                         acc[d][4 * i + 3] * by);
+        }
+}
+
+// attend_alone for each of a wave's rows from `first` on; `put` takes (row of the wave, its place, its sums, its elements).
+template <typename T, int DP, typename A, typename Put>
+__device__ __forceinline__ void rows_alone(const A &a, const Sequence &seq, uint32_t b, uint32_t kv_head, uint32_t split,
+                                           int32_t first, int32_t rows, int32_t from, int32_t to, int32_t step, int32_t part,
+                                           Put put) {
+    for (int r = 0; r < 32 && first + r < rows; ++r) {
+        const int32_t t = fast_quotient(first + r, a.group);
+        const RowOut place(a, seq, kv_head, t, first + r - t * a.group.divisor, split);
+        const T *query = reinterpret_cast<const T *>(a.query + place.index * a.query_token + place.head * a.query_head);
+        float o[DP / 64];
+        const float2 sums = attend_alone<T, DP>(a, query, seen_by(a, seq, t), from, to, step, part, a.table + b * a.table_stride,
+                                                a.keys.data + kv_head * a.keys.head_stride,
+                                                a.values.data + kv_head * a.values.head_stride, o);
+        put(r, place, sums, o);
+    }
+}
+
+// A wave's 32 rows to memory.
+template <typename T, int DP, int KB, typename A>
+__device__ __forceinline__ void put_rows(const A &a, const Sequence &seq, uint32_t b, uint32_t kv_head, uint32_t split,
+                                         const RowTile &tile, int32_t rows, int32_t step, const Core<T, DP, KB> &core) {
+    const int lane = threadIdx.x % 64, half = lane / 32;
+    const int head_dim = a.head_dim;
+    if (core.special) {
+        rows_alone<T, DP>(a, seq, b, kv_head, split, tile.row - threadIdx.x % 32, rows, tile.low + tile.from * step,
+                          tile.low + tile.to * step, step, step,
+                          [&](int, const RowOut &place, const float2 &sums, const float (&o)[DP / 64]) {
+                              if (lane == 0) place.put_sums(a, sums.x, sums.y);
+                              const float by = a.splits > 1 ? 1.0f : (sums.y == 0.0f ? 0.0f : 1.0f / sums.y);
+                              for (int k = 0; k < DP / 64; ++k)
+                                  if (lane + 64 * k < head_dim)
+                                      put_as(a.splits > 1 ? QXT_TYPE_F32 : a.out_type, place.row(a), lane + 64 * k, o[k] * by);
+                          });
+        return;
+    }
+    const float total = add_halves(core.sum);
+    if (tile.row >= rows) return;
+    const RowOut place(a, seq, kv_head, tile.token, tile.in_group, split);
+    if (half == 0) place.put_sums(a, core.top == kNone ? kNone : core.top * a.scale2, total);
+    char *out = place.row(a);
+    if (a.splits > 1) {
+        if (total != 0.0f) put_row<float>(out, core.acc, 1.0f, half, head_dim);
+        return;
+    }
+    const float by = total == 0.0f ? 0.0f : 1.0f / total;
+    if (a.out_type == QXT_TYPE_BF16)
+        put_row<bf16_t>(out, core.acc, by, half, head_dim);
+    else if (a.out_type == QXT_TYPE_F16)
+        put_row<f16_t>(out, core.acc, by, half, head_dim);
+    else
+        put_row<float>(out, core.acc, by, half, head_dim);
+}
+
+// kv_heads x tiles x splits x sequences, kv_heads fastest.
+struct Place {
+    uint32_t head, tile, split, b;
+    template <typename A>
+    __device__ __forceinline__ explicit Place(const A &a) {
+        uint32_t id = blockIdx.x;
+        head = id % a.kv_heads;
+        id /= a.kv_heads;
+        tile = id % a.tiles;
+        id /= a.tiles;
+        split = id % a.splits;
+        b = id / a.splits;
+    }
+};
+
 template <int DP, int WQ, int WK>
 struct Shape {
     static constexpr int kKeys = DP <= 128 && WQ >= 4 ? 64 : 32;  // keys of one step and key part
@@ -127,299 +405,133 @@ struct Shape {
 
 // Two waves a SIMD (256 registers each) up to 128 elements of head size, one above.
 template <typename T, int DP, int WQ, int WK>
-__global__ __launch_bounds__(64 * WQ * WK, DP <= 128 ? 2 : 1) void paged_attention_kernel(PagedArgs a) {
+__global__ __launch_bounds__(64 * WQ * WK, DP <= 128 ? 2 : 1) void paged_attention_kernel(PagedArgs) {
+    Kernarg<PagedArgs> *const args = kernargs<PagedArgs>();
+    Kernarg<PagedArgs> &a = *args;
     using S = Shape<DP, WQ, WK>;
-    using TL = Tile<DP>;
-    using M = Mfma<T>;
-    typedef typename M::frag frag;
+    using C = Core<T, DP, S::kKeys / 32>;
+    typedef typename C::frag frag;
     extern __shared__ __align__(16) char lds[];
-    constexpr int kBlocks = S::kKeys / 32, kCols = DP / 32;
-
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int wq = wave % WQ, wk = wave / WQ, col = lane % 32, half = lane / 32;
-    uint32_t id = blockIdx.x;
-    const uint32_t head = id % a.kv_heads;
-    id /= a.kv_heads;
-    const uint32_t first_tile = id % a.tiles;
-    id /= a.tiles;
-    const uint32_t split = id % a.splits, b = id / a.splits;
-    const Sequence seq = sequence_of(a, b);
-    const int32_t group = a.group.divisor, rows = seq.tokens * group;
-    const int32_t tiles = (rows + 32 * WQ - 1) / (32 * WQ);
-
+    const Place at(a);
+    const Sequence seq = sequence_of(a, at.b);
+    const int32_t rows = seq.tokens * a.group.divisor, tiles = (rows + 32 * WQ - 1) / (32 * WQ);
     Stager<DP, S::kRows> stager;
-    stager.table = a.table + b * a.table_stride;
-    const char *keys = a.keys.data + head * a.keys.head_stride, *values = a.values.data + head * a.values.head_stride;
-    char *const my_keys = lds + 2 * S::kTileBytes * wk;  // this key part's tiles of stage 0
+    stager.start(a, at.b, at.head);
+    C core;
+    core.place(lane);
+    const char *const my_keys = lds + 2 * S::kTileBytes * wk;  // this key part's tiles of stage 0
+    const uint32_t my_rows = lds_offset(my_keys) + wq * S::kRows * Tile<DP>::kRowBytes;
 
-    // Operand addresses within a tile (bytes), without the block's own offset.
-    const int key_at = col * TL::kRowBytes + ((half ^ TL::key_turn(col)) * 16);
-    const int vr = 4 * half + (lane % 16) / 4;
-    const int value_chunk = (2 * ((lane / 16) % 2) + (lane % 4) / 2) ^ TL::value_turn(vr);
-    const int value_at = vr * TL::kRowBytes + value_chunk * 16 + (lane % 2) * 8;
-
-    for (int32_t turn = first_tile; turn < tiles; turn += a.tiles) {
-        // The longest rows first: the last tiles of a causal sequence.
-        const int32_t tile = tiles - 1 - turn;
-        const int32_t row = tile * 32 * WQ + 32 * wq + col, held = min(row, rows - 1);
-        const int32_t token = fast_quotient(held, a.group), in_group = held - token * group;
-        const Range mine = seen_by(a, seq, token);
-        const Range first = seen_by(a, seq, fast_quotient(tile * 32 * WQ, a.group));
-        const Range last = seen_by(a, seq, fast_quotient(min(rows, (tile + 1) * 32 * WQ) - 1, a.group));
-        const int32_t low = first.low, high = last.high;
-        // What this wave's rows see, all of them or any.
-        const int32_t any_low = __builtin_amdgcn_readlane(mine.low, 0), all_low = __builtin_amdgcn_readlane(mine.low, 31);
-        const int32_t all_high = __builtin_amdgcn_readlane(mine.high, 0), any_high = __builtin_amdgcn_readlane(mine.high, 31);
-        const int32_t steps = (high - low + S::kStep - 1) / S::kStep, share = (steps + a.splits - 1) / a.splits;
-        const int32_t from = min<int32_t>(split * share, steps), to = min<int32_t>(from + share, steps);
-
-        const char *query_row = a.query + (seq.start + token) * a.query_token +
-                                static_cast<int64_t>(head * group + in_group) * a.query_head;
-        frag q[DP / 16];
-#pragma unroll
-        for (int s = 0; s < DP / 16; ++s) {
-            q[s] = frag{};
-            if (16 * s + 8 * half < static_cast<int>(a.head_dim))
-                q[s] = *reinterpret_cast<const frag *>(query_row + (16 * s + 8 * half) * 2);
-        }
-
-        f32x16 acc[kCols];
-#pragma unroll
-        for (int d = 0; d < kCols; ++d) acc[d] = f32x16{};
-        bool special = false;           // unseen values that are no numbers reached acc
-        float top = kNone, sum = 0.0f;  // top in logit units (unscaled), sum over this lane's keys
-
-        // Slot of this lane's staged row in step t.
-        const int stage_row = wq * S::kRows + lane % S::kRows;
-        auto staged_slot = [&](int32_t t) { return low + t * S::kStep + wk * S::kKeys + stage_row; };
+    for (int32_t turn = at.tile; turn < tiles; turn += a.tiles) {
+        const int32_t tile = tiles - 1 - turn;  // the longest rows first: the last tiles of a causal sequence
+        Kernarg<PagedArgs> &y = *late(args);
+        const RowTile rt(y, seq, tile, 32 * WQ, 32 * wq, rows, at.split, S::kStep);
+        core.begin(y.query + (seq.start + rt.token) * y.query_token +
+                       static_cast<int64_t>(at.head * y.group.divisor + rt.in_group) * y.query_head,
+                   half, y.head_dim);
         auto stage = [&](int32_t t) {
-            char *to = my_keys + (t & 1) * S::kStageBytes + wq * S::kRows * TL::kRowBytes;
-            const int32_t slot = staged_slot(t);
-            stager.template load<true>(keys, stager.offset_in(a, a.keys, slot), to, lane, wq * S::kRows, a.head_dim);
-            stager.template load<false>(values, stager.offset_in(a, a.values, slot), to + S::kTileBytes, lane,
-                                        wq * S::kRows, a.head_dim);
+            const uint32_t to = my_rows + (t & 1) * S::kStageBytes;
+            stager.stage(a, rt.low + t * S::kStep + wk * S::kKeys + wq * S::kRows, rt.high, to, to + S::kTileBytes, wq * S::kRows);
         };
-
-        if (from < to) {
-            stager.look_up(a, staged_slot(from), high);
-            stage(from);
-            stager.look_up(a, staged_slot(from + 1), high);
-        }
-        for (int32_t t = from; t < to; ++t) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's rows of step t have landed
-            if (WQ > 1) __builtin_amdgcn_s_barrier();         // everyone's have, and step t - 1 has been read
-            asm volatile("" ::: "memory");
-            __builtin_amdgcn_sched_barrier(0);
-            if (t + 1 < to) {
-                stage(t + 1);
-                stager.look_up(a, staged_slot(t + 2), high);
-            }
-            const int32_t base = low + t * S::kStep + wk * S::kKeys;
-            if (base >= any_high || base + S::kKeys <= any_low) continue;
+        auto compute = [&](int32_t t) {
+            const int32_t base = rt.low + t * S::kStep + wk * S::kKeys;
+            if (base >= rt.any_high || base + S::kKeys <= rt.any_low) return;
             const char *kt = my_keys + (t & 1) * S::kStageBytes, *vt = kt + S::kTileBytes;
-
-            f32x16 s[kBlocks];
-#pragma unroll
-            for (int kb = 0; kb < kBlocks; ++kb) {
-                s[kb] = f32x16{};
-#pragma unroll
-                for (int c = 0; c < DP / 16; ++c) {
-                    const frag k = *reinterpret_cast<const frag *>(kt + kb * 32 * TL::kRowBytes + (key_at ^ (32 * c)));
-                    s[kb] = M::run(k, q[c], s[kb]);
-                }
-            }
-            const bool partial = base < all_low || base + S::kKeys > all_high;
-            if (partial) {
-#pragma unroll
-                for (int kb = 0; kb < kBlocks; ++kb)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int32_t slot = base + 32 * kb + 8 * (i / 4) + 4 * half + i % 4;
-                        if (slot < mine.low || slot >= mine.high) s[kb][i] = kNone;
-                    }
-            }
-            float most = s[0][0];
-#pragma unroll
-            for (int kb = 0; kb < kBlocks; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) most = fmaxf(most, s[kb][i]);
-            most = max_halves(most);
-            // A row without a maximum yet takes any; others wait for the slack.
-            if (__any(most * a.scale2 > top * a.scale2 + kSlack)) {
-                const float next = fmaxf(top, most);
-                const float factor = next == kNone ? 1.0f : __builtin_amdgcn_exp2f((top - next) * a.scale2);
-                top = next;
-                sum *= factor;
-#pragma unroll
-                for (int d = 0; d < kCols; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[d][i] *= factor;
-            }
-            const float shift = top == kNone ? 0.0f : top * a.scale2;
-            frag p[kBlocks][2];
-#pragma unroll
-            for (int kb = 0; kb < kBlocks; ++kb) {
-                float part = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float w = __builtin_amdgcn_exp2f(fmaf(s[kb][i], a.scale2, -shift));
-                    part += w;
-                    p[kb][i / 8][i % 8] = static_cast<T>(w);
-                }
-                sum += part;
-            }
-            // Sixteen values of columns 32 d + col, in the order of p[kb][h].
-            auto value_frag = [&](int kb, int h, int d) {
-                const char *at = vt + (32 * kb + 16 * h) * TL::kRowBytes + (value_at ^ (64 * d));
-                const uint2 v0 = read_transposed(at), v1 = read_transposed(at + 8 * TL::kRowBytes);
-                return uint4{v0.x, v0.y, v1.x, v1.y};
-            };
-            // A weight of 0 times an infinite or NaN value is NaN: where this wave's rows see different slots, such
-            // values may belong to slots that a row does not see, and the rows are taken one by one below.
-            if (partial && (any_low != all_low || any_high != all_high)) {
-                uint32_t found = 0;
-#pragma unroll 1
-                for (int x = 0; x < 2 * kBlocks; ++x)
-#pragma unroll
-                    for (int d = 0; d < kCols; ++d) {
-                        const uint4 v = value_frag(x / 2, x % 2, d);
-                        found |= M::special(v.x) | M::special(v.y) | M::special(v.z) | M::special(v.w);
-                    }
-                special = special || __any(found & 0x80008000u);
-            }
-#pragma unroll
-            for (int kb = 0; kb < kBlocks; ++kb)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int d = 0; d < kCols; ++d)
-                        acc[d] = M::run(__builtin_bit_cast(frag, value_frag(kb, h, d)), p[kb][h], acc[d]);
-        }
-        sum = add_halves(sum);
-        // Rows' results: row `row`, elements 32 d + 8 (i / 4) + 4 half + i % 4 in acc[d][i].
-        const int64_t token_index = seq.start + token;
-        const int64_t query_head = static_cast<int64_t>(head) * group + in_group;
-        const int64_t part_row = (static_cast<int64_t>(split) * a.tokens + token_index) * (a.kv_heads * group) + query_head;
-        const float top2 = top == kNone ? kNone : top * a.scale2;
-        // attend_alone for each of this wave's rows; `put` stores (row of the wave, row, its sums, its elements).
-        auto rows_alone = [&](auto put) {
-            for (int r = 0; r < 32; ++r) {
-                const int32_t one = tile * 32 * WQ + 32 * wq + r;
-                if (one >= rows) break;
-                const int32_t t = fast_quotient(one, a.group), h = one - t * group;
-                const T *q_row = reinterpret_cast<const T *>(a.query + (seq.start + t) * a.query_token +
-                                                             static_cast<int64_t>(head * group + h) * a.query_head);
-                float o[DP / 64];
-                const float2 sums = attend_alone<T, DP>(a, q_row, seen_by(a, seq, t), low + from * S::kStep + wk * S::kKeys,
-                                                        low + to * S::kStep, S::kStep, S::kKeys, stager.table, keys, values, o);
-                put(r, static_cast<int64_t>(seq.start + t), static_cast<int64_t>(head) * group + h, sums, o);
-            }
+            f32x16 s[S::kKeys / 32];
+            frag p[S::kKeys / 32][2];
+            core.logits(kt, s);
+            const bool partial = base < rt.all_low || base + S::kKeys > rt.all_high;
+            if (partial) C::hide(s, base, half, rt.mine);
+            core.weigh(s, a.scale2, p);
+            if (partial && (rt.any_low != rt.all_low || rt.any_high != rt.all_high)) core.inspect(vt);
+            core.add_values(vt, p);
         };
-        if (WK == 1) {
-            if (special) {
-                rows_alone([&](int, int64_t index, int64_t h, const float2 &sums, const float (&o)[DP / 64]) {
-                    const int64_t at = (static_cast<int64_t>(split) * a.tokens + index) * (a.kv_heads * group) + h;
-                    const bool parts = a.splits > 1;
-                    if (lane == 0 && parts) a.part_sum[at] = sums;
-                    if (lane == 0 && !parts && a.lse != nullptr) a.lse[index * a.lse_token + h] = lse_of(sums.x, sums.y);
-                    const float by = parts ? 1.0f : (sums.y == 0.0f ? 0.0f : 1.0f / sums.y);
-                    for (int k = 0; k < DP / 64; ++k) {
-                        const int e = lane + 64 * k;
-                        if (e >= static_cast<int>(a.head_dim)) continue;
-                        if (parts)
-                            a.part_out[at * a.head_dim + e] = o[k];
-                        else
-                            put_as(a.out_type, a.out + index * a.out_token + h * a.out_head, e, o[k] * by);
-                    }
-                });
-            } else if (row < rows) {
-                if (a.splits > 1) {
-                    if (half == 0) a.part_sum[part_row] = make_float2(top2, sum);
-                } else if (a.lse != nullptr && half == 0) {
-                    a.lse[token_index * a.lse_token + query_head] = lse_of(top2, sum);
-                }
-                const float by = a.splits > 1 ? 1.0f : (sum == 0.0f ? 0.0f : 1.0f / sum);
-                char *out = a.splits > 1 ? reinterpret_cast<char *>(a.part_out + part_row * a.head_dim)
-                                         : a.out + token_index * a.out_token + query_head * a.out_head;
-                const uint32_t type = a.splits > 1 ? QXT_TYPE_F32 : a.out_type;
-                if (a.splits == 1 || sum != 0.0f) {
-#pragma unroll
-                    for (int d = 0; d < kCols; ++d)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int e = 32 * d + 8 * i + 4 * half;
-                            if (e < static_cast<int>(a.head_dim))
-                                put4_as(type, out, e, acc[d][4 * i] * by, acc[d][4 * i + 1] * by, acc[d][4 * i + 2] * by,
-                                        acc[d][4 * i + 3] * by);
-                        }
+        if constexpr (WQ == 1) {
+            // The wave reads only what it staged itself: two steps are in flight, and no one is waited for.
+            if (rt.from < rt.to) stage(rt.from);
+            if (rt.from + 1 < rt.to) stage(rt.from + 1);
+            core.hold_queries();
+            for (int32_t t = rt.from; t < rt.to; ++t) {
+                if (t + 1 < rt.to)
+                    landed<2 * Stager<DP, S::kRows>::kLoads>();
+                else
+                    landed<0>();
+                compute(t);
+                if (t + 2 < rt.to) {
+                    reads_done();
+                    stage(t + 2);
                 }
             }
-            if (WQ > 1) __syncthreads();  // before the next tile's staging
-            continue;
-        }
-
-        // Join the key parts: every wave scales to the common maximum and puts
-        // its outputs in LDS, then each wave adds up and stores its share of the elements.
-        constexpr int kPitch = DP + 4;  // floats a row
-        float *joined = reinterpret_cast<float *>(lds);                          // [WK][32 WQ][kPitch]
-        float2 *sums = reinterpret_cast<float2 *>(joined + WK * 32 * WQ * kPitch);  // [WK][32 WQ]
-        __syncthreads();  // staged tiles have been read
-        const int part_at = wk * 32 * WQ + 32 * wq;  // this wave's rows
-        if (special) {
-            rows_alone([&](int r, int64_t, int64_t, const float2 &one, const float (&o)[DP / 64]) {
-                if (lane == 0) sums[part_at + r] = one;
-                for (int k = 0; k < DP / 64; ++k) joined[(part_at + r) * kPitch + lane + 64 * k] = o[k];
-            });
         } else {
-            if (half == 0) sums[part_at + col] = make_float2(top2, sum);
-#pragma unroll
-            for (int d = 0; d < kCols; ++d)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<float4 *>(joined + (part_at + col) * kPitch + 32 * d + 8 * i + 4 * half) =
-                        make_float4(acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]);
+            if (rt.from < rt.to) stage(rt.from);
+            core.hold_queries();
+            for (int32_t t = rt.from; t < rt.to; ++t) {
+                landed<0>();  // this wave's rows of step t
+                meet();       // everyone's, and step t - 1 has been read
+                if (t + 1 < rt.to) stage(t + 1);
+                compute(t);
+            }
         }
-        __syncthreads();
-        constexpr int kLanes = DP / 4;  // threads a row, four elements each
-        for (int r = threadIdx.x / kLanes; r < 32 * WQ; r += S::kThreads / kLanes) {
-            const int32_t out_row = tile * 32 * WQ + r;
-            if (out_row >= rows) break;
-            const int e = 4 * (threadIdx.x % kLanes);
-            float most = kNone, total = 0.0f;
-            float2 ms[WK];
-#pragma unroll
-            for (int w = 0; w < WK; ++w) {
-                ms[w] = sums[w * 32 * WQ + r];
-                most = fmaxf(most, ms[w].x);
-            }
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < WK; ++w) {
-                if (ms[w].y == 0.0f) continue;  // saw nothing (its maximum is -inf)
-                const float f = __builtin_amdgcn_exp2f(ms[w].x - (most == kNone ? 0.0f : most));
-                const float g = ms[w].x == kNone ? 1.0f : f;
-                const float4 y = *reinterpret_cast<const float4 *>(joined + (w * 32 * WQ + r) * kPitch + e);
-                total += ms[w].y * g;
-                x.x += y.x * g;
-                x.y += y.y * g;
-                x.z += y.z * g;
-                x.w += y.w * g;
-            }
-            const int32_t t = fast_quotient(out_row, a.group);
-            const int64_t index = seq.start + t, h = static_cast<int64_t>(head) * group + (out_row - t * group);
-            if (a.splits > 1) {
-                const int64_t at = (static_cast<int64_t>(split) * a.tokens + index) * (a.kv_heads * group) + h;
-                if (e == 0) a.part_sum[at] = make_float2(most, total);
-                if (total != 0.0f && e < static_cast<int>(a.head_dim))
-                    *reinterpret_cast<float4 *>(a.part_out + at * a.head_dim + e) = x;
+        Kernarg<PagedArgs> &z = *late(args);
+        if constexpr (WK == 1) {
+            put_rows<T, DP>(z, seq, at.b, at.head, at.split, rt, rows, S::kStep, core);
+            if (WQ > 1) __syncthreads();  // before the next tile's staging
+        } else {
+            // Join the key parts: every wave puts its outputs in LDS, then the threads add up and store shares of the elements.
+            constexpr int kPitch = DP + 4;  // floats a row
+            float *joined = reinterpret_cast<float *>(lds);                              // [WK][32 WQ][kPitch]
+            float2 *sums = reinterpret_cast<float2 *>(joined + WK * 32 * WQ * kPitch);   // [WK][32 WQ]
+            __syncthreads();                                                             // staged tiles have been read
+            const int part_at = wk * 32 * WQ + 32 * wq;                                  // this wave's rows
+            if (core.special) {
+                rows_alone<T, DP>(z, seq, at.b, at.head, at.split, tile * 32 * WQ + 32 * wq, rows,
+                                  rt.low + rt.from * S::kStep + wk * S::kKeys, rt.low + rt.to * S::kStep, S::kStep, S::kKeys,
+                                  [&](int r, const RowOut &, const float2 &one, const float (&o)[DP / 64]) {
+                                      if (lane == 0) sums[part_at + r] = one;
+                                      for (int k = 0; k < DP / 64; ++k) joined[(part_at + r) * kPitch + lane + 64 * k] = o[k];
+                                  });
             } else {
-                if (e == 0 && a.lse != nullptr) a.lse[index * a.lse_token + h] = lse_of(most, total);
-                const float by = total == 0.0f ? 0.0f : 1.0f / total;
-                if (e < static_cast<int>(a.head_dim))
-                    put4_as(a.out_type, a.out + index * a.out_token + h * a.out_head, e, x.x * by, x.y * by, x.z * by, x.w * by);
+                const float total = add_halves(core.sum);
+                if (half == 0) sums[part_at + col] = make_float2(core.top == kNone ? kNone : core.top * z.scale2, total);
+                put_row<float>(reinterpret_cast<char *>(joined + (part_at + col) * kPitch), core.acc, 1.0f, half, DP);
             }
+            __syncthreads();
+            constexpr int kLanes = DP / 4;  // threads a row, four elements each
+            for (int r = threadIdx.x / kLanes; r < 32 * WQ; r += S::kThreads / kLanes) {
+                const int32_t out_row = tile * 32 * WQ + r;
+                if (out_row >= rows) break;
+                const int e = 4 * (threadIdx.x % kLanes);
+                float most = kNone, total = 0.0f;
+                float2 ms[WK];
+#pragma unroll
+                for (int w = 0; w < WK; ++w) {
+                    ms[w] = sums[w * 32 * WQ + r];
+                    most = fmaxf(most, ms[w].x);
+                }
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < WK; ++w) {
+                    if (ms[w].y == 0.0f) continue;  // saw nothing
+                    const float f = ms[w].x == kNone ? 1.0f : __builtin_amdgcn_exp2f(ms[w].x - most);
+                    const float4 y = *reinterpret_cast<const float4 *>(joined + (w * 32 * WQ + r) * kPitch + e);
+                    total += ms[w].y * f;
+                    x.x += y.x * f;
+                    x.y += y.y * f;
+                    x.z += y.z * f;
+                    x.w += y.w * f;
+                }
+                const int32_t t = fast_quotient(out_row, z.group);
+                const RowOut place(z, seq, at.head, t, out_row - t * z.group.divisor, at.split);
+                if (e == 0) place.put_sums(z, most, total);
+                if (e < static_cast<int>(z.head_dim)) {
+                    const float by = z.splits > 1 ? 1.0f : (total == 0.0f ? 0.0f : 1.0f / total);
+                    put4_as(z.splits > 1 ? QXT_TYPE_F32 : z.out_type, place.row(z), e, x.x * by, x.y * by, x.z * by, x.w * by);
+                }
+            }
+            __syncthreads();
         }
-        __syncthreads();
     }
 }
 

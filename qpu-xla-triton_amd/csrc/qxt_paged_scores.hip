@@ -101,7 +101,7 @@ __global__ __launch_bounds__(64 * kScoreWaves, DP <= 128 ? 2 : 1) void paged_sco
                     const int chunk = (lane % TL::kChunks) ^ TL::key_turn(r);
                     const char *src = a.query + (seq.start + token) * a.query_token +
                                       static_cast<int64_t>(head * group + h) * a.query_head + chunk * 16;
-                    if (chunk * 8 >= static_cast<int>(a.head_dim)) src = reinterpret_cast<const char *>(&kZeroRow);
+                    if (chunk * 8 >= static_cast<int>(a.head_dim)) src = reinterpret_cast<const char *>(kZeroRow);
                     __builtin_amdgcn_global_load_lds(
                         (const __attribute__((address_space(1))) void *)src,
                         (__attribute__((address_space(3))) void *)(rows_lds[buffer] + wave * kOwn * TL::kRowBytes + i * 1024),
