@@ -28,13 +28,14 @@ inline bool all_multiples(size_t of, std::initializer_list<size_t> values) {
 // n / d and n % d for n < 2^31 and a divisor known at launch.  With s =
 // ceil(log2 d) and m = floor(2^(31 + s) / d) + 1 the error of m is below
 // 2^s / 2^(31 + s) relative to 1 / d, so floor(n m / 2^(31 + s)) is exact for
-// every n < 2^31, and m < 2^32.  d = 1 is passed through.
+// every n < 2^31, and m < 2^32.  d = 1 passes n through (without a branch).
 struct FastDiv {
-    uint32_t divisor, magic, shift;
+    uint32_t divisor, magic, shift, pass;
 };
 inline FastDiv fast_div(uint32_t d) {
-    FastDiv f{d, 0, 0};
+    FastDiv f{d, 0, 0, 0xFFFFFFFFu};
     if (d <= 1) return f;
+    f.pass = 0;
     uint32_t s = 0;
     while ((1ull << s) < d) ++s;
     f.magic = static_cast<uint32_t>((1ull << (31 + s)) / d + 1);
@@ -44,8 +45,7 @@ inline FastDiv fast_div(uint32_t d) {
 // (F: FastDiv, in any address space.)
 template <typename F>
 __host__ __device__ __forceinline__ uint32_t fast_quotient(uint32_t n, const F &f) {
-    if (f.divisor <= 1) return n;
-    return static_cast<uint32_t>((static_cast<uint64_t>(n) * f.magic) >> 32) >> f.shift;
+    return (static_cast<uint32_t>((static_cast<uint64_t>(n) * f.magic) >> 32) + (n & f.pass)) >> f.shift;
 }
 
 // One cache (keys or values): pages of page_size slots, a row of head_dim

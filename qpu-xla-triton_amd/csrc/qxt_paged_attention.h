@@ -207,13 +207,22 @@ struct Stager {
         }
     }
 
+    template <typename A>
+    __device__ __forceinline__ void load_keys(const A &a, const Row &r, uint32_t to, int row0) const {
+        load<true>(address(keys, a.keys, r), to, row0, a.head_dim);
+    }
+    template <typename A>
+    __device__ __forceinline__ void load_values(const A &a, const Row &r, uint32_t to, int row0) const {
+        load<false>(address(values, a.values, r), to, row0, a.head_dim);
+    }
+
     // Both tiles' rows; keys at `to`, values at `to_values`.
     template <typename A>
     __device__ __forceinline__ void stage(const A &a, int32_t slot0, int32_t high, uint32_t to, uint32_t to_values,
                                           int row0) {
         const Row r = locate(a, slot0, high);
-        load<true>(address(keys, a.keys, r), to, row0, a.head_dim);
-        load<false>(address(values, a.values, r), to_values, row0, a.head_dim);
+        load_keys(a, r, to, row0);
+        load_values(a, r, to_values, row0);
     }
 };
 

@@ -345,8 +345,9 @@ __device__ __forceinline__ void rows_alone(const A &a, const Sequence &seq, uint
 template <typename T, int DP, int KB, typename A>
 __device__ __forceinline__ void put_rows(const A &a, const Sequence &seq, uint32_t b, uint32_t kv_head, uint32_t split,
                                          const RowTile &tile, int32_t rows, int32_t step, const Core<T, DP, KB> &core) {
-    const int lane = threadIdx.x % 64, half = lane / 32;
-    const int head_dim = a.head_dim;
+    int lane = threadIdx.x % 64;
+    asm volatile("" : "+v"(lane));  // keeps the elements' offsets out of the main loop's registers
+    const int half = lane / 32, head_dim = a.head_dim;
     if (core.special) {
         rows_alone<T, DP>(a, seq, b, kv_head, split, tile.row - threadIdx.x % 32, rows, tile.low + tile.from * step,
                           tile.low + tile.to * step, step, step,
@@ -535,6 +536,111 @@ __global__ __launch_bounds__(64 * WQ * WK, DP <= 128 ? 2 : 1) void paged_attenti
     }
 }
 
+// Many rows (heads of up to 128 elements): eight waves of 32 rows over steps of
+// 64 keys, two waves on each SIMD in opposite phases.  While waves 0-3 feed the
+// matrix cores (logits of step t, outputs of step t - 1), waves 4-7, on the same
+// SIMDs, turn their logits into weights on the vector unit, and at the next
+// barrier they change places; in step, both units idle in turns.
+// Three buffers each of keys and values: a wave stages its share of keys t + 2
+// and values t + 1 at the start of its matrix phase t, into buffers last read a
+// phase ago, and waits for them two phases later, before the barrier after which
+// the first wave reads them.
+template <typename T, int DP>
+__global__ __launch_bounds__(512, 2) void paged_attention_long_kernel(PagedArgs) {
+    constexpr int kKeys = 64, kWaveRows = kKeys / 8, kTileBytes = kKeys * DP * 2, kRing = 3;
+    using C = Core<T, DP, kKeys / 32>;
+    using St = Stager<DP, kWaveRows>;
+    typedef typename C::frag frag;
+    extern __shared__ __align__(16) char lds[];  // kRing tiles of keys, kRing of values
+    Kernarg<PagedArgs> *const args = kernargs<PagedArgs>();
+    Kernarg<PagedArgs> &a = *args;
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), half = lane / 32;
+    const bool second = wave >= 4;
+    const Place at(a);
+    const Sequence seq = sequence_of(a, at.b);
+    const int32_t rows = seq.tokens * a.group.divisor, tiles = (rows + 255) / 256;
+    St stager;
+    stager.start(a, at.b, at.head);
+    C core;
+    core.place(lane);
+    const uint32_t my_rows = lds_offset(lds) + wave * kWaveRows * Tile<DP>::kRowBytes;
+
+    for (int32_t turn = at.tile; turn < tiles; turn += a.tiles) {
+        const int32_t tile = tiles - 1 - turn;  // the longest rows first: the last tiles of a causal sequence
+        Kernarg<PagedArgs> &y = *late(args);
+        const RowTile rt(y, seq, tile, 256, 32 * wave, rows, at.split, kKeys);
+        core.begin(y.query + (seq.start + rt.token) * y.query_token +
+                       static_cast<int64_t>(at.head * y.group.divisor + rt.in_group) * y.query_head,
+                   half, y.head_dim);
+        const int32_t end = min(rt.high, rt.low + rt.to * kKeys);  // steps past the last stage rows of zeros
+        auto locate = [&](int32_t t) { return stager.locate(a, rt.low + t * kKeys + wave * kWaveRows, end); };
+        auto load_keys = [&](const typename St::Row &r, int place) {
+            stager.load_keys(a, r, my_rows + place * kTileBytes, wave * kWaveRows);
+        };
+        auto load_values = [&](const typename St::Row &r, int place) {
+            stager.load_values(a, r, my_rows + (kRing + place) * kTileBytes, wave * kWaveRows);
+        };
+        auto shown = [&](int32_t t) {  // some row of this wave sees some slot of step t
+            const int32_t base = rt.low + t * kKeys;
+            return t >= rt.from && t < rt.to && base < rt.any_high && base + kKeys > rt.any_low;
+        };
+        typename St::Row next = locate(rt.from);
+        load_keys(next, 0);
+        load_values(next, 0);
+        next = locate(rt.from + 1);
+        load_keys(next, 1);
+        core.hold_queries();
+        landed<0>();
+        meet();
+        if (second) meet();
+
+        f32x16 s[kKeys / 32];
+        frag p[kKeys / 32][2];
+        int place = 0, before = kRing - 1;  // buffers of steps t and t - 1
+        bool pending = false, ragged = false;  // step t - 1 has weights; its rows see different slots
+        for (int32_t t = rt.from; t < rt.to; ++t) {
+            // Matrix phase: the buffers of keys t - 1 and values t - 2 are free.
+            const int after = place == kRing - 1 ? 0 : place + 1;
+            const typename St::Row third = locate(t + 2);
+            load_keys(third, before);
+            load_values(next, after);
+            next = third;
+            const int32_t base = rt.low + t * kKeys;
+            const bool live = shown(t);
+            if (live) core.logits(lds + place * kTileBytes, s);
+            if (pending) {
+                const char *vt = lds + (kRing + before) * kTileBytes;
+                if (ragged) core.inspect(vt);
+                core.add_values(vt, p);
+            }
+            if (second) landed<2 * St::kLoads>();
+            meet();
+            // Vector phase.
+            if (live) {
+                const bool partial = base < rt.all_low || base + kKeys > rt.all_high;
+                if (partial) C::hide(s, base, half, rt.mine);
+                core.weigh(s, a.scale2, p);
+                ragged = partial && (rt.any_low != rt.all_low || rt.any_high != rt.all_high);
+            }
+            pending = live;
+            before = place;
+            place = after;
+            if (!second) landed<2 * St::kLoads>();
+            meet();
+        }
+        if (pending) {
+            const char *vt = lds + (kRing + before) * kTileBytes;
+            if (ragged) core.inspect(vt);
+            core.add_values(vt, p);
+        }
+        if (!second) meet();
+        landed<0>();
+        Kernarg<PagedArgs> &z = *late(args);
+        put_rows<T, DP>(z, seq, at.b, at.head, at.split, rt, rows, kKeys, core);
+        __syncthreads();  // before the next tile's staging
+    }
+}
+
 // Join the parts of rows whose slots were split over workgroups: a wave a row,
 // four elements a lane.
 __global__ __launch_bounds__(256) void paged_attention_join_kernel(PagedArgs a) {
@@ -615,7 +721,9 @@ int launch_attention_shape(const PagedArgs &a, const Plan &p, uint32_t grid, hip
     if (p.wq == 1) return launch_attention<T, DP, 1, wide ? 2 : 4>(a, grid, stream);
     if (p.wq == 2) return launch_attention<T, DP, 2, wide ? 1 : 2>(a, grid, stream);
     if (p.wq == 4) return launch_attention<T, DP, 4, 1>(a, grid, stream);
-    if constexpr (!wide) return launch_attention<T, DP, 8, 1>(a, grid, stream);
+    if constexpr (!wide)
+        return launch("paged_attention_long_kernel", paged_attention_long_kernel<T, DP>, dim3(grid), dim3(512), 6 * 64 * DP * 2,
+                      stream, a);
     return fail(QXT_INTERNAL_ERROR, "paged attention: no launch for %u waves", p.wq);
 }
 
