@@ -20,6 +20,7 @@ struct PagedArgs {
     FastDiv group;  // query heads per key head
     float scale, scale2;  // scale2 = scale * log2(e)
     int32_t causal, window;
+    uint32_t even;   // units of eight slots lie in one page, at 32-bit strides, in rows of DP elements
     uint32_t tiles, splits;  // grid: kv_heads x tiles x splits x sequences, kv_heads fastest
     char *out;
     int64_t out_token, out_head;
@@ -45,6 +46,12 @@ template <typename A>
 __device__ __forceinline__ A *late(A *args) {
     asm volatile("" : "+s"(args));
     return args;
+}
+
+// A wave-uniform value that stays in a register from here on.
+template <typename V>
+__device__ __forceinline__ void keep(V &value) {
+    asm volatile("" : "+s"(value));
 }
 
 // (A: PagedArgs, in any address space.)
@@ -95,8 +102,8 @@ struct Tile {
     static constexpr int kChunks = DP / 8;               // 16-byte chunks a row
     static constexpr int kRowBytes = DP * 2;
     static constexpr int kRowsPerLoad = 64 / kChunks;    // rows of one wave-wide 16-byte DMA
-    static __device__ __forceinline__ int key_turn(int row) { return row & (kChunks < 16 ? kChunks - 1 : 15); }
-    static __device__ __forceinline__ int value_turn(int row) { return 2 * (row & (kChunks < 16 ? 3 : 7)); }
+    static __device__ __forceinline__ int key_turn(int row) { return row & (kChunks < 16 ? 7 : 15); }
+    static __device__ __forceinline__ int value_turn(int row) { return kChunks < 16 ? 2 * (row & 3) : 4 * (row & 3); }
 };
 
 // Source of rows that are not in the cache: slots past a sequence's end, pages
@@ -112,6 +119,10 @@ __device__ __constant__ const uint4 kZeroRow[32] = {};
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void dma16(const char *src, uint32_t to) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(src) : "memory", "m0");
+}
+// The same from a wave-uniform address plus each lane's offset.
+__device__ __forceinline__ void dma16_at(uint64_t base, uint32_t offset, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(offset), "s"(base) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 
@@ -139,91 +150,145 @@ __device__ __forceinline__ uint32_t lds_offset(const char *p) {
         reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char *)p)));
 }
 
-// One wave's share of staging: ROWS consecutive slots of a tile, one row per
-// lane for the address work (lanes past ROWS repeat).  Each lane holds the page
-// id of one of 64 consecutive table entries, refetched when the slots leave
-// them, so that a tile's addresses wait for no load.
+// One wave's share of staging: ROWS consecutive slots of a tile.  Rows go in
+// units of eight.  Where pages hold whole units (`even`), a unit's address is
+// the same for the wave and the lanes' offsets in it never change: scalar
+// arithmetic and one instruction a load.  Otherwise, and for the units at a
+// sequence's end, each lane works out a row's address and the lanes that load
+// it fetch it from there.  Each lane holds the page id of one of 64 consecutive
+// table entries, refetched when the slots leave them, so that a tile's
+// addresses wait for no load.
 template <int DP, int ROWS>
 struct Stager {
     using TL = Tile<DP>;
     static constexpr int kLoads = ROWS / TL::kRowsPerLoad;  // of keys, and as many of values
+    static constexpr int kUnit = 8, kUnits = ROWS / kUnit, kUnitLoads = kUnit / TL::kRowsPerLoad;
+    // Arguments that the main loops need, in registers: left in the kernarg segment they are loaded, and
+    // waited for, at every use.
     const int32_t *table;
-    const char *keys, *values;  // of this head
+    uint64_t keys, values;  // of this head
+    FastDiv page;
+    uint32_t pages, even, head_dim;
+    uint32_t key_page, key_slot, value_page, value_slot;  // strides in 16 bytes
     int32_t held, page0;        // page id of entry page0 + lane
+    int32_t holes;              // some of them name no page
+    // Of this lane's 16 bytes within a unit; keys of even and odd units (of a wave's single unit: its own).
+    static constexpr int kKinds = kUnits > 1 ? 2 : 1;
+    uint32_t key_offset[kKinds][kUnitLoads], value_offset[kUnitLoads];
 
     template <typename A>
-    __device__ __forceinline__ void start(const A &a, uint32_t b, uint32_t head) {
+    __device__ __forceinline__ void start(const A &a, uint32_t b, uint32_t head, int first_row) {
         table = a.table + b * a.table_stride;
-        keys = a.keys.data + head * a.keys.head_stride;
-        values = a.values.data + head * a.values.head_stride;
+        keys = reinterpret_cast<uint64_t>(a.keys.data + head * a.keys.head_stride);
+        values = reinterpret_cast<uint64_t>(a.values.data + head * a.values.head_stride);
+        page = FastDiv{a.page.divisor, a.page.magic, a.page.shift, a.page.pass};
+        pages = a.pages;
+        even = a.even;
+        head_dim = a.head_dim;
+        key_page = static_cast<uint32_t>(a.keys.page_stride / 16);
+        key_slot = static_cast<uint32_t>(a.keys.slot_stride / 16);
+        value_page = static_cast<uint32_t>(a.values.page_stride / 16);
+        value_slot = static_cast<uint32_t>(a.values.slot_stride / 16);
+        keep(table);
+        keep(keys);
+        keep(values);
+        keep(page.divisor);
+        keep(page.magic);
+        keep(page.shift);
+        keep(page.pass);
+        keep(pages);
+        keep(even);
+        keep(head_dim);
+        keep(key_page);
+        keep(key_slot);
+        keep(value_page);
+        keep(value_slot);
         held = -1;
         page0 = -64;
+        holes = 0;
+        const int lane = threadIdx.x % 64;
+#pragma unroll
+        for (int i = 0; i < kUnitLoads; ++i) {
+            const int r = i * TL::kRowsPerLoad + lane / TL::kChunks, chunk = lane % TL::kChunks;
+#pragma unroll
+            for (int k = 0; k < kKinds; ++k)
+                key_offset[k][i] = r * static_cast<uint32_t>(a.keys.slot_stride) + (chunk ^ TL::key_turn(first_row + 8 * k + r)) * 16;
+            value_offset[i] = r * static_cast<uint32_t>(a.values.slot_stride) + (chunk ^ TL::value_turn(r)) * 16;
+        }
     }
 
-    // Page entry and place in the page of this lane's row (slot slot0 + lane % ROWS), or entry -1 from `high` on.
-    struct Row {
-        int32_t id;
+    // The rows of slots slot0 .. slot0 + ROWS - 1 (those from `high` on are zeros).
+    struct Rows {
+        int32_t slot0;
+        bool whole;       // wave-uniform: units by scalar addresses
+        int32_t id;       // else page id (or -1) and place in the page of this lane's row slot0 + lane % ROWS
         uint32_t in_page;
     };
-    template <typename A>
-    __device__ __forceinline__ Row locate(const A &a, int32_t slot0, int32_t high) {
+
+    __device__ __forceinline__ Rows locate(int32_t slot0, int32_t high) {
         const int lane = threadIdx.x % 64;
+        Rows r;
+        r.slot0 = slot0;
         if (slot0 < high) {
-            const int32_t first = fast_quotient(slot0, a.page), last = fast_quotient(min(slot0 + ROWS, high) - 1, a.page);
+            const int32_t first = fast_quotient(slot0, page), last = fast_quotient(min(slot0 + ROWS, high) - 1, page);
             if (first < page0 || last >= page0 + 64) {
                 page0 = first;
-                const int32_t entry = first + lane, end = fast_quotient(high - 1, a.page);
-                held = table[min(entry, end)];
+                held = table[min(first + lane, static_cast<int32_t>(fast_quotient(high - 1, page)))];
+                holes = __any(static_cast<uint32_t>(held) >= pages) ? 1 : 0;
+                asm volatile("" : "+v"(held));  // waited for here, not (with every DMA in flight) at each use
             }
         }
-        const int32_t slot = slot0 + lane % ROWS;
-        const uint32_t page = fast_quotient(static_cast<uint32_t>(slot), a.page);
-        Row r;
-        r.in_page = static_cast<uint32_t>(slot) - page * a.page.divisor;
-        const int32_t id = __shfl(held, static_cast<int>(page) - page0, 64);
-        r.id = slot < high && static_cast<uint32_t>(id) < a.pages ? id : -1;
+        r.id = -1;
+        r.in_page = 0;
+        // At the last rows and among entries without a page the lanes work on their own.
+        r.whole = even != 0 && holes == 0 && slot0 + ROWS <= high;
+        if (!r.whole) {
+            const int32_t slot = slot0 + lane % ROWS;
+            const uint32_t entry = fast_quotient(static_cast<uint32_t>(slot), page);
+            r.in_page = static_cast<uint32_t>(slot) - entry * page.divisor;
+            const int32_t id = __shfl(held, static_cast<int>(entry) - page0, 64);
+            r.id = slot < high && static_cast<uint32_t>(id) < pages ? id : -1;
+        }
         return r;
     }
 
-    template <typename V>
-    __device__ __forceinline__ static uint64_t address(const char *base, const V &c, const Row &r) {
-        const char *at = base + static_cast<int64_t>(r.id) * c.page_stride + static_cast<int64_t>(r.in_page) * c.slot_stride;
-        return reinterpret_cast<uint64_t>(r.id < 0 ? reinterpret_cast<const char *>(kZeroRow) : at);
-    }
-
-    // DMA this wave's rows, row0 .. of the tile, to LDS offset `to`.
     template <bool KEYS>
-    __device__ __forceinline__ static void load(uint64_t row, uint32_t to, int row0, uint32_t head_dim) {
+    __device__ __forceinline__ void load(const Rows &rows, uint32_t to, int first_row) const {
+        const uint64_t base = KEYS ? keys : values;
+        const uint32_t page_stride = KEYS ? key_page : value_page, slot_stride = KEYS ? key_slot : value_slot;
+        auto address = [&](int32_t id, uint32_t in_page) {
+            return base + ((static_cast<uint64_t>(static_cast<uint32_t>(id)) * page_stride +
+                            static_cast<uint64_t>(in_page) * slot_stride) << 4);
+        };
+        if (rows.whole) {
+#pragma unroll
+            for (int u = 0; u < kUnits; ++u) {
+                const uint32_t slot = rows.slot0 + u * kUnit, entry = fast_quotient(slot, page);
+                const uint32_t id = __builtin_amdgcn_readlane(held, entry - page0);
+                const uint64_t at = address(id, slot - entry * page.divisor);
+#pragma unroll
+                for (int i = 0; i < kUnitLoads; ++i)
+                    dma16_at(at, KEYS ? key_offset[u % kKinds][i] : value_offset[i], to + (u * kUnitLoads + i) * 1024);
+            }
+            return;
+        }
         const int lane = threadIdx.x % 64;
+        const uint64_t row = rows.id < 0 ? reinterpret_cast<uint64_t>(kZeroRow) : address(rows.id, rows.in_page);
         const int lo = static_cast<int>(row), hi = static_cast<int>(row >> 32);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int r = i * TL::kRowsPerLoad + lane / TL::kChunks;
             const uint64_t at = (static_cast<uint64_t>(static_cast<uint32_t>(__shfl(hi, r, 64))) << 32) |
                                 static_cast<uint32_t>(__shfl(lo, r, 64));
-            const int chunk = (lane % TL::kChunks) ^ (KEYS ? TL::key_turn(row0 + r) : TL::value_turn(row0 + r));
+            const int chunk = (lane % TL::kChunks) ^ (KEYS ? TL::key_turn(first_row + r) : TL::value_turn(r));
             const uint64_t src = chunk * 8 < static_cast<int>(head_dim) ? at + chunk * 16 : reinterpret_cast<uint64_t>(kZeroRow);
             dma16(reinterpret_cast<const char *>(src), to + i * 1024);
         }
     }
-
-    template <typename A>
-    __device__ __forceinline__ void load_keys(const A &a, const Row &r, uint32_t to, int row0) const {
-        load<true>(address(keys, a.keys, r), to, row0, a.head_dim);
+    __device__ __forceinline__ void load_keys(const Rows &rows, uint32_t to, int first_row) const {
+        load<true>(rows, to, first_row);
     }
-    template <typename A>
-    __device__ __forceinline__ void load_values(const A &a, const Row &r, uint32_t to, int row0) const {
-        load<false>(address(values, a.values, r), to, row0, a.head_dim);
-    }
-
-    // Both tiles' rows; keys at `to`, values at `to_values`.
-    template <typename A>
-    __device__ __forceinline__ void stage(const A &a, int32_t slot0, int32_t high, uint32_t to, uint32_t to_values,
-                                          int row0) {
-        const Row r = locate(a, slot0, high);
-        load_keys(a, r, to, row0);
-        load_values(a, r, to_values, row0);
-    }
+    __device__ __forceinline__ void load_values(const Rows &rows, uint32_t to) const { load<false>(rows, to, 0); }
 };
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));

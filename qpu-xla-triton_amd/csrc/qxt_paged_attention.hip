@@ -148,18 +148,37 @@ struct Core {
         special = false;
     }
 
+    // Operands are read a few products before their use: in this order in the source, since where scalar registers are
+    // short the compiler keeps the source's order, and by `ahead` where it reorders.
+    static constexpr int kKeysAhead = 6, kValuesAhead = 4;
+    // The surrounding block's LDS reads (READS a product) go AHEAD products before their use.
+    template <int PRODUCTS, int READS, int AHEAD>
+    __device__ __forceinline__ static void ahead() {
+        __builtin_amdgcn_sched_group_barrier(0x100, READS * AHEAD, 0);  // LDS reads
+#pragma unroll
+        for (int i = 0; i < PRODUCTS - AHEAD; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix instructions
+            __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+    }
+
     // s[kb][i]: logit of this lane's row with key 32 kb + 8 (i / 4) + 4 half + i % 4 of the tile.
     __device__ __forceinline__ void logits(const char *keys, f32x16 (&s)[KB]) const {
+        constexpr int kProducts = KB * kSteps, kAhead = kKeysAhead < kProducts ? kKeysAhead : kProducts;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) s[kb] = f32x16{};
+        frag k[kAhead];
 #pragma unroll
-        for (int c = 0; c < kSteps; ++c)
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-                const frag k = *reinterpret_cast<const frag *>(keys + kb * 32 * TL::kRowBytes + (key_at ^ (32 * c)));
-                s[kb] = M::run(k, q[c], s[kb]);
+        for (int i = 0; i < kProducts + kAhead; ++i) {
+            if (i >= kAhead) {
+                const int j = i - kAhead, kb = j % KB, c = j / KB;
+                s[kb] = M::run(k[j % kAhead], q[c], s[kb]);
             }
-        ahead<KB * kSteps, 1, kKeysAhead>();
+            if (i < kProducts)
+                k[i % kAhead] = *reinterpret_cast<const frag *>(keys + (i % KB) * 32 * TL::kRowBytes + (key_at ^ (32 * (i / KB))));
+        }
+        ahead<kProducts, 1, kAhead>();
     }
 
     __device__ __forceinline__ static void hide(f32x16 (&s)[KB], int32_t base, int half, const Range &mine) {
@@ -227,28 +246,17 @@ struct Core {
     }
 
     __device__ __forceinline__ void add_values(const char *values, const frag (&p)[KB][2]) {
+        constexpr int kProducts = KB * 2 * kCols, kAhead = kValuesAhead < kProducts ? kValuesAhead : kProducts;
+        uint4 v[kAhead];
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int d = 0; d < kCols; ++d)
-                    acc[d] = M::run(__builtin_bit_cast(frag, value_frag(values, kb, h, d)), p[kb][h], acc[d]);
-        ahead<KB * 2 * kCols, 2, kValuesAhead>();
-    }
-
-    // The compiler would wait for every operand read right before its product; this orders the surrounding block's
-    // LDS reads (READS a product) AHEAD products before their use.
-    static constexpr int kKeysAhead = 4, kValuesAhead = 4;
-    template <int PRODUCTS, int READS, int AHEAD>
-    __device__ __forceinline__ static void ahead() {
-        __builtin_amdgcn_sched_group_barrier(0x100, READS * AHEAD, 0);  // LDS reads
-#pragma unroll
-        for (int i = 0; i < PRODUCTS - AHEAD; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix instructions
-            __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+        for (int i = 0; i < kProducts + kAhead; ++i) {
+            if (i >= kAhead) {
+                const int j = i - kAhead, d = j % kCols, x = j / kCols;
+                acc[d] = M::run(__builtin_bit_cast(frag, v[j % kAhead]), p[x / 2][x % 2], acc[d]);
+            }
+            if (i < kProducts) v[i % kAhead] = value_frag(values, i / kCols / 2, i / kCols % 2, i % kCols);
         }
-        __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+        ahead<kProducts, 2, kAhead>();
     }
 
     // Have the queries arrive here: left to their first use, the compiler waits for all loads in flight at every step.
@@ -262,7 +270,7 @@ struct Core {
 struct RowTile {
     int32_t row, token, in_group;           // this lane's row (its last one repeated past the end)
     Range mine;
-    int32_t low, high;                      // any row of the workgroup's
+    int32_t low, high;                      // any row of the workgroup's (low rounded down)
     int32_t any_low, all_low, all_high, any_high;  // this wave's rows, any of them or all
     int32_t from, to;                       // steps of this split
 
@@ -273,7 +281,7 @@ struct RowTile {
         token = fast_quotient(min(row, rows - 1), a.group);
         in_group = min(row, rows - 1) - token * a.group.divisor;
         mine = seen_by(a, seq, token);
-        low = seen_by(a, seq, fast_quotient(tile * tile_rows, a.group)).low;
+        low = seen_by(a, seq, fast_quotient(tile * tile_rows, a.group)).low & ~7;  // whole units
         high = seen_by(a, seq, fast_quotient(min(rows, (tile + 1) * tile_rows) - 1, a.group)).high;
         any_low = __builtin_amdgcn_readlane(mine.low, 0);
         all_low = __builtin_amdgcn_readlane(mine.low, 31);
@@ -282,6 +290,11 @@ struct RowTile {
         const int32_t steps = (high - low + step - 1) / step, share = (steps + a.splits - 1) / a.splits;
         from = min<int32_t>(split * share, steps);
         to = min<int32_t>(from + share, steps);
+    }
+
+    // A step from slot `base` on may hold real slots that some row of the wave does not see.
+    __device__ __forceinline__ bool mixed(int32_t base) const {
+        return any_low != all_low || any_high != all_high || base < all_low || any_high != high;
     }
 };
 
@@ -419,7 +432,9 @@ __global__ __launch_bounds__(64 * WQ * WK, DP <= 128 ? 2 : 1) void paged_attenti
     const Sequence seq = sequence_of(a, at.b);
     const int32_t rows = seq.tokens * a.group.divisor, tiles = (rows + 32 * WQ - 1) / (32 * WQ);
     Stager<DP, S::kRows> stager;
-    stager.start(a, at.b, at.head);
+    stager.start(a, at.b, at.head, wq * S::kRows);
+    float scale2 = a.scale2;
+    keep(scale2);
     C core;
     core.place(lane);
     const char *const my_keys = lds + 2 * S::kTileBytes * wk;  // this key part's tiles of stage 0
@@ -434,7 +449,9 @@ __global__ __launch_bounds__(64 * WQ * WK, DP <= 128 ? 2 : 1) void paged_attenti
                    half, y.head_dim);
         auto stage = [&](int32_t t) {
             const uint32_t to = my_rows + (t & 1) * S::kStageBytes;
-            stager.stage(a, rt.low + t * S::kStep + wk * S::kKeys + wq * S::kRows, rt.high, to, to + S::kTileBytes, wq * S::kRows);
+            const auto staged = stager.locate(rt.low + t * S::kStep + wk * S::kKeys + wq * S::kRows, rt.high);
+            stager.load_keys(staged, to, wq * S::kRows);
+            stager.load_values(staged, to + S::kTileBytes);
         };
         auto compute = [&](int32_t t) {
             const int32_t base = rt.low + t * S::kStep + wk * S::kKeys;
@@ -445,8 +462,8 @@ __global__ __launch_bounds__(64 * WQ * WK, DP <= 128 ? 2 : 1) void paged_attenti
             core.logits(kt, s);
             const bool partial = base < rt.all_low || base + S::kKeys > rt.all_high;
             if (partial) C::hide(s, base, half, rt.mine);
-            core.weigh(s, a.scale2, p);
-            if (partial && (rt.any_low != rt.all_low || rt.any_high != rt.all_high)) core.inspect(vt);
+            core.weigh(s, scale2, p);
+            if (partial && rt.mixed(base)) core.inspect(vt);
             core.add_values(vt, p);
         };
         if constexpr (WQ == 1) {
@@ -541,10 +558,12 @@ __global__ __launch_bounds__(64 * WQ * WK, DP <= 128 ? 2 : 1) void paged_attenti
 // matrix cores (logits of step t, outputs of step t - 1), waves 4-7, on the same
 // SIMDs, turn their logits into weights on the vector unit, and at the next
 // barrier they change places; in step, both units idle in turns.
-// Three buffers each of keys and values: a wave stages its share of keys t + 2
-// and values t + 1 at the start of its matrix phase t, into buffers last read a
-// phase ago, and waits for them two phases later, before the barrier after which
-// the first wave reads them.
+// Three buffers each of keys and values, staged in the vector phases: in that of
+// step t the first four waves ask for keys t + 2 and values t + 1, the others,
+// whose vector phase t comes one phase later, for keys t + 3 and values t + 2;
+// all of these buffers were last read a phase or more before.  Each wave waits
+// for its share two phases on, before the barrier after which the first wave
+// reads it, with the loads of its next vector phase already under way.
 template <typename T, int DP>
 __global__ __launch_bounds__(512, 2) void paged_attention_long_kernel(PagedArgs) {
     constexpr int kKeys = 64, kWaveRows = kKeys / 8, kTileBytes = kKeys * DP * 2, kRing = 3;
@@ -560,7 +579,9 @@ __global__ __launch_bounds__(512, 2) void paged_attention_long_kernel(PagedArgs)
     const Sequence seq = sequence_of(a, at.b);
     const int32_t rows = seq.tokens * a.group.divisor, tiles = (rows + 255) / 256;
     St stager;
-    stager.start(a, at.b, at.head);
+    stager.start(a, at.b, at.head, wave * kWaveRows);
+    float scale2 = a.scale2;
+    keep(scale2);
     C core;
     core.place(lane);
     const uint32_t my_rows = lds_offset(lds) + wave * kWaveRows * Tile<DP>::kRowBytes;
@@ -573,22 +594,27 @@ __global__ __launch_bounds__(512, 2) void paged_attention_long_kernel(PagedArgs)
                        static_cast<int64_t>(at.head * y.group.divisor + rt.in_group) * y.query_head,
                    half, y.head_dim);
         const int32_t end = min(rt.high, rt.low + rt.to * kKeys);  // steps past the last stage rows of zeros
-        auto locate = [&](int32_t t) { return stager.locate(a, rt.low + t * kKeys + wave * kWaveRows, end); };
-        auto load_keys = [&](const typename St::Row &r, int place) {
-            stager.load_keys(a, r, my_rows + place * kTileBytes, wave * kWaveRows);
+        auto locate = [&](int32_t t) { return stager.locate(rt.low + t * kKeys + wave * kWaveRows, end); };
+        auto load_keys = [&](const typename St::Rows &r, int place) {
+            stager.load_keys(r, my_rows + place * kTileBytes, wave * kWaveRows);
         };
-        auto load_values = [&](const typename St::Row &r, int place) {
-            stager.load_values(a, r, my_rows + (kRing + place) * kTileBytes, wave * kWaveRows);
+        auto load_values = [&](const typename St::Rows &r, int place) {
+            stager.load_values(r, my_rows + (kRing + place) * kTileBytes);
         };
         auto shown = [&](int32_t t) {  // some row of this wave sees some slot of step t
             const int32_t base = rt.low + t * kKeys;
             return t >= rt.from && t < rt.to && base < rt.any_high && base + kKeys > rt.any_low;
         };
-        typename St::Row next = locate(rt.from);
+        typename St::Rows next = locate(rt.from);
         load_keys(next, 0);
         load_values(next, 0);
         next = locate(rt.from + 1);
         load_keys(next, 1);
+        if (second) {
+            load_values(next, 1);
+            next = locate(rt.from + 2);
+            load_keys(next, 2);
+        }
         core.hold_queries();
         landed<0>();
         meet();
@@ -599,12 +625,8 @@ __global__ __launch_bounds__(512, 2) void paged_attention_long_kernel(PagedArgs)
         int place = 0, before = kRing - 1;  // buffers of steps t and t - 1
         bool pending = false, ragged = false;  // step t - 1 has weights; its rows see different slots
         for (int32_t t = rt.from; t < rt.to; ++t) {
-            // Matrix phase: the buffers of keys t - 1 and values t - 2 are free.
+            // Matrix phase.
             const int after = place == kRing - 1 ? 0 : place + 1;
-            const typename St::Row third = locate(t + 2);
-            load_keys(third, before);
-            load_values(next, after);
-            next = third;
             const int32_t base = rt.low + t * kKeys;
             const bool live = shown(t);
             if (live) core.logits(lds + place * kTileBytes, s);
@@ -615,12 +637,16 @@ __global__ __launch_bounds__(512, 2) void paged_attention_long_kernel(PagedArgs)
             }
             if (second) landed<2 * St::kLoads>();
             meet();
-            // Vector phase.
+            // Vector phase.  Keys two (three) steps on take the buffer of keys t - 1 (t), values one less that of t - 2 (t - 1).
+            const typename St::Rows later = locate(t + (second ? 3 : 2));
+            load_keys(later, second ? place : before);
+            load_values(next, second ? before : after);
+            next = later;
             if (live) {
                 const bool partial = base < rt.all_low || base + kKeys > rt.all_high;
                 if (partial) C::hide(s, base, half, rt.mine);
-                core.weigh(s, a.scale2, p);
-                ragged = partial && (rt.any_low != rt.all_low || rt.any_high != rt.all_high);
+                core.weigh(s, scale2, p);
+                ragged = partial && rt.mixed(base);
             }
             pending = live;
             before = place;
@@ -751,6 +777,8 @@ int check_paged_cache(const char *name, const qxt_paged_cache *c, bool needs_val
         (needs_values &&
          (!aligned(c->values, 16) || !all_multiples(16, {c->value_page_stride, c->value_slot_stride, c->value_head_stride}))))
         return fail(QXT_INVALID_ARGUMENT, "%s: cache rows must be 16-byte aligned", name);
+    if ((c->key_page_stride | c->value_page_stride | c->key_slot_stride | c->value_slot_stride) >> 36)
+        return fail(QXT_INVALID_ARGUMENT, "%s: page or slot strides of 64 GiB or more", name);
     if (c->block_table_stride % 4 || !aligned(c->block_table, 4) || !aligned(c->context_lens, 4))
         return fail(QXT_INVALID_ARGUMENT, "%s: misaligned block table or lengths", name);
     return QXT_OK;
@@ -824,6 +852,9 @@ int qxt_paged_attention(const void *query, size_t query_token_stride, size_t que
     a.scale2 = static_cast<float>(scale * 1.4426950408889634);
     a.causal = causal;
     a.window = static_cast<int32_t>(window);
+    // Pages in whole units, 32-bit strides within a unit and a page table, head sizes without padding.
+    a.even = cache->page_size % 8 == 0 && cache->head_dim == (cache->head_dim <= 64 ? 64u : cache->head_dim <= 128 ? 128u : 256u) &&
+             std::max(cache->key_slot_stride, cache->value_slot_stride) < (1u << 27);
     a.tiles = p.tiles;
     a.splits = p.splits;
     a.out = static_cast<char *>(out);

@@ -192,6 +192,10 @@ def test_what_unused_slots_hold_does_not_matter(lens, dtype) -> None:
     ([(66, 30)], 2, 1, 256, 16, 0),     # 60 rows, wide
     ([(3000, 10)], 4, 1, 128, 16, 0),   # split
     ([(75, 25)], 4, 1, 128, 16, 30),    # 100 rows with a window
+    ([(90, 20)], 32, 1, 128, 16, 0),    # 640 rows: a wave's rows are one token's, the workgroup's are not
+    ([(90, 20)], 32, 1, 128, 16, 11),
+    ([(90, 20)], 32, 1, 64, 12, 11),    # pages that hold no whole units
+    ([(200, 8)], 32, 1, 64, 16, 50),
 ])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_infinite_and_nan_slots_reach_only_rows_that_see_them(case, dtype) -> None:
