@@ -20,7 +20,7 @@ struct PagedArgs {
     FastDiv group;  // query heads per key head
     float scale, scale2;  // scale2 = scale * log2(e)
     int32_t causal, window;
-    uint32_t even;   // units of eight slots lie in one page, at 32-bit strides, in rows of DP elements
+    uint32_t even;   // units of eight slots lie in one page, in rows of DP elements; keys and values at one distance
     uint32_t tiles, splits;  // grid: kv_heads x tiles x splits x sequences, kv_heads fastest
     char *out;
     int64_t out_token, out_head;
@@ -219,61 +219,74 @@ struct Stager {
 
     // The rows of slots slot0 .. slot0 + ROWS - 1 (those from `high` on are zeros).
     struct Rows {
-        int32_t slot0;
-        bool whole;       // wave-uniform: units by scalar addresses
-        int32_t id;       // else page id (or -1) and place in the page of this lane's row slot0 + lane % ROWS
+        int32_t whole;                           // wave-uniform: units by the addresses below
+        uint64_t at[kUnits];                     // (of keys; values lie at one distance from them)
+        int32_t id;                              // else page id (or -1) and place in the page of this lane's row
         uint32_t in_page;
     };
 
+    // Page ids of the entries from `first` on (the last one repeated).
+    __device__ __forceinline__ void fetch(int32_t first, int32_t high) {
+        page0 = first;
+        held = table[min(first + static_cast<int32_t>(threadIdx.x % 64), static_cast<int32_t>(fast_quotient(high - 1, page)))];
+        holes = __any(static_cast<uint32_t>(held) >= pages) ? 1 : 0;
+        asm volatile("" : "+v"(held));  // waited for here, not (with every DMA in flight) at each use
+    }
+    __device__ __forceinline__ static uint64_t address(uint64_t base, uint32_t page_stride, uint32_t slot_stride, uint32_t id,
+                                                       uint32_t in_page) {
+        return base + ((static_cast<uint64_t>(id) * page_stride + static_cast<uint64_t>(in_page) * slot_stride) << 4);
+    }
+
     __device__ __forceinline__ Rows locate(int32_t slot0, int32_t high) {
-        const int lane = threadIdx.x % 64;
         Rows r;
-        r.slot0 = slot0;
-        if (slot0 < high) {
-            const int32_t first = fast_quotient(slot0, page), last = fast_quotient(min(slot0 + ROWS, high) - 1, page);
-            if (first < page0 || last >= page0 + 64) {
-                page0 = first;
-                held = table[min(first + lane, static_cast<int32_t>(fast_quotient(high - 1, page)))];
-                holes = __any(static_cast<uint32_t>(held) >= pages) ? 1 : 0;
-                asm volatile("" : "+v"(held));  // waited for here, not (with every DMA in flight) at each use
-            }
-        }
         r.id = -1;
         r.in_page = 0;
-        // At the last rows and among entries without a page the lanes work on their own.
-        r.whole = even != 0 && holes == 0 && slot0 + ROWS <= high;
-        if (!r.whole) {
-            const int32_t slot = slot0 + lane % ROWS;
-            const uint32_t entry = fast_quotient(static_cast<uint32_t>(slot), page);
-            r.in_page = static_cast<uint32_t>(slot) - entry * page.divisor;
-            const int32_t id = __shfl(held, static_cast<int>(entry) - page0, 64);
-            r.id = slot < high && static_cast<uint32_t>(id) < pages ? id : -1;
+        r.whole = 0;
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) r.at[u] = 0;
+        if (even != 0 && slot0 + ROWS <= high) {
+            const int32_t last = fast_quotient(slot0 + ROWS - kUnit, page);
+            const int32_t first = kUnits > 1 ? static_cast<int32_t>(fast_quotient(slot0, page)) : last;
+            if (first < page0 || last >= page0 + 64) fetch(first, high);
+            if (holes == 0) {
+                r.whole = 1;
+#pragma unroll
+                for (int u = 0; u < kUnits; ++u) {
+                    const uint32_t slot = slot0 + u * kUnit, entry = fast_quotient(slot, page), in_page = slot - entry * page.divisor;
+                    const uint32_t id = __builtin_amdgcn_readlane(held, entry - page0);
+                    r.at[u] = keys + ((static_cast<uint64_t>(id) * key_page + in_page * key_slot) << 4);
+                }
+                return r;
+            }
         }
+        // At the last rows, in other pages and among entries without a page the lanes work on their own.
+        if (slot0 < high) {
+            const int32_t first = fast_quotient(slot0, page), last = fast_quotient(min(slot0 + ROWS, high) - 1, page);
+            if (first < page0 || last >= page0 + 64) fetch(first, high);
+        }
+        const int32_t slot = slot0 + static_cast<int32_t>(threadIdx.x % 64) % ROWS;
+        const uint32_t entry = fast_quotient(static_cast<uint32_t>(slot), page);
+        r.in_page = static_cast<uint32_t>(slot) - entry * page.divisor;
+        const int32_t id = __shfl(held, static_cast<int>(entry) - page0, 64);
+        r.id = slot < high && static_cast<uint32_t>(id) < pages ? id : -1;
         return r;
     }
 
     template <bool KEYS>
     __device__ __forceinline__ void load(const Rows &rows, uint32_t to, int first_row) const {
-        const uint64_t base = KEYS ? keys : values;
-        const uint32_t page_stride = KEYS ? key_page : value_page, slot_stride = KEYS ? key_slot : value_slot;
-        auto address = [&](int32_t id, uint32_t in_page) {
-            return base + ((static_cast<uint64_t>(static_cast<uint32_t>(id)) * page_stride +
-                            static_cast<uint64_t>(in_page) * slot_stride) << 4);
-        };
         if (rows.whole) {
 #pragma unroll
-            for (int u = 0; u < kUnits; ++u) {
-                const uint32_t slot = rows.slot0 + u * kUnit, entry = fast_quotient(slot, page);
-                const uint32_t id = __builtin_amdgcn_readlane(held, entry - page0);
-                const uint64_t at = address(id, slot - entry * page.divisor);
+            for (int u = 0; u < kUnits; ++u)
 #pragma unroll
                 for (int i = 0; i < kUnitLoads; ++i)
-                    dma16_at(at, KEYS ? key_offset[u % kKinds][i] : value_offset[i], to + (u * kUnitLoads + i) * 1024);
-            }
+                    dma16_at(KEYS ? rows.at[u] : rows.at[u] + (values - keys), KEYS ? key_offset[u % kKinds][i] : value_offset[i],
+                             to + (u * kUnitLoads + i) * 1024);
             return;
         }
         const int lane = threadIdx.x % 64;
-        const uint64_t row = rows.id < 0 ? reinterpret_cast<uint64_t>(kZeroRow) : address(rows.id, rows.in_page);
+        const uint64_t row = rows.id < 0 ? reinterpret_cast<uint64_t>(kZeroRow)
+                             : KEYS      ? address(keys, key_page, key_slot, rows.id, rows.in_page)
+                                         : address(values, value_page, value_slot, rows.id, rows.in_page);
         const int lo = static_cast<int>(row), hi = static_cast<int>(row >> 32);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {

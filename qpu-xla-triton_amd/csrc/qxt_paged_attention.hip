@@ -273,10 +273,12 @@ struct RowTile {
     int32_t low, high;                      // any row of the workgroup's (low rounded down)
     int32_t any_low, all_low, all_high, any_high;  // this wave's rows, any of them or all
     int32_t from, to;                       // steps of this split
+    int32_t tile;                           // its number, below 0: none
 
     template <typename A>
     __device__ __forceinline__ RowTile(const A &a, const Sequence &seq, int32_t tile, int tile_rows, int wave_row,
-                                       int32_t rows, uint32_t split, int step) {
+                                       int32_t rows, uint32_t split, int step)
+        : tile(tile) {
         row = tile * tile_rows + wave_row + threadIdx.x % 32;
         token = fast_quotient(min(row, rows - 1), a.group);
         in_group = min(row, rows - 1) - token * a.group.divisor;
@@ -575,24 +577,33 @@ __global__ __launch_bounds__(512, 2) void paged_attention_long_kernel(PagedArgs)
     Kernarg<PagedArgs> &a = *args;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), half = lane / 32;
     const bool second = wave >= 4;
-    const Place at(a);
-    const Sequence seq = sequence_of(a, at.b);
-    const int32_t rows = seq.tokens * a.group.divisor, tiles = (rows + 255) / 256;
     St stager;
-    stager.start(a, at.b, at.head, wave * kWaveRows);
+    {
+        const Place at(a);
+        stager.start(a, at.b, at.head, wave * kWaveRows);
+    }
     float scale2 = a.scale2;
     keep(scale2);
     C core;
     core.place(lane);
     const uint32_t my_rows = lds_offset(lds) + wave * kWaveRows * Tile<DP>::kRowBytes;
 
-    for (int32_t turn = at.tile; turn < tiles; turn += a.tiles) {
-        const int32_t tile = tiles - 1 - turn;  // the longest rows first: the last tiles of a causal sequence
+    for (int32_t round = 0;; ++round) {
+        // (Where the workgroup stands is worked out anew before and after the main loop.)
         Kernarg<PagedArgs> &y = *late(args);
-        const RowTile rt(y, seq, tile, 256, 32 * wave, rows, at.split, kKeys);
-        core.begin(y.query + (seq.start + rt.token) * y.query_token +
-                       static_cast<int64_t>(at.head * y.group.divisor + rt.in_group) * y.query_head,
-                   half, y.head_dim);
+        const RowTile rt = [&] {
+            const Place at(y);
+            const Sequence seq = sequence_of(y, at.b);
+            const int32_t rows = seq.tokens * y.group.divisor, tiles = (rows + 255) / 256;
+            const int32_t tile = tiles - 1 - static_cast<int32_t>(at.tile) - round * static_cast<int32_t>(y.tiles);
+            RowTile r(y, seq, tile, 256, 32 * wave, rows, at.split, kKeys);
+            if (tile >= 0)
+                core.begin(y.query + (seq.start + r.token) * y.query_token +
+                               static_cast<int64_t>(at.head * y.group.divisor + r.in_group) * y.query_head,
+                           half, y.head_dim);
+            return r;
+        }();
+        if (rt.tile < 0) break;
         const int32_t end = min(rt.high, rt.low + rt.to * kKeys);  // steps past the last stage rows of zeros
         auto locate = [&](int32_t t) { return stager.locate(rt.low + t * kKeys + wave * kWaveRows, end); };
         auto load_keys = [&](const typename St::Rows &r, int place) {
@@ -623,7 +634,7 @@ __global__ __launch_bounds__(512, 2) void paged_attention_long_kernel(PagedArgs)
         f32x16 s[kKeys / 32];
         frag p[kKeys / 32][2];
         int place = 0, before = kRing - 1;  // buffers of steps t and t - 1
-        bool pending = false, ragged = false;  // step t - 1 has weights; its rows see different slots
+        int32_t pending = 0, ragged = 0;  // step t - 1 has weights; its rows see different slots
         for (int32_t t = rt.from; t < rt.to; ++t) {
             // Matrix phase.
             const int after = place == kRing - 1 ? 0 : place + 1;
@@ -646,9 +657,9 @@ __global__ __launch_bounds__(512, 2) void paged_attention_long_kernel(PagedArgs)
                 const bool partial = base < rt.all_low || base + kKeys > rt.all_high;
                 if (partial) C::hide(s, base, half, rt.mine);
                 core.weigh(s, scale2, p);
-                ragged = partial && rt.mixed(base);
+                ragged = partial && rt.mixed(base) ? 1 : 0;
             }
-            pending = live;
+            pending = live ? 1 : 0;
             before = place;
             place = after;
             if (!second) landed<2 * St::kLoads>();
@@ -662,38 +673,68 @@ __global__ __launch_bounds__(512, 2) void paged_attention_long_kernel(PagedArgs)
         if (!second) meet();
         landed<0>();
         Kernarg<PagedArgs> &z = *late(args);
-        put_rows<T, DP>(z, seq, at.b, at.head, at.split, rt, rows, kKeys, core);
+        const Place at(z);
+        const Sequence seq = sequence_of(z, at.b);
+        put_rows<T, DP>(z, seq, at.b, at.head, at.split, rt, seq.tokens * z.group.divisor, kKeys, core);
         __syncthreads();  // before the next tile's staging
     }
 }
 
-// Join the parts of rows whose slots were split over workgroups: a wave a row,
-// four elements a lane.
+// Join the parts of rows whose slots were split over workgroups.  LANES lanes a
+// row, four elements each; the row's sums are read at once, the parts with four
+// in flight (read one after another, eight parts took 7 us at any size).
+template <int LANES>
 __global__ __launch_bounds__(256) void paged_attention_join_kernel(PagedArgs a) {
     const uint32_t heads = a.kv_heads * a.group.divisor;
-    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * 4 + threadIdx.x / 64;
+    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
     const uint64_t rows = static_cast<uint64_t>(a.tokens) * heads;
-    if (row >= rows) return;
+    if (row >= rows) return;  // whole groups of LANES leave together
     const int64_t token = row / heads, head = row - token * heads;
     if (a.starts != nullptr && (token < a.starts[0] || token >= a.starts[a.sequences])) return;  // nobody's row
-    const int lane = threadIdx.x % 64;
-    float top = kNone;
-    for (uint32_t s = lane; s < a.splits; s += 64) top = fmaxf(top, a.part_sum[s * rows + row].x);
-    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-    float total = 0.0f;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    const uint32_t lane = threadIdx.x % LANES;
     const int e = 4 * lane;
-    for (uint32_t s = 0; s < a.splits; ++s) {
-        const float2 part = a.part_sum[s * rows + row];
-        if (part.y == 0.0f) continue;
-        const float f = part.x == kNone ? 1.0f : __builtin_amdgcn_exp2f(part.x - top);
-        total += part.y * f;
-        if (e < static_cast<int>(a.head_dim)) {
-            const float4 y = *reinterpret_cast<const float4 *>(a.part_out + (s * rows + row) * a.head_dim + e);
-            x.x += y.x * f;
-            x.y += y.y * f;
-            x.z += y.z * f;
-            x.w += y.w * f;
+    float top = kNone, total = 0.0f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t s0 = 0; s0 < a.splits; s0 += LANES) {
+        // This round's parts: their sums in the lanes, their common maximum.
+        const uint32_t count = min<uint32_t>(LANES, a.splits - s0);
+        float2 mine = make_float2(kNone, 0.0f);
+        if (lane < count) mine = a.part_sum[(s0 + lane) * rows + row];
+        float most = mine.x;
+#pragma unroll
+        for (int off = LANES / 2; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor(most, off, LANES));
+        const float next = fmaxf(top, most), back = top == kNone ? 0.0f : __builtin_amdgcn_exp2f(top - next);
+        if (s0 > 0) {
+            const float old = next == kNone ? 1.0f : back;
+            total *= old;
+            x.x *= old;
+            x.y *= old;
+            x.z *= old;
+            x.w *= old;
+        }
+        top = next;
+        // A part without a maximum is empty (sum 0, no outputs written), or NaN throughout.
+        const float factor = mine.y == 0.0f ? 0.0f : mine.x == kNone ? 1.0f : __builtin_amdgcn_exp2f(mine.x - top);
+        for (uint32_t s1 = 0; s1 < count; s1 += 4) {
+            float4 y[4];
+            float f[4];
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {
+                const uint32_t s = min(s1 + k, count - 1);
+                const float sum = __shfl(mine.y, s, LANES);
+                f[k] = s1 + k < count ? __shfl(factor, s, LANES) : 0.0f;
+                total += s1 + k < count && sum != 0.0f ? sum * f[k] : 0.0f;
+                y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (s1 + k < count && sum != 0.0f && e < static_cast<int>(a.head_dim))
+                    y[k] = *reinterpret_cast<const float4 *>(a.part_out + ((s0 + s) * rows + row) * a.head_dim + e);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                x.x += y[k].x * f[k];
+                x.y += y[k].y * f[k];
+                x.z += y[k].z * f[k];
+                x.w += y[k].w * f[k];
+            }
         }
     }
     if (lane == 0 && a.lse != nullptr) a.lse[token * a.lse_token + head] = lse_of(top, total);
@@ -709,8 +750,14 @@ struct Plan {
 };
 
 // Waves by the rows that share a key head (new tokens of the longest chunk
-// times heads of a group), then workgroups until the chip has work: the slots
-// of each row tile are split when tiles, heads and sequences alone are fewer.
+// times heads of a group).  A CU holds one workgroup of most shapes, so the slots
+// of each row tile are split while tiles, heads and sequences alone leave CUs
+// idle, up to one workgroup a CU, each with two steps at least (four of the long
+// shapes).  Measured, main kernel and join: a 512-token chunk over 32k slots (64
+// workgroups) 848 us whole, 455 in two, 281 in four, 301 in eight; one TinyLlama
+// token over 1900 slots (4) 16.7 us whole, 11.6 in four, 10.1 in eight.  Of few
+// rows, whose contexts differ most, eight workgroups a CU even out: 64 sequences
+// of 3k to 16k slots (512 workgroups) 506 us whole, 463 in four, 481 in eight.
 Plan plan_of(uint32_t head_dim, uint32_t group, uint32_t kv_heads, uint32_t sequences, uint32_t tokens,
              uint32_t max_query, uint32_t max_context) {
     const uint64_t rows = static_cast<uint64_t>(std::max(1u, std::min(max_query, tokens))) * group;
@@ -719,11 +766,18 @@ Plan plan_of(uint32_t head_dim, uint32_t group, uint32_t kv_heads, uint32_t sequ
     p.wq = rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 || wide ? 4 : 8;
     p.wk = p.wq == 1 ? (wide ? 2 : 4) : p.wq == 2 ? (wide ? 1 : 2) : 1;
     p.tiles = static_cast<uint32_t>((rows + 32 * p.wq - 1) / (32 * p.wq));
-    const uint64_t base = static_cast<uint64_t>(p.tiles) * kv_heads * sequences;
-    const uint64_t wanted = 2ull * compute_units();
+    const uint64_t base = static_cast<uint64_t>(p.tiles) * kv_heads * sequences, cus = compute_units();
     const uint32_t step = (p.wq >= 4 && !wide ? 64 : 32) * p.wk;
-    const uint64_t most = std::max<uint64_t>(1, max_context / (4 * step));  // four steps a split at least
-    p.splits = static_cast<uint32_t>(std::min<uint64_t>({(wanted + base - 1) / base, most, 256}));
+    uint64_t splits = 1;
+    if (2 * base <= cus)
+        splits = cus / base;
+    else if (p.wq <= 2)
+        splits = std::min<uint64_t>((8 * cus + base - 1) / base, 8);
+    else if (base < 2 * cus)
+        for (uint64_t s = 2; s <= 4; ++s)  // rounds of workgroups per part
+            if ((base * s + cus - 1) / cus * splits < (base * splits + cus - 1) / cus * s) splits = s;
+    const uint64_t most = std::max<uint64_t>(1, max_context / ((p.wq <= 2 ? 2 : 4) * step));
+    p.splits = static_cast<uint32_t>(std::min<uint64_t>({splits, most, 64}));
     return p;
 }
 
@@ -852,9 +906,12 @@ int qxt_paged_attention(const void *query, size_t query_token_stride, size_t que
     a.scale2 = static_cast<float>(scale * 1.4426950408889634);
     a.causal = causal;
     a.window = static_cast<int32_t>(window);
-    // Pages in whole units, 32-bit strides within a unit and a page table, head sizes without padding.
-    a.even = cache->page_size % 8 == 0 && cache->head_dim == (cache->head_dim <= 64 ? 64u : cache->head_dim <= 128 ? 128u : 256u) &&
-             std::max(cache->key_slot_stride, cache->value_slot_stride) < (1u << 27);
+    // Pages in whole units; one layout of keys and values, whose places in a page 32 bits (of 16 bytes) hold; head
+    // sizes without padding.
+    const uint32_t dim = cache->head_dim <= 64 ? 64 : cache->head_dim <= 128 ? 128 : 256;
+    a.even = cache->page_size % 8 == 0 && cache->head_dim == dim && cache->key_page_stride == cache->value_page_stride &&
+             cache->key_slot_stride == cache->value_slot_stride && cache->key_slot_stride < (1u << 28) &&
+             static_cast<uint64_t>(cache->page_size) * (cache->key_slot_stride / 16) <= UINT32_MAX;
     a.tiles = p.tiles;
     a.splits = p.splits;
     a.out = static_cast<char *>(out);
@@ -872,8 +929,13 @@ int qxt_paged_attention(const void *query, size_t query_token_stride, size_t que
                        : launch_attention_dim<f16_t>(a, p, static_cast<uint32_t>(grid), as_stream(stream));
     if (rc != QXT_OK || p.splits == 1) return rc;
     const uint64_t rows = static_cast<uint64_t>(tokens) * query_heads;
-    return launch("paged_attention_join_kernel", paged_attention_join_kernel, dim3(static_cast<uint32_t>((rows + 3) / 4)),
-                  dim3(256), 0, as_stream(stream), a);
+    auto join = [&](auto kernel, uint32_t lanes) {
+        return launch("paged_attention_join_kernel", kernel, dim3(static_cast<uint32_t>((rows * lanes + 255) / 256)), dim3(256), 0,
+                      as_stream(stream), a);
+    };
+    if (cache->head_dim <= 64) return join(paged_attention_join_kernel<16>, 16);
+    if (cache->head_dim <= 128) return join(paged_attention_join_kernel<32>, 32);
+    return join(paged_attention_join_kernel<64>, 64);
 }
 
 }  // extern "C"
