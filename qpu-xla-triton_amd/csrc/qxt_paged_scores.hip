@@ -233,7 +233,7 @@ __global__ __launch_bounds__(64 * kScoreWaves, DP <= 128 ? 2 : 1) void paged_sco
 // own, `run` slots each (at most kRun).  Keys go through a ring of tiles in LDS:
 // a lane that fetched its own key's row straight into registers would touch
 // every cache line four times, and more lines are in flight than L1 holds (92 us
-// over 215 MB of keys, this way 45).  Totals wait in LDS until the run is done, so
+// over 215 MB of keys, this way 57).  Totals wait in LDS until the run is done, so
 // that no wait for a score to add to drains the ring.
 constexpr int kRun = 1024;
 template <int DP>
@@ -286,20 +286,25 @@ __global__ __launch_bounds__(64 * kScoreWaves, 1) void paged_scores_few_kernel(S
                 if (16 * c + 8 * half < head_dim) q[c] = *reinterpret_cast<const frag *>(query + (16 * c + 8 * half) * 2);
         }
         float lse[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {  // all asked for at once, before any is looked at
+            lse[i] = 0.0f;
+            if (rows > 0) {
+                const int32_t r = min(row0 + 8 * (i / 4) + 4 * half + i % 4, rows - 1);
+                const int32_t t = fast_quotient(static_cast<uint32_t>(r), a.group);
+                lse[i] = a.lse[(seq.start + t) * a.lse_token + static_cast<int64_t>(head) * group + (r - t * group)];
+            }
+        }
         uint32_t counts = 0;
         int32_t all_low = 0, all_high = INT32_MAX;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const int32_t r = row0 + 8 * (i / 4) + 4 * half + i % 4;
-            lse[i] = 0.0f;
-            if (r >= rows) continue;
-            const int32_t t = fast_quotient(static_cast<uint32_t>(r), a.group);
-            lse[i] = a.lse[(seq.start + t) * a.lse_token + static_cast<int64_t>(head) * group + (r - t * group)];
-            const Range sees = seen_by(a, seq, t);
-            if (lse[i] == -__builtin_inff() || sees.high == 0) continue;
-            counts |= 1u << i;
-            all_low = max(all_low, sees.low);
-            all_high = min(all_high, sees.high);
+            const Range sees = seen_by(a, seq, fast_quotient(static_cast<uint32_t>(min(r, max(rows - 1, 0))), a.group));
+            const bool one = r < rows && lse[i] != -__builtin_inff() && sees.high > 0;
+            counts |= one ? 1u << i : 0u;
+            all_low = max(all_low, one ? sees.low : 0);
+            all_high = min(all_high, one ? sees.high : INT32_MAX);
         }
         all_low = __builtin_amdgcn_readfirstlane(max(all_low, __shfl_xor(all_low, 32, 64)));
         all_high = __builtin_amdgcn_readfirstlane(min(all_high, __shfl_xor(all_high, 32, 64)));
@@ -391,9 +396,10 @@ ScorePlan score_plan(uint32_t group, uint32_t kv_heads, uint32_t sequences, uint
     const uint64_t rows = static_cast<uint64_t>(std::min(max_query, tokens)) * group, cus = compute_units();
     p.splits = 1;
     if (rows <= 32) {
-        // Eight waves a CU, of 64 slots at least.
+        // One workgroup a CU where sequences are alike, waves of 64 slots at least (16 sequences of 4k to 8k slots:
+        // 56 us, with two 61, with four 68).
         const uint64_t all = static_cast<uint64_t>(std::max(1u, max_context)) * kv_heads * sequences;
-        p.run = static_cast<int32_t>(std::min<uint64_t>(kRun, std::max<uint64_t>(64, (all / (8 * cus) + 63) / 64 * 64)));
+        p.run = static_cast<int32_t>(std::min<uint64_t>(kRun, std::max<uint64_t>(64, (all / (4 * cus) + 63) / 64 * 64)));
         p.tiles = std::max<uint32_t>(1, static_cast<uint32_t>((max_context + static_cast<uint64_t>(p.run) * kScoreWaves - 1) /
                                                               (static_cast<uint64_t>(p.run) * kScoreWaves)));
         return p;

@@ -51,6 +51,7 @@ def _check(problem, budget, recent, **options):
 @pytest.mark.parametrize("lens,budget,recent", [
     ([65], 64, 8), ([300, 64, 20, 0, 1], 64, 64), ([257, 130, 129], 128, 0), ([1000], 1, 0), ([1000], 1, 1), ([2], 1, 1),
     ([1000, 999, 513], 512, 100), ([100, 90], 99, 10), ([100], 200, 10), ([4097, 5000], 4096, 512),
+    ([68, 67, 66], 64, 62), ([5, 4, 3], 2, 1), ([132, 131, 130, 129], 128, 3),  # a few over: one launch, slot by slot
 ])
 @pytest.mark.parametrize("ties", [False, True])
 def test_against_the_definition(lens, budget, recent, ties) -> None:
