@@ -50,6 +50,8 @@ SOURCE_FLAGS = {
     "qxt_q4_0_tiled.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "qxt_q4_0.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "qxt_q4_0_rows.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "qxt_paged_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "qxt_paged_scores.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 
