@@ -36,6 +36,17 @@ def empty_for(stream: Any, shape: tuple[int, ...], dtype: torch.dtype, device: t
     return tensor
 
 
+def like_for(stream: Any, t: torch.Tensor, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``empty_for`` of a tensor's shape, type (or ``dtype``) and device (a third of its time on the current stream)."""
+    if stream is None:
+        return torch.empty_like(t) if dtype is None or dtype is t.dtype else torch.empty_like(t, dtype=dtype)
+    return empty_for(stream, t.shape, t.dtype if dtype is None else dtype, t.device)
+
+
+def workspace_for(stream: Any, size: int, device: torch.device) -> torch.Tensor | None:
+    return empty_for(stream, (size,), torch.uint8, device) if size else None
+
+
 def require_one_gpu(name: str, first: torch.Tensor, *others: torch.Tensor | None) -> None:
     index = first.get_device()
     for t in others:
@@ -102,7 +113,7 @@ def dense_last(t: torch.Tensor) -> bool:
 
 
 def check_index(name: str, what: str, t: torch.Tensor, dtype: torch.dtype, count: int) -> None:
-    if t.dtype is not dtype or t.shape != (count,) or not t.is_contiguous():
+    if t.dtype is not dtype or t.dim() != 1 or t.numel() != count or not t.is_contiguous():
         raise ValueError(f"{name}: {what} must be contiguous {str(dtype).removeprefix('torch.')} [{count}]")
 
 

@@ -29,9 +29,11 @@ from qpu_xla_amd._paged import (
     check_size,
     empty_for,
     head_rows,
+    like_for,
     paged_cache,
     per_slot,
     require_one_gpu,
+    workspace_for,
 )
 from qpu_xla_amd._tensors import ptr, stream_handle
 from qpu_xla_amd.errors import KernelError
@@ -102,7 +104,7 @@ def paged_attention(
     scale, window, max_query, max_context = _sizes(name, shape, slots, query_starts, scale, window, max_query, max_context)
     tokens, query_heads, head_dim = shape
     if out is None:
-        out = empty_for(stream, shape, query.dtype, query.device)
+        out = like_for(stream, query)
     out_shape, out_code, *out_strides = head_rows(name, "out", out)
     if out_shape != shape:
         raise ValueError(f"{name}: out must have the query's shape")
@@ -112,7 +114,7 @@ def paged_attention(
         return out
     size = (_lib._lib or _lib.load()).qxt_paged_attention_workspace(query_heads, heads, head_dim, sequences, tokens,
                                                                     max_query, max_context)
-    workspace = empty_for(stream, (size,), torch.uint8, query.device) if size else None
+    workspace = workspace_for(stream, size, query.device)
     _lib.call(
         "qxt_paged_attention", query.data_ptr(), *strides, cache, ptr(query_starts), out.data_ptr(), *out_strides, out_code,
         ptr(lse), lse_stride, tokens, query_heads, scale, 1 if causal else 0, window, max_query, max_context,
@@ -152,14 +154,14 @@ def paged_attention_scores(
     scores_shape = (sequences, heads, slots)
     before = (0, 0) if scores is None else per_slot(name, "scores", scores, torch.float32, scores_shape)
     if out is None:
-        out = empty_for(stream, scores_shape, torch.float32, query.device)
+        out = empty_for(stream, scores_shape, torch.float32, query.device) if scores is None else like_for(stream, scores)
     after = per_slot(name, "out", out, torch.float32, scores_shape)
     require_one_gpu(name, query, key_cache, block_table, context_lens, lse, query_starts, scores, out)
     if sequences == 0:
         return out
     size = (_lib._lib or _lib.load()).qxt_paged_attention_scores_workspace(query_heads, heads, sequences, tokens, slots,
                                                                            max_query, max_context)
-    workspace = empty_for(stream, (size,), torch.uint8, query.device) if size else None
+    workspace = workspace_for(stream, size, query.device)
     _lib.call(
         "qxt_paged_attention_scores", query.data_ptr(), *strides, cache, ptr(query_starts), lse.data_ptr(), lse_stride,
         ptr(scores), *before, out.data_ptr(), *after, tokens, query_heads, scale, 1 if causal else 0, window, max_query,

@@ -20,7 +20,7 @@ from typing import Any
 import torch
 
 from qpu_xla_amd import _lib
-from qpu_xla_amd._paged import check_index, check_size, empty_for, paged_cache, per_slot, require_one_gpu
+from qpu_xla_amd._paged import check_index, check_size, like_for, paged_cache, per_slot, require_one_gpu, workspace_for
 from qpu_xla_amd._tensors import stream_handle
 from qpu_xla_amd.errors import KernelError
 from qpu_xla_amd.kernel import Kernel
@@ -58,13 +58,12 @@ def paged_cache_evict(
     slots = width * page_size
     max_context = slots if max_context is None else min(slots, check_size(name, "max_context", max_context))
     shape = (sequences, heads, slots)
-    device = key_cache.device
     if scores_out is None:
-        scores_out = empty_for(stream, shape, torch.float32, device)
+        scores_out = like_for(stream, scores)
     if positions_out is None:
-        positions_out = empty_for(stream, shape, torch.int32, device)
+        positions_out = like_for(stream, positions)
     if lens_out is None:
-        lens_out = empty_for(stream, (sequences,), torch.int32, device)
+        lens_out = like_for(stream, context_lens)
     else:
         check_index(name, "lens_out", lens_out, torch.int32, sequences)
     strides = [per_slot(name, what, t, dtype, shape)
@@ -75,7 +74,7 @@ def paged_cache_evict(
     if sequences == 0:
         return lens_out, scores_out, positions_out
     size = (_lib._lib or _lib.load()).qxt_paged_cache_evict_workspace(heads, sequences, slots, budget)
-    workspace = empty_for(stream, (size,), torch.uint8, device)
+    workspace = workspace_for(stream, size, key_cache.device)
     _lib.call(
         "qxt_paged_cache_evict", cache, scores.data_ptr(), *strides[0], scores_out.data_ptr(), *strides[1],
         positions.data_ptr(), *strides[2], positions_out.data_ptr(), *strides[3], lens_out.data_ptr(), budget, recent,

@@ -22,7 +22,7 @@ from typing import Any
 import torch
 
 from qpu_xla_amd import _lib
-from qpu_xla_amd._paged import check_index, empty_for, head_rows, paged_cache, require_one_gpu
+from qpu_xla_amd._paged import check_index, head_rows, like_for, paged_cache, require_one_gpu
 from qpu_xla_amd._tensors import ptr, stream_handle
 from qpu_xla_amd.errors import KernelError
 from qpu_xla_amd.kernel import Kernel
@@ -72,9 +72,9 @@ def qk_norm_rope(
     tokens, query_heads, head_dim = shape
     rows, half = _check_tables(name, tokens, head_dim, cos, sin, positions, query_weight, key_weight)
     if query_out is None:
-        query_out = empty_for(stream, shape, query.dtype if key_out is None else key_out.dtype, query.device)
+        query_out = like_for(stream, query, None if key_out is None else key_out.dtype)
     if key_out is None:
-        key_out = empty_for(stream, key_shape, query_out.dtype, query.device)
+        key_out = like_for(stream, key, query_out.dtype)
     query_out_shape, out_code, *query_out_strides = head_rows(name, "query_out", query_out)
     key_out_shape, key_code, *key_out_strides = head_rows(name, "key_out", key_out)
     if query_out_shape != shape or key_out_shape != key_shape or out_code != key_code:
@@ -121,7 +121,7 @@ def qk_norm_rope_cache(
         raise ValueError(f"{name}: the cache must hold the keys' heads and head size")
     check_index(name, "slots", slots, torch.int64, tokens)
     if query_out is None:
-        query_out = empty_for(stream, shape, key_cache.dtype, query.device)
+        query_out = like_for(stream, query, key_cache.dtype)
     out_shape, out_code, *out_strides = head_rows(name, "query_out", query_out)
     if out_shape != shape or out_code != cache_code:
         raise ValueError(f"{name}: query_out must have the query's shape and the cache's type")
