@@ -420,6 +420,10 @@ struct Shape {
 };
 
 // Two waves a SIMD (256 registers each) up to 128 elements of head size, one above.
+// Measured: one token for each of 64 sequences of 3k to 16k slots (2.6 GB of keys
+// and values, heads of 128) 464 us, 5.5 TB/s: bound by memory.  Seven chunks of 1
+// to 300 tokens with a window, heads of 256: 62 us for 17.5 GFLOP, matrix units
+// 23 % busy, vector units 25 %: with one wave a SIMD nothing covers its waits.
 template <typename T, int DP, int WQ, int WK>
 __global__ __launch_bounds__(64 * WQ * WK, DP <= 128 ? 2 : 1) void paged_attention_kernel(PagedArgs) {
     Kernarg<PagedArgs> *const args = kernargs<PagedArgs>();
@@ -566,6 +570,11 @@ __global__ __launch_bounds__(64 * WQ * WK, DP <= 128 ? 2 : 1) void paged_attenti
 // all of these buffers were last read a phase or more before.  Each wave waits
 // for its share two phases on, before the barrier after which the first wave
 // reads it, with the loads of its next vector phase already under way.
+// Measured: 8192 new tokens, 32 heads of 128 over 8 key heads, causal, 577 us
+// (0.95 PFLOP/s; a library product of two 8192 x 8192 matrices 1.37); in step
+// 651 us; the DMA issued in the matrix phases instead 653.  Bound by the vector
+// phases, about 2000 cycles a step against 1350 of matrix work: half of them the
+// softmax, the rest page look-ups, addresses and DMA issue of the staging.
 template <typename T, int DP>
 __global__ __launch_bounds__(512, 2) void paged_attention_long_kernel(PagedArgs) {
     constexpr int kKeys = 64, kWaveRows = kKeys / 8, kTileBytes = kKeys * DP * 2, kRing = 3;

@@ -13,6 +13,9 @@
 // budget-th largest; ties at it go to the lowest slots by a scan in slot order.
 // One workgroup does that for a (sequence, head); a second launch over all of
 // them moves the rows.
+// Measured: 32k slots to 4k for 32 (sequence, head) pairs 55 us to select
+// (32 of 256 CUs work, their vector units 52 % busy with the passes over the
+// keys), and 20 to move, near the rate of a copy; one slot over for 256 pairs 8 us.
 #include <algorithm>
 
 #include "qxt_paged.h"
