@@ -225,7 +225,10 @@ struct Stager {
         uint32_t in_page;
     };
 
-    // Page ids of the entries from `first` on (the last one repeated).
+    // Before a tile whose `high` may be larger than the one before: what is held repeats the last entry below the old one.
+    __device__ __forceinline__ void forget() { page0 = -64; }
+
+    // Page ids of the entries from `first` on (the last one below `high` repeated: right while `high` does not grow).
     __device__ __forceinline__ void fetch(int32_t first, int32_t high) {
         page0 = first;
         held = table[min(first + static_cast<int32_t>(threadIdx.x % 64), static_cast<int32_t>(fast_quotient(high - 1, page)))];

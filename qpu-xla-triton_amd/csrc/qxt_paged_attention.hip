@@ -615,6 +615,7 @@ __global__ __launch_bounds__(512, 2) void paged_attention_long_kernel(PagedArgs)
         }();
         if (rt.tile < 0) break;
         const int32_t end = min(rt.high, rt.low + rt.to * kKeys);  // steps past the last stage rows of zeros
+        stager.forget();  // (with a window a later tile's share of the slots may end above an earlier one's)
         auto locate = [&](int32_t t) { return stager.locate(rt.low + t * kKeys + wave * kWaveRows, end); };
         auto load_keys = [&](const typename St::Rows &r, int place) {
             stager.load_keys(r, my_rows + place * kTileBytes, wave * kWaveRows);
