@@ -192,19 +192,24 @@ __global__ __launch_bounds__(64 * kScoreWaves, DP <= 128 ? 2 : 1) void paged_sco
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int at = 32 * rb + 8 * i + 4 * half;
-                        const float4 l = *reinterpret_cast<const float4 *>(&row_lse[buffer][at]);
-                        const float *ls = &l.x;
+                        float4 l = *reinterpret_cast<const float4 *>(&row_lse[buffer][at]);
+                        float *ls = &l.x;
                         if (partial) {
+                            // (A NaN log-sum goes into the logits of what its row sees: -inf minus NaN would not hide the rest.)
                             const int4 lo = *reinterpret_cast<const int4 *>(&row_low[buffer][at]);
                             const int4 hi = *reinterpret_cast<const int4 *>(&row_high[buffer][at]);
                             const int32_t *los = &lo.x, *his = &hi.x;
 #pragma unroll
-                            for (int kb = 0; kb < 2; ++kb)
+                            for (int e = 0; e < 4; ++e) {
+                                const bool none = ls[e] != ls[e];
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) {
+                                for (int kb = 0; kb < 2; ++kb) {
                                     const int32_t slot = mine0 + 32 * kb + col;
-                                    if (slot < los[e] || slot >= his[e]) s[kb][4 * i + e] = -__builtin_inff();
+                                    const float logit = none ? ls[e] : s[kb][4 * i + e];
+                                    s[kb][4 * i + e] = slot < los[e] || slot >= his[e] ? -__builtin_inff() : logit;
                                 }
+                                ls[e] = none ? 0.0f : ls[e];
+                            }
                         }
 #pragma unroll
                         for (int kb = 0; kb < 2; ++kb)
@@ -341,12 +346,13 @@ __global__ __launch_bounds__(64 * kScoreWaves, 1) void paged_scores_few_kernel(S
                     reads_done();
                     stage(t + F::kRing);
                 }
+                uint32_t enter = counts;  // rows whose weights enter (left out is the weight: the log-sum may be NaN)
                 if (base < all_low || base + 32 > all_high) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int32_t r = min(row0 + 8 * (i / 4) + 4 * half + i % 4, rows - 1);
                         const Range sees = seen_by(a, seq, fast_quotient(static_cast<uint32_t>(r), a.group));
-                        if (slot < sees.low || slot >= sees.high) s[i] = -__builtin_inff();
+                        if (slot < sees.low || slot >= sees.high) enter &= ~(1u << i);
                     }
                 }
                 float total = 0.0f;
@@ -354,7 +360,7 @@ __global__ __launch_bounds__(64 * kScoreWaves, 1) void paged_scores_few_kernel(S
                 for (int i = 0; i < 16; ++i) {
                     // The difference first: its rounding, not the log-sum's, bounds the weight's error.
                     const float w = __builtin_amdgcn_exp2f(fmaf(s[i], scale, -lse[i]) * kLog2e);
-                    total += counts >> i & 1 ? w : 0.0f;
+                    total += enter >> i & 1 ? w : 0.0f;
                 }
                 total = add_halves(total);
                 if (half == 0) totals[32 * t + col] = total;
