@@ -448,7 +448,8 @@ size_t qxt_paged_attention_scores_workspace(uint32_t query_heads, uint32_t kv_he
                                             uint32_t slots, uint32_t max_query, uint32_t max_context) {
     if (kv_heads == 0 || query_heads == 0 || query_heads % kv_heads || sequences == 0) return 0;
     return qxt::score_workspace(
-        qxt::score_plan(query_heads / kv_heads, kv_heads, sequences, tokens, max_query, max_context), sequences, kv_heads, slots);
+        qxt::score_plan(query_heads / kv_heads, kv_heads, sequences, tokens, max_query, std::min(max_context, slots)), sequences,
+        kv_heads, slots);
 }
 
 int qxt_paged_attention_scores(const void *query, size_t query_token_stride, size_t query_head_stride,
