@@ -456,9 +456,10 @@ int qxt_qk_norm_rope_cache(const void *query, size_t query_token_stride, size_t 
  * log sum_j p_j; a row that sees nothing gets 0 and -inf, whatever unseen slots
  * hold.  Tokens of no sequence are left alone.  max_query and max_context
  * (longest chunk and context) only size the launch: larger ones in the device's
- * arrays are still computed, more slowly.  workspace: 16-byte aligned, of at
- * least qxt_paged_attention_workspace() bytes for the same sizes, free again
- * when the stream has passed the call. */
+ * arrays are still computed, more slowly; without query_starts max_query is 1,
+ * whatever it says.  workspace: 16-byte aligned, of at least
+ * qxt_paged_attention_workspace() bytes for the same arguments, free again when
+ * the stream has passed the call. */
 size_t qxt_paged_attention_workspace(uint32_t query_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t sequences,
                                      uint32_t tokens, uint32_t max_query, uint32_t max_context);
 int qxt_paged_attention(const void *query, size_t query_token_stride, size_t query_head_stride,

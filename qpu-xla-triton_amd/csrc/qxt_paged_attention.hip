@@ -856,8 +856,12 @@ extern "C" {
 size_t qxt_paged_attention_workspace(uint32_t query_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t sequences,
                                      uint32_t tokens, uint32_t max_query, uint32_t max_context) {
     if (kv_heads == 0 || query_heads % kv_heads || query_heads == 0 || sequences == 0 || tokens == 0) return 0;
-    const qxt::Plan p = qxt::plan_of(head_dim, query_heads / kv_heads, kv_heads, sequences, tokens, max_query, max_context);
-    return qxt::workspace_of(p, tokens, query_heads, head_dim);
+    auto bytes = [&](uint32_t longest) {
+        return qxt::workspace_of(
+            qxt::plan_of(head_dim, query_heads / kv_heads, kv_heads, sequences, tokens, longest, max_context), tokens, query_heads,
+            head_dim);
+    };
+    return tokens == sequences ? std::max(bytes(max_query), bytes(1)) : bytes(max_query);  // a call without starts plans for 1
 }
 
 int qxt_paged_attention(const void *query, size_t query_token_stride, size_t query_head_stride,

@@ -447,9 +447,12 @@ extern "C" {
 size_t qxt_paged_attention_scores_workspace(uint32_t query_heads, uint32_t kv_heads, uint32_t sequences, uint32_t tokens,
                                             uint32_t slots, uint32_t max_query, uint32_t max_context) {
     if (kv_heads == 0 || query_heads == 0 || query_heads % kv_heads || sequences == 0) return 0;
-    return qxt::score_workspace(
-        qxt::score_plan(query_heads / kv_heads, kv_heads, sequences, tokens, max_query, std::min(max_context, slots)), sequences,
-        kv_heads, slots);
+    auto bytes = [&](uint32_t longest) {
+        return qxt::score_workspace(
+            qxt::score_plan(query_heads / kv_heads, kv_heads, sequences, tokens, longest, std::min(max_context, slots)), sequences,
+            kv_heads, slots);
+    };
+    return tokens == sequences ? std::max(bytes(max_query), bytes(1)) : bytes(max_query);  // a call without starts plans for 1
 }
 
 int qxt_paged_attention_scores(const void *query, size_t query_token_stride, size_t query_head_stride,

@@ -49,3 +49,12 @@ def _attention(slots, sequences, tokens, starts, max_query, max_context):
 def test_contexts_up_to_and_past_the_slots(stopped, call, max_context, tokens, sequences) -> None:
     for max_query in {1, 7, tokens, 2 * tokens}:
         assert call(4096, sequences, tokens, FAKE, max_query, max_context) == _lib.SUBMISSION_FAILED, _lib.last_error()
+
+
+@pytest.mark.parametrize("call", [_scores, _attention])
+@pytest.mark.parametrize("sequences", [1, 2, 7, 64, 300])
+@pytest.mark.parametrize("max_query", [0, 1, 2, 9, 64, 2**32 - 1])
+def test_one_token_a_sequence_whatever_max_query_says(stopped, call, sequences, max_query) -> None:
+    for max_context in (1, 700, 4096, 65536):
+        assert call(65536, sequences, sequences, None, max_query, max_context) == _lib.SUBMISSION_FAILED, _lib.last_error()
+        assert call(65536, sequences, sequences, FAKE, max_query, max_context) == _lib.SUBMISSION_FAILED, _lib.last_error()
