@@ -82,6 +82,9 @@ __device__ __forceinline__ Sequence sequence_of(const A &a, uint32_t b) {
 struct Range {
     int32_t low, high;
 };
+// A window as seen_by takes it: at - window + 1 stays in 32 bits (at > -2^30), and 2^30 covers every slot.
+inline int32_t window_of(uint32_t window) { return static_cast<int32_t>(window < (1u << 30) ? window : 1u << 30); }
+
 template <typename A>
 __device__ __forceinline__ Range seen_by(const A &a, const Sequence &s, int32_t token) {
     const int32_t at = s.length - s.tokens + token;  // its own slot

@@ -920,7 +920,7 @@ int qxt_paged_attention(const void *query, size_t query_token_stride, size_t que
     a.scale = scale;
     a.scale2 = static_cast<float>(scale * 1.4426950408889634);
     a.causal = causal;
-    a.window = static_cast<int32_t>(window);
+    a.window = window_of(window);
     // Pages in whole units; one layout of keys and values, whose places in a page 32 bits (of 16 bytes) hold; head
     // sizes without padding.
     const uint32_t dim = cache->head_dim <= 64 ? 64 : cache->head_dim <= 128 ? 128 : 256;

@@ -514,7 +514,7 @@ int qxt_paged_attention_scores(const void *query, size_t query_token_stride, siz
     a.group = fast_div(group);
     a.scale = scale;
     a.causal = causal;
-    a.window = static_cast<int32_t>(window);
+    a.window = window_of(window);
     const uint32_t dim = cache->head_dim <= 64 ? 64 : cache->head_dim <= 128 ? 128 : 256;
     a.even = cache->page_size % 8 == 0 && cache->head_dim == dim && cache->key_slot_stride < (1u << 28) &&
              static_cast<uint64_t>(cache->page_size) * (cache->key_slot_stride / 16) <= UINT32_MAX;
