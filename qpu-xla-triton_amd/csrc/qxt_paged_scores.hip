@@ -99,7 +99,8 @@ __global__ __launch_bounds__(64 * kScoreWaves, DP <= 128 ? 2 : 1) void paged_sco
         int32_t first = 0, last = seq.tokens;
         const int32_t before = seq.length - seq.tokens;
         if (a.causal) first = max(0, key0 - before);
-        if (a.window > 0) last = static_cast<int32_t>(min<int64_t>(last, static_cast<int64_t>(key_end) - 1 + a.window - before));
+        if (a.window > 0)
+            last = static_cast<int32_t>(max<int64_t>(0, min<int64_t>(last, static_cast<int64_t>(key_end) - 1 + a.window - before)));
         const int32_t row_first = first * group, row_last = last * group;
         if (key0 < key_end && row_first < row_last) {
             frag k[2][DP / 16];
