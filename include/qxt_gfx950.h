@@ -492,9 +492,10 @@ int qxt_paged_attention_scores(const void *query, size_t query_token_stride, siz
  * use; a NaN score is the least.  Kept slots below budget stay; the i-th slot
  * below it that is given up takes key row, value row, score and position of the
  * i-th kept slot at or above it.  Slots from budget to the old length get score
- * 0 and position -1; lens_out[b] = min(length, budget) (not the context_lens
- * array itself).  scores fp32 and positions int32 [sequences, heads, table_width
- * * page_size], strides in bytes, dense in the slot; outputs may be the inputs.
+ * 0 and position -1; lens_out[b] = min(length, budget) (apart from the
+ * context_lens array).  scores fp32 and positions int32 [sequences, heads,
+ * table_width * page_size], strides in bytes, dense in the slot; outputs may be
+ * the inputs, and share no memory with them otherwise, nor row with row.
  * No page may belong to two sequences.  workspace (8-byte aligned):
  * qxt_paged_cache_evict_workspace() bytes. */
 size_t qxt_paged_cache_evict_workspace(uint32_t heads, uint32_t sequences, uint32_t slots, uint32_t budget);

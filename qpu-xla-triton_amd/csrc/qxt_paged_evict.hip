@@ -17,6 +17,7 @@
 // (32 of 256 CUs work, their vector units 52 % busy with the passes over the
 // keys), and 20 to move, near the rate of a copy; one slot over for 256 pairs 8 us.
 #include <algorithm>
+#include <utility>
 
 #include "qxt_paged.h"
 
@@ -366,6 +367,38 @@ int32_t most_moves(uint64_t slots, uint32_t budget) {
     return slots <= budget ? 0 : static_cast<int32_t>(std::min<uint64_t>(budget, slots - budget));
 }
 
+// One row of `bytes` for each (sequence, head).
+struct RowSet {
+    const void *data;
+    size_t sequence, head;  // strides in bytes
+};
+
+// Whether rows of x and y share memory, those at one place in both (in place) aside.  A workgroup whose scores others
+// write meanwhile would count them differently from pass to pass, and follow moves of which one end was never written.
+bool rows_overlap(RowSet x, RowSet y, uint32_t sequences, uint32_t heads, size_t bytes) {
+    if (sequences == 1) x.sequence = y.sequence = 0;
+    if (heads == 1) x.head = y.head = 0;
+    const int64_t apart = static_cast<int64_t>(reinterpret_cast<uintptr_t>(y.data) - reinterpret_cast<uintptr_t>(x.data));
+    auto span = [&](const RowSet &r) { return static_cast<int64_t>((sequences - 1) * r.sequence + (heads - 1) * r.head + bytes); };
+    if (apart >= span(x) || -apart >= span(y)) return false;
+    if (x.sequence != y.sequence || x.head != y.head) return true;  // interleaved in two ways: not worth telling apart
+    if (apart == 0) {
+        // The usual orders: whole sequences one after another, or whole heads.
+        const bool by_head = heads > 1 && (sequences == 1 || x.head < x.sequence);
+        const size_t inner = by_head ? x.head : x.sequence, outer = by_head ? x.sequence : x.head;
+        const uint32_t inner_rows = by_head ? heads : sequences, outer_rows = by_head ? sequences : heads;
+        if ((inner_rows == 1 || inner >= bytes) && (outer_rows == 1 || outer >= (inner_rows - 1) * inner + bytes)) return false;
+    }
+    const int64_t row = static_cast<int64_t>(bytes);
+    for (int64_t i = 1 - static_cast<int64_t>(sequences); i < static_cast<int64_t>(sequences); ++i)
+        for (int64_t j = 1 - static_cast<int64_t>(heads); j < static_cast<int64_t>(heads); ++j) {
+            if (apart == 0 && i == 0 && j == 0) continue;
+            const int64_t between = apart + i * static_cast<int64_t>(x.sequence) + j * static_cast<int64_t>(x.head);
+            if (between < row && -between < row) return true;
+        }
+    return false;
+}
+
 template <int THREADS, bool MOVE>
 int launch_plan(const EvictArgs &a, uint32_t sequences, size_t lds, hipStream_t stream) {
     return launch("paged_evict_plan_kernel", paged_evict_plan_kernel<THREADS, MOVE>, dim3(a.heads, sequences), dim3(THREADS),
@@ -392,7 +425,8 @@ int qxt_paged_cache_evict(const qxt_paged_cache *cache, const float *scores, siz
     if (cache->sequences == 0) return QXT_OK;
     if (scores == nullptr || scores_out == nullptr || positions == nullptr || positions_out == nullptr || lens_out == nullptr)
         return fail(QXT_INVALID_ARGUMENT, "paged cache evict: null pointer");
-    if (lens_out == cache->context_lens)  // other heads' workgroups still read them
+    if (lens_out < cache->context_lens + cache->sequences && cache->context_lens < lens_out + cache->sequences)
+        // (other workgroups still read the old ones)
         return fail(QXT_INVALID_ARGUMENT, "paged cache evict: new lengths must not replace the old ones in place");
     if (budget == 0 || budget > INT32_MAX / 2 || recent > budget)
         return fail(QXT_INVALID_ARGUMENT, "paged cache evict: budget must be positive and recent at most the budget");
@@ -404,6 +438,13 @@ int qxt_paged_cache_evict(const qxt_paged_cache *cache, const float *scores, siz
     if (cache->heads > 65535 || cache->sequences > 65535)
         return fail(QXT_INVALID_ARGUMENT, "paged cache evict: more than 65535 heads or sequences");
     const uint32_t slots = cache->page_size * cache->table_width;
+    for (const auto &[in, out] : {std::pair<RowSet, RowSet>{{scores, scores_sequence_stride, scores_head_stride},
+                                                            {scores_out, scores_out_sequence_stride, scores_out_head_stride}},
+                                  {{positions, positions_sequence_stride, positions_head_stride},
+                                   {positions_out, positions_out_sequence_stride, positions_out_head_stride}}})
+        if (rows_overlap(out, out, cache->sequences, cache->heads, 4 * static_cast<size_t>(slots)) ||
+            rows_overlap(in, out, cache->sequences, cache->heads, 4 * static_cast<size_t>(slots)))
+            return fail(QXT_INVALID_ARGUMENT, "paged cache evict: output rows share memory with other rows");
     const size_t needed = qxt_paged_cache_evict_workspace(cache->heads, cache->sequences, slots, budget);
     if (workspace == nullptr || workspace_bytes < needed || !aligned(workspace, 8))
         return fail(QXT_INVALID_ARGUMENT, "paged cache evict: workspace of %zu bytes needed", needed);

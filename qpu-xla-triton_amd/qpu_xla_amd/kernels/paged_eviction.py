@@ -44,7 +44,8 @@ def paged_cache_evict(
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Evict in the cache; returns (new lengths int32 [B], scores, positions), new tensors unless outputs are given.
 
-    ``scores_out`` and ``positions_out`` may be the inputs themselves; ``lens_out`` must not be ``context_lens``.
+    ``scores_out`` and ``positions_out`` may be the inputs themselves, and share no memory with them otherwise, nor row
+    with row; ``lens_out`` lies apart from ``context_lens``.
     ``max_context`` is the host's bound of the lengths and sizes the launch.
     """
     name = "paged_cache_evict"
