@@ -454,7 +454,11 @@ int qxt_qk_norm_rope_cache(const void *query, size_t query_token_stride, size_t 
  * context_lens[b] - n + i; query heads share key head h / (query_heads / heads).
  * out = sum_j p_j v_j / sum_j p_j, p_j = exp(scale * q.k_j), and lse (or NULL) =
  * log sum_j p_j; a row that sees nothing gets 0 and -inf, whatever unseen slots
- * hold.  Tokens of no sequence are left alone.  max_query and max_context
+ * hold.  Computed in fp32, but for the weights p_j, which are rounded to the
+ * cache's type for the product with the values, whatever out_type is.  Infinite
+ * or NaN values among slots that some of a chunk's rows see and others do not
+ * are handled row by row, many times more slowly.  Tokens of no sequence are
+ * left alone (out and lse keep what they held).  max_query and max_context
  * (longest chunk and context) only size the launch: larger ones in the device's
  * arrays are still computed, more slowly; without query_starts max_query is 1,
  * whatever it says.  workspace: 16-byte aligned, of at least
@@ -472,9 +476,11 @@ int qxt_paged_attention(const void *query, size_t query_token_stride, size_t que
  * sum over sequence b's tokens t and the query heads h of key head `head` of
  * exp(scale * q.k_j - lse[t, h]), for the slots j that t sees (as
  * qxt_paged_attention, whose lse this takes: then each row's weights add up to
- * 1).  Rows with lse = -inf add nothing.  previous and scores: fp32 [sequences,
- * heads, table_width * page_size], strides in bytes, dense in j; they may be
- * the same.  Slots at and above a sequence's length keep their previous value.
+ * 1).  Rows with lse = -inf add nothing, those with a NaN lse make the slots that
+ * they see NaN, and no other.  previous and scores: fp32 [sequences, heads,
+ * table_width * page_size], strides in bytes, dense in j; they may be the same.
+ * Slots at and above a sequence's length keep their previous value; all of the
+ * table's width is read and written, so wide tables cost time.
  * The order of the sum is fixed by the arguments. */
 size_t qxt_paged_attention_scores_workspace(uint32_t query_heads, uint32_t kv_heads, uint32_t sequences, uint32_t tokens,
                                             uint32_t slots, uint32_t max_query, uint32_t max_context);

@@ -317,7 +317,6 @@ struct Mfma;
 template <>
 struct Mfma<bf16_t> {
     typedef bf16_t frag __attribute__((ext_vector_type(8)));
-    static constexpr uint32_t kMantissa = 0x7F;
     // Bits 15 and 31 are set where the element in bits 0-15 or 16-31 is infinite or NaN.
     static __device__ __forceinline__ uint32_t special(uint32_t two) { return (two & 0x7F807F80u) + 0x00800080u; }
     static __device__ __forceinline__ f32x16 run(frag a, frag b, f32x16 c) {
@@ -327,7 +326,6 @@ struct Mfma<bf16_t> {
 template <>
 struct Mfma<f16_t> {
     typedef f16_t frag __attribute__((ext_vector_type(8)));
-    static constexpr uint32_t kMantissa = 0x3FF;
     static __device__ __forceinline__ uint32_t special(uint32_t two) { return (two & 0x7C007C00u) + 0x04000400u; }
     static __device__ __forceinline__ f32x16 run(frag a, frag b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);

@@ -14,6 +14,13 @@
 // and sum need one exchange between half-waves, and the rounded weights are
 // already the second operand of O^T = V^T P^T: the sum over keys may run in any
 // order, so V^T is read (transposed, from LDS) in the order the lanes hold.
+//
+// The matrix units take weights in the cache's type, and so they are rounded for
+// the product with the values, also where the output is fp32; the sum that
+// divides keeps them in 32 bits.  Relative error of outputs against 64 bits, one
+// token over 3000 slots, heads of 128: bf16 cache 2.3e-3 in bf16 (the output's
+// own rounding is 1.7e-3), 1.5e-3 in fp32; fp16 cache 2.8e-4 in fp16, 1.9e-4 in
+// fp32.  In fp16 weights below 2^-25 of the largest add to the sum alone.
 #include <algorithm>
 
 #include "qxt_paged_attention.h"
@@ -22,9 +29,9 @@ namespace qxt {
 namespace {
 
 constexpr float kNone = -__builtin_inff();
-// The running maximum moves only when a logit exceeds it by 2^8: weights stay
-// below 256 (exact in the sums' 32 bits, in range of fp16) and the rescaling of
-// the outputs is rare.
+// The running maximum moves only when a logit exceeds it by this much (in log2
+// units): weights stay up to 2^8, in range of fp16, and the rescaling of the
+// outputs is rare.
 constexpr float kSlack = 8.0f;
 
 template <typename TO>
@@ -55,6 +62,10 @@ __device__ __forceinline__ float lse_of(float top2, float sum) {
 // sees enter.  For the rare waves whose rows see different slots of a step that
 // holds infinite or NaN values.  Lane l gets elements l + 64 k; the slots are
 // [from, to) in parts of `part` every `step`.
+// Right, and slow: keys are read element by element, the rows one after another,
+// and the call waits for its slowest wave.  One such value three slots from the
+// end: 8k prompt of 32 heads of 128 0.64 -> 201 ms, 512 tokens over 32k slots
+// 0.31 -> 166 ms, 9 tokens over 1k slots 14 us -> 1.1 ms.
 template <typename T, int DP, typename A>
 __device__ __forceinline__ float2 attend_alone(const A &a, const T *query, const Range &mine, int32_t from,
                                                int32_t to, int32_t step, int32_t part, const int32_t *table,

@@ -97,7 +97,12 @@ def paged_attention(
     lse: torch.Tensor | None = None,
     stream: Any = None,
 ) -> torch.Tensor:
-    """Attention outputs [T, Hq, D] (the query's type, or ``out``'s); ``lse`` float32 [T, Hq] receives the log-sums."""
+    """Attention outputs [T, Hq, D] (the query's type, or ``out``'s); ``lse`` float32 [T, Hq] receives the log-sums.
+
+    Rows of tokens that belong to no sequence (padding outside ``query_starts``) are not written: ``out`` and ``lse`` keep
+    what they held there, and without ``out`` those rows are uninitialised.  The softmax weights are rounded to the
+    cache's type for the product with the values, also for a float32 ``out``.
+    """
     name = "paged_attention"
     shape, strides, heads, sequences, slots, cache = _check(name, query, key_cache, value_cache, block_table, context_lens,
                                                             query_starts)
@@ -143,7 +148,8 @@ def paged_attention_scores(
     """Weight that each slot received, float32 [B, Hkv, W * page_size], on top of ``scores`` (None: zeros).
 
     ``lse`` are the log-sums that ``paged_attention`` wrote for the same queries, cache and masks; a row's weights then
-    add up to 1.  ``out`` may be ``scores`` itself.
+    add up to 1.  ``out`` may be ``scores`` itself.  A row with a NaN log-sum makes the slots that it sees NaN.  Every slot
+    of the table's width is read and written.
     """
     name = "paged_attention_scores"
     shape, strides, heads, sequences, slots, cache = _check(name, query, key_cache, None, block_table, context_lens,

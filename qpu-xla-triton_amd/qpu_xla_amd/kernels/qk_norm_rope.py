@@ -7,8 +7,8 @@
 ``y = x * rsqrt(mean(x^2) + epsilon) * weight`` per row (skipped where a weight is None), then the pairs
 ``(y[i], y[i + R/2])``, or ``(y[2i], y[2i + 1])`` with ``interleaved``, turn by ``cos[position, i]``,
 ``sin[position, i]`` (fp32 [P, R/2]); elements past R stay.  Everything is computed in fp32 and rounded once.  Tokens
-and heads may have any stride (slices of one q/k/v projection), rows are dense.  A position outside the table gives a
-NaN row, a negative slot (padding) is not stored.
+and heads may have any stride (slices of one q/k/v projection), rows are dense.  A position outside the table makes the
+row's rotated part NaN, a negative slot (padding) is not stored.
 
 The reference's rotation and norm programs (``src/qpu_xla/kernels``) are separate fp32 launches; no counterpart of
 the fused form or of the paged cache exists there.
