@@ -581,8 +581,8 @@ __global__ __launch_bounds__(64 * WQ * WK, DP <= 128 ? 2 : 1) void paged_attenti
 // all of these buffers were last read a phase or more before.  Each wave waits
 // for its share two phases on, before the barrier after which the first wave
 // reads it, with the loads of its next vector phase already under way.
-// Measured: 8192 new tokens, 32 heads of 128, 32 key heads, causal, 577 us
-// (0.95 PFLOP/s; a library product of two 8192 x 8192 matrices 1.37).  When this
+// Measured: 8192 new tokens, 32 heads of 128, 32 key heads, causal, 570 us
+// (0.96 PFLOP/s; a library product of two 8192 x 8192 matrices 1.37).  When this
 // took 600 us, all waves in step took 651; at 620, the DMA issued in the matrix
 // phases instead 653.  Bound by the vector phases, about 2000 cycles a step
 // against 1350 of matrix work: half of them the softmax, the rest page look-ups,

@@ -12,8 +12,8 @@
 // are too few workgroups, the steps are dealt out over splits, whose sums a
 // second launch adds in order.  Bound by the matrix and vector units together:
 // 32 MFMAs and 64 exponentials with three more operations each a wave and step.
-// Measured: a 4k prompt, 32 heads of 128 over 8 key heads, causal, 154 us for
-// 68.7 GFLOP; the vector units are busy 55 % of the time, the matrix units 28 %.
+// Measured: a 4k prompt, 32 heads of 128 over 8 key heads, causal, 156 us for
+// 68.7 GFLOP; the vector units are busy 54 % of the time, the matrix units 28 %.
 //
 // Every score of the table's width is read and written, in place too, so tables
 // wider than the contexts cost: one token each of 16 sequences of 6k slots, 8 key
