@@ -512,6 +512,91 @@ int qxt_paged_cache_evict(const qxt_paged_cache *cache, const float *scores, siz
                           size_t positions_out_head_stride, int32_t *lens_out, uint32_t budget, uint32_t recent,
                           uint32_t max_context, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ------------------------------------------- microscaling blocks and norms */
+
+/* No counterpart in the reference for anything in this section: its block
+ * formats are ggml's, its norms are separate fp32 launches. */
+
+/* Block formats: 32 elements under one shared power of two (OCP Microscaling
+ * Formats).  Values are packed element by element in a row (4-bit ones two a
+ * byte, the lower index in the low half), scales are one byte E a block in a
+ * plane of their own, of value 2^(E - 127); 255: the whole block is NaN. */
+#define QXT_MX_FP4 0u /* e2m1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives */
+#define QXT_MX_FP8 1u /* e4m3 up to 448 */
+
+/* Quantised row kinds of qxt_add_rms_norm and qxt_mxfp4_gated_*, next to QXT_TYPE_F32, _BF16 and _F16. */
+#define QXT_ROWS_INT8 3u  /* int8 values, one fp32 scale a row: as qxt_quantize_rows_int8 */
+#define QXT_ROWS_Q8_0 4u  /* 34-byte blocks: as qxt_quantize_q8_0 */
+#define QXT_ROWS_MXFP8 5u /* QXT_MX_FP8 values and scales */
+#define QXT_ROWS_MXFP4 6u /* QXT_MX_FP4 values and scales */
+
+/* Rows of blocks.  Strides in bytes. */
+typedef struct qxt_mx_matrix {
+    const void *values;
+    size_t row_stride;
+    const uint8_t *scales;
+    size_t scales_row_stride;
+} qxt_mx_matrix;
+
+/* Rows [rows, columns] of floats (strides free, elements dense) to blocks and
+ * back; columns a multiple of 32.  With a block's largest magnitude A, E - 127 =
+ * floor(log2 A) - floor(log2 largest element), at least -127 (zero blocks too);
+ * elements are x / 2^(E - 127) rounded to nearest even and cut to the largest
+ * element (6, 448).  A block that holds an infinity or a NaN becomes NaN.
+ * Reading back is exact but for the rounding to bf16 or fp16. */
+int qxt_quantize_mx(const void *x, size_t x_row_stride, uint32_t type, void *values, size_t values_row_stride,
+                    uint8_t *scales, size_t scales_row_stride, uint32_t rows, uint32_t columns, uint32_t format,
+                    void *stream);
+int qxt_dequantize_mx(const void *values, size_t values_row_stride, const uint8_t *scales, size_t scales_row_stride,
+                      void *x, size_t x_row_stride, uint32_t type, uint32_t rows, uint32_t columns, uint32_t format,
+                      void *stream);
+
+/* sum = x + residual, rounded to the residual's type; y = sum * f * weight with
+ * f = 1 / sqrt(mean(sum^2) + epsilon), from the rounded sum.  Without a residual
+ * (NULL; sum is not written then) y is of x.  The mean and f are computed in 64
+ * bits, f and both products are rounded to fp32, and that y is rounded to out_kind
+ * or quantised by its rule, so every code is defined.  out: a float type's rows,
+ * int8 rows (scales: fp32 [rows]), Q8_0 blocks (no scales) or microscaling values
+ * (scales: bytes, rows scales_row_stride apart; columns a multiple of 32 for any
+ * blocks).  sum may be the residual or x, and float outputs may be x, where types
+ * and strides are the same; no other memory may be shared. */
+int qxt_add_rms_norm(const void *x, size_t x_row_stride, uint32_t x_type, const void *residual,
+                     size_t residual_row_stride, uint32_t residual_type, void *sum, size_t sum_row_stride,
+                     const float *weight, double epsilon, void *out, size_t out_row_stride, void *scales,
+                     size_t scales_row_stride, uint32_t out_kind, uint32_t rows, uint32_t columns, void *stream);
+
+/* y [m, n] = a w^T (+ bias), over activations a [m, k] in blocks of `format` and
+ * weights w [n, k] in blocks of QXT_MX_FP4 (values in rows aligned to 16 bytes,
+ * k a multiple of 32).  Products are exact and sums are fp32; for 8-bit activations
+ * and results other than float32 the matrix instruction drops what lies more than 13
+ * bits below the largest of eight neighbouring products (1e-5 of a result's size).
+ * y_type: QXT_TYPE_*, rounded once.  qxt_mxfp4_linear takes activations as floats and
+ * quantises them as qxt_quantize_mx does.  workspace (16-byte aligned):
+ * qxt_mxfp4_linear_workspace() bytes for one weight, free again when the stream
+ * has passed the call. */
+size_t qxt_mxfp4_linear_workspace(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, uint32_t format);
+int qxt_mxfp4_gemm(const qxt_mx_matrix *a, uint32_t format, const qxt_mx_matrix *w, const float *bias, void *y, size_t ldy,
+                   uint32_t y_type, uint32_t m, uint32_t n, uint32_t k, void *workspace, size_t workspace_bytes, void *stream);
+int qxt_mxfp4_linear(const void *x, size_t ldx, uint32_t x_type, uint32_t format, const qxt_mx_matrix *w, const float *bias,
+                     void *y, size_t ldy, uint32_t y_type, uint32_t m, uint32_t n, uint32_t k, void *workspace,
+                     size_t workspace_bytes, void *stream);
+
+/* Gate functions: g / (1 + exp(-g)), and g (1 + erf(g / sqrt 2)) / 2. */
+#define QXT_GATE_SILU 0u
+#define QXT_GATE_GELU 1u
+
+/* h [m, n] = f(a gate^T) * (a up^T), operands as above and f a gate function of
+ * the fp32 sums; h_kind: QXT_TYPE_*, QXT_ROWS_MXFP8 or QXT_ROWS_MXFP4 (n a multiple
+ * of 32; h_scales takes the scales).  workspace: qxt_mxfp4_linear_workspace() bytes
+ * for two weights. */
+int qxt_mxfp4_gated_gemm(const qxt_mx_matrix *a, uint32_t format, const qxt_mx_matrix *gate, const qxt_mx_matrix *up,
+                         uint32_t gate_function, void *h, size_t ldh, uint8_t *h_scales, size_t ldhs, uint32_t h_kind,
+                         uint32_t m, uint32_t n, uint32_t k, void *workspace, size_t workspace_bytes, void *stream);
+int qxt_mxfp4_gated_linear(const void *x, size_t ldx, uint32_t x_type, uint32_t format, const qxt_mx_matrix *gate,
+                           const qxt_mx_matrix *up, uint32_t gate_function, void *h, size_t ldh, uint8_t *h_scales,
+                           size_t ldhs, uint32_t h_kind, uint32_t m, uint32_t n, uint32_t k, void *workspace,
+                           size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,121 @@
+// Quantising rows to microscaling blocks (qxt_mx.h has the rule) and reading
+// them back.
+//
+// Both are bound by their bytes: each element is read and written once, and the
+// arithmetic is a maximum over a block and one conversion an element.  A thread
+// holds eight elements, one or two 16-byte pieces, and four neighbouring lanes a
+// block, so its maximum takes two exchanges and no element is read twice.
+#include "qxt_mx.h"
+
+namespace qxt {
+namespace {
+
+constexpr int kThreads = 256;
+
+struct MxRows {
+    char *x;
+    int64_t x_stride;
+    uint32_t type;
+    char *values;
+    int64_t values_stride;
+    uint8_t *scales;
+    int64_t scales_stride;
+    uint32_t pieces;  // of eight elements, of all rows
+    FastDiv row;      // by the pieces of a row
+};
+
+template <bool FP8, bool VEC>
+__global__ __launch_bounds__(kThreads) void quantize_mx_kernel(MxRows a) {
+    const uint32_t piece = blockIdx.x * kThreads + threadIdx.x;
+    if (piece >= a.pieces) return;  // whole blocks leave together
+    const uint32_t row = fast_quotient(piece, a.row), at = piece - row * a.row.divisor;
+    const Eight e = load_eight<VEC>(a.type, a.x + row * a.x_stride, at * 8);
+    const uint32_t scale = block_scale<FP8>(e);
+    char *values = a.values + row * a.values_stride;
+    if constexpr (FP8) *reinterpret_cast<u2 *>(values + static_cast<size_t>(at) * 8) = fp8_of(e, scale);
+    else *reinterpret_cast<uint32_t *>(values + static_cast<size_t>(at) * 4) = fp4_of(e, scale);
+    if (at % 4 == 0) a.scales[row * a.scales_stride + at / 4] = static_cast<uint8_t>(scale);
+}
+
+template <bool FP8, bool VEC>
+__global__ __launch_bounds__(kThreads) void dequantize_mx_kernel(MxRows a) {
+    const uint32_t piece = blockIdx.x * kThreads + threadIdx.x;
+    if (piece >= a.pieces) return;
+    const uint32_t row = fast_quotient(piece, a.row), at = piece - row * a.row.divisor;
+    const char *values = a.values + row * a.values_stride;
+    const float scale = mx_value(a.scales[row * a.scales_stride + at / 4]);
+    Eight e;
+    if constexpr (FP8) e = fp8_values(*reinterpret_cast<const u2 *>(values + static_cast<size_t>(at) * 8), scale);
+    else e = fp4_values(*reinterpret_cast<const uint32_t *>(values + static_cast<size_t>(at) * 4), scale);
+    store_eight<VEC>(a.type, a.x + row * a.x_stride, at * 8, e);
+}
+
+int run_mx(bool quantize, MxRows &a, uint32_t rows, uint32_t columns, uint32_t format, void *stream) {
+    const char *name = quantize ? "quantize mx" : "dequantize mx";
+    if (!known_type(a.type)) return fail(QXT_INVALID_ARGUMENT, "%s: unknown element type", name);
+    if (!known_mx(format)) return fail(QXT_INVALID_ARGUMENT, "%s: unknown block format", name);
+    if (columns == 0 || columns % kMxBlock)
+        return fail(QXT_INVALID_ARGUMENT, "%s: columns must be a positive multiple of 32", name);
+    const uint64_t pieces = static_cast<uint64_t>(rows) * (columns / 8);
+    if (pieces > INT32_MAX) return fail(QXT_INVALID_ARGUMENT, "%s: more than 2^34 elements", name);
+    if (rows == 0) return QXT_OK;
+    if (a.x == nullptr || a.values == nullptr || a.scales == nullptr)
+        return fail(QXT_INVALID_ARGUMENT, "%s: null pointer", name);
+    const size_t element = type_bytes(a.type), piece = format == QXT_MX_FP8 ? 8 : 4;
+    const size_t x_stride = static_cast<size_t>(a.x_stride), v_stride = static_cast<size_t>(a.values_stride);
+    if (!aligned(a.x, element) || x_stride % element || !aligned(a.values, piece) || v_stride % piece)
+        return fail(QXT_INVALID_ARGUMENT, "%s: misaligned rows", name);
+    if (rows > 1 && (x_stride < columns * element || v_stride < mx_row_bytes(format, columns) ||
+                     static_cast<size_t>(a.scales_stride) < columns / kMxBlock))
+        return fail(QXT_INVALID_ARGUMENT, "%s: a row stride is below the row", name);
+    if (int rc = injected(QXT_FAIL_SUBMISSION)) return rc;
+    a.pieces = static_cast<uint32_t>(pieces);
+    a.row = fast_div(columns / 8);
+    const bool vec = aligned(a.x, 16) && x_stride % 16 == 0;
+    const dim3 grid((a.pieces + kThreads - 1) / kThreads);
+    const bool fp8 = format == QXT_MX_FP8;
+    if (quantize)
+        return launch("quantize_mx_kernel",
+                      fp8 ? (vec ? quantize_mx_kernel<true, true> : quantize_mx_kernel<true, false>)
+                          : (vec ? quantize_mx_kernel<false, true> : quantize_mx_kernel<false, false>),
+                      grid, dim3(kThreads), 0, as_stream(stream), a);
+    return launch("dequantize_mx_kernel",
+                  fp8 ? (vec ? dequantize_mx_kernel<true, true> : dequantize_mx_kernel<true, false>)
+                      : (vec ? dequantize_mx_kernel<false, true> : dequantize_mx_kernel<false, false>),
+                  grid, dim3(kThreads), 0, as_stream(stream), a);
+}
+
+}  // namespace
+}  // namespace qxt
+
+extern "C" {
+
+int qxt_quantize_mx(const void *x, size_t x_row_stride, uint32_t type, void *values, size_t values_row_stride,
+                    uint8_t *scales, size_t scales_row_stride, uint32_t rows, uint32_t columns, uint32_t format,
+                    void *stream) {
+    qxt::MxRows a{};
+    a.x = static_cast<char *>(const_cast<void *>(x));
+    a.x_stride = static_cast<int64_t>(x_row_stride);
+    a.type = type;
+    a.values = static_cast<char *>(values);
+    a.values_stride = static_cast<int64_t>(values_row_stride);
+    a.scales = scales;
+    a.scales_stride = static_cast<int64_t>(scales_row_stride);
+    return qxt::run_mx(true, a, rows, columns, format, stream);
+}
+
+int qxt_dequantize_mx(const void *values, size_t values_row_stride, const uint8_t *scales, size_t scales_row_stride,
+                      void *x, size_t x_row_stride, uint32_t type, uint32_t rows, uint32_t columns, uint32_t format,
+                      void *stream) {
+    qxt::MxRows a{};
+    a.x = static_cast<char *>(x);
+    a.x_stride = static_cast<int64_t>(x_row_stride);
+    a.type = type;
+    a.values = static_cast<char *>(const_cast<void *>(values));
+    a.values_stride = static_cast<int64_t>(values_row_stride);
+    a.scales = const_cast<uint8_t *>(scales);
+    a.scales_stride = static_cast<int64_t>(scales_row_stride);
+    return qxt::run_mx(false, a, rows, columns, format, stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,127 @@
+// Shared by the kernels of linears over microscaling 4-bit weights: arguments,
+// the scaled matrix instruction, the gate functions and the store of results.
+#pragma once
+
+#include "qxt_mx.h"
+
+namespace qxt {
+
+struct MxOperand {
+    const char *values;
+    int64_t stride;
+    const uint8_t *scales;
+    int64_t scale_stride;
+};
+
+struct MxLinearArgs {
+    MxOperand a;     // activations [m, blocks]
+    MxOperand w[2];  // weights [n, blocks]; the second one: up, of a gated product
+    const float *bias;
+    char *y;
+    int64_t y_stride;
+    uint8_t *y_scales;
+    int64_t y_scale_stride;
+    uint32_t m, n, blocks;
+    uint32_t out_kind, gate;
+    uint32_t vec_out;  // y's rows are aligned to 16 bytes
+};
+
+typedef int i8 __attribute__((ext_vector_type(8)));
+typedef int i4 __attribute__((ext_vector_type(4)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+
+// How activations enter the matrix instruction.  Among products of 8-bit elements it drops what lies more than 13 bits
+// below the largest of eight neighbours' powers of two (measured: 4e-6 to 2e-5 of a result's size whatever K is, with
+// either sign): less than results in half types or blocks lose to their rounding.  For float32 results the 8-bit elements
+// go through it in two parts, those of magnitude 2 and above and those below it (their bit 6 tells): within a part no
+// product's last bit lies more than 13 bits below another's power of two, so nothing is dropped.
+enum Act { kAct4 = 0, kAct8 = 1, kAct8Parts = 2 };
+
+__device__ __forceinline__ int large_bytes(int word) {
+    const uint32_t bit = (static_cast<uint32_t>(word) >> 6) & 0x01010101u;
+    return static_cast<int>((bit << 8) - bit);  // 0xFF in each byte whose bit 6 is set
+}
+
+__device__ __forceinline__ i8 low_half(u4 v) {
+    return i8{static_cast<int>(v[0]), static_cast<int>(v[1]), static_cast<int>(v[2]), static_cast<int>(v[3]), 0, 0, 0, 0};
+}
+__device__ __forceinline__ i8 both_halves(u4 a, u4 b) {
+    return i8{static_cast<int>(a[0]), static_cast<int>(a[1]), static_cast<int>(a[2]), static_cast<int>(a[3]),
+              static_cast<int>(b[0]), static_cast<int>(b[1]), static_cast<int>(b[2]), static_cast<int>(b[3])};
+}
+
+// Activation operands of one instruction, and acc += W A over 128 elements of K: 16 weight rows (4-bit) by 16 activation
+// rows.  Lane l holds weight row l % 16 and activation row l % 16; of 4-bit rows the 32 elements of block l / 16, of 8-bit
+// ones bytes 16 (l / 16) + [0, 16) and 64 + the same; and of both rows byte J of a word of scales: that of block l / 16.
+// It receives weight rows 4 (l / 16) + [0, 4) of activation row l % 16.
+template <int ACT>
+struct ActPiece {
+    i8 v, rest;
+    __device__ __forceinline__ ActPiece(u4 a, u4 b) {
+        if constexpr (ACT == kAct4) {
+            v = low_half(a);
+        } else {
+            v = both_halves(a, b);
+            if constexpr (ACT == kAct8Parts) {
+                const i8 all = v;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int large = large_bytes(all[i]);
+                    v[i] = all[i] & large;
+                    rest[i] = all[i] & ~large;
+                }
+            }
+        }
+    }
+};
+
+template <int ACT, int J>
+__device__ __forceinline__ f4 mx_mfma(u4 w, const ActPiece<ACT> &a, f4 acc, uint32_t w_scales, uint32_t a_scales) {
+    constexpr int form = ACT == kAct4 ? 4 : 0;
+    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(low_half(w), a.v, acc, 4, form, J, w_scales, J, a_scales);
+    if constexpr (ACT == kAct8Parts)
+        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(low_half(w), a.rest, acc, 4, form, J, w_scales, J, a_scales);
+    return acc;
+}
+
+// exp(-g) through the hardware's power of two: the part of g log2(e) that its
+// rounding loses is put back to first order, so the error is a few units of fp32
+// for every g (without it, |g| units).
+__device__ __forceinline__ float gated(uint32_t gate, float g, float up) {
+    if (gate == QXT_GATE_SILU) {
+        const float t = fminf(fmaxf(g * -1.442695041f, -126.0f), 200.0f);
+        const float rest = fmaf(g, -1.442695041f, -t) + g * -1.925963033e-8f;
+        const float e = __builtin_amdgcn_exp2f(t) * (1.0f + 0.6931471806f * (fabsf(g) < 87.0f ? rest : 0.0f));
+        return g * __builtin_amdgcn_rcpf(1.0f + e) * up;
+    }
+    return 0.5f * g * (1.0f + erff(g * 0.7071067812f)) * up;
+}
+
+// Eight results of activation row m at columns n .. n + 7; block outputs: four neighbouring lanes hold a whole block.
+__device__ __forceinline__ void store_results(const MxLinearArgs &a, uint32_t m, uint32_t n, Eight e) {
+    if (a.out_kind >= QXT_ROWS_MXFP8) {
+        const bool fp8 = a.out_kind == QXT_ROWS_MXFP8;
+        const uint32_t scale = fp8 ? block_scale<true>(e) : block_scale<false>(e);
+        if (m >= a.m || n >= a.n) return;
+        char *row = a.y + m * a.y_stride;
+        if (fp8) *reinterpret_cast<u2 *>(row + n) = fp8_of(e, scale);
+        else *reinterpret_cast<uint32_t *>(row + n / 2) = fp4_of(e, scale);
+        if (n % 32 == 0) a.y_scales[m * a.y_scale_stride + n / 32] = static_cast<uint8_t>(scale);
+        return;
+    }
+    if (m >= a.m || n >= a.n) return;
+    char *row = a.y + m * a.y_stride;
+    if (a.vec_out && n + 8 <= a.n) {
+        store_eight<true>(a.out_kind, row, n, e);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (n + i >= a.n) return;
+        if (a.out_kind == QXT_TYPE_F32) reinterpret_cast<float *>(row)[n + i] = e.v[i];
+        else if (a.out_kind == QXT_TYPE_BF16) reinterpret_cast<bf16_t *>(row)[n + i] = static_cast<bf16_t>(e.v[i]);
+        else reinterpret_cast<f16_t *>(row)[n + i] = static_cast<f16_t>(e.v[i]);
+    }
+}
+
+}  // namespace qxt

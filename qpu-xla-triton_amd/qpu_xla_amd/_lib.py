@@ -16,6 +16,7 @@ from ctypes import (
     Structure,
     c_char,
     c_char_p,
+    c_double,
     c_float,
     c_int,
     c_int32,
@@ -59,6 +60,14 @@ TYPE_F32 = 0
 TYPE_BF16 = 1
 TYPE_F16 = 2
 ROPE_INTERLEAVED = 1
+MX_FP4 = 0
+MX_FP8 = 1
+ROWS_INT8 = 3
+ROWS_Q8_0 = 4
+ROWS_MXFP8 = 5
+ROWS_MXFP4 = 6
+GATE_SILU = 0
+GATE_GELU = 1
 
 
 class DeviceInfo(Structure):
@@ -101,6 +110,7 @@ class Q4Task(Structure):
 
 # ``qxt_paged_cache`` in C's layout, packed by struct (a ctypes Structure of its 18 fields takes 2 us to fill).
 PAGED_CACHE = struct.Struct("PNNNPNNNPNPIIIIIII0P")
+MX_MATRIX = struct.Struct("PNPN")  # ``qxt_mx_matrix``
 
 
 class LlamaContextConfig(Structure):
@@ -207,6 +217,17 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "qxt_paged_cache_evict_workspace": (_SZ, [_U] * 4),
     "qxt_paged_cache_evict": (
         c_int, [_P, _P, _SZ, _SZ, _P, _SZ, _SZ, _P, _SZ, _SZ, _P, _SZ, _SZ, _P, _U, _U, _U, _P, _SZ, _P]),
+    "qxt_quantize_mx": (c_int, [_P, _SZ, _U, _P, _SZ, _P, _SZ, _U, _U, _U, _P]),
+    "qxt_dequantize_mx": (c_int, [_P, _SZ, _P, _SZ, _P, _SZ, _U, _U, _U, _U, _P]),
+    "qxt_add_rms_norm": (
+        c_int, [_P, _SZ, _U, _P, _SZ, _U, _P, _SZ, _P, c_double, _P, _SZ, _P, _SZ, _U, _U, _U, _P]),
+    "qxt_mxfp4_linear_workspace": (_SZ, [_U] * 5),
+    "qxt_mxfp4_gemm": (c_int, [_P, _U, _P, _P, _P, _SZ, _U, _U, _U, _U, _P, _SZ, _P]),
+    "qxt_mxfp4_linear": (c_int, [_P, _SZ, _U, _U, _P, _P, _P, _SZ, _U, _U, _U, _U, _P, _SZ, _P]),
+    "qxt_mxfp4_gated_gemm": (
+        c_int, [_P, _U, _P, _P, _U, _P, _SZ, _P, _SZ, _U, _U, _U, _U, _P, _SZ, _P]),
+    "qxt_mxfp4_gated_linear": (
+        c_int, [_P, _SZ, _U, _U, _P, _P, _U, _P, _SZ, _P, _SZ, _U, _U, _U, _U, _P, _SZ, _P]),
     "qxt_llama_context_create": (c_int, [POINTER(LlamaContextConfig), POINTER(c_void_p)]),
     "qxt_llama_context_destroy": (None, [_P]),
     "qxt_llama_context_last_error": (c_char_p, [_P]),

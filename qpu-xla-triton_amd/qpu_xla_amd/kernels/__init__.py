@@ -1,5 +1,15 @@
 """gfx950 kernels of the quantized-linear path, one module per reference kernel module."""
 
+from qpu_xla_amd.kernels.add_rms_norm import (  # noqa: F401
+    ADD_RMS_NORM_KERNEL,
+    AddRmsNormOptions,
+    add_rms_norm,
+    add_rms_norm_grid,
+    add_rms_norm_int8,
+    add_rms_norm_mxfp4,
+    add_rms_norm_mxfp8,
+    add_rms_norm_q8_0,
+)
 from qpu_xla_amd.kernels.gemm_int8 import (  # noqa: F401
     TILED_W8A8_GEMM_DEQUANTIZE_KERNEL,
     TILED_W8A8_GEMM_KERNEL,
@@ -43,6 +53,20 @@ from qpu_xla_amd.kernels.ggml_q8_0 import (  # noqa: F401
     GGML_Q8_0_Q8_0_LINEAR_M4_KERNEL,
     ggml_q8_0_q8_0_linear,
     supports_ggml_q8_0_q8_0_linear_m4,
+)
+from qpu_xla_amd.kernels.mxfp4 import (  # noqa: F401
+    MXFP4_GATED_GEMM_KERNEL,
+    MXFP4_GEMM_KERNEL,
+    Mxfp4GatedOptions,
+    dequantize_mxfp4,
+    dequantize_mxfp8,
+    mxfp4_gated_gemm,
+    mxfp4_gated_linear,
+    mxfp4_gemm,
+    mxfp4_gemm_grid,
+    mxfp4_linear,
+    quantize_mxfp4,
+    quantize_mxfp8,
 )
 from qpu_xla_amd.kernels.paged_attention import (  # noqa: F401
     PAGED_ATTENTION_KERNEL,
