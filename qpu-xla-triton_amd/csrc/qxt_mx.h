@@ -186,4 +186,19 @@ __device__ __forceinline__ Eight fp8_values(u2 word, float scale) {
     return e;
 }
 
+// Arguments of quantising and reading back (qxt_mx_quantize.hip), and their checks and launch.
+struct MxRows {
+    char *x;
+    int64_t x_stride;
+    uint32_t type;
+    char *values;
+    int64_t values_stride;
+    uint8_t *scales;
+    int64_t scales_stride;
+    uint32_t scale_pad;  // bytes to clear after a row's last scale
+    uint32_t pieces;     // of eight elements, of all rows
+    FastDiv row;         // by the pieces of a row
+};
+int run_mx(bool quantize, MxRows &a, uint32_t rows, uint32_t columns, uint32_t format, void *stream);
+
 }  // namespace qxt

@@ -12,18 +12,6 @@ namespace {
 
 constexpr int kThreads = 256;
 
-struct MxRows {
-    char *x;
-    int64_t x_stride;
-    uint32_t type;
-    char *values;
-    int64_t values_stride;
-    uint8_t *scales;
-    int64_t scales_stride;
-    uint32_t pieces;  // of eight elements, of all rows
-    FastDiv row;      // by the pieces of a row
-};
-
 template <bool FP8, bool VEC>
 __global__ __launch_bounds__(kThreads) void quantize_mx_kernel(MxRows a) {
     const uint32_t piece = blockIdx.x * kThreads + threadIdx.x;
@@ -34,7 +22,10 @@ __global__ __launch_bounds__(kThreads) void quantize_mx_kernel(MxRows a) {
     char *values = a.values + row * a.values_stride;
     if constexpr (FP8) *reinterpret_cast<u2 *>(values + static_cast<size_t>(at) * 8) = fp8_of(e, scale);
     else *reinterpret_cast<uint32_t *>(values + static_cast<size_t>(at) * 4) = fp4_of(e, scale);
-    if (at % 4 == 0) a.scales[row * a.scales_stride + at / 4] = static_cast<uint8_t>(scale);
+    uint8_t *scales = a.scales + row * a.scales_stride;
+    if (at % 4 == 0) scales[at / 4] = static_cast<uint8_t>(scale);
+    if (a.scale_pad != 0 && at + 1 == a.row.divisor)
+        for (uint32_t i = 0; i < a.scale_pad; ++i) scales[at / 4 + 1 + i] = 0;
 }
 
 template <bool FP8, bool VEC>
@@ -49,6 +40,8 @@ __global__ __launch_bounds__(kThreads) void dequantize_mx_kernel(MxRows a) {
     else e = fp4_values(*reinterpret_cast<const uint32_t *>(values + static_cast<size_t>(at) * 4), scale);
     store_eight<VEC>(a.type, a.x + row * a.x_stride, at * 8, e);
 }
+
+}  // namespace
 
 int run_mx(bool quantize, MxRows &a, uint32_t rows, uint32_t columns, uint32_t format, void *stream) {
     const char *name = quantize ? "quantize mx" : "dequantize mx";
@@ -85,7 +78,6 @@ int run_mx(bool quantize, MxRows &a, uint32_t rows, uint32_t columns, uint32_t f
                   grid, dim3(kThreads), 0, as_stream(stream), a);
 }
 
-}  // namespace
 }  // namespace qxt
 
 extern "C" {

@@ -97,6 +97,10 @@ __device__ __forceinline__ float gated(uint32_t gate, float g, float up) {
     return 0.5f * g * (1.0f + erff(g * 0.7071067812f)) * up;
 }
 
+// The tile kernels (qxt_mxfp4_tile.hip): every row stride of values below 2^23 bytes; every row of scales aligned to four
+// bytes and readable up to a multiple of four, with no NaN there.
+int mxfp4_tiles(const MxLinearArgs &a, int act, bool gated, hipStream_t stream);
+
 // Eight results of activation row m at columns n .. n + 7; block outputs: four neighbouring lanes hold a whole block.
 __device__ __forceinline__ void store_results(const MxLinearArgs &a, uint32_t m, uint32_t n, Eight e) {
     if (a.out_kind >= QXT_ROWS_MXFP8) {

@@ -124,6 +124,19 @@ int launch_stream(const MxLinearArgs &a, bool words, hipStream_t stream) {
                   dim3(static_cast<uint32_t>(grid)), dim3(64 * WAVES), 0, stream, a);
 }
 
+// Scales in rows of words, zeros behind the last.
+__global__ __launch_bounds__(256) void pad_scales_kernel(const uint8_t *from, int64_t stride, uint32_t blocks, uint32_t *to,
+                                                         uint32_t words, uint32_t total, FastDiv row) {
+    const uint32_t at = blockIdx.x * 256 + threadIdx.x;
+    if (at >= total) return;
+    const uint32_t y = fast_quotient(at, row), x = at - y * words;
+    uint32_t word = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j)
+        if (4 * x + j < blocks) word |= static_cast<uint32_t>(from[y * stride + 4 * x + j]) << (8 * j);
+    to[at] = word;
+}
+
 template <int ACT>
 int launch_act(const MxLinearArgs &a, bool is_gated, bool words, hipStream_t stream) {
     return is_gated ? launch_stream<ACT, true>(a, words, stream) : launch_stream<ACT, false>(a, words, stream);
@@ -143,10 +156,30 @@ MxOperand operand(const qxt_mx_matrix *m) {
             static_cast<int64_t>(m->scales_row_stride)};
 }
 
-// Bytes that quantised activations take in the workspace: values, then scales.
-size_t quantised_bytes(uint32_t m, uint32_t k, uint32_t format) {
-    return static_cast<size_t>(m) * mx_row_bytes(format, k) + static_cast<size_t>(m) * (k / kMxBlock);
-}
+size_t up16(size_t bytes) { return (bytes + 15) / 16 * 16; }
+uint32_t padded(uint32_t blocks) { return (blocks + 3) / 4 * 4; }
+
+// More activation rows than this go to the tile kernels.
+constexpr uint32_t kStreamRows = 16;
+
+// The workspace: quantised activations (values, scales in rows of words), and for the tile kernels room for each
+// operand's scales in rows of words.
+struct Workspace {
+    size_t values = 0, scales = 0, a_scales = 0, w_scales = 0, w_each = 0, bytes = 0;
+    Workspace(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, uint32_t format, bool floats) {
+        const size_t pad = padded(k / kMxBlock);
+        if (floats) {
+            scales = up16(m * mx_row_bytes(format, k));
+            bytes = scales + up16(m * pad);
+        }
+        if (m <= kStreamRows) return;
+        a_scales = bytes;
+        if (!floats) bytes += up16(m * pad);
+        w_scales = bytes;
+        w_each = up16(n * pad);
+        bytes += weights * w_each;
+    }
+};
 
 struct Floats {
     const void *x;
@@ -170,18 +203,19 @@ int run_linear(MxLinearArgs &a, const Floats *x, uint32_t format, bool is_gated,
     a.blocks = k / kMxBlock;
     if (a.m == 0 || a.n == 0) return QXT_OK;
     if (a.y == nullptr || (blocks_out && a.y_scales == nullptr)) return fail(QXT_INVALID_ARGUMENT, "%s: null pointer", name);
+    const Workspace room(a.m, a.n, k, is_gated ? 2 : 1, format, x != nullptr);
     if (x != nullptr) {
         const size_t element = type_bytes(x->type);
         if (x->x == nullptr) return fail(QXT_INVALID_ARGUMENT, "%s: null pointer", name);
         if (!aligned(x->x, element) || x->stride % element || (a.m > 1 && x->stride < k * element))
             return fail(QXT_INVALID_ARGUMENT, "%s: bad strides or alignment", name);
-        if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < quantised_bytes(a.m, k, format))
-            return fail(QXT_INVALID_ARGUMENT, "%s: workspace too small or not aligned to 16 bytes", name);
         a.a.values = static_cast<const char *>(workspace);
         a.a.stride = static_cast<int64_t>(mx_row_bytes(format, k));
-        a.a.scales = reinterpret_cast<const uint8_t *>(workspace) + static_cast<size_t>(a.m) * mx_row_bytes(format, k);
-        a.a.scale_stride = a.blocks;
+        a.a.scales = static_cast<const uint8_t *>(workspace) + room.scales;
+        a.a.scale_stride = padded(a.blocks);
     }
+    if (room.bytes != 0 && (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < room.bytes))
+        return fail(QXT_INVALID_ARGUMENT, "%s: workspace too small or not aligned to 16 bytes", name);
     if (int rc = check_operand(name, a.a, format, a.m, a.blocks)) return rc;
     for (int w = 0; w < (is_gated ? 2 : 1); ++w)
         if (int rc = check_operand(name, a.w[w], QXT_MX_FP4, a.n, a.blocks)) return rc;
@@ -194,16 +228,44 @@ int run_linear(MxLinearArgs &a, const Floats *x, uint32_t format, bool is_gated,
     if (int rc = injected(QXT_FAIL_SUBMISSION)) return rc;
     a.vec_out = aligned(a.y, 16) && a.y_stride % 16 == 0;
     if (x != nullptr) {
-        const int rc = qxt_quantize_mx(x->x, x->stride, x->type, const_cast<char *>(a.a.values), a.a.stride,
-                                       const_cast<uint8_t *>(a.a.scales), a.a.scale_stride, a.m, k, format, stream);
-        if (rc != QXT_OK) return rc;
+        MxRows rows{};
+        rows.x = static_cast<char *>(const_cast<void *>(x->x));
+        rows.x_stride = static_cast<int64_t>(x->stride);
+        rows.type = x->type;
+        rows.values = const_cast<char *>(a.a.values);
+        rows.values_stride = a.a.stride;
+        rows.scales = const_cast<uint8_t *>(a.a.scales);
+        rows.scales_stride = a.a.scale_stride;
+        rows.scale_pad = static_cast<uint32_t>(a.a.scale_stride) - a.blocks;
+        if (int rc = run_mx(true, rows, a.m, k, format, stream)) return rc;
     }
-    bool words = a.blocks % 4 == 0 && aligned(a.a.scales, 4) && a.a.scale_stride % 4 == 0;
-    for (int w = 0; w < (is_gated ? 2 : 1); ++w)
-        words = words && aligned(a.w[w].scales, 4) && a.w[w].scale_stride % 4 == 0;
     const hipStream_t s = as_stream(stream);
-    if (format == QXT_MX_FP4) return launch_act<kAct4>(a, is_gated, words, s);
-    return a.out_kind == QXT_TYPE_F32 ? launch_act<kAct8Parts>(a, is_gated, words, s) : launch_act<kAct8>(a, is_gated, words, s);
+    const int act = format == QXT_MX_FP4 ? kAct4 : a.out_kind == QXT_TYPE_F32 ? kAct8Parts : kAct8;
+    constexpr int64_t kTileStride = 1 << 23;
+    const bool tiles = a.m > kStreamRows && a.a.stride < kTileStride && a.w[0].stride < kTileStride && a.w[1].stride < kTileStride;
+    bool words = true;  // every row of scales in words
+    for (int o = 0; o < (is_gated ? 3 : 2); ++o) {
+        MxOperand &operand = o == 0 ? a.a : a.w[o - 1];
+        if (o == 0 && x != nullptr) continue;  // written so
+        if (a.blocks % 4 == 0 && aligned(operand.scales, 4) && operand.scale_stride % 4 == 0) continue;
+        words = false;
+        if (!tiles) break;
+        const uint32_t rows = o == 0 ? a.m : a.n, row = padded(a.blocks) / 4;
+        if (static_cast<uint64_t>(rows) * row > INT32_MAX) return fail(QXT_INVALID_ARGUMENT, "%s: too many blocks", name);
+        uint8_t *to = static_cast<uint8_t *>(workspace) + (o == 0 ? room.a_scales : room.w_scales + (o - 1) * room.w_each);
+        if (int rc = launch("pad_scales_kernel", pad_scales_kernel, dim3((rows * row + 255) / 256), dim3(256), 0, s, operand.scales,
+                            operand.scale_stride, a.blocks, reinterpret_cast<uint32_t *>(to), row, rows * row, fast_div(row)))
+            return rc;
+        operand.scales = to;
+        operand.scale_stride = 4 * row;
+    }
+    if (tiles) return mxfp4_tiles(a, act, is_gated, s);
+    words = words && a.blocks % 4 == 0;
+    switch (act) {
+        case kAct4: return launch_act<kAct4>(a, is_gated, words, s);
+        case kAct8: return launch_act<kAct8>(a, is_gated, words, s);
+        default: return launch_act<kAct8Parts>(a, is_gated, words, s);
+    }
 }
 
 MxLinearArgs linear_args(const qxt_mx_matrix *w, const qxt_mx_matrix *up, void *y, size_t ldy, uint32_t kind, uint32_t m, uint32_t n) {
@@ -225,9 +287,9 @@ using namespace qxt;
 
 extern "C" {
 
-size_t qxt_mxfp4_linear_workspace(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, uint32_t format) {
+size_t qxt_mxfp4_linear_workspace(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, uint32_t format, uint32_t floats) {
     if (!known_mx(format) || k == 0 || k % kMxBlock || weights == 0 || weights > 2 || m == 0 || n == 0) return 0;
-    return (quantised_bytes(m, k, format) + 15) / 16 * 16;
+    return Workspace(m, n, k, weights, format, floats != 0).bytes;
 }
 
 int qxt_mxfp4_gemm(const qxt_mx_matrix *a, uint32_t format, const qxt_mx_matrix *w, const float *bias, void *y, size_t ldy,
