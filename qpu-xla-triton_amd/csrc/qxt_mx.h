@@ -54,11 +54,11 @@ __device__ __forceinline__ Eight eight_of(uint32_t type, u4 a, u4 b) {
 // Two elements rounded to a half type, packed.
 __device__ __forceinline__ uint32_t half_pair(uint32_t type, float x, float y) {
     if (type == QXT_TYPE_BF16) {
-        const bf16_t a = static_cast<bf16_t>(x), b = static_cast<bf16_t>(y);
-        return __builtin_bit_cast(uint16_t, a) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, b)) << 16;
+        typedef bf16_t pair __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, pair{static_cast<bf16_t>(x), static_cast<bf16_t>(y)});
     }
-    const f16_t a = static_cast<f16_t>(x), b = static_cast<f16_t>(y);
-    return __builtin_bit_cast(uint16_t, a) | static_cast<uint32_t>(__builtin_bit_cast(uint16_t, b)) << 16;
+    typedef f16_t pair __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, pair{static_cast<f16_t>(x), static_cast<f16_t>(y)});
 }
 
 // Eight elements from / to element `index` of a row (16-byte pieces), or one by one where rows are not aligned.
@@ -151,15 +151,19 @@ __device__ __forceinline__ u2 fp8_of(const Eight &e, uint32_t scale) {
     return word;
 }
 
+// The largest of four neighbouring lanes (lanes 4i to 4i + 3, all of which take part).
+__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
+    v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xB1, 0xF, 0xF, true)));  // lanes 1 0 3 2
+    return max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x4E, 0xF, 0xF, true)));  // 2 3 0 1
+}
+
 // Four neighbouring lanes hold a block, eight elements each (all four take part).  Returns its scale byte.
 template <bool FP8>
 __device__ __forceinline__ uint32_t block_scale(const Eight &e) {
     uint32_t largest = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) largest = max(largest, magnitude(e.v[i]));
-    largest = max(largest, static_cast<uint32_t>(__shfl_xor(static_cast<int>(largest), 1, 4)));
-    largest = max(largest, static_cast<uint32_t>(__shfl_xor(static_cast<int>(largest), 2, 4)));
-    return mx_scale<FP8>(largest);
+    return mx_scale<FP8>(quad_max(largest));
 }
 
 // Values of eight elements.

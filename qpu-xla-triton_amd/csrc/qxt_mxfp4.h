@@ -2,6 +2,8 @@
 // the scaled matrix instruction, the gate functions and the store of results.
 #pragma once
 
+#include <type_traits>
+
 #include "qxt_mx.h"
 
 namespace qxt {
@@ -101,30 +103,48 @@ __device__ __forceinline__ float gated(uint32_t gate, float g, float up) {
 // bytes and readable up to a multiple of four, with no NaN there.
 int mxfp4_tiles(const MxLinearArgs &a, int act, bool gated, hipStream_t stream);
 
-// Eight results of activation row m at columns n .. n + 7; block outputs: four neighbouring lanes hold a whole block.
-__device__ __forceinline__ void store_results(const MxLinearArgs &a, uint32_t m, uint32_t n, Eight e) {
-    if (a.out_kind >= QXT_ROWS_MXFP8) {
-        const bool fp8 = a.out_kind == QXT_ROWS_MXFP8;
-        const uint32_t scale = fp8 ? block_scale<true>(e) : block_scale<false>(e);
-        if (m >= a.m || n >= a.n) return;
+// Eight results of activation row m at columns n .. n + 7 as KIND; block kinds: four neighbouring lanes hold a whole block.
+// `whole`: all eight columns lie in the row, and rows are aligned to 16 bytes.
+template <int KIND>
+__device__ __forceinline__ void store_results(const MxLinearArgs &a, uint32_t m, uint32_t n, bool whole, const Eight &e) {
+    if constexpr (KIND == QXT_ROWS_MXFP8 || KIND == QXT_ROWS_MXFP4) {
+        constexpr bool fp8 = KIND == QXT_ROWS_MXFP8;
+        const uint32_t scale = block_scale<fp8>(e);
+        if (m >= a.m || n >= a.n) return;  // (the row's length is a multiple of 32)
         char *row = a.y + m * a.y_stride;
-        if (fp8) *reinterpret_cast<u2 *>(row + n) = fp8_of(e, scale);
+        if constexpr (fp8) *reinterpret_cast<u2 *>(row + n) = fp8_of(e, scale);
         else *reinterpret_cast<uint32_t *>(row + n / 2) = fp4_of(e, scale);
         if (n % 32 == 0) a.y_scales[m * a.y_scale_stride + n / 32] = static_cast<uint8_t>(scale);
-        return;
-    }
-    if (m >= a.m || n >= a.n) return;
-    char *row = a.y + m * a.y_stride;
-    if (a.vec_out && n + 8 <= a.n) {
-        store_eight<true>(a.out_kind, row, n, e);
-        return;
-    }
+    } else {
+        if (m >= a.m) return;
+        char *row = a.y + m * a.y_stride;
+        if (whole) {
+            store_eight<true>(KIND, row, n, e);
+            return;
+        }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if (n + i >= a.n) return;
-        if (a.out_kind == QXT_TYPE_F32) reinterpret_cast<float *>(row)[n + i] = e.v[i];
-        else if (a.out_kind == QXT_TYPE_BF16) reinterpret_cast<bf16_t *>(row)[n + i] = static_cast<bf16_t>(e.v[i]);
-        else reinterpret_cast<f16_t *>(row)[n + i] = static_cast<f16_t>(e.v[i]);
+        for (int i = 0; i < 8; ++i) {
+            if (n + i >= a.n) return;
+            if (KIND == QXT_TYPE_F32) reinterpret_cast<float *>(row)[n + i] = e.v[i];
+            else if (KIND == QXT_TYPE_BF16) reinterpret_cast<bf16_t *>(row)[n + i] = static_cast<bf16_t>(e.v[i]);
+            else reinterpret_cast<f16_t *>(row)[n + i] = static_cast<f16_t>(e.v[i]);
+        }
+    }
+}
+
+// `f` with the output's kind as a constant.  (Float32 results are those of kAct8Parts and of kAct4.)
+template <int ACT, bool GATED, typename F>
+__device__ __forceinline__ void with_kind(uint32_t kind, F &&f) {
+    if constexpr (ACT != kAct8) {
+        if (kind == QXT_TYPE_F32) return f(std::integral_constant<int, QXT_TYPE_F32>{});
+    }
+    if constexpr (ACT != kAct8Parts) {
+        if (kind == QXT_TYPE_BF16) return f(std::integral_constant<int, QXT_TYPE_BF16>{});
+        if (kind == QXT_TYPE_F16) return f(std::integral_constant<int, QXT_TYPE_F16>{});
+        if constexpr (GATED) {
+            if (kind == QXT_ROWS_MXFP8) return f(std::integral_constant<int, QXT_ROWS_MXFP8>{});
+            f(std::integral_constant<int, QXT_ROWS_MXFP4>{});
+        }
     }
 }
 

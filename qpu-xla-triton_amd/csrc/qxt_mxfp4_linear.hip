@@ -88,30 +88,32 @@ __global__ __launch_bounds__(64 * WAVES) void mxfp4_stream_kernel(MxLinearArgs a
         for (int t = 0; t < RT; ++t) *reinterpret_cast<f4 *>(&sums[wave][w][t][r][4 * c]) = acc[w][t];
     __syncthreads();
     // 2 RT threads an activation row, eight columns each.
-    for (uint32_t i = threadIdx.x; i < 32 * RT; i += 64 * WAVES) {
-        const uint32_t m = i / (2 * RT), at = i % (2 * RT), n = n0 + 8 * at;
-        Eight e[W];
+    with_kind<ACT, GATED>(a.out_kind, [&](auto kind) {
+        for (uint32_t i = threadIdx.x; i < 32 * RT; i += 64 * WAVES) {
+            const uint32_t m = i / (2 * RT), at = i % (2 * RT), n = n0 + 8 * at;
+            Eight e[W];
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float *from = &sums[0][w][at / 2][m][8 * (at % 2)];
+            for (int w = 0; w < W; ++w) {
+                const float *from = &sums[0][w][at / 2][m][8 * (at % 2)];
 #pragma unroll
-            for (int x = 0; x < 8; ++x) e[w].v[x] = from[x];
-            for (int s = 1; s < WAVES; ++s) {
-                from += W * RT * 256;
+                for (int x = 0; x < 8; ++x) e[w].v[x] = from[x];
+                for (int s = 1; s < WAVES; ++s) {
+                    from += W * RT * 256;
 #pragma unroll
-                for (int x = 0; x < 8; ++x) e[w].v[x] += from[x];
+                    for (int x = 0; x < 8; ++x) e[w].v[x] += from[x];
+                }
             }
-        }
-        if constexpr (GATED) {
+            if constexpr (GATED) {
 #pragma unroll
-            for (int x = 0; x < 8; ++x) e[0].v[x] = gated(a.gate, e[0].v[x], e[1].v[x]);
-        } else if (a.bias != nullptr) {
+                for (int x = 0; x < 8; ++x) e[0].v[x] = gated(a.gate, e[0].v[x], e[1].v[x]);
+            } else if (a.bias != nullptr) {
 #pragma unroll
-            for (int x = 0; x < 8; ++x)
-                if (n + x < a.n) e[0].v[x] += a.bias[n + x];
+                for (int x = 0; x < 8; ++x)
+                    if (n + x < a.n) e[0].v[x] += a.bias[n + x];
+            }
+            store_results<decltype(kind)::value>(a, m0 + m, n, a.vec_out && n + 8 <= a.n, e[0]);
         }
-        store_results(a, m0 + m, n, e[0]);
-    }
+    });
 }
 
 template <int ACT, bool GATED>

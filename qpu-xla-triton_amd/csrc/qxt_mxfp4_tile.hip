@@ -31,9 +31,6 @@ __device__ __forceinline__ void dma16(uint64_t base, uint32_t offset, uint32_t t
 __device__ __forceinline__ void dma16_from(const char *src, uint32_t to) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(src) : "memory", "m0");
 }
-__device__ __forceinline__ void dma4_from(const uint8_t *src, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(to), "v"(src) : "memory", "m0");
-}
 #pragma clang diagnostic pop
 
 // Wait until all but the wave's N youngest loads are done, and all of its LDS reads.
@@ -44,7 +41,9 @@ __device__ __forceinline__ void landed() {
 }
 __device__ __forceinline__ void meet() {
     asm volatile("" : : : "memory");
+    __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
     asm volatile("" : : : "memory");
 }
 
@@ -59,26 +58,36 @@ __device__ __forceinline__ void xcd_tile(uint32_t id, uint32_t tm, uint32_t tn, 
     tx = in / rows;
 }
 
-template <int ACT, bool GATED, int TW, int TA, int WN, int WM, int RING>
+template <int ACT, bool GATED, int TW, int TA, int WN, int WM, int SUB, int RING>
 struct Tiles {
     static constexpr bool FP8 = ACT != kAct4;
     static constexpr int WAVES = WN * WM, THREADS = 64 * WAVES;
     static constexpr int BN = 16 * TW * WN, BM = 16 * TA * WM;  // weight rows (of both weights), activation rows
-    static constexpr int ROW = FP8 ? 128 : 64;                 // bytes of an activation row a stage
-    static constexpr int W_BYTES = BN * 64, A_BYTES = BM * ROW, S_BYTES = (BN + BM) * 4;
-    static constexpr int STAGE = W_BYTES + A_BYTES + S_BYTES;
+    static constexpr int W_ROW = 64 * SUB, A_ROW = (FP8 ? 128 : 64) * SUB;  // bytes of a row a stage
+    static constexpr int W_BYTES = BN * W_ROW, A_BYTES = BM * A_ROW, STAGE = W_BYTES + A_BYTES;
     static constexpr int W_LOADS = W_BYTES / 1024, A_LOADS = A_BYTES / 1024, S_LOADS = (BN + BM) / 64;
     static constexpr int W_EACH = W_LOADS / WAVES, A_EACH = A_LOADS / WAVES, S_EACH = (S_LOADS + WAVES - 1) / WAVES;
-    static constexpr int LOADS = W_EACH + A_EACH + S_EACH;  // of each wave a stage
+    static constexpr int LOADS = W_EACH + A_EACH;           // of each wave a stage, but for scales
+    static constexpr int GROUP = 4 / SUB;                   // stages that share a row's 16 bytes of scales
+    static constexpr int SCALES = (BN + BM) * 16;           // bytes of a group
     static constexpr int OUT = 16 * TW / (GATED ? 2 : 1);   // result columns of a wave
     static constexpr int OUT_ROW = OUT + 4;                 // floats, in LDS
-    static constexpr int LDS = RING * STAGE > WAVES * 16 * OUT_ROW * 4 ? RING * STAGE : WAVES * 16 * OUT_ROW * 4;
+    static constexpr int OPERANDS = RING * STAGE + 2 * SCALES, RESULTS = WAVES * 16 * OUT_ROW * 4;
+    static constexpr int LDS = OPERANDS > RESULTS ? OPERANDS : RESULTS;
     static_assert(W_LOADS % WAVES == 0 && A_LOADS % WAVES == 0 && LDS <= 160 * 1024, "tile shape");
+    static_assert(RING <= GROUP, "a group's scales are fetched with the last stage of the group before");
 };
 
-template <int ACT, bool GATED, int TW, int TA, int WN, int WM, int RING>
+// Where piece p (16 bytes) of row r of a stage lies, in pieces from the row's start.
+template <int ROW>
+__device__ __forceinline__ uint32_t turned(uint32_t p, uint32_t r) {
+    static_assert(ROW == 64 || ROW == 128, "");
+    return ROW == 64 ? p ^ (r / 2 % 4) : p ^ (r % 8);
+}
+
+template <int ACT, bool GATED, int TW, int TA, int WN, int WM, int SUB, int RING>
 __global__ __launch_bounds__(64 * WN * WM) void mxfp4_tile_kernel(MxLinearArgs a) {
-    typedef Tiles<ACT, GATED, TW, TA, WN, WM, RING> T;
+    typedef Tiles<ACT, GATED, TW, TA, WN, WM, SUB, RING> T;
     __shared__ __attribute__((aligned(16))) char lds[T::LDS];
     const uint32_t lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % WN, wm = wave / WN;
@@ -88,29 +97,28 @@ __global__ __launch_bounds__(64 * WN * WM) void mxfp4_tile_kernel(MxLinearArgs a
     const uint32_t m0 = ty * T::BM, n0 = tx * kColumns;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)));
 
-    // What this wave fetches: weight row tiles wave * W_EACH + i, activation pieces wave * A_EACH + i, scales of 64 rows.
-    // Rows past the last are the last one again: their results are not stored.
-    const uint32_t wrow = lane / 4, wpiece = (lane % 4) ^ (wrow / 2 % 4);
+    // What this wave fetches: loads wave * W_EACH + i of the weights, wave * A_EACH + i of the activations, each of whole
+    // rows, and 16 bytes of the scales of 64 rows.  Rows past the last are the last one again: their results are not stored.
+    constexpr uint32_t kWPieces = T::W_ROW / 16, kWRows = 64 / kWPieces, kAPieces = T::A_ROW / 16, kARows = 64 / kAPieces;
+    const uint32_t wrow = lane / kWPieces, arow = lane / kAPieces;
+    const uint32_t wpiece = turned<T::W_ROW>(lane % kWPieces, wrow);
+    const uint32_t apiece = turned<T::A_ROW>(lane % kAPieces, arow);
+    static_assert(kWRows >= 8 && (kARows >= 8), "a load's rows turn alike");
     uint64_t w_base[T::W_EACH];
     uint32_t w_off[T::W_EACH];
 #pragma unroll
     for (int i = 0; i < T::W_EACH; ++i) {
-        const uint32_t t = wave * T::W_EACH + i, which = GATED ? t & 1 : 0, first = n0 + 16 * (GATED ? t / 2 : t);
-        const MxOperand &w = a.w[0], &u = a.w[1];
-        const int64_t stride = which ? u.stride : w.stride;
-        const uint32_t base = min(first, a.n - 1);
-        w_base[i] = reinterpret_cast<uint64_t>((which ? u.values : w.values) + base * stride);
-        w_off[i] = min(wrow, a.n - 1 - base) * static_cast<uint32_t>(stride) + wpiece * 16;
+        const uint32_t row = (wave * T::W_EACH + i) * kWRows, t = row / 16, which = GATED ? t & 1 : 0;
+        const uint32_t first = min(n0 + (GATED ? t / 2 * 16 + row % 16 : row), a.n - 1);
+        const int64_t stride = which ? a.w[1].stride : a.w[0].stride;
+        w_base[i] = reinterpret_cast<uint64_t>((which ? a.w[1].values : a.w[0].values) + first * stride);
+        w_off[i] = min(wrow, a.n - 1 - first) * static_cast<uint32_t>(stride) + wpiece * 16;
     }
-    constexpr uint32_t kPieces = T::ROW / 16, kRowsPerLoad = 64 / kPieces;
-    const uint32_t arow = lane / kPieces, apiece = (lane % kPieces) ^ (T::FP8 ? arow % 8 : arow / 2 % 4);
-    uint64_t a_base = reinterpret_cast<uint64_t>(a.a.values + m0 * a.a.stride);
+    const uint64_t a_base = reinterpret_cast<uint64_t>(a.a.values + m0 * a.a.stride);
     uint32_t a_off[T::A_EACH];
 #pragma unroll
-    for (int i = 0; i < T::A_EACH; ++i) {
-        const uint32_t row = (wave * T::A_EACH + i) * kRowsPerLoad + arow;
-        a_off[i] = min(row, a.m - 1 - m0) * static_cast<uint32_t>(a.a.stride) + apiece * 16;
-    }
+    for (int i = 0; i < T::A_EACH; ++i)
+        a_off[i] = min((wave * T::A_EACH + i) * kARows + arow, a.m - 1 - m0) * static_cast<uint32_t>(a.a.stride) + apiece * 16;
     const uint8_t *scales[T::S_EACH];
 #pragma unroll
     for (int i = 0; i < T::S_EACH; ++i) {
@@ -121,36 +129,45 @@ __global__ __launch_bounds__(64 * WN * WM) void mxfp4_tile_kernel(MxLinearArgs a
         scales[i] = o.scales + at * o.scale_stride;
         if (GATED && row < T::BN && t % 2 == 1) scales[i] = a.w[1].scales + at * a.w[1].scale_stride;
     }
-    const uint32_t stages = (a.blocks + 3) / 4, blocks = a.blocks;
-    auto fetch = [&](uint32_t s, uint32_t buffer) {
-        const uint32_t to = lds0 + buffer * T::STAGE;
-        const bool whole = 4 * s + 4 <= blocks;
-#pragma unroll
-        for (int i = 0; i < T::W_EACH; ++i) {
-            const uint32_t at = to + (wave * T::W_EACH + i) * 1024;
-            if (whole) {
-                dma16(w_base[i] + s * 64ull, w_off[i], at);
-            } else {
-                const char *src = reinterpret_cast<const char *>(w_base[i] + s * 64ull + w_off[i]);
-                dma16_from(4 * s + wpiece < blocks ? src : reinterpret_cast<const char *>(&kZeroPiece), at);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < T::A_EACH; ++i) {
-            const uint32_t at = to + T::W_BYTES + (wave * T::A_EACH + i) * 1024;
-            if (whole) {
-                dma16(a_base + s * static_cast<uint64_t>(T::ROW), a_off[i], at);
-            } else {
-                const char *src = reinterpret_cast<const char *>(a_base + s * static_cast<uint64_t>(T::ROW) + a_off[i]);
-                const uint32_t block = 4 * s + (T::FP8 ? apiece / 2 : apiece);
-                dma16_from(block < blocks ? src : reinterpret_cast<const char *>(&kZeroPiece), at);
-            }
-        }
+    const uint32_t blocks = a.blocks, steps = (blocks + 3) / 4, stages = (steps + SUB - 1) / SUB;
+    // Scales of blocks 16 g to 16 g + 15.  (Waves past the last load fetch that one again, to the same place with the same
+    // bytes.)
+    auto fetch_scales = [&](uint32_t g) {
+        const uint32_t at = RING * T::STAGE + g % 2 * T::SCALES;
 #pragma unroll
         for (int i = 0; i < T::S_EACH; ++i) {
-            // (Waves past the last load fetch that one again, to the same place with the same bytes.)
-            const uint32_t at = to + T::W_BYTES + T::A_BYTES + min(wave * T::S_EACH + i, T::S_LOADS - 1u) * 256;
-            dma4_from(scales[i] + s * 4ull, at);
+            const uint32_t to = at + min(wave * T::S_EACH + i, T::S_LOADS - 1u) * 1024;
+            if (16 * g + 16 <= blocks) {
+                dma16_from(reinterpret_cast<const char *>(scales[i] + g * 16ull), lds0 + to);
+            } else {  // the last words of a row, and nothing behind them
+                u4 v;
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j)
+                    v[j] = 16 * g + 4 * j < blocks ? *reinterpret_cast<const uint32_t *>(scales[i] + g * 16ull + 4 * j) : 0u;
+                *reinterpret_cast<u4 *>(lds + to + lane * 16) = v;
+            }
+        }
+    };
+    auto fetch = [&](uint32_t s, uint32_t buffer) {
+        if (s % T::GROUP == T::GROUP - 1 && (s + 1) * SUB < steps) fetch_scales((s + 1) / T::GROUP);
+        const uint32_t to = lds0 + buffer * T::STAGE;
+        const uint32_t w_to = to + wave * T::W_EACH * 1024, a_to = to + T::W_BYTES + wave * T::A_EACH * 1024;
+        const uint64_t w_skip = s * static_cast<uint64_t>(T::W_ROW), a_from = a_base + s * static_cast<uint64_t>(T::A_ROW);
+        if (4 * SUB * (s + 1) <= blocks) {
+#pragma unroll
+            for (int i = 0; i < T::W_EACH; ++i) dma16(w_base[i] + w_skip, w_off[i], w_to + i * 1024);
+#pragma unroll
+            for (int i = 0; i < T::A_EACH; ++i) dma16(a_from, a_off[i], a_to + i * 1024);
+        } else {  // the last stage of a K that does not fill it: zeros past the rows' ends
+            const char *zero = reinterpret_cast<const char *>(&kZeroPiece);
+#pragma unroll
+            for (int i = 0; i < T::W_EACH; ++i)
+                dma16_from(4 * SUB * s + wpiece < blocks ? reinterpret_cast<const char *>(w_base[i] + w_skip + w_off[i]) : zero,
+                           w_to + i * 1024);
+            const bool in = 4 * SUB * s + (T::FP8 ? apiece / 2 : apiece) < blocks;
+#pragma unroll
+            for (int i = 0; i < T::A_EACH; ++i)
+                dma16_from(in ? reinterpret_cast<const char *>(a_from + a_off[i]) : zero, a_to + i * 1024);
         }
     };
 
@@ -160,47 +177,94 @@ __global__ __launch_bounds__(64 * WN * WM) void mxfp4_tile_kernel(MxLinearArgs a
 #pragma unroll
         for (int j = 0; j < TA; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
 
-    // Where this lane's operands lie in a stage.
-    const uint32_t w_at = (wn * TW * 16 + r) * 64 + (c ^ (r / 2 % 4)) * 16;
-    const uint32_t a_row = wm * TA * 16 + r;
-    const uint32_t a_lo = T::W_BYTES + a_row * T::ROW + (T::FP8 ? c ^ (r % 8) : c ^ (r / 2 % 4)) * 16;
-    const uint32_t a_hi = T::FP8 ? T::W_BYTES + a_row * T::ROW + ((4 + c) ^ (r % 8)) * 16 : a_lo;
-    const uint32_t ws_at = T::W_BYTES + T::A_BYTES + (wn * TW * 16 + r) * 4 + c;
-    const uint32_t as_at = T::W_BYTES + T::A_BYTES + (T::BN + a_row) * 4 + c;
-
-#pragma unroll
-    for (int s = 0; s < RING - 1; ++s)
-        if (s < static_cast<int>(stages)) fetch(s, s);
-    uint32_t buffer = 0;
-    for (uint32_t s = 0; s < stages; ++s) {
-        // Stage s has landed when at most the younger ones that are in flight are left.
-        const uint32_t younger = min(stages - 1 - s, static_cast<uint32_t>(RING - 2));
-        if (RING > 3 && younger == 2) landed<2 * T::LOADS>();
-        else if (younger == 1) landed<T::LOADS>();
-        else landed<0>();
-        meet();  // all of it, from every wave; and every wave has read stage s - 1, whose buffer the next fetch fills
-        if (s + RING - 1 < stages) fetch(s + RING - 1, buffer == 0 ? RING - 1 : buffer - 1);
+    // Where this lane's operands of a stage's first step lie, and its scales of a group's.  (The pieces of the second step
+    // lie where bit 6 of the address is turned.)
+    const uint32_t w_row = wn * TW * 16 + r, a_row = wm * TA * 16 + r;
+    const uint32_t w_at = w_row * T::W_ROW + turned<T::W_ROW>(c, r) * 16;
+    const uint32_t a_lo = T::W_BYTES + a_row * T::A_ROW + turned<T::A_ROW>(c, r) * 16;
+    const uint32_t a_hi = T::W_BYTES + a_row * T::A_ROW + turned<T::A_ROW>(4 + c, r) * 16;
+    const uint32_t ws_at = RING * T::STAGE + w_row * 16 + c, as_at = RING * T::STAGE + (T::BN + a_row) * 16 + c;
+    uint32_t wscale[TW], ascale[TA];
+    u4 w[TW], lo[TA], hi[TA];
+    auto read = [&](uint32_t step, uint32_t buffer) {
         const char *from = lds + buffer * T::STAGE;
-        uint32_t wscale[TW], ascale[TA];
-        u4 w[TW], lo[TA], hi[TA];
+        const char *from_scales = lds + step / 4 % 2 * T::SCALES + step % 4 * 4;
+        const uint32_t turn = step % SUB * 64;
 #pragma unroll
         for (int j = 0; j < TA; ++j) {
-            lo[j] = *reinterpret_cast<const u4 *>(from + a_lo + j * 16 * T::ROW);
-            hi[j] = T::FP8 ? *reinterpret_cast<const u4 *>(from + a_hi + j * 16 * T::ROW) : lo[j];
-            ascale[j] = *reinterpret_cast<const uint8_t *>(from + as_at + j * 64);
+            lo[j] = *reinterpret_cast<const u4 *>(from + (a_lo ^ turn) + j * 16 * T::A_ROW);
+            hi[j] = T::FP8 ? *reinterpret_cast<const u4 *>(from + a_hi + j * 16 * T::A_ROW) : lo[j];
+            ascale[j] = *reinterpret_cast<const uint8_t *>(from_scales + as_at + j * 256);
         }
 #pragma unroll
         for (int i = 0; i < TW; ++i) {
-            w[i] = *reinterpret_cast<const u4 *>(from + w_at + i * 1024);
-            wscale[i] = *reinterpret_cast<const uint8_t *>(from + ws_at + i * 64);
+            w[i] = *reinterpret_cast<const u4 *>(from + (w_at ^ turn) + i * 16 * T::W_ROW);
+            wscale[i] = *reinterpret_cast<const uint8_t *>(from_scales + ws_at + i * 256);
         }
+    };
+    auto multiply = [&]() {
 #pragma unroll
         for (int j = 0; j < TA; ++j) {
             const ActPiece<ACT> act(lo[j], hi[j]);
 #pragma unroll
             for (int i = 0; i < TW; ++i) acc[i][j] = mx_mfma<ACT, 0>(w[i], act, acc[i][j], wscale[i], ascale[j]);
         }
-        buffer = buffer + 1 == RING ? 0 : buffer + 1;
+    };
+    // All but the youngest `younger` stages in flight have landed.  (A group's scales are fetched before a stage's rows,
+    // so they have landed with them, or before.)
+    auto landed_but = [&](uint32_t younger) {
+        if (RING > 3 && younger == 2) landed<2 * T::LOADS>();
+        else if (RING > 2 && younger == 1) landed<T::LOADS>();
+        else landed<0>();
+    };
+
+    fetch_scales(0);
+#pragma unroll
+    for (int s = 0; s < RING - 1; ++s)
+        if (s < static_cast<int>(stages)) fetch(s, s);
+    uint32_t buffer = 0;
+    if constexpr (T::WAVES == 8) {
+        // The waves of a SIMD take turns: waves 0 - 3 read a step's operands while waves 4 - 7 multiply those of the one
+        // before, and the other way round.  A buffer is free once waves 4 - 7 have read it; the next stage has to be there
+        // when waves 0 - 3 begin to read it, so they wait after their products, waves 4 - 7 (a phase behind) after their
+        // reads.
+        const bool second = wave >= 4;
+        landed_but(min(stages - 1, static_cast<uint32_t>(RING - 2)));
+        meet();
+        if (second) meet();
+        uint32_t s = 0;
+        for (uint32_t step = 0; step < stages * SUB; ++step) {
+            // In flight behind stage s + 1 once the next fetch is issued.
+            const uint32_t younger = s + 2 < stages ? min(stages - 2 - s, static_cast<uint32_t>(RING - 2)) : 0u;
+            const bool last = SUB == 1 || step % SUB == SUB - 1;  // of its stage
+            if ((SUB == 1 || step % SUB == 0) && s + RING - 1 < stages) fetch(s + RING - 1, buffer == 0 ? RING - 1 : buffer - 1);
+            read(step, buffer);
+            if (second && last) landed_but(younger);
+            else landed<63>();
+            meet();
+            __builtin_amdgcn_s_setprio(1);
+            multiply();
+            __builtin_amdgcn_s_setprio(0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (!second && last) landed_but(younger);
+            meet();
+            if (last) {
+                ++s;
+                buffer = buffer + 1 == RING ? 0 : buffer + 1;
+            }
+        }
+        if (!second) meet();
+    } else {
+        for (uint32_t s = 0; s < stages; ++s) {
+            landed_but(min(stages - 1 - s, static_cast<uint32_t>(RING - 2)));
+            meet();  // all of stage s, from every wave; and every wave has read stage s - 1, whose buffer the fetch fills
+            if (s + RING - 1 < stages) fetch(s + RING - 1, buffer == 0 ? RING - 1 : buffer - 1);
+            for (uint32_t u = 0; u < SUB; ++u) {
+                read(s * SUB + u, buffer);
+                multiply();
+            }
+            buffer = buffer + 1 == RING ? 0 : buffer + 1;
+        }
     }
 
     // Results by 16 rows through LDS, so that a lane stores eight neighbouring columns.
@@ -213,53 +277,55 @@ __global__ __launch_bounds__(64 * WN * WM) void mxfp4_tile_kernel(MxLinearArgs a
 #pragma unroll
         for (int e = 0; e < 8; ++e) bias[e] = a.bias != nullptr && out_n + e < a.n ? a.bias[out_n + e] : 0.0f;
     }
+    const bool whole = a.vec_out && out_n + 8 <= a.n;
+    with_kind<ACT, GATED>(a.out_kind, [&](auto kind) {
 #pragma unroll
-    for (int j = 0; j < TA; ++j) {
+        for (int j = 0; j < TA; ++j) {
 #pragma unroll
-        for (int i = 0; i < TW / (GATED ? 2 : 1); ++i) {
-            f4 v;
-            if constexpr (GATED) {
+            for (int i = 0; i < TW / (GATED ? 2 : 1); ++i) {
+                f4 v;
+                if constexpr (GATED) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = gated(a.gate, acc[2 * i][j][e], acc[2 * i + 1][j][e]);
-            } else {
-                v = acc[i][j];
+                    for (int e = 0; e < 4; ++e) v[e] = gated(a.gate, acc[2 * i][j][e], acc[2 * i + 1][j][e]);
+                } else {
+                    v = acc[i][j];
+                }
+                *reinterpret_cast<f4 *>(mine + r * T::OUT_ROW + 16 * i + 4 * c) = v;
             }
-            *reinterpret_cast<f4 *>(mine + r * T::OUT_ROW + 16 * i + 4 * c) = v;
-        }
-        __builtin_amdgcn_wave_barrier();
-        asm volatile("" : : : "memory");
+            __builtin_amdgcn_wave_barrier();
+            asm volatile("" : : : "memory");
 #pragma unroll
-        for (uint32_t step = 0; step < 16; step += kRows) {
-            const uint32_t row = step + lane / kEights;
-            const float *from = mine + row * T::OUT_ROW + lane % kEights * 8;
-            const f4 x = *reinterpret_cast<const f4 *>(from), y = *reinterpret_cast<const f4 *>(from + 4);
-            Eight e{{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}};
-            if constexpr (!GATED) {
-                if (a.bias != nullptr) {
+            for (uint32_t step = 0; step < 16; step += kRows) {
+                const uint32_t row = step + lane / kEights;
+                const float *from = mine + row * T::OUT_ROW + lane % kEights * 8;
+                const f4 x = *reinterpret_cast<const f4 *>(from), y = *reinterpret_cast<const f4 *>(from + 4);
+                Eight e{{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}};
+                if constexpr (!GATED) {
 #pragma unroll
                     for (int q = 0; q < 8; ++q) e.v[q] += bias[q];
                 }
+                store_results<decltype(kind)::value>(a, m0 + wm * TA * 16 + j * 16 + row, out_n, whole, e);
             }
-            store_results(a, m0 + wm * TA * 16 + j * 16 + row, out_n, e);
+            asm volatile("" : : : "memory");
+            __builtin_amdgcn_wave_barrier();
         }
-        asm volatile("" : : : "memory");
-        __builtin_amdgcn_wave_barrier();
-    }
+    });
 }
 
-template <int ACT, bool GATED, int TW, int TA, int WN, int WM, int RING>
+template <int ACT, bool GATED, int TW, int TA, int WN, int WM, int SUB, int RING>
 int launch_tile(const MxLinearArgs &a, hipStream_t stream) {
-    typedef Tiles<ACT, GATED, TW, TA, WN, WM, RING> T;
+    typedef Tiles<ACT, GATED, TW, TA, WN, WM, SUB, RING> T;
     constexpr uint32_t columns = T::BN / (GATED ? 2 : 1);
     const uint64_t grid = static_cast<uint64_t>((a.m + T::BM - 1) / T::BM) * ((a.n + columns - 1) / columns);
     if (grid > INT32_MAX) return fail(QXT_INVALID_ARGUMENT, "mxfp4 linear: too many outputs");
-    return launch("mxfp4_tile_kernel", mxfp4_tile_kernel<ACT, GATED, TW, TA, WN, WM, RING>, dim3(static_cast<uint32_t>(grid)),
+    return launch("mxfp4_tile_kernel", mxfp4_tile_kernel<ACT, GATED, TW, TA, WN, WM, SUB, RING>, dim3(static_cast<uint32_t>(grid)),
                   dim3(T::THREADS), 0, stream, a);
 }
 
 template <int ACT, bool GATED>
 int launch_tiles(const MxLinearArgs &a, hipStream_t stream) {
-    return launch_tile<ACT, GATED, 8, 4, 2, 4, 3>(a, stream);
+    if constexpr (ACT == kAct4) return launch_tile<ACT, GATED, 8, 4, 2, 4, 2, 2>(a, stream);
+    else return launch_tile<ACT, GATED, 8, 4, 2, 4, 1, 3>(a, stream);
 }
 
 }  // namespace
