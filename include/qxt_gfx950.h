@@ -573,8 +573,9 @@ int qxt_add_rms_norm(const void *x, size_t x_row_stride, uint32_t x_type, const 
  * y_type: QXT_TYPE_*, rounded once.  qxt_mxfp4_linear takes activations as floats and
  * quantises them as qxt_quantize_mx does.  workspace (16-byte aligned):
  * qxt_mxfp4_linear_workspace() bytes for one weight (floats: 1 where activations are
- * floats), free again when the stream has passed the call. */
-size_t qxt_mxfp4_linear_workspace(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, uint32_t format, uint32_t floats);
+ * floats; out_kind: y_type, or h_kind below), free again when the stream has passed the call. */
+size_t qxt_mxfp4_linear_workspace(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, uint32_t format, uint32_t floats,
+                                  uint32_t out_kind);
 int qxt_mxfp4_gemm(const qxt_mx_matrix *a, uint32_t format, const qxt_mx_matrix *w, const float *bias, void *y, size_t ldy,
                    uint32_t y_type, uint32_t m, uint32_t n, uint32_t k, void *workspace, size_t workspace_bytes, void *stream);
 int qxt_mxfp4_linear(const void *x, size_t ldx, uint32_t x_type, uint32_t format, const qxt_mx_matrix *w, const float *bias,

@@ -26,6 +26,9 @@ struct MxLinearArgs {
     uint32_t m, n, blocks;
     uint32_t out_kind, gate;
     uint32_t vec_out;  // y's rows are aligned to 16 bytes
+    // Tile kernels that split K: every split's sums, fp32 [splits, weights, m, part_row].
+    float *parts;
+    uint32_t part_row, splits, split_steps;  // split_steps: K / 128 of a split, a multiple of four
 };
 
 typedef int i8 __attribute__((ext_vector_type(8)));
@@ -99,9 +102,18 @@ __device__ __forceinline__ float gated(uint32_t gate, float g, float up) {
     return 0.5f * g * (1.0f + erff(g * 0.7071067812f)) * up;
 }
 
-// The tile kernels (qxt_mxfp4_tile.hip): every row stride of values below 2^23 bytes; every row of scales aligned to four
-// bytes and readable up to a multiple of four, with no NaN there.
-int mxfp4_tiles(const MxLinearArgs &a, int act, bool gated, hipStream_t stream);
+// How the tile kernels (qxt_mxfp4_tile.hip) take a product: the tile, and into how many parts K is split.
+struct TilePlan {
+    uint32_t tile, splits;
+};
+TilePlan plan_tiles(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, int act);
+inline int act_of(uint32_t format, uint32_t out_kind) {
+    return format == QXT_MX_FP4 ? kAct4 : out_kind == QXT_TYPE_F32 ? kAct8Parts : kAct8;
+}
+inline uint32_t part_row(uint32_t n) { return (n + 7) / 8 * 8; }
+// Every row stride of values below 2^23 bytes; every row of scales aligned to four bytes and readable up to a multiple of
+// four, with no NaN there; `a.parts` of the plan's size where it splits.
+int mxfp4_tiles(MxLinearArgs &a, int act, bool gated, const TilePlan &plan, hipStream_t stream);
 
 // Eight results of activation row m at columns n .. n + 7 as KIND; block kinds: four neighbouring lanes hold a whole block.
 // `whole`: all eight columns lie in the row, and rows are aligned to 16 bytes.

@@ -165,10 +165,10 @@ uint32_t padded(uint32_t blocks) { return (blocks + 3) / 4 * 4; }
 constexpr uint32_t kStreamRows = 16;
 
 // The workspace: quantised activations (values, scales in rows of words), and for the tile kernels room for each
-// operand's scales in rows of words.
+// operand's scales in rows of words, and the sums of the parts of K.
 struct Workspace {
-    size_t values = 0, scales = 0, a_scales = 0, w_scales = 0, w_each = 0, bytes = 0;
-    Workspace(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, uint32_t format, bool floats) {
+    size_t scales = 0, a_scales = 0, w_scales = 0, w_each = 0, parts = 0, bytes = 0;
+    Workspace(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, uint32_t format, uint32_t out_kind, bool floats) {
         const size_t pad = padded(k / kMxBlock);
         if (floats) {
             scales = up16(m * mx_row_bytes(format, k));
@@ -180,6 +180,9 @@ struct Workspace {
         w_scales = bytes;
         w_each = up16(n * pad);
         bytes += weights * w_each;
+        parts = bytes;
+        const TilePlan plan = plan_tiles(m, n, k, weights, act_of(format, out_kind));
+        if (plan.splits > 1) bytes += static_cast<size_t>(plan.splits) * weights * m * part_row(n) * sizeof(float);
     }
 };
 
@@ -205,7 +208,7 @@ int run_linear(MxLinearArgs &a, const Floats *x, uint32_t format, bool is_gated,
     a.blocks = k / kMxBlock;
     if (a.m == 0 || a.n == 0) return QXT_OK;
     if (a.y == nullptr || (blocks_out && a.y_scales == nullptr)) return fail(QXT_INVALID_ARGUMENT, "%s: null pointer", name);
-    const Workspace room(a.m, a.n, k, is_gated ? 2 : 1, format, x != nullptr);
+    const Workspace room(a.m, a.n, k, is_gated ? 2 : 1, format, a.out_kind, x != nullptr);
     if (x != nullptr) {
         const size_t element = type_bytes(x->type);
         if (x->x == nullptr) return fail(QXT_INVALID_ARGUMENT, "%s: null pointer", name);
@@ -242,7 +245,7 @@ int run_linear(MxLinearArgs &a, const Floats *x, uint32_t format, bool is_gated,
         if (int rc = run_mx(true, rows, a.m, k, format, stream)) return rc;
     }
     const hipStream_t s = as_stream(stream);
-    const int act = format == QXT_MX_FP4 ? kAct4 : a.out_kind == QXT_TYPE_F32 ? kAct8Parts : kAct8;
+    const int act = act_of(format, a.out_kind);
     constexpr int64_t kTileStride = 1 << 23;
     const bool tiles = a.m > kStreamRows && a.a.stride < kTileStride && a.w[0].stride < kTileStride && a.w[1].stride < kTileStride;
     bool words = true;  // every row of scales in words
@@ -261,7 +264,10 @@ int run_linear(MxLinearArgs &a, const Floats *x, uint32_t format, bool is_gated,
         operand.scales = to;
         operand.scale_stride = 4 * row;
     }
-    if (tiles) return mxfp4_tiles(a, act, is_gated, s);
+    if (tiles) {
+        a.parts = reinterpret_cast<float *>(static_cast<char *>(workspace) + room.parts);
+        return mxfp4_tiles(a, act, is_gated, plan_tiles(a.m, a.n, k, is_gated ? 2 : 1, act), s);
+    }
     words = words && a.blocks % 4 == 0;
     switch (act) {
         case kAct4: return launch_act<kAct4>(a, is_gated, words, s);
@@ -289,9 +295,10 @@ using namespace qxt;
 
 extern "C" {
 
-size_t qxt_mxfp4_linear_workspace(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, uint32_t format, uint32_t floats) {
+size_t qxt_mxfp4_linear_workspace(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, uint32_t format, uint32_t floats,
+                                  uint32_t out_kind) {
     if (!known_mx(format) || k == 0 || k % kMxBlock || weights == 0 || weights > 2 || m == 0 || n == 0) return 0;
-    return Workspace(m, n, k, weights, format, floats != 0).bytes;
+    return Workspace(m, n, k, weights, format, out_kind, floats != 0).bytes;
 }
 
 int qxt_mxfp4_gemm(const qxt_mx_matrix *a, uint32_t format, const qxt_mx_matrix *w, const float *bias, void *y, size_t ldy,

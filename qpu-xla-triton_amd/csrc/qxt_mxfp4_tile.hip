@@ -65,16 +65,17 @@ struct Tiles {
     static constexpr int BN = 16 * TW * WN, BM = 16 * TA * WM;  // weight rows (of both weights), activation rows
     static constexpr int W_ROW = 64 * SUB, A_ROW = (FP8 ? 128 : 64) * SUB;  // bytes of a row a stage
     static constexpr int W_BYTES = BN * W_ROW, A_BYTES = BM * A_ROW, STAGE = W_BYTES + A_BYTES;
-    static constexpr int W_LOADS = W_BYTES / 1024, A_LOADS = A_BYTES / 1024, S_LOADS = (BN + BM) / 64;
+    static constexpr int W_LOADS = W_BYTES / 1024, A_LOADS = A_BYTES / 1024, S_LOADS = (BN + BM + 63) / 64;
     static constexpr int W_EACH = W_LOADS / WAVES, A_EACH = A_LOADS / WAVES, S_EACH = (S_LOADS + WAVES - 1) / WAVES;
     static constexpr int LOADS = W_EACH + A_EACH;           // of each wave a stage, but for scales
     static constexpr int GROUP = 4 / SUB;                   // stages that share a row's 16 bytes of scales
-    static constexpr int SCALES = (BN + BM) * 16;           // bytes of a group
+    static constexpr int SCALES = S_LOADS * 1024;          // bytes of a group
     static constexpr int OUT = 16 * TW / (GATED ? 2 : 1);   // result columns of a wave
     static constexpr int OUT_ROW = OUT + 4;                 // floats, in LDS
     static constexpr int OPERANDS = RING * STAGE + 2 * SCALES, RESULTS = WAVES * 16 * OUT_ROW * 4;
     static constexpr int LDS = OPERANDS > RESULTS ? OPERANDS : RESULTS;
     static_assert(W_LOADS % WAVES == 0 && A_LOADS % WAVES == 0 && LDS <= 160 * 1024, "tile shape");
+    static_assert(OUT % 32 == 0 && OUT <= 128, "a wave's results hold whole blocks, and 64 lanes at most 16 rows of them");
     static_assert(RING <= GROUP, "a group's scales are fetched with the last stage of the group before");
 };
 
@@ -93,8 +94,10 @@ __global__ __launch_bounds__(64 * WN * WM) void mxfp4_tile_kernel(MxLinearArgs a
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % WN, wm = wave / WN;
     constexpr uint32_t kColumns = T::BN / (GATED ? 2 : 1);  // result columns of the workgroup
     uint32_t ty, tx;
-    xcd_tile(blockIdx.x, (a.m + T::BM - 1) / T::BM, (a.n + kColumns - 1) / kColumns, 4, ty, tx);
+    const uint32_t tiles = gridDim.x / a.splits, split = blockIdx.x / tiles;
+    xcd_tile(blockIdx.x - split * tiles, (a.m + T::BM - 1) / T::BM, (a.n + kColumns - 1) / kColumns, 4, ty, tx);
     const uint32_t m0 = ty * T::BM, n0 = tx * kColumns;
+    const uint32_t first_block = split * a.split_steps * 4, blocks = min(a.blocks - first_block, a.split_steps * 4);
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)));
 
     // What this wave fetches: loads wave * W_EACH + i of the weights, wave * A_EACH + i of the activations, each of whole
@@ -111,10 +114,10 @@ __global__ __launch_bounds__(64 * WN * WM) void mxfp4_tile_kernel(MxLinearArgs a
         const uint32_t row = (wave * T::W_EACH + i) * kWRows, t = row / 16, which = GATED ? t & 1 : 0;
         const uint32_t first = min(n0 + (GATED ? t / 2 * 16 + row % 16 : row), a.n - 1);
         const int64_t stride = which ? a.w[1].stride : a.w[0].stride;
-        w_base[i] = reinterpret_cast<uint64_t>((which ? a.w[1].values : a.w[0].values) + first * stride);
+        w_base[i] = reinterpret_cast<uint64_t>((which ? a.w[1].values : a.w[0].values) + first * stride + first_block * 16ull);
         w_off[i] = min(wrow, a.n - 1 - first) * static_cast<uint32_t>(stride) + wpiece * 16;
     }
-    const uint64_t a_base = reinterpret_cast<uint64_t>(a.a.values + m0 * a.a.stride);
+    const uint64_t a_base = reinterpret_cast<uint64_t>(a.a.values + m0 * a.a.stride + first_block * (T::FP8 ? 32ull : 16ull));
     uint32_t a_off[T::A_EACH];
 #pragma unroll
     for (int i = 0; i < T::A_EACH; ++i)
@@ -128,8 +131,9 @@ __global__ __launch_bounds__(64 * WN * WM) void mxfp4_tile_kernel(MxLinearArgs a
         const MxOperand &o = row >= T::BN ? a.a : a.w[0];
         scales[i] = o.scales + at * o.scale_stride;
         if (GATED && row < T::BN && t % 2 == 1) scales[i] = a.w[1].scales + at * a.w[1].scale_stride;
+        scales[i] += first_block;
     }
-    const uint32_t blocks = a.blocks, steps = (blocks + 3) / 4, stages = (steps + SUB - 1) / SUB;
+    const uint32_t steps = (blocks + 3) / 4, stages = (steps + SUB - 1) / SUB;
     // Scales of blocks 16 g to 16 g + 15.  (Waves past the last load fetch that one again, to the same place with the same
     // bytes.)
     auto fetch_scales = [&](uint32_t g) {
@@ -267,6 +271,23 @@ __global__ __launch_bounds__(64 * WN * WM) void mxfp4_tile_kernel(MxLinearArgs a
         }
     }
 
+    if (a.splits > 1) {  // sums of a part of K, joined by another kernel: four columns a lane
+        const uint64_t plane = static_cast<uint64_t>(a.m) * a.part_row;
+        float *to = a.parts + split * (GATED ? 2 : 1) * plane;
+#pragma unroll
+        for (int j = 0; j < TA; ++j) {
+            const uint32_t m = m0 + (wm * TA + j) * 16 + r;
+            if (m >= a.m) continue;
+#pragma unroll
+            for (int i = 0; i < TW; ++i) {
+                const uint32_t n = n0 + wn * T::OUT + (GATED ? i / 2 : i) * 16 + 4 * c;
+                if (n < a.part_row)
+                    *reinterpret_cast<f4 *>(to + (GATED && i % 2 ? plane : 0) + static_cast<uint64_t>(m) * a.part_row + n) = acc[i][j];
+            }
+        }
+        return;
+    }
+
     // Results by 16 rows through LDS, so that a lane stores eight neighbouring columns.
     __syncthreads();
     float *mine = reinterpret_cast<float *>(lds) + wave * 16 * T::OUT_ROW;
@@ -312,29 +333,115 @@ __global__ __launch_bounds__(64 * WN * WM) void mxfp4_tile_kernel(MxLinearArgs a
     });
 }
 
-template <int ACT, bool GATED, int TW, int TA, int WN, int WM, int SUB, int RING>
-int launch_tile(const MxLinearArgs &a, hipStream_t stream) {
-    typedef Tiles<ACT, GATED, TW, TA, WN, WM, SUB, RING> T;
-    constexpr uint32_t columns = T::BN / (GATED ? 2 : 1);
-    const uint64_t grid = static_cast<uint64_t>((a.m + T::BM - 1) / T::BM) * ((a.n + columns - 1) / columns);
-    if (grid > INT32_MAX) return fail(QXT_INVALID_ARGUMENT, "mxfp4 linear: too many outputs");
-    return launch("mxfp4_tile_kernel", mxfp4_tile_kernel<ACT, GATED, TW, TA, WN, WM, SUB, RING>, dim3(static_cast<uint32_t>(grid)),
-                  dim3(T::THREADS), 0, stream, a);
+// Joins the parts of K: a thread adds up eight columns of a row, in the order of the parts.
+template <int ACT, bool GATED>
+__global__ __launch_bounds__(256) void mxfp4_join_kernel(MxLinearArgs a, FastDiv row) {
+    const uint32_t at = blockIdx.x * 256 + threadIdx.x, m = fast_quotient(at, row), n = (at - m * row.divisor) * 8;
+    if (m >= a.m) return;  // (rows of four lanes leave together where blocks are stored)
+    const uint64_t plane = static_cast<uint64_t>(a.m) * a.part_row;
+    const float *from = a.parts + static_cast<uint64_t>(m) * a.part_row + n;
+    f4 sum[GATED ? 2 : 1][2] = {};
+    for (uint32_t s = 0; s < a.splits; ++s)
+#pragma unroll
+        for (int w = 0; w < (GATED ? 2 : 1); ++w, from += plane)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) sum[w][h] += *reinterpret_cast<const f4 *>(from + 4 * h);
+    Eight e;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        e.v[i] = sum[0][i / 4][i % 4];
+        if constexpr (GATED) e.v[i] = gated(a.gate, e.v[i], sum[1][i / 4][i % 4]);
+        else if (a.bias != nullptr && n + i < a.n) e.v[i] += a.bias[n + i];
+    }
+    with_kind<ACT, GATED>(a.out_kind, [&](auto kind) {
+        store_results<decltype(kind)::value>(a, m, n, a.vec_out && n + 8 <= a.n, e);
+    });
 }
 
-template <int ACT, bool GATED>
-int launch_tiles(const MxLinearArgs &a, hipStream_t stream) {
-    if constexpr (ACT == kAct4) return launch_tile<ACT, GATED, 8, 4, 2, 4, 2, 2>(a, stream);
-    else return launch_tile<ACT, GATED, 8, 4, 2, 4, 1, 3>(a, stream);
+template <int ACT, bool GATED, int TW, int TA, int WN, int WM, int SUB, int RING>
+int launch_tile(MxLinearArgs &a, uint32_t splits, hipStream_t stream) {
+    typedef Tiles<ACT, GATED, TW, TA, WN, WM, SUB, RING> T;
+    constexpr uint32_t columns = T::BN / (GATED ? 2 : 1);
+    const uint32_t groups = (a.blocks + 15) / 16;
+    a.split_steps = (groups + splits - 1) / splits * 4;
+    a.splits = (groups + a.split_steps / 4 - 1) / (a.split_steps / 4);  // none is empty
+    a.part_row = part_row(a.n);
+    const uint64_t grid = static_cast<uint64_t>((a.m + T::BM - 1) / T::BM) * ((a.n + columns - 1) / columns) * a.splits;
+    const uint32_t row = a.part_row / 8;
+    const uint64_t joins = (static_cast<uint64_t>(a.m) * row + 255) / 256;
+    if (grid > INT32_MAX || (a.splits > 1 && joins * 256 > INT32_MAX)) return fail(QXT_INVALID_ARGUMENT, "mxfp4 linear: too many outputs");
+    const int rc = launch("mxfp4_tile_kernel", mxfp4_tile_kernel<ACT, GATED, TW, TA, WN, WM, SUB, RING>,
+                          dim3(static_cast<uint32_t>(grid)), dim3(T::THREADS), 0, stream, a);
+    if (rc != QXT_OK || a.splits == 1) return rc;
+    return launch("mxfp4_join_kernel", mxfp4_join_kernel<ACT, GATED>, dim3(static_cast<uint32_t>(joins)), dim3(256), 0, stream, a,
+                  fast_div(row));
 }
+
+// The tiles of a plan, weight rows by activation rows.  The first has eight waves, which take turns, the others four, and
+// two to four workgroups a CU.
+constexpr uint32_t kTiles = 5;
+constexpr uint32_t kTileRows[kTiles][2] = {{256, 256}, {128, 128}, {128, 64}, {64, 64}, {128, 32}};
+
+template <int ACT, bool GATED>
+int launch_tiles(MxLinearArgs &a, const TilePlan &plan, hipStream_t stream) {
+    // 4-bit rows take two steps of K a stage, for whole cache lines.
+    constexpr int SUB = ACT == kAct4 ? 2 : 1, RING = ACT == kAct4 ? 2 : 3, DEEP = ACT == kAct4 ? 2 : 4;
+    switch (plan.tile) {
+        case 0: return launch_tile<ACT, GATED, 8, 4, 2, 4, SUB, RING>(a, plan.splits, stream);
+        case 1: return launch_tile<ACT, GATED, 4, 4, 2, 2, SUB, RING>(a, plan.splits, stream);
+        case 2: return launch_tile<ACT, GATED, 4, 2, 2, 2, SUB, RING>(a, plan.splits, stream);
+        case 3: return launch_tile<ACT, GATED, 4, 1, 1, 4, SUB, DEEP>(a, plan.splits, stream);
+        default: return launch_tile<ACT, GATED, 4, 1, 2, 2, SUB, DEEP>(a, plan.splits, stream);
+    }
+}
+
+// Estimated microseconds of a launch: a step of 128 elements of K takes `step` where few workgroups run and half of that
+// plus `share` for each 256 workgroups where many do; `edge`: filling the ring and storing the results, for each 256
+// workgroups.  Fitted to 4093 measured calls (17 to 4096 rows, K 512 to 14336, 1024 to 14336 columns, every tile and up to
+// 16 parts; rms error 8 %); the least estimate is on average 2 % slower than the fastest of them, at most 24 %.
+struct TileCost {
+    float step, share, edge;
+};
+constexpr TileCost kCosts[3][kTiles] = {
+    {{0.92f, 0.65f, 5.4f}, {0.37f, 0.26f, 2.3f}, {0.29f, 0.18f, 1.5f}, {0.25f, 0.11f, 0.7f}, {0.27f, 0.15f, 0.8f}},  // kAct4
+    {{1.10f, 0.87f, 5.5f}, {0.61f, 0.36f, 2.2f}, {0.36f, 0.25f, 1.6f}, {0.30f, 0.17f, 0.8f}, {0.29f, 0.21f, 1.1f}},  // kAct8
+    {{2.36f, 1.53f, 6.1f}, {1.01f, 0.61f, 2.9f}, {0.58f, 0.34f, 2.1f}, {0.44f, 0.25f, 1.3f}, {0.44f, 0.26f, 1.6f}},  // kAct8Parts
+};
+// The second kernel that parts of K need, and a megabyte of their sums.
+constexpr float kJoin = 2.7f, kJoinMegabyte = 0.09f;
+constexpr uint32_t kMostSplits = 16;
 
 }  // namespace
 
-int mxfp4_tiles(const MxLinearArgs &a, int act, bool gated, hipStream_t stream) {
+TilePlan plan_tiles(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, int act) {
+    TilePlan best{0, 1};
+    float least = 0.0f;
+    const uint32_t steps = (k + 127) / 128, groups = (steps + 3) / 4;
+    const float sums = static_cast<float>(weights) * static_cast<float>(m) * static_cast<float>(n) * 4e-6f;
+    for (uint32_t t = 0; t < kTiles; ++t) {
+        const float tiles = static_cast<float>((m + kTileRows[t][1] - 1) / kTileRows[t][1]) *
+                            static_cast<float>((static_cast<uint64_t>(n) * weights + kTileRows[t][0] - 1) / kTileRows[t][0]);
+        for (uint32_t wanted = 1; wanted <= kMostSplits && wanted <= groups; ++wanted) {
+            const uint32_t each = (groups + wanted - 1) / wanted, splits = (groups + each - 1) / each;
+            if (splits < wanted) continue;  // the same as fewer
+            const TileCost &c = kCosts[act][t];
+            const float load = tiles * static_cast<float>(splits) / 256.0f, depth = static_cast<float>(min(4 * each, steps));
+            float cost = depth * fmaxf(c.step, 0.5f * c.step + c.share * load) + c.edge * fmaxf(load, 1.0f);
+            if (splits > 1) cost += kJoin + kJoinMegabyte * 2.0f * static_cast<float>(splits) * sums;
+            if (least == 0.0f || cost < least) {
+                least = cost;
+                best = {t, splits};
+            }
+        }
+    }
+    return best;
+}
+
+int mxfp4_tiles(MxLinearArgs &a, int act, bool gated, const TilePlan &plan, hipStream_t stream) {
     switch (act) {
-        case kAct4: return gated ? launch_tiles<kAct4, true>(a, stream) : launch_tiles<kAct4, false>(a, stream);
-        case kAct8: return gated ? launch_tiles<kAct8, true>(a, stream) : launch_tiles<kAct8, false>(a, stream);
-        default: return gated ? launch_tiles<kAct8Parts, true>(a, stream) : launch_tiles<kAct8Parts, false>(a, stream);
+        case kAct4: return gated ? launch_tiles<kAct4, true>(a, plan, stream) : launch_tiles<kAct4, false>(a, plan, stream);
+        case kAct8: return gated ? launch_tiles<kAct8, true>(a, plan, stream) : launch_tiles<kAct8, false>(a, plan, stream);
+        default: return gated ? launch_tiles<kAct8Parts, true>(a, plan, stream) : launch_tiles<kAct8Parts, false>(a, plan, stream);
     }
 }
 

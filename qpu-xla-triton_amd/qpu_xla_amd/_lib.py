@@ -221,7 +221,7 @@ SIGNATURES: dict[str, tuple[Any, list[Any]]] = {
     "qxt_dequantize_mx": (c_int, [_P, _SZ, _P, _SZ, _P, _SZ, _U, _U, _U, _U, _P]),
     "qxt_add_rms_norm": (
         c_int, [_P, _SZ, _U, _P, _SZ, _U, _P, _SZ, _P, c_double, _P, _SZ, _P, _SZ, _U, _U, _U, _P]),
-    "qxt_mxfp4_linear_workspace": (_SZ, [_U] * 6),
+    "qxt_mxfp4_linear_workspace": (_SZ, [_U] * 7),
     "qxt_mxfp4_gemm": (c_int, [_P, _U, _P, _P, _P, _SZ, _U, _U, _U, _U, _P, _SZ, _P]),
     "qxt_mxfp4_linear": (c_int, [_P, _SZ, _U, _U, _P, _P, _P, _SZ, _U, _U, _U, _U, _P, _SZ, _P]),
     "qxt_mxfp4_gated_gemm": (

@@ -105,9 +105,9 @@ def _float_out(name: str, out: torch.Tensor | None, dtype: torch.dtype, rows: in
     return out, code, stride
 
 
-def _workspace(rows: int, columns: int, depth: int, weights: int, fmt: int, floats: int, stream: Any,
+def _workspace(rows: int, columns: int, depth: int, weights: int, fmt: int, floats: int, kind: int, stream: Any,
                device: torch.device) -> tuple[torch.Tensor | None, int]:
-    size = (_lib._lib or _lib.load()).qxt_mxfp4_linear_workspace(rows, columns, depth, weights, fmt, floats)
+    size = (_lib._lib or _lib.load()).qxt_mxfp4_linear_workspace(rows, columns, depth, weights, fmt, floats, kind)
     return workspace_for(stream, size, device), size
 
 
@@ -132,7 +132,7 @@ def mxfp4_gemm(
     dtype = dtype if dtype is not None else torch.float32 if out is None else out.dtype
     out, code, stride = _float_out(name, out, dtype, m, n, stream, a_values.device)
     require_current_gpu(name, a_values, a_scales, w_values, w_scales, bias, out)
-    workspace, size = _workspace(m, n, k, 1, fmt, 0, stream, a_values.device)
+    workspace, size = _workspace(m, n, k, 1, fmt, 0, code, stream, a_values.device)
     _lib.call("qxt_mxfp4_gemm", a, fmt, w, bias_at, out.data_ptr(), stride, code, m, n, k,
               None if workspace is None else workspace.data_ptr(), size, stream_handle(stream))
     return out
@@ -160,7 +160,7 @@ def mxfp4_linear(
     dtype = dtype if dtype is not None else x.dtype if out is None else out.dtype
     out, code, stride = _float_out(name, out, dtype, m, n, stream, x.device)
     require_current_gpu(name, x, w_values, w_scales, bias, out)
-    workspace, size = _workspace(m, n, k, 1, fmt, 1, stream, x.device)
+    workspace, size = _workspace(m, n, k, 1, fmt, 1, code, stream, x.device)
     _lib.call("qxt_mxfp4_linear", x.data_ptr(), x_stride, x_code, fmt, w, bias_at, out.data_ptr(), stride, code, m, n, k,
               None if workspace is None else workspace.data_ptr(), size, stream_handle(stream))
     return out
@@ -222,7 +222,7 @@ def mxfp4_gated_gemm(
     function = _gate_function(name, gate)
     result, tensors, kind, places = _gated_out(name, output, out, m, n, stream, a_values.device)
     require_current_gpu(name, a_values, a_scales, gate_values, gate_scales, up_values, up_scales, *tensors)
-    workspace, size = _workspace(m, n, k, 2, fmt, 0, stream, a_values.device)
+    workspace, size = _workspace(m, n, k, 2, fmt, 0, kind, stream, a_values.device)
     _lib.call("qxt_mxfp4_gated_gemm", a, fmt, gate_at, up_at, function, *places, kind, m, n, k,
               None if workspace is None else workspace.data_ptr(), size, stream_handle(stream))
     return result
@@ -251,7 +251,7 @@ def mxfp4_gated_linear(
         output = out.dtype if isinstance(out, torch.Tensor) else x.dtype
     result, tensors, kind, places = _gated_out(name, output, out, m, n, stream, x.device)
     require_current_gpu(name, x, gate_values, gate_scales, up_values, up_scales, *tensors)
-    workspace, size = _workspace(m, n, k, 2, fmt, 1, stream, x.device)
+    workspace, size = _workspace(m, n, k, 2, fmt, 1, kind, stream, x.device)
     _lib.call("qxt_mxfp4_gated_linear", x.data_ptr(), x_stride, x_code, fmt, gate_at, up_at, function, *places, kind, m, n, k,
               None if workspace is None else workspace.data_ptr(), size, stream_handle(stream))
     return result

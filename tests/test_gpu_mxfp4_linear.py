@@ -44,7 +44,9 @@ def _stored(x, fmt):
 # One token, tiles with one row or column too many, K of one block, blocks that do not fill an instruction, long K, many rows.
 SHAPES = [(1, 32, 32), (1, 5632, 2048), (1, 17, 96), (2, 64, 128), (3, 100, 160), (8, 257, 512), (15, 48, 1056), (16, 96, 2048),
           (17, 33, 544), (31, 130, 4096), (33, 200, 352), (64, 512, 1024), (77, 300, 3008), (128, 256, 2048), (130, 129, 640),
-          (200, 1030, 96), (257, 260, 1152), (300, 520, 4096), (515, 777, 256)]
+          (200, 1030, 96), (257, 260, 1152), (300, 520, 4096), (515, 777, 256),
+          # K in many parts (whole groups of 512 elements or not), every tile.
+          (20, 96, 9248), (70, 200, 8192), (150, 130, 6176), (260, 300, 12288), (1030, 2060, 544), (2050, 2310, 256), (700, 1500, 1024)]
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -81,7 +83,7 @@ def test_linear_quantises_as_the_quantiser_does(shape, dtype, fmt) -> None:
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("gate", ["silu", "gelu"])
 @pytest.mark.parametrize("shape", [(1, 64, 2048), (1, 5632, 512), (5, 96, 160), (16, 160, 1024), (20, 33, 96), (40, 96, 4096), (130, 352, 640),
-                                   (260, 288, 1024)])
+                                   (260, 288, 1024), (24, 64, 8224), (100, 160, 6144), (1100, 1312, 256), (600, 1440, 512)])
 def test_gated_against_the_definition(shape, gate, fmt) -> None:
     m, n, k = shape
     a, g, u = _operands(m, n, k, fmt, weights=2)
