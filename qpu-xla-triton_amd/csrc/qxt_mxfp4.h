@@ -26,6 +26,7 @@ struct MxLinearArgs {
     uint32_t m, n, blocks;
     uint32_t out_kind, gate;
     uint32_t vec_out;  // y's rows are aligned to 16 bytes
+    uint32_t a_words;  // activations' rows of scales are words
     // Tile kernels that split K: every split's sums, fp32 [splits, weights, m, part_row].
     float *parts;
     uint32_t part_row, splits, split_steps;  // split_steps: K / 128 of a split, a multiple of four
@@ -100,6 +101,45 @@ __device__ __forceinline__ float gated(uint32_t gate, float g, float up) {
         return g * __builtin_amdgcn_rcpf(1.0f + e) * up;
     }
     return 0.5f * g * (1.0f + erff(g * 0.7071067812f)) * up;
+}
+
+// Source of what lies past a row's last block.
+__device__ __constant__ const uint4 kZeroPiece = {};
+
+// 64 lanes' 16 or 4 bytes, from a wave-uniform address plus each lane's offset or from each lane's address, to LDS at `to`
+// + 16 (or 4) * lane.  Inline
+// assembly because the compiler waits for every such load in flight before it reads any of LDS; the waits here are the
+// kernel's own.  There is no register output.
+// (The compiler warns that it may not preserve m0; it has no other use for it here.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void dma16(uint64_t base, uint32_t offset, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(offset), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void dma16_from(const char *src, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(src) : "memory", "m0");
+}
+__device__ __forceinline__ void dma4_from(const char *src, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(to), "v"(src) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// Wait until all but the wave's N youngest loads are done, and all of its LDS reads.
+template <int N>
+__device__ __forceinline__ void landed() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(N) : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+__device__ __forceinline__ void reads_done() {
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+__device__ __forceinline__ void meet() {
+    asm volatile("" : : : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" : : : "memory");
 }
 
 // How the tile kernels (qxt_mxfp4_tile.hip) take a product: the tile, and into how many parts K is split.

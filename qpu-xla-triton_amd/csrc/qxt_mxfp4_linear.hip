@@ -9,99 +9,218 @@
 namespace qxt {
 namespace {
 
-// A workgroup owns 16 RT weight rows (of each weight) and 16 activation rows; its waves take every WAVES-th
-// group of 512 elements of K, read their operands straight into registers, and add their sums through LDS.  Within a
-// group lane (r, c) holds blocks 4c .. 4c + 3 of its rows, one for each of four instructions (K may be permuted as long
-// as both operands agree), so that a word of scales serves all four.
-template <int ACT, bool GATED, int RT, int WAVES, bool WORDS>
-__global__ __launch_bounds__(64 * WAVES) void mxfp4_stream_kernel(MxLinearArgs a) {
-    constexpr int W = GATED ? 2 : 1;
-    __shared__ __attribute__((aligned(16))) float sums[WAVES][W][RT][16][16];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, c = lane >> 4;
-    const uint32_t column_tiles = (a.n + 16 * RT - 1) / (16 * RT);
-    const uint32_t mt = blockIdx.x / column_tiles, nt = blockIdx.x - mt * column_tiles;
-    const uint32_t m0 = mt * 16, n0 = nt * 16 * RT;
-    const uint32_t arow = min(m0 + r, a.m - 1);  // rows past the last are computed from it and not stored
-    const char *av = a.a.values + arow * a.a.stride;
-    const uint8_t *as = a.a.scales + arow * a.a.scale_stride;
-    const char *wv[W][RT];
-    const uint8_t *ws[W][RT];
-#pragma unroll
-    for (int w = 0; w < W; ++w)
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            const uint32_t row = min(n0 + 16 * t + r, a.n - 1);
-            wv[w][t] = a.w[w].values + row * a.w[w].stride;
-            ws[w][t] = a.w[w].scales + row * a.w[w].scale_stride;
+// Few activation rows: bound by the weights' bytes.  A workgroup owns 16 RT rows of each weight and all of the (at most 16)
+// activation rows, which lie in LDS for the whole of K, and its waves take every WAVES-th unit of 256 elements of K: 128
+// bytes of each weight row, a cache line, fetched by DMA into one of the wave's SLOTS own LDS buffers, where it lies so
+// that the reads of a piece (16 bytes) over 16 rows touch all banks.  Nothing but its own loads is waited for by a wave
+// until the sums of all are added up.  Float activations come into LDS as they are and are quantised there, by every
+// workgroup for itself: less than a launch where they are few.  Activations too are fetched by DMA, ahead of the first
+// weights: waiting for a load into registers would wait for every weight requested after it.
+struct Floats {
+    const char *x;
+    int64_t stride;
+    uint32_t type;
+};
+
+// LDS of the activations: rows of whole units and 16 bytes more (so that rows start in different banks), then their scales.
+struct ActRows {
+    uint32_t row, scale_row, scales, bytes;
+};
+template <int ACT>
+__host__ __device__ inline ActRows act_rows(uint32_t m, uint32_t blocks) {
+    const uint32_t units = (blocks + 7) / 8;
+    ActRows r;
+    r.row = units * (ACT == kAct4 ? 128 : 256) + 16;
+    r.scale_row = units * 8 + 4;
+    r.scales = m * r.row;
+    r.bytes = (r.scales + m * r.scale_row + 15) / 16 * 16;
+    return r;
+}
+
+// Bytes of a float row in LDS.
+__host__ __device__ inline uint32_t float_row(uint32_t type, uint32_t blocks) { return blocks * (type == QXT_TYPE_F32 ? 128 : 64); }
+
+template <int ACT, bool GATED, bool FLOATS, bool WORDS, int RT, int WAVES, int SLOTS>
+__global__ __launch_bounds__(64 * WAVES) void mxfp4_stream_kernel(MxLinearArgs a, Floats f) {
+    constexpr int W = GATED ? 2 : 1, TILES = W * RT, THREADS = 64 * WAVES;
+    constexpr int DATA = 2 * TILES, SCALES = WORDS ? (TILES + 1) / 2 : 0, LOADS = DATA + SCALES;  // loads of a unit
+    constexpr uint32_t kSlot = TILES * 2048 + (TILES + 1) / 2 * 256;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const uint32_t lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t n0 = blockIdx.x * 16 * RT, blocks = a.blocks, units = (blocks + 7) / 8;
+    const ActRows rows = act_rows<ACT>(a.m, blocks);
+    const uint32_t slots = rows.bytes + wave * SLOTS * kSlot;
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)));
+
+    // Rows of `bytes` (a multiple of 16) to LDS, `pitch` apart: the waves take 1024 bytes in turn.
+    auto fetch_rows = [&](const char *src, int64_t stride, uint32_t bytes, uint32_t to, uint32_t pitch) {
+        const uint32_t loads = (bytes + 1023) / 1024;
+        uint32_t row = 0, at = wave;
+        while (at >= loads && row < a.m) at -= loads, ++row;
+        while (row < a.m) {
+            const uint32_t byte = at * 1024 + lane * 16;
+            if (byte < bytes) dma16_from(src + row * stride + byte, lds0 + to + row * pitch + at * 1024);
+            at += WAVES;
+            while (at >= loads && row < a.m) at -= loads, ++row;
         }
-    auto piece = [](const char *p, bool in) { return in ? *reinterpret_cast<const u4 *>(p) : u4{0, 0, 0, 0}; };
-    auto scale_word = [&](const uint8_t *p, uint32_t b) {
-        if (WORDS) return b < a.blocks ? *reinterpret_cast<const uint32_t *>(p + b) : 0u;
-        uint32_t word = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (b + j < a.blocks) word |= static_cast<uint32_t>(p[b + j]) << (8 * j);
-        return word;
     };
-    f4 acc[W][RT] = {};
-    for (uint32_t first = 16 * wave; first < a.blocks; first += 16 * WAVES) {
-        const uint32_t b0 = first + 4 * c;
-        u4 wp[W][RT][4], ap[4][2];
-        uint32_t wscale[W][RT];
-#pragma unroll
-        for (int w = 0; w < W; ++w)
-#pragma unroll
-            for (int t = 0; t < RT; ++t) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) wp[w][t][j] = piece(wv[w][t] + static_cast<size_t>(b0 + j) * 16, b0 + j < a.blocks);
-                wscale[w][t] = scale_word(ws[w][t], b0);
-            }
-        const uint32_t ascale = scale_word(as, b0);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (ACT != kAct4) {
-                const uint32_t lo = first + 4 * (c >> 1) + j, hi = lo + 8;
-                ap[j][0] = piece(av + static_cast<size_t>(lo) * 32 + 16 * (c & 1), lo < a.blocks);
-                ap[j][1] = piece(av + static_cast<size_t>(hi) * 32 + 16 * (c & 1), hi < a.blocks);
-            } else {
-                ap[j][0] = piece(av + static_cast<size_t>(b0 + j) * 16, b0 + j < a.blocks);
-                ap[j][1] = ap[j][0];
+    const uint32_t raw = rows.bytes + WAVES * SLOTS * kSlot, raw_row = FLOATS ? float_row(f.type, blocks) : 0;
+    if constexpr (FLOATS) {
+        fetch_rows(f.x, f.stride, raw_row, raw, raw_row);
+    } else {
+        if (a.a_words) {
+            for (uint32_t row = 0; row < a.m; ++row)
+                for (uint32_t at = wave * 64; at < blocks / 4; at += THREADS)
+                    if (at + lane < blocks / 4)
+                        dma4_from(reinterpret_cast<const char *>(a.a.scales + row * a.a.scale_stride + (at + lane) * 4),
+                                  lds0 + rows.scales + row * rows.scale_row + at * 4);
+        } else {  // through registers: nothing else is in flight yet
+            for (uint32_t i = threadIdx.x; i < a.m * blocks; i += THREADS) {
+                const uint32_t row = i / blocks, at = i - row * blocks;
+                lds[rows.scales + row * rows.scale_row + at] = static_cast<char>(a.a.scales[row * a.a.scale_stride + at]);
             }
         }
-        auto step = [&](auto jc) {
-            constexpr int j = decltype(jc)::value;
-            const ActPiece<ACT> act(ap[j][0], ap[j][1]);
-#pragma unroll
-            for (int w = 0; w < W; ++w)
-#pragma unroll
-                for (int t = 0; t < RT; ++t)
-                    acc[w][t] = mx_mfma<ACT, j>(wp[w][t][j], act, acc[w][t], wscale[w][t], ascale);
-        };
-        step(std::integral_constant<int, 0>{});
-        step(std::integral_constant<int, 1>{});
-        step(std::integral_constant<int, 2>{});
-        step(std::integral_constant<int, 3>{});
+        fetch_rows(a.a.values, a.a.stride, blocks * (ACT == kAct4 ? 16 : 32), 0, rows.row);
     }
+
+    // A unit's weights: a load is eight rows of 128 bytes; its scales: a load is 32 rows of eight bytes.
+    const uint32_t wrow = lane / 8, wpiece = (lane % 8) ^ wrow;
+    const char *w_from[TILES][2];
+    const uint8_t *s_from[(TILES + 1) / 2];
 #pragma unroll
-    for (int w = 0; w < W; ++w)
+    for (int t = 0; t < TILES; ++t)
 #pragma unroll
-        for (int t = 0; t < RT; ++t) *reinterpret_cast<f4 *>(&sums[wave][w][t][r][4 * c]) = acc[w][t];
+        for (int h = 0; h < 2; ++h) {
+            const MxOperand &o = a.w[t % W];
+            w_from[t][h] = o.values + min(n0 + t / W * 16 + h * 8 + wrow, a.n - 1) * o.stride + wpiece * 16;
+        }
+#pragma unroll
+    for (int i = 0; i < (TILES + 1) / 2; ++i) {
+        const uint32_t row = min(i * 32 + lane / 2, TILES * 16 - 1u), t = row / 16;
+        const uint32_t at = min(n0 + t / W * 16 + row % 16, a.n - 1);
+        s_from[i] = a.w[0].scales + at * a.w[0].scale_stride;
+        if (W == 2 && t % 2 == 1) s_from[i] = a.w[1].scales + at * a.w[1].scale_stride;
+    }
+    auto fetch = [&](uint32_t unit, uint32_t slot) {
+        const uint32_t to = slots + slot * kSlot;
+        const bool whole = 8 * unit + 8 <= blocks;
+        const char *zero = reinterpret_cast<const char *>(&kZeroPiece);
+#pragma unroll
+        for (int i = 0; i < (TILES + 1) / 2; ++i) {
+            const uint32_t block = 8 * unit + lane % 2 * 4, at = to + TILES * 2048 + i * 256;
+            if constexpr (WORDS) {
+                const char *src = reinterpret_cast<const char *>(s_from[i] + block);
+                dma4_from(block < blocks ? src : zero, lds0 + at);
+            } else {
+                uint32_t word = 0;
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j)
+                    if (block + j < blocks) word |= static_cast<uint32_t>(s_from[i][block + j]) << (8 * j);
+                *reinterpret_cast<uint32_t *>(lds + at + lane * 4) = word;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const char *src = w_from[t][h] + unit * 128ull;
+                dma16_from(whole || 8 * unit + wpiece < blocks ? src : zero, lds0 + to + t * 2048 + h * 1024);
+            }
+    };
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s)
+        if (wave + s * WAVES < units) fetch(wave + s * WAVES, s);
+
+    // The activations have landed when only the weights are left in flight.
+    const uint32_t mine = wave < units ? min((units - 1 - wave) / WAVES + 1, static_cast<uint32_t>(SLOTS)) : 0u;
+    if (SLOTS > 1 && mine == 2) landed<2 * LOADS>();
+    else if (mine == 1) landed<LOADS>();
+    else landed<0>();
+    if constexpr (FLOATS) {
+        meet();
+        for (uint32_t row = 0; row < a.m; ++row) {
+            const char *from = lds + raw + row * raw_row;
+            char *to = lds + row * rows.row;
+            for (uint32_t at = threadIdx.x; at < blocks * 4; at += THREADS) {  // four neighbouring threads a block
+                const Eight e = load_eight<true>(f.type, from, at * 8);
+                const uint32_t scale = block_scale<ACT != kAct4>(e);
+                if constexpr (ACT == kAct4) *reinterpret_cast<uint32_t *>(to + at * 4) = fp4_of(e, scale);
+                else *reinterpret_cast<u2 *>(to + at * 8) = fp8_of(e, scale);
+                if (at % 4 == 0) lds[rows.scales + row * rows.scale_row + at / 4] = static_cast<char>(scale);
+            }
+        }
+    }
+    // Zeros from the last block to the end of its unit.
+    const uint32_t pad = units * 8 - blocks, block_bytes = ACT == kAct4 ? 16 : 32;
+    if (threadIdx.x < a.m * 8 && threadIdx.x % 8 < pad) {
+        const uint32_t row = threadIdx.x / 8, block = blocks + threadIdx.x % 8;
+        char *to = lds + row * rows.row + block * block_bytes;
+        *reinterpret_cast<u4 *>(to) = u4{0, 0, 0, 0};
+        if (ACT != kAct4) *reinterpret_cast<u4 *>(to + 16) = u4{0, 0, 0, 0};
+        lds[rows.scales + row * rows.scale_row + block] = 0;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    reads_done();
+    meet();
+
+    const uint32_t arow = min(r, a.m - 1);  // rows past the last are computed from it and not stored
+    const char *a_at = lds + arow * rows.row + c * 16;
+    const char *as_at = lds + rows.scales + arow * rows.scale_row + c;
+    f4 acc[TILES] = {};
+    uint32_t slot = 0;
+    for (uint32_t unit = wave; unit < units; unit += WAVES) {
+        // Units behind this one that are in flight.
+        const uint32_t younger = min((units - 1 - unit) / WAVES, static_cast<uint32_t>(SLOTS - 1));
+        if (SLOTS > 1 && younger == 1) landed<LOADS>();
+        else landed<0>();
+        const char *from = lds + slots + slot * kSlot;
+        u4 w[TILES][2], lo[2], hi[2];
+        uint32_t wscale[TILES][2], ascale[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const uint32_t step = 2 * unit + u;
+            lo[u] = *reinterpret_cast<const u4 *>(a_at + step * (ACT == kAct4 ? 64 : 128));
+            hi[u] = ACT == kAct4 ? lo[u] : *reinterpret_cast<const u4 *>(a_at + step * 128 + 64);
+            ascale[u] = *reinterpret_cast<const uint8_t *>(as_at + step * 4);
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+                w[t][u] = *reinterpret_cast<const u4 *>(from + t * 2048 + r * 128 + ((4 * u + c) ^ (r % 8)) * 16);
+                wscale[t][u] = *reinterpret_cast<const uint8_t *>(from + TILES * 2048 + t * 128 + r * 8 + 4 * u + c);
+            }
+        }
+        reads_done();
+        if (unit + SLOTS * WAVES < units) fetch(unit + SLOTS * WAVES, slot);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const ActPiece<ACT> act(lo[u], hi[u]);
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) acc[t] = mx_mfma<ACT, 0>(w[t][u], act, acc[t], wscale[t][u], ascale[u]);
+        }
+        slot = slot + 1 == SLOTS ? 0 : slot + 1;
+    }
+
+    // The waves' sums lie where the units were.
+    __syncthreads();
+    float *sums = reinterpret_cast<float *>(lds + rows.bytes);  // [WAVES][TILES][16 rows][16 columns]
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) *reinterpret_cast<f4 *>(sums + ((wave * TILES + t) * 16 + r) * 16 + 4 * c) = acc[t];
     __syncthreads();
     // 2 RT threads an activation row, eight columns each.
     with_kind<ACT, GATED>(a.out_kind, [&](auto kind) {
-        for (uint32_t i = threadIdx.x; i < 32 * RT; i += 64 * WAVES) {
+        for (uint32_t i = threadIdx.x; i < a.m * 2 * RT; i += THREADS) {
             const uint32_t m = i / (2 * RT), at = i % (2 * RT), n = n0 + 8 * at;
             Eight e[W];
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                const float *from = &sums[0][w][at / 2][m][8 * (at % 2)];
+                const float *from = sums + ((at / 2 * W + w) * 16 + m) * 16 + 8 * (at % 2);
+                f4 x = {}, y = {};
 #pragma unroll
-                for (int x = 0; x < 8; ++x) e[w].v[x] = from[x];
-                for (int s = 1; s < WAVES; ++s) {
-                    from += W * RT * 256;
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) e[w].v[x] += from[x];
+                for (int s = 0; s < WAVES; ++s) {
+                    x += *reinterpret_cast<const f4 *>(from + s * TILES * 256);
+                    y += *reinterpret_cast<const f4 *>(from + s * TILES * 256 + 4);
                 }
+                e[w] = Eight{{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]}};
             }
             if constexpr (GATED) {
 #pragma unroll
@@ -111,19 +230,9 @@ __global__ __launch_bounds__(64 * WAVES) void mxfp4_stream_kernel(MxLinearArgs a
                 for (int x = 0; x < 8; ++x)
                     if (n + x < a.n) e[0].v[x] += a.bias[n + x];
             }
-            store_results<decltype(kind)::value>(a, m0 + m, n, a.vec_out && n + 8 <= a.n, e[0]);
+            store_results<decltype(kind)::value>(a, m, n, a.vec_out && n + 8 <= a.n, e[0]);
         }
     });
-}
-
-template <int ACT, bool GATED>
-int launch_stream(const MxLinearArgs &a, bool words, hipStream_t stream) {
-    constexpr int RT = 2, WAVES = 8;
-    const uint64_t grid = static_cast<uint64_t>((a.m + 15) / 16) * ((a.n + 16 * RT - 1) / (16 * RT));
-    if (grid > INT32_MAX) return fail(QXT_INVALID_ARGUMENT, "mxfp4 linear: too many outputs");
-    return launch("mxfp4_stream_kernel",
-                  words ? mxfp4_stream_kernel<ACT, GATED, RT, WAVES, true> : mxfp4_stream_kernel<ACT, GATED, RT, WAVES, false>,
-                  dim3(static_cast<uint32_t>(grid)), dim3(64 * WAVES), 0, stream, a);
 }
 
 // Scales in rows of words, zeros behind the last.
@@ -139,14 +248,44 @@ __global__ __launch_bounds__(256) void pad_scales_kernel(const uint8_t *from, in
     to[at] = word;
 }
 
-template <int ACT>
-int launch_act(const MxLinearArgs &a, bool is_gated, bool words, hipStream_t stream) {
-    return is_gated ? launch_stream<ACT, true>(a, words, stream) : launch_stream<ACT, false>(a, words, stream);
+template <int ACT, bool GATED, int RT, int WAVES, int SLOTS>
+constexpr size_t stream_lds(const MxLinearArgs &a, const Floats *f) {
+    constexpr uint32_t tiles = RT * (GATED ? 2 : 1), slot = tiles * 2048 + (tiles + 1) / 2 * 256;
+    static_assert(SLOTS >= 1 && SLOTS <= 2 && slot >= tiles * 1024, "the sums lie where the units were");
+    return act_rows<ACT>(a.m, a.blocks).bytes + WAVES * SLOTS * slot + (f != nullptr ? a.m * float_row(f->type, a.blocks) : 0);
 }
+
+template <int ACT, bool GATED, int RT, int WAVES, int SLOTS>
+int launch_stream(const MxLinearArgs &a, const Floats *f, bool words, hipStream_t stream) {
+    auto kernel = f != nullptr ? (words ? mxfp4_stream_kernel<ACT, GATED, true, true, RT, WAVES, SLOTS>
+                                        : mxfp4_stream_kernel<ACT, GATED, true, false, RT, WAVES, SLOTS>)
+                               : (words ? mxfp4_stream_kernel<ACT, GATED, false, true, RT, WAVES, SLOTS>
+                                        : mxfp4_stream_kernel<ACT, GATED, false, false, RT, WAVES, SLOTS>);
+    return launch("mxfp4_stream_kernel", kernel, dim3((a.n + 16 * RT - 1) / (16 * RT)), dim3(64 * WAVES),
+                  stream_lds<ACT, GATED, RT, WAVES, SLOTS>(a, f), stream, a, f != nullptr ? *f : Floats{});
+}
+
+// Which rows, waves and buffers.  Gated products hold 32 rows of each weight, for whole blocks of results; two buffers a
+// wave where two workgroups fit a CU all the same (one row, K = 4096, N = 14336, 8-bit rows: 14.0 -> 13.7 us; with them
+// where only one fits, as with bf16 rows: 13.6 -> 16.8 us).  A single weight of many columns, or of a short K, in 32 rows
+// by four waves (one row, K = 4096, N = 14336: 8.1 us, with 16 rows by eight waves 8.9; K = 2048, N = 5632 4.8, 5.2), else
+// in 16 rows by eight waves (K = 14336, N = 4096: 8.2 us, with 32 rows by four 8.9; K = 4096 4.4, 5.1).
+template <int ACT>
+int launch_act(const MxLinearArgs &a, const Floats *f, bool is_gated, bool words, hipStream_t stream) {
+    if (is_gated) {
+        if (stream_lds<ACT, true, 2, 4, 2>(a, f) <= 80 * 1024) return launch_stream<ACT, true, 2, 4, 2>(a, f, words, stream);
+        return launch_stream<ACT, true, 2, 4, 1>(a, f, words, stream);
+    }
+    if (a.n >= 12288 || a.blocks <= 64) return launch_stream<ACT, false, 2, 4, 2>(a, f, words, stream);
+    return launch_stream<ACT, false, 1, 8, 2>(a, f, words, stream);
+}
+
+constexpr uint32_t kMostK = 1u << 22;
 
 int check_operand(const char *name, const MxOperand &o, uint32_t format, uint32_t rows, uint32_t blocks) {
     if (o.values == nullptr || o.scales == nullptr) return fail(QXT_INVALID_ARGUMENT, "%s: null pointer", name);
     if (!aligned(o.values, 16) || o.stride % 16) return fail(QXT_INVALID_ARGUMENT, "%s: values must be in rows aligned to 16 bytes", name);
+    if (rows > 1 && o.stride >= 1 << 23) return fail(QXT_INVALID_ARGUMENT, "%s: rows of values must lie less than 8 MiB apart", name);
     if (rows > 1 && (static_cast<size_t>(o.stride) < mx_row_bytes(format, blocks * kMxBlock) ||
                      static_cast<size_t>(o.scale_stride) < blocks))
         return fail(QXT_INVALID_ARGUMENT, "%s: a row stride is below the row", name);
@@ -161,8 +300,18 @@ MxOperand operand(const qxt_mx_matrix *m) {
 size_t up16(size_t bytes) { return (bytes + 15) / 16 * 16; }
 uint32_t padded(uint32_t blocks) { return (blocks + 3) / 4 * 4; }
 
-// More activation rows than this go to the tile kernels.
-constexpr uint32_t kStreamRows = 16;
+// Activation rows that the streaming kernel takes: up to 16, as long as they leave room in LDS for the weights.
+constexpr size_t kStreamBytes = 48 * 1024;
+// Bytes of float activations that every workgroup of it quantises for itself.
+constexpr size_t kFusedBytes = 32 * 1024;
+bool streams(uint32_t m, uint32_t k, uint32_t format) {
+    const uint32_t blocks = k / kMxBlock;
+    return m <= 16 && (format == QXT_MX_FP4 ? act_rows<kAct4>(m, blocks) : act_rows<kAct8>(m, blocks)).bytes <= kStreamBytes;
+}
+bool fuses(const Floats &x, uint32_t m, uint32_t k, uint32_t format) {
+    return streams(m, k, format) && m * static_cast<size_t>(float_row(x.type, k / kMxBlock)) <= kFusedBytes &&
+           aligned(x.x, 16) && (m == 1 || x.stride % 16 == 0);
+}
 
 // The workspace: quantised activations (values, scales in rows of words), and for the tile kernels room for each
 // operand's scales in rows of words, and the sums of the parts of K.
@@ -174,7 +323,7 @@ struct Workspace {
             scales = up16(m * mx_row_bytes(format, k));
             bytes = scales + up16(m * pad);
         }
-        if (m <= kStreamRows) return;
+        if (streams(m, k, format)) return;
         a_scales = bytes;
         if (!floats) bytes += up16(m * pad);
         w_scales = bytes;
@@ -186,18 +335,12 @@ struct Workspace {
     }
 };
 
-struct Floats {
-    const void *x;
-    size_t stride;
-    uint32_t type;
-};
-
 // Checks shared by the four entry points, then the launches.  `x`: activations in floats, quantised into the workspace.
 int run_linear(MxLinearArgs &a, const Floats *x, uint32_t format, bool is_gated, uint32_t k, void *workspace,
                size_t workspace_bytes, void *stream) {
     const char *name = is_gated ? "mxfp4 gated" : "mxfp4 linear";
     if (!known_mx(format)) return fail(QXT_INVALID_ARGUMENT, "%s: unknown block format", name);
-    if (k == 0 || k % kMxBlock || k > INT32_MAX) return fail(QXT_INVALID_ARGUMENT, "%s: K must be a positive multiple of 32", name);
+    if (k == 0 || k % kMxBlock || k > kMostK) return fail(QXT_INVALID_ARGUMENT, "%s: K must be a positive multiple of 32 below 2^22", name);
     if (a.m > INT32_MAX / 32 || a.n > INT32_MAX / 32) return fail(QXT_INVALID_ARGUMENT, "%s: too many rows or columns", name);
     const bool blocks_out = a.out_kind == QXT_ROWS_MXFP8 || a.out_kind == QXT_ROWS_MXFP4;
     if (!known_type(a.out_kind) && !(is_gated && blocks_out))
@@ -212,16 +355,21 @@ int run_linear(MxLinearArgs &a, const Floats *x, uint32_t format, bool is_gated,
     if (x != nullptr) {
         const size_t element = type_bytes(x->type);
         if (x->x == nullptr) return fail(QXT_INVALID_ARGUMENT, "%s: null pointer", name);
-        if (!aligned(x->x, element) || x->stride % element || (a.m > 1 && x->stride < k * element))
+        if (!aligned(x->x, element) || static_cast<size_t>(x->stride) % element ||
+            (a.m > 1 && static_cast<size_t>(x->stride) < k * element))
             return fail(QXT_INVALID_ARGUMENT, "%s: bad strides or alignment", name);
+    }
+    const bool fused = x != nullptr && fuses(*x, a.m, k, format);
+    if (x != nullptr && !fused) {
         a.a.values = static_cast<const char *>(workspace);
         a.a.stride = static_cast<int64_t>(mx_row_bytes(format, k));
         a.a.scales = static_cast<const uint8_t *>(workspace) + room.scales;
         a.a.scale_stride = padded(a.blocks);
     }
-    if (room.bytes != 0 && (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < room.bytes))
+    if (!fused && room.bytes != 0 && (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < room.bytes))
         return fail(QXT_INVALID_ARGUMENT, "%s: workspace too small or not aligned to 16 bytes", name);
-    if (int rc = check_operand(name, a.a, format, a.m, a.blocks)) return rc;
+    if (!fused)
+        if (int rc = check_operand(name, a.a, format, a.m, a.blocks)) return rc;
     for (int w = 0; w < (is_gated ? 2 : 1); ++w)
         if (int rc = check_operand(name, a.w[w], QXT_MX_FP4, a.n, a.blocks)) return rc;
     const size_t out_align = blocks_out ? (a.out_kind == QXT_ROWS_MXFP8 ? 8 : 4) : type_bytes(a.out_kind);
@@ -232,10 +380,10 @@ int run_linear(MxLinearArgs &a, const Floats *x, uint32_t format, bool is_gated,
         return fail(QXT_INVALID_ARGUMENT, "%s: bad strides or alignment", name);
     if (int rc = injected(QXT_FAIL_SUBMISSION)) return rc;
     a.vec_out = aligned(a.y, 16) && a.y_stride % 16 == 0;
-    if (x != nullptr) {
+    if (x != nullptr && !fused) {
         MxRows rows{};
-        rows.x = static_cast<char *>(const_cast<void *>(x->x));
-        rows.x_stride = static_cast<int64_t>(x->stride);
+        rows.x = const_cast<char *>(x->x);
+        rows.x_stride = x->stride;
         rows.type = x->type;
         rows.values = const_cast<char *>(a.a.values);
         rows.values_stride = a.a.stride;
@@ -246,15 +394,14 @@ int run_linear(MxLinearArgs &a, const Floats *x, uint32_t format, bool is_gated,
     }
     const hipStream_t s = as_stream(stream);
     const int act = act_of(format, a.out_kind);
-    constexpr int64_t kTileStride = 1 << 23;
-    const bool tiles = a.m > kStreamRows && a.a.stride < kTileStride && a.w[0].stride < kTileStride && a.w[1].stride < kTileStride;
-    bool words = true;  // every row of scales in words
+    const bool tiles = !streams(a.m, k, format);
+    bool words = true;  // the weights' rows of scales are in words
     for (int o = 0; o < (is_gated ? 3 : 2); ++o) {
         MxOperand &operand = o == 0 ? a.a : a.w[o - 1];
-        if (o == 0 && x != nullptr) continue;  // written so
+        if (o == 0 && (x != nullptr || !tiles)) continue;  // written so, or read byte by byte
         if (a.blocks % 4 == 0 && aligned(operand.scales, 4) && operand.scale_stride % 4 == 0) continue;
         words = false;
-        if (!tiles) break;
+        if (!tiles) continue;
         const uint32_t rows = o == 0 ? a.m : a.n, row = padded(a.blocks) / 4;
         if (static_cast<uint64_t>(rows) * row > INT32_MAX) return fail(QXT_INVALID_ARGUMENT, "%s: too many blocks", name);
         uint8_t *to = static_cast<uint8_t *>(workspace) + (o == 0 ? room.a_scales : room.w_scales + (o - 1) * room.w_each);
@@ -264,15 +411,17 @@ int run_linear(MxLinearArgs &a, const Floats *x, uint32_t format, bool is_gated,
         operand.scales = to;
         operand.scale_stride = 4 * row;
     }
+    a.a_words = a.blocks % 4 == 0 && aligned(a.a.scales, 4) && a.a.scale_stride % 4 == 0;
     if (tiles) {
         a.parts = reinterpret_cast<float *>(static_cast<char *>(workspace) + room.parts);
         return mxfp4_tiles(a, act, is_gated, plan_tiles(a.m, a.n, k, is_gated ? 2 : 1, act), s);
     }
-    words = words && a.blocks % 4 == 0;
+    Floats f{};
+    if (fused) f = *x;
     switch (act) {
-        case kAct4: return launch_act<kAct4>(a, is_gated, words, s);
-        case kAct8: return launch_act<kAct8>(a, is_gated, words, s);
-        default: return launch_act<kAct8Parts>(a, is_gated, words, s);
+        case kAct4: return launch_act<kAct4>(a, fused ? &f : nullptr, is_gated, words, s);
+        case kAct8: return launch_act<kAct8>(a, fused ? &f : nullptr, is_gated, words, s);
+        default: return launch_act<kAct8Parts>(a, fused ? &f : nullptr, is_gated, words, s);
     }
 }
 
@@ -316,7 +465,7 @@ int qxt_mxfp4_linear(const void *x, size_t ldx, uint32_t x_type, uint32_t format
     if (w == nullptr) return fail(QXT_INVALID_ARGUMENT, "mxfp4 linear: null pointer");
     MxLinearArgs args = linear_args(w, nullptr, y, ldy, y_type, m, n);
     args.bias = bias;
-    const Floats floats{x, ldx, x_type};
+    const Floats floats{static_cast<const char *>(x), static_cast<int64_t>(ldx), x_type};
     return run_linear(args, &floats, format, false, k, workspace, workspace_bytes, stream);
 }
 
@@ -341,7 +490,7 @@ int qxt_mxfp4_gated_linear(const void *x, size_t ldx, uint32_t x_type, uint32_t 
     args.gate = gate_function;
     args.y_scales = h_scales;
     args.y_scale_stride = static_cast<int64_t>(ldhs);
-    const Floats floats{x, ldx, x_type};
+    const Floats floats{static_cast<const char *>(x), static_cast<int64_t>(ldx), x_type};
     return run_linear(args, &floats, format, true, k, workspace, workspace_bytes, stream);
 }
 

@@ -15,38 +15,6 @@
 namespace qxt {
 namespace {
 
-// Source of what lies past a row's last block.
-__device__ __constant__ const uint4 kZeroPiece = {};
-
-// 64 lanes' 16 or 4 bytes, from a wave-uniform address plus each lane's offset or from each lane's address, to LDS at `to`
-// + 16 (or 4) * lane.  Inline
-// assembly because the compiler waits for every such load in flight before it reads any of LDS; the waits here are the
-// kernel's own.  There is no register output.
-// (The compiler warns that it may not preserve m0; it has no other use for it here.)
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void dma16(uint64_t base, uint32_t offset, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(offset), "s"(base) : "memory", "m0");
-}
-__device__ __forceinline__ void dma16_from(const char *src, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(src) : "memory", "m0");
-}
-#pragma clang diagnostic pop
-
-// Wait until all but the wave's N youngest loads are done, and all of its LDS reads.
-template <int N>
-__device__ __forceinline__ void landed() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(N) : "memory");
-    __builtin_amdgcn_sched_barrier(0);
-}
-__device__ __forceinline__ void meet() {
-    asm volatile("" : : : "memory");
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("" : : : "memory");
-}
-
 // Output tile (ty, tx) of a workgroup.  Workgroups go to the eight XCDs in turn, each with its own L2: every XCD takes a
 // contiguous run of a grouped order (`gm` tile rows at a time, column by column), so that what it runs together shares
 // panels.
