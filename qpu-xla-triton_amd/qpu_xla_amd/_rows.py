@@ -1,4 +1,8 @@
-"""Checks and C-ABI arguments of the operators over rows: floats, microscaling blocks, and where they live."""
+"""Checks and C-ABI arguments of the operators over rows: floats, microscaling blocks, and where they live.
+
+They run at every call, and a call of few rows is bound by them: shapes and strides are read once each, devices are
+compared as integers, and outputs made here are not looked at again.
+"""
 
 from __future__ import annotations
 
@@ -7,7 +11,7 @@ from typing import Any
 import torch
 
 from qpu_xla_amd import _lib
-from qpu_xla_amd._paged import TYPES, require_one_gpu
+from qpu_xla_amd._paged import TYPES, empty_for
 
 MX_BLOCK = 32
 FP8 = torch.float8_e4m3fn
@@ -17,9 +21,23 @@ _SCALES = (torch.uint8, torch.float8_e8m0fnu)
 
 def require_current_gpu(name: str, first: torch.Tensor, *others: torch.Tensor | None) -> None:
     """All tensors on the current HIP device: streams and launches belong to it."""
-    require_one_gpu(name, first, *others)
-    if first.get_device() != torch._C._cuda_getDevice():
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            index = -1
+    if index < 0:
+        raise ValueError(f"{name}: all tensors must live on one HIP device (no CPU fallback)")
+    if index != torch._C._cuda_getDevice():
         raise ValueError(f"{name}: the tensors must live on the current HIP device")
+
+
+def new_rows(stream: Any, like: torch.Tensor, shape: tuple[int, ...], dtype: torch.dtype) -> torch.Tensor:
+    """``empty_for`` on a tensor's device; on the current stream at two thirds of its time where the shapes agree."""
+    if stream is None:
+        if like.shape == shape:
+            return torch.empty_like(like, dtype=dtype, memory_format=torch.contiguous_format)
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    return empty_for(stream, shape, dtype, like.device)
 
 
 def float_rows(name: str, what: str, t: torch.Tensor) -> tuple[int, int, int, int]:
@@ -63,28 +81,40 @@ def mx_format(name: str, what: str) -> int:
 
 def mx_rows(name: str, what: str, values: torch.Tensor, scales: torch.Tensor, formats: tuple[int, ...] = (0, 1)) -> tuple[int, int, int, bytes]:
     """(rows, columns, format, ``qxt_mx_matrix``) of stored blocks: the values' type tells the format."""
-    fp8 = values.dtype is FP8
-    if (_lib.MX_FP8 if fp8 else _lib.MX_FP4) not in formats:
-        raise ValueError(f"{name}: {what} values must be packed 4-bit elements, uint8 [rows, columns / 2]")
-    stride = _byte_rows(name, f"{what} values", values, (FP8,) if fp8 else _FP4_STORED, None)
-    rows, stored = values.shape
-    columns = stored if fp8 else 2 * stored
+    dtype, shape, scale_shape = values.dtype, values.shape, scales.shape
+    fmt = _lib.MX_FP8 if dtype is FP8 else _lib.MX_FP4
+    if fmt not in formats or (fmt == _lib.MX_FP4 and dtype not in _FP4_STORED) or len(shape) != 2:
+        raise ValueError(f"{name}: {what} values must be packed 4-bit elements, uint8 [rows, columns / 2]"
+                         + (", or float8_e4m3fn [rows, columns]" if _lib.MX_FP8 in formats else ""))
+    rows, columns = shape
+    if fmt == _lib.MX_FP4:
+        columns *= 2
     if columns == 0 or columns % MX_BLOCK:
         raise ValueError(f"{name}: {what} must have columns in positive multiples of {MX_BLOCK}")
-    scale_stride = _byte_rows(name, f"{what} scales", scales, _SCALES, (rows, columns // MX_BLOCK))
-    packed = _lib.MX_MATRIX.pack(values.data_ptr(), stride, scales.data_ptr(), scale_stride)
-    return rows, columns, _lib.MX_FP8 if fp8 else _lib.MX_FP4, packed
+    if scales.dtype not in _SCALES or len(scale_shape) != 2 or scale_shape[0] != rows or scale_shape[1] != columns // MX_BLOCK:
+        raise ValueError(f"{name}: {what} scales must be uint8 or float8_e8m0fnu [{rows}, {columns // MX_BLOCK}]")
+    stride, element = values.stride()
+    scale_stride, scale_element = scales.stride()
+    if element != 1 or (scale_element != 1 and scale_shape[1] > 1) or (rows > 1 and (
+            stride < shape[1] or scale_stride < scale_shape[1])):
+        raise ValueError(f"{name}: {what} must have dense rows of values and scales")
+    if rows <= 1:  # torch gives a single row any stride
+        stride = scale_stride = 0
+    return rows, columns, fmt, _lib.MX_MATRIX.pack(values.data_ptr(), stride, scales.data_ptr(), scale_stride)
 
 
-def mx_outputs(name: str, rows: int, columns: int, fp8: bool, values: torch.Tensor | None, scales: torch.Tensor | None,
-               empty: Any) -> tuple[torch.Tensor, int, torch.Tensor, int]:
-    """(values, byte stride, scales, byte stride) to write blocks into; ``empty(shape, dtype)`` makes what is not given."""
+def mx_outputs(name: str, like: torch.Tensor, rows: int, columns: int, fp8: bool, values: torch.Tensor | None,
+               scales: torch.Tensor | None, stream: Any) -> tuple[torch.Tensor, int, torch.Tensor, int]:
+    """(values, byte stride, scales, byte stride) to write blocks into, made on ``like``'s device where not given."""
     if columns == 0 or columns % MX_BLOCK:
         raise ValueError(f"{name}: columns must be a positive multiple of {MX_BLOCK}")
     shape = (rows, columns if fp8 else columns // 2)
     if values is None:
-        values = empty(shape, FP8 if fp8 else torch.uint8)
+        values, stride = new_rows(stream, like, shape, FP8 if fp8 else torch.uint8), shape[1]
+    else:
+        stride = _byte_rows(name, "values", values, (FP8,) if fp8 else _FP4_STORED, shape)
     if scales is None:
-        scales = empty((rows, columns // MX_BLOCK), torch.uint8)
-    return (values, _byte_rows(name, "values", values, (FP8,) if fp8 else _FP4_STORED, shape),
-            scales, _byte_rows(name, "scales", scales, _SCALES, (rows, columns // MX_BLOCK)))
+        scales, scale_stride = new_rows(stream, like, (rows, columns // MX_BLOCK), torch.uint8), columns // MX_BLOCK
+    else:
+        scale_stride = _byte_rows(name, "scales", scales, _SCALES, (rows, columns // MX_BLOCK))
+    return values, stride, scales, scale_stride

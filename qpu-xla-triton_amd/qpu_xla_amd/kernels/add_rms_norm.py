@@ -23,53 +23,54 @@ from typing import Any
 import torch
 
 from qpu_xla_amd import _lib
-from qpu_xla_amd._paged import TYPES, empty_for
-from qpu_xla_amd._rows import MX_BLOCK, float_rows, mx_outputs, require_current_gpu, vector
-from qpu_xla_amd._tensors import row_stride, rows_are_dense, stream_handle
+from qpu_xla_amd._paged import TYPES
+from qpu_xla_amd._rows import MX_BLOCK, float_rows, mx_outputs, new_rows, require_current_gpu, vector
+from qpu_xla_amd._tensors import rows_are_dense, stream_handle
 from qpu_xla_amd.errors import KernelError
 from qpu_xla_amd.kernel import Kernel
 from qpu_xla_amd.kernels.quantize import Q8_0_BLOCK_BYTES
 
 
-class _Call:
-    """The arguments that every form shares."""
-
-    def __init__(self, name: str, x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None,
-                 residual_out: torch.Tensor | None, epsilon: float, stream: Any) -> None:
-        self.name, self.stream, self.device = name, stream, x.device
-        self.rows, self.columns, x_code, x_stride = float_rows(name, "x", x)
-        if self.columns == 0:
-            raise ValueError(f"{name}: rows must not be empty")
-        if not epsilon >= 0.0:
-            raise ValueError(f"{name}: epsilon must not be negative")
-        weight_at = vector(name, "weight", weight, self.columns)
-        self.tensors = [weight, residual]
-        head = [x.data_ptr(), x_stride, x_code]
-        if residual is None:
-            if residual_out is not None:
-                raise ValueError(f"{name}: residual_out without a residual")
-            head += [None, 0, 0, None, 0]
+def _run(name: str, kind: int, x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None, epsilon: float,
+         out: torch.Tensor, out_stride: int, scales: torch.Tensor | None, scales_stride: int,
+         residual_out: torch.Tensor | None, stream: Any) -> torch.Tensor | None:
+    """The checks and the call that every form shares; the sum."""
+    rows, columns, x_code, x_stride = float_rows(name, "x", x)
+    if columns == 0:
+        raise ValueError(f"{name}: rows must not be empty")
+    if not epsilon >= 0.0:
+        raise ValueError(f"{name}: epsilon must not be negative")
+    weight_at = vector(name, "weight", weight, columns)
+    residual_at = sum_at = None
+    code = stride = sum_stride = 0
+    if residual is None:
+        if residual_out is not None:
+            raise ValueError(f"{name}: residual_out without a residual")
+        require_current_gpu(name, x, weight, out, scales)
+    else:
+        r_rows, r_columns, code, stride = float_rows(name, "residual", residual)
+        if r_rows != rows or r_columns != columns:
+            raise ValueError(f"{name}: residual must have x's shape")
+        if residual_out is None:
+            residual_out, sum_stride = new_rows(stream, residual, (rows, columns), residual.dtype), columns * (2 if code else 4)
         else:
-            rows, columns, code, stride = float_rows(name, "residual", residual)
-            if residual_out is None:
-                residual_out = self.empty((rows, columns), residual.dtype)
-            elif residual_out.dtype is not residual.dtype:
+            if residual_out.dtype is not residual.dtype:
                 raise ValueError(f"{name}: residual_out must have the residual's type")
-            out_rows, out_columns, _, out_stride = float_rows(name, "residual_out", residual_out)
-            if (rows, columns) != (self.rows, self.columns) or (out_rows, out_columns) != (rows, columns):
-                raise ValueError(f"{name}: residual and residual_out must have x's shape")
-            head += [residual.data_ptr(), stride, code, residual_out.data_ptr(), out_stride]
-        self.sum = residual_out
-        self.head = [*head, weight_at, epsilon]
-        self.x = x
+            s_rows, s_columns, _, sum_stride = float_rows(name, "residual_out", residual_out)
+            if s_rows != rows or s_columns != columns:
+                raise ValueError(f"{name}: residual_out must have x's shape")
+        residual_at, sum_at = residual.data_ptr(), residual_out.data_ptr()
+        require_current_gpu(name, x, weight, residual, residual_out, out, scales)
+    _lib.call("qxt_add_rms_norm", x.data_ptr(), x_stride, x_code, residual_at, stride, code, sum_at, sum_stride, weight_at,
+              epsilon, out.data_ptr(), out_stride, None if scales is None else scales.data_ptr(), scales_stride, kind, rows,
+              columns, stream_handle(stream))
+    return residual_out
 
-    def empty(self, shape: tuple[int, ...], dtype: torch.dtype) -> torch.Tensor:
-        return empty_for(self.stream, shape, dtype, self.device)
 
-    def run(self, out: torch.Tensor, out_stride: int, scales: torch.Tensor | None, scales_stride: int, kind: int) -> None:
-        require_current_gpu(self.name, self.x, *self.tensors, self.sum, out, scales)
-        _lib.call("qxt_add_rms_norm", *self.head, out.data_ptr(), out_stride, None if scales is None else scales.data_ptr(),
-                  scales_stride, kind, self.rows, self.columns, stream_handle(self.stream))
+def _shape(name: str, x: torch.Tensor) -> tuple[int, int]:
+    if x.dim() != 2:
+        raise ValueError(f"{name}: x must be float32, bfloat16 or float16 [rows, columns] with dense rows")
+    return tuple(x.shape)
 
 
 def add_rms_norm(
@@ -83,14 +84,13 @@ def add_rms_norm(
     stream: Any = None,
 ) -> tuple[torch.Tensor, torch.Tensor | None]:
     """(y, sum) of float rows x [T, D], fp32 weight [D] and residual [T, D]; y in x's type unless ``out`` is given."""
-    call = _Call("add_rms_norm", x, weight, residual, residual_out, epsilon, stream)
+    shape = _shape("add_rms_norm", x)
     if out is None:
-        out = call.empty((call.rows, call.columns), x.dtype)
-    rows, columns, code, stride = float_rows(call.name, "out", out)
-    if (rows, columns) != (call.rows, call.columns):
+        out = new_rows(stream, x, shape, x.dtype)
+    rows, columns, code, stride = float_rows("add_rms_norm", "out", out)
+    if (rows, columns) != shape:
         raise ValueError("add_rms_norm: out must have x's shape")
-    call.run(out, stride, None, 0, code)
-    return out, call.sum
+    return out, _run("add_rms_norm", code, x, weight, residual, epsilon, out, stride, None, 0, residual_out, stream)
 
 
 def add_rms_norm_int8(
@@ -106,16 +106,20 @@ def add_rms_norm_int8(
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
     """(int8 [T, D], fp32 scales [T], sum): y through ``quantize_rows_int8``'s rule."""
     name = "add_rms_norm_int8"
-    call = _Call(name, x, weight, residual, residual_out, epsilon, stream)
-    shape = (call.rows, call.columns)
-    out = call.empty(shape, torch.int8) if out is None else out
-    scales = call.empty(shape[:1], torch.float32) if scales is None else scales
-    if out.dtype is not torch.int8 or tuple(out.shape) != shape or (call.rows and not rows_are_dense(out)) or (
-            call.rows > 1 and out.stride(0) < call.columns):
-        raise ValueError(f"{name}: out must be int8 {list(shape)} with dense rows")
-    vector(name, "scales", scales, call.rows)
-    call.run(out, out.stride(0) if call.rows > 1 else 0, scales, 0, _lib.ROWS_INT8)
-    return out, scales, call.sum
+    shape = _shape(name, x)
+    if out is None:
+        out, stride = new_rows(stream, x, shape, torch.int8), shape[1]
+    else:
+        if out.dtype is not torch.int8 or tuple(out.shape) != shape or (shape[1] > 1 and out.stride(1) != 1) or (
+                shape[0] > 1 and out.stride(0) < shape[1]):
+            raise ValueError(f"{name}: out must be int8 {list(shape)} with dense rows")
+        stride = out.stride(0) if shape[0] > 1 else 0
+    if scales is None:
+        scales = new_rows(stream, x, shape[:1], torch.float32)
+    else:
+        vector(name, "scales", scales, shape[0])
+    total = _run(name, _lib.ROWS_INT8, x, weight, residual, epsilon, out, stride, scales, 0, residual_out, stream)
+    return out, scales, total
 
 
 def add_rms_norm_q8_0(
@@ -130,25 +134,26 @@ def add_rms_norm_q8_0(
 ) -> tuple[torch.Tensor, torch.Tensor | None]:
     """(Q8_0 blocks uint8 [T, D/32, 34], sum): y through ``quantize_q8_0``'s rule."""
     name = "add_rms_norm_q8_0"
-    call = _Call(name, x, weight, residual, residual_out, epsilon, stream)
-    if call.columns % MX_BLOCK:
-        raise ValueError(f"{name}: columns must be a multiple of 32")
-    shape = (call.rows, call.columns // MX_BLOCK, Q8_0_BLOCK_BYTES)
-    out = call.empty(shape, torch.uint8) if out is None else out
-    if out.dtype is not torch.uint8 or tuple(out.shape) != shape or (call.rows and not rows_are_dense(out)) or (
-            call.rows > 1 and out.stride(0) < shape[1] * Q8_0_BLOCK_BYTES):
+    rows, columns = _shape(name, x)
+    if columns == 0 or columns % MX_BLOCK:
+        raise ValueError(f"{name}: columns must be a positive multiple of 32")
+    shape = (rows, columns // MX_BLOCK, Q8_0_BLOCK_BYTES)
+    if out is None:
+        out = new_rows(stream, x, shape, torch.uint8)
+    elif out.dtype is not torch.uint8 or tuple(out.shape) != shape or (rows and not rows_are_dense(out)) or (
+            rows > 1 and out.stride(0) < shape[1] * Q8_0_BLOCK_BYTES):
         raise ValueError(f"{name}: out must be uint8 {list(shape)} with dense rows")
-    call.run(out, row_stride(out) if call.rows > 1 else 0, None, 0, _lib.ROWS_Q8_0)
-    return out, call.sum
+    stride = out.stride(0) if rows > 1 else 0
+    return out, _run(name, _lib.ROWS_Q8_0, x, weight, residual, epsilon, out, stride, None, 0, residual_out, stream)
 
 
 def _mx(name: str, kind: int, x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None, epsilon: float,
         values: torch.Tensor | None, scales: torch.Tensor | None, residual_out: torch.Tensor | None,
         stream: Any) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
-    call = _Call(name, x, weight, residual, residual_out, epsilon, stream)
-    values, stride, scales, scales_stride = mx_outputs(name, call.rows, call.columns, kind == _lib.ROWS_MXFP8, values, scales, call.empty)
-    call.run(values, stride, scales, scales_stride, kind)
-    return values, scales, call.sum
+    rows, columns = _shape(name, x)
+    values, stride, scales, scales_stride = mx_outputs(name, x, rows, columns, kind == _lib.ROWS_MXFP8, values, scales, stream)
+    total = _run(name, kind, x, weight, residual, epsilon, values, stride, scales, scales_stride, residual_out, stream)
+    return values, scales, total
 
 
 def add_rms_norm_mxfp8(

@@ -24,8 +24,8 @@ from typing import Any
 import torch
 
 from qpu_xla_amd import _lib
-from qpu_xla_amd._paged import TYPES, empty_for, workspace_for
-from qpu_xla_amd._rows import FP8, MX_BLOCK, float_rows, mx_format, mx_outputs, mx_rows, require_current_gpu, vector
+from qpu_xla_amd._paged import TYPES, workspace_for
+from qpu_xla_amd._rows import FP8, MX_BLOCK, float_rows, mx_format, mx_outputs, mx_rows, new_rows, require_current_gpu, vector
 from qpu_xla_amd._tensors import stream_handle
 from qpu_xla_amd.errors import KernelError
 from qpu_xla_amd.kernel import Kernel
@@ -37,8 +37,7 @@ _BLOCK_KINDS = {"mxfp8": _lib.ROWS_MXFP8, "mxfp4": _lib.ROWS_MXFP4}
 def _quantize(name: str, fp8: bool, x: torch.Tensor, values: torch.Tensor | None, scales: torch.Tensor | None,
               stream: Any) -> tuple[torch.Tensor, torch.Tensor]:
     rows, columns, code, stride = float_rows(name, "x", x)
-    values, v_stride, scales, s_stride = mx_outputs(name, rows, columns, fp8, values, scales,
-                                                    lambda shape, dtype: empty_for(stream, shape, dtype, x.device))
+    values, v_stride, scales, s_stride = mx_outputs(name, x, rows, columns, fp8, values, scales, stream)
     require_current_gpu(name, x, values, scales)
     _lib.call("qxt_quantize_mx", x.data_ptr(), stride, code, values.data_ptr(), v_stride, scales.data_ptr(), s_stride, rows,
               columns, _lib.MX_FP8 if fp8 else _lib.MX_FP4, stream_handle(stream))
@@ -63,7 +62,7 @@ def _dequantize(name: str, fmt: int, values: torch.Tensor, scales: torch.Tensor,
     if found != fmt:
         raise ValueError(f"{name}: the values are of another block format")
     if out is None:
-        out = empty_for(stream, (rows, columns), torch.float32 if dtype is None else dtype, values.device)
+        out = new_rows(stream, values, (rows, columns), torch.float32 if dtype is None else dtype)
     elif dtype is not None and out.dtype is not dtype:
         raise ValueError(f"{name}: out is not of the given dtype")
     out_rows, out_columns, code, stride = float_rows(name, "out", out)
@@ -90,14 +89,15 @@ def dequantize_mxfp8(values: torch.Tensor, scales: torch.Tensor, out: torch.Tens
 # -------------------------------------------------------------------- linears
 
 
-def _float_out(name: str, out: torch.Tensor | None, dtype: torch.dtype, rows: int, columns: int, stream: Any,
-               device: torch.device) -> tuple[torch.Tensor, int, int]:
+def _float_out(name: str, like: torch.Tensor, out: torch.Tensor | None, dtype: torch.dtype, rows: int, columns: int,
+               stream: Any) -> tuple[torch.Tensor, int, int]:
     """(out, type code, byte stride)."""
     if out is None:
-        if dtype not in TYPES:
+        code = TYPES.get(dtype)
+        if code is None:
             raise ValueError(f"{name}: the output must be float32, bfloat16 or float16")
-        out = empty_for(stream, (rows, columns), dtype, device)
-    elif out.dtype is not dtype:
+        return new_rows(stream, like, (rows, columns), dtype), code, columns * (2 if code else 4)
+    if out.dtype is not dtype:
         raise ValueError(f"{name}: out is not of the output's type")
     got_rows, got_columns, code, stride = float_rows(name, "out", out)
     if (got_rows, got_columns) != (rows, columns):
@@ -108,7 +108,7 @@ def _float_out(name: str, out: torch.Tensor | None, dtype: torch.dtype, rows: in
 def _workspace(rows: int, columns: int, depth: int, weights: int, fmt: int, floats: int, kind: int, stream: Any,
                device: torch.device) -> tuple[torch.Tensor | None, int]:
     size = (_lib._lib or _lib.load()).qxt_mxfp4_linear_workspace(rows, columns, depth, weights, fmt, floats, kind)
-    return workspace_for(stream, size, device), size
+    return (workspace_for(stream, size, device), size) if size else (None, 0)
 
 
 def mxfp4_gemm(
@@ -130,7 +130,7 @@ def mxfp4_gemm(
         raise ValueError(f"{name}: a and w differ in K")
     bias_at = vector(name, "bias", bias, n)
     dtype = dtype if dtype is not None else torch.float32 if out is None else out.dtype
-    out, code, stride = _float_out(name, out, dtype, m, n, stream, a_values.device)
+    out, code, stride = _float_out(name, a_values, out, dtype, m, n, stream)
     require_current_gpu(name, a_values, a_scales, w_values, w_scales, bias, out)
     workspace, size = _workspace(m, n, k, 1, fmt, 0, code, stream, a_values.device)
     _lib.call("qxt_mxfp4_gemm", a, fmt, w, bias_at, out.data_ptr(), stride, code, m, n, k,
@@ -158,7 +158,7 @@ def mxfp4_linear(
         raise ValueError(f"{name}: x and w differ in K")
     bias_at = vector(name, "bias", bias, n)
     dtype = dtype if dtype is not None else x.dtype if out is None else out.dtype
-    out, code, stride = _float_out(name, out, dtype, m, n, stream, x.device)
+    out, code, stride = _float_out(name, x, out, dtype, m, n, stream)
     require_current_gpu(name, x, w_values, w_scales, bias, out)
     workspace, size = _workspace(m, n, k, 1, fmt, 1, code, stream, x.device)
     _lib.call("qxt_mxfp4_linear", x.data_ptr(), x_stride, x_code, fmt, w, bias_at, out.data_ptr(), stride, code, m, n, k,
@@ -166,7 +166,7 @@ def mxfp4_linear(
     return out
 
 
-def _gated_out(name: str, output: Any, out: Any, m: int, n: int, stream: Any, device: torch.device) -> tuple[Any, list, int, list]:
+def _gated_out(name: str, like: torch.Tensor, output: Any, out: Any, m: int, n: int, stream: Any) -> tuple[Any, list, int, list]:
     """(what is returned, its tensors, kind, [address, stride, scales' address, stride])."""
     if isinstance(output, str):
         kind = _BLOCK_KINDS.get(output)
@@ -175,12 +175,11 @@ def _gated_out(name: str, output: Any, out: Any, m: int, n: int, stream: Any, de
         if out is not None and not (isinstance(out, tuple) and len(out) == 2):
             raise ValueError(f"{name}: out must be (values, scales)")
         values, scales = (None, None) if out is None else out
-        values, stride, scales, scale_stride = mx_outputs(
-            name, m, n, output == "mxfp8", values, scales, lambda shape, dtype: empty_for(stream, shape, dtype, device))
+        values, stride, scales, scale_stride = mx_outputs(name, like, m, n, output == "mxfp8", values, scales, stream)
         return (values, scales), [values, scales], kind, [values.data_ptr(), stride, scales.data_ptr(), scale_stride]
     if out is not None and not isinstance(out, torch.Tensor):
         raise ValueError(f"{name}: out must be a tensor")
-    out, kind, stride = _float_out(name, out, output, m, n, stream, device)
+    out, kind, stride = _float_out(name, like, out, output, m, n, stream)
     return out, [out], kind, [out.data_ptr(), stride, None, 0]
 
 
@@ -220,7 +219,7 @@ def mxfp4_gated_gemm(
     m, k, fmt, a = mx_rows(name, "a", a_values, a_scales)
     n, gate_at, up_at = _gate_weights(name, k, gate_values, gate_scales, up_values, up_scales)
     function = _gate_function(name, gate)
-    result, tensors, kind, places = _gated_out(name, output, out, m, n, stream, a_values.device)
+    result, tensors, kind, places = _gated_out(name, a_values, output, out, m, n, stream)
     require_current_gpu(name, a_values, a_scales, gate_values, gate_scales, up_values, up_scales, *tensors)
     workspace, size = _workspace(m, n, k, 2, fmt, 0, kind, stream, a_values.device)
     _lib.call("qxt_mxfp4_gated_gemm", a, fmt, gate_at, up_at, function, *places, kind, m, n, k,
@@ -249,7 +248,7 @@ def mxfp4_gated_linear(
     function = _gate_function(name, gate)
     if output is None:
         output = out.dtype if isinstance(out, torch.Tensor) else x.dtype
-    result, tensors, kind, places = _gated_out(name, output, out, m, n, stream, x.device)
+    result, tensors, kind, places = _gated_out(name, x, output, out, m, n, stream)
     require_current_gpu(name, x, gate_values, gate_scales, up_values, up_scales, *tensors)
     workspace, size = _workspace(m, n, k, 2, fmt, 1, kind, stream, x.device)
     _lib.call("qxt_mxfp4_gated_linear", x.data_ptr(), x_stride, x_code, fmt, gate_at, up_at, function, *places, kind, m, n, k,
