@@ -207,7 +207,7 @@ __global__ __launch_bounds__(64 * WAVES) void mxfp4_stream_kernel(MxLinearArgs a
     for (int t = 0; t < TILES; ++t) *reinterpret_cast<f4 *>(sums + ((wave * TILES + t) * 16 + r) * 16 + 4 * c) = acc[t];
     __syncthreads();
     // 2 RT threads an activation row, eight columns each.
-    with_kind<ACT, GATED>(a.out_kind, [&](auto kind) {
+    with_kind<ACT, GATED, true>(a.out_kind, [&](auto kind) {
         for (uint32_t i = threadIdx.x; i < a.m * 2 * RT; i += THREADS) {
             const uint32_t m = i / (2 * RT), at = i % (2 * RT), n = n0 + 8 * at;
             Eight e[W];
@@ -393,7 +393,6 @@ int run_linear(MxLinearArgs &a, const Floats *x, uint32_t format, bool is_gated,
         if (int rc = run_mx(true, rows, a.m, k, format, stream)) return rc;
     }
     const hipStream_t s = as_stream(stream);
-    const int act = act_of(format, a.out_kind);
     const bool tiles = !streams(a.m, k, format);
     bool words = true;  // the weights' rows of scales are in words
     for (int o = 0; o < (is_gated ? 3 : 2); ++o) {
@@ -414,15 +413,13 @@ int run_linear(MxLinearArgs &a, const Floats *x, uint32_t format, bool is_gated,
     a.a_words = a.blocks % 4 == 0 && aligned(a.a.scales, 4) && a.a.scale_stride % 4 == 0;
     if (tiles) {
         a.parts = reinterpret_cast<float *>(static_cast<char *>(workspace) + room.parts);
+        const int act = act_of(format, a.out_kind);
         return mxfp4_tiles(a, act, is_gated, plan_tiles(a.m, a.n, k, is_gated ? 2 : 1, act), s);
     }
     Floats f{};
     if (fused) f = *x;
-    switch (act) {
-        case kAct4: return launch_act<kAct4>(a, fused ? &f : nullptr, is_gated, words, s);
-        case kAct8: return launch_act<kAct8>(a, fused ? &f : nullptr, is_gated, words, s);
-        default: return launch_act<kAct8Parts>(a, fused ? &f : nullptr, is_gated, words, s);
-    }
+    if (format == QXT_MX_FP4) return launch_act<kAct4>(a, fused ? &f : nullptr, is_gated, words, s);
+    return launch_act<kAct8Parts>(a, fused ? &f : nullptr, is_gated, words, s);
 }
 
 MxLinearArgs linear_args(const qxt_mx_matrix *w, const qxt_mx_matrix *up, void *y, size_t ldy, uint32_t kind, uint32_t m, uint32_t n) {

@@ -267,7 +267,7 @@ __global__ __launch_bounds__(64 * WN * WM) void mxfp4_tile_kernel(MxLinearArgs a
         for (int e = 0; e < 8; ++e) bias[e] = a.bias != nullptr && out_n + e < a.n ? a.bias[out_n + e] : 0.0f;
     }
     const bool whole = a.vec_out && out_n + 8 <= a.n;
-    with_kind<ACT, GATED>(a.out_kind, [&](auto kind) {
+    with_kind<ACT, GATED, false>(a.out_kind, [&](auto kind) {
 #pragma unroll
         for (int j = 0; j < TA; ++j) {
 #pragma unroll
@@ -321,7 +321,7 @@ __global__ __launch_bounds__(256) void mxfp4_join_kernel(MxLinearArgs a, FastDiv
         if constexpr (GATED) e.v[i] = gated(a.gate, e.v[i], sum[1][i / 4][i % 4]);
         else if (a.bias != nullptr && n + i < a.n) e.v[i] += a.bias[n + i];
     }
-    with_kind<ACT, GATED>(a.out_kind, [&](auto kind) {
+    with_kind<ACT, GATED, false>(a.out_kind, [&](auto kind) {
         store_results<decltype(kind)::value>(a, m, n, a.vec_out && n + 8 <= a.n, e);
     });
 }
