@@ -572,9 +572,12 @@ int qxt_add_rms_norm(const void *x, size_t x_row_stride, uint32_t x_type, const 
  * matrix instruction drops what lies more than 13 bits below the largest of eight
  * neighbouring products (1e-5 of a result's size).  y_type: QXT_TYPE_*, rounded once.  qxt_mxfp4_linear takes activations as floats and
  * quantises them as qxt_quantize_mx does.  workspace (16-byte aligned):
- * qxt_mxfp4_linear_workspace() bytes for one weight (floats: 1 where activations are
- * floats; out_kind: y_type, or h_kind below), free again when the stream has passed the call. */
-size_t qxt_mxfp4_linear_workspace(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, uint32_t format, uint32_t floats,
+ * qxt_mxfp4_linear_workspace() bytes for one weight (x_kind: 0 for activations in
+ * blocks, 1 + QXT_TYPE_* for floats, with QXT_ROWS_ALIGNED added where x and its row
+ * stride are multiples of 16 bytes; out_kind: y_type, or h_kind below), free again when
+ * the stream has passed the call; NULL where that is 0. */
+#define QXT_ROWS_ALIGNED 16u
+size_t qxt_mxfp4_linear_workspace(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, uint32_t format, uint32_t x_kind,
                                   uint32_t out_kind);
 int qxt_mxfp4_gemm(const qxt_mx_matrix *a, uint32_t format, const qxt_mx_matrix *w, const float *bias, void *y, size_t ldy,
                    uint32_t y_type, uint32_t m, uint32_t n, uint32_t k, void *workspace, size_t workspace_bytes, void *stream);

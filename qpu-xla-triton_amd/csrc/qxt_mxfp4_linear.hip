@@ -308,18 +308,24 @@ bool streams(uint32_t m, uint32_t k, uint32_t format) {
     const uint32_t blocks = k / kMxBlock;
     return m <= 16 && (format == QXT_MX_FP4 ? act_rows<kAct4>(m, blocks) : act_rows<kAct8>(m, blocks)).bytes <= kStreamBytes;
 }
-bool fuses(const Floats &x, uint32_t m, uint32_t k, uint32_t format) {
-    return streams(m, k, format) && m * static_cast<size_t>(float_row(x.type, k / kMxBlock)) <= kFusedBytes &&
-           aligned(x.x, 16) && (m == 1 || x.stride % 16 == 0);
+// x_kind: 0 for blocks, else 1 + the floats' type, with QXT_ROWS_ALIGNED where rows start at multiples of 16 bytes.
+uint32_t kind_of(const Floats *x, uint32_t m) {
+    if (x == nullptr) return 0;
+    return 1 + x->type + (aligned(x->x, 16) && (m == 1 || x->stride % 16 == 0) ? QXT_ROWS_ALIGNED : 0);
+}
+bool fuses(uint32_t x_kind, uint32_t m, uint32_t k, uint32_t format) {
+    return (x_kind & QXT_ROWS_ALIGNED) != 0 && streams(m, k, format) &&
+           m * static_cast<size_t>(float_row((x_kind & ~QXT_ROWS_ALIGNED) - 1, k / kMxBlock)) <= kFusedBytes;
 }
 
 // The workspace: quantised activations (values, scales in rows of words), and for the tile kernels room for each
 // operand's scales in rows of words, and the sums of the parts of K.
 struct Workspace {
     size_t scales = 0, a_scales = 0, w_scales = 0, w_each = 0, parts = 0, bytes = 0;
-    Workspace(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, uint32_t format, uint32_t out_kind, bool floats) {
+    Workspace(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, uint32_t format, uint32_t x_kind, uint32_t out_kind) {
         const size_t pad = padded(k / kMxBlock);
-        if (floats) {
+        const bool floats = x_kind != 0;
+        if (floats && !fuses(x_kind, m, k, format)) {
             scales = up16(m * mx_row_bytes(format, k));
             bytes = scales + up16(m * pad);
         }
@@ -340,7 +346,7 @@ int run_linear(MxLinearArgs &a, const Floats *x, uint32_t format, bool is_gated,
                size_t workspace_bytes, void *stream) {
     const char *name = is_gated ? "mxfp4 gated" : "mxfp4 linear";
     if (!known_mx(format)) return fail(QXT_INVALID_ARGUMENT, "%s: unknown block format", name);
-    if (k == 0 || k % kMxBlock || k > kMostK) return fail(QXT_INVALID_ARGUMENT, "%s: K must be a positive multiple of 32 below 2^22", name);
+    if (k == 0 || k % kMxBlock || k >= kMostK) return fail(QXT_INVALID_ARGUMENT, "%s: K must be a positive multiple of 32 below 2^22", name);
     if (a.m > INT32_MAX / 32 || a.n > INT32_MAX / 32) return fail(QXT_INVALID_ARGUMENT, "%s: too many rows or columns", name);
     const bool blocks_out = a.out_kind == QXT_ROWS_MXFP8 || a.out_kind == QXT_ROWS_MXFP4;
     if (!known_type(a.out_kind) && !(is_gated && blocks_out))
@@ -351,7 +357,8 @@ int run_linear(MxLinearArgs &a, const Floats *x, uint32_t format, bool is_gated,
     a.blocks = k / kMxBlock;
     if (a.m == 0 || a.n == 0) return QXT_OK;
     if (a.y == nullptr || (blocks_out && a.y_scales == nullptr)) return fail(QXT_INVALID_ARGUMENT, "%s: null pointer", name);
-    const Workspace room(a.m, a.n, k, is_gated ? 2 : 1, format, a.out_kind, x != nullptr);
+    const uint32_t x_kind = kind_of(x, a.m);
+    const Workspace room(a.m, a.n, k, is_gated ? 2 : 1, format, x_kind, a.out_kind);
     if (x != nullptr) {
         const size_t element = type_bytes(x->type);
         if (x->x == nullptr) return fail(QXT_INVALID_ARGUMENT, "%s: null pointer", name);
@@ -359,14 +366,14 @@ int run_linear(MxLinearArgs &a, const Floats *x, uint32_t format, bool is_gated,
             (a.m > 1 && static_cast<size_t>(x->stride) < k * element))
             return fail(QXT_INVALID_ARGUMENT, "%s: bad strides or alignment", name);
     }
-    const bool fused = x != nullptr && fuses(*x, a.m, k, format);
+    const bool fused = fuses(x_kind, a.m, k, format);
     if (x != nullptr && !fused) {
         a.a.values = static_cast<const char *>(workspace);
         a.a.stride = static_cast<int64_t>(mx_row_bytes(format, k));
         a.a.scales = static_cast<const uint8_t *>(workspace) + room.scales;
         a.a.scale_stride = padded(a.blocks);
     }
-    if (!fused && room.bytes != 0 && (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < room.bytes))
+    if (room.bytes != 0 && (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < room.bytes))
         return fail(QXT_INVALID_ARGUMENT, "%s: workspace too small or not aligned to 16 bytes", name);
     if (!fused)
         if (int rc = check_operand(name, a.a, format, a.m, a.blocks)) return rc;
@@ -441,10 +448,12 @@ using namespace qxt;
 
 extern "C" {
 
-size_t qxt_mxfp4_linear_workspace(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, uint32_t format, uint32_t floats,
+size_t qxt_mxfp4_linear_workspace(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, uint32_t format, uint32_t x_kind,
                                   uint32_t out_kind) {
-    if (!known_mx(format) || k == 0 || k % kMxBlock || weights == 0 || weights > 2 || m == 0 || n == 0) return 0;
-    return Workspace(m, n, k, weights, format, out_kind, floats != 0).bytes;
+    if (!known_mx(format) || k == 0 || k % kMxBlock || k >= kMostK || weights == 0 || weights > 2 || m == 0 || n == 0 ||
+        (x_kind & ~QXT_ROWS_ALIGNED) > 1 + QXT_TYPE_F16)
+        return 0;
+    return Workspace(m, n, k, weights, format, x_kind, out_kind).bytes;
 }
 
 int qxt_mxfp4_gemm(const qxt_mx_matrix *a, uint32_t format, const qxt_mx_matrix *w, const float *bias, void *y, size_t ldy,

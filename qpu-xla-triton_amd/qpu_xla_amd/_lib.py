@@ -68,6 +68,7 @@ ROWS_MXFP8 = 5
 ROWS_MXFP4 = 6
 GATE_SILU = 0
 GATE_GELU = 1
+ROWS_ALIGNED = 16
 
 
 class DeviceInfo(Structure):

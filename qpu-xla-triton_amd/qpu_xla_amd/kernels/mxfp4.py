@@ -105,10 +105,18 @@ def _float_out(name: str, like: torch.Tensor, out: torch.Tensor | None, dtype: t
     return out, code, stride
 
 
-def _workspace(rows: int, columns: int, depth: int, weights: int, fmt: int, floats: int, kind: int, stream: Any,
-               device: torch.device) -> tuple[torch.Tensor | None, int]:
-    size = (_lib._lib or _lib.load()).qxt_mxfp4_linear_workspace(rows, columns, depth, weights, fmt, floats, kind)
-    return (workspace_for(stream, size, device), size) if size else (None, 0)
+def _workspace(rows: int, columns: int, depth: int, weights: int, fmt: int, x_kind: int, kind: int, stream: Any,
+               device: torch.device) -> tuple[torch.Tensor | None, int | None, int]:
+    """(the workspace, its address, its size)."""
+    size = (_lib._lib or _lib.load()).qxt_mxfp4_linear_workspace(rows, columns, depth, weights, fmt, x_kind, kind)
+    if not size:
+        return None, None, 0
+    workspace = workspace_for(stream, size, device)
+    return workspace, workspace.data_ptr(), size
+
+
+def _x_kind(x: torch.Tensor, code: int, stride: int) -> int:
+    return 1 + code if (x.data_ptr() | stride) % 16 else 1 + code + _lib.ROWS_ALIGNED
 
 
 def mxfp4_gemm(
@@ -132,9 +140,9 @@ def mxfp4_gemm(
     dtype = dtype if dtype is not None else torch.float32 if out is None else out.dtype
     out, code, stride = _float_out(name, a_values, out, dtype, m, n, stream)
     require_current_gpu(name, a_values, a_scales, w_values, w_scales, bias, out)
-    workspace, size = _workspace(m, n, k, 1, fmt, 0, code, stream, a_values.device)
-    _lib.call("qxt_mxfp4_gemm", a, fmt, w, bias_at, out.data_ptr(), stride, code, m, n, k,
-              None if workspace is None else workspace.data_ptr(), size, stream_handle(stream))
+    workspace, at, size = _workspace(m, n, k, 1, fmt, 0, code, stream, a_values.device)
+    _lib.call("qxt_mxfp4_gemm", a, fmt, w, bias_at, out.data_ptr(), stride, code, m, n, k, at, size,
+              stream_handle(stream))
     return out
 
 
@@ -160,9 +168,9 @@ def mxfp4_linear(
     dtype = dtype if dtype is not None else x.dtype if out is None else out.dtype
     out, code, stride = _float_out(name, x, out, dtype, m, n, stream)
     require_current_gpu(name, x, w_values, w_scales, bias, out)
-    workspace, size = _workspace(m, n, k, 1, fmt, 1, code, stream, x.device)
-    _lib.call("qxt_mxfp4_linear", x.data_ptr(), x_stride, x_code, fmt, w, bias_at, out.data_ptr(), stride, code, m, n, k,
-              None if workspace is None else workspace.data_ptr(), size, stream_handle(stream))
+    workspace, at, size = _workspace(m, n, k, 1, fmt, _x_kind(x, x_code, x_stride), code, stream, x.device)
+    _lib.call("qxt_mxfp4_linear", x.data_ptr(), x_stride, x_code, fmt, w, bias_at, out.data_ptr(), stride, code, m, n, k, at, size,
+              stream_handle(stream))
     return out
 
 
@@ -221,9 +229,9 @@ def mxfp4_gated_gemm(
     function = _gate_function(name, gate)
     result, tensors, kind, places = _gated_out(name, a_values, output, out, m, n, stream)
     require_current_gpu(name, a_values, a_scales, gate_values, gate_scales, up_values, up_scales, *tensors)
-    workspace, size = _workspace(m, n, k, 2, fmt, 0, kind, stream, a_values.device)
-    _lib.call("qxt_mxfp4_gated_gemm", a, fmt, gate_at, up_at, function, *places, kind, m, n, k,
-              None if workspace is None else workspace.data_ptr(), size, stream_handle(stream))
+    workspace, at, size = _workspace(m, n, k, 2, fmt, 0, kind, stream, a_values.device)
+    _lib.call("qxt_mxfp4_gated_gemm", a, fmt, gate_at, up_at, function, *places, kind, m, n, k, at, size,
+              stream_handle(stream))
     return result
 
 
@@ -250,9 +258,9 @@ def mxfp4_gated_linear(
         output = out.dtype if isinstance(out, torch.Tensor) else x.dtype
     result, tensors, kind, places = _gated_out(name, x, output, out, m, n, stream)
     require_current_gpu(name, x, gate_values, gate_scales, up_values, up_scales, *tensors)
-    workspace, size = _workspace(m, n, k, 2, fmt, 1, kind, stream, x.device)
-    _lib.call("qxt_mxfp4_gated_linear", x.data_ptr(), x_stride, x_code, fmt, gate_at, up_at, function, *places, kind, m, n, k,
-              None if workspace is None else workspace.data_ptr(), size, stream_handle(stream))
+    workspace, at, size = _workspace(m, n, k, 2, fmt, _x_kind(x, x_code, x_stride), kind, stream, x.device)
+    _lib.call("qxt_mxfp4_gated_linear", x.data_ptr(), x_stride, x_code, fmt, gate_at, up_at, function, *places, kind, m, n, k, at, size,
+              stream_handle(stream))
     return result
 
 
