@@ -19,6 +19,10 @@ Host-side mirror of the reference's W8A8 contract owner,
   ``supported-win`` candidates of the exact shape class from a
   ``CandidateRegistry``.  There is no CPU reference path: a shape without a
   GPU or hybrid winner raises instead of running on the host.
+
+Next to them, with no counterpart there, weights in microscaling 4-bit blocks:
+``QuantizedMatrixMxfp4``, ``quantize_matrix_mxfp4``, ``mxfp4_linear`` and
+``mxfp4_feed_forward`` (norm, gated product and the linear down).
 """
 
 from __future__ import annotations
@@ -32,6 +36,8 @@ from qpu_xla_amd import _lib
 from qpu_xla_amd._tensors import ptr, require_gpu, row_stride, rows_are_dense, stream_handle
 from qpu_xla_amd.candidates import CandidateRecord, CandidateRegistry
 from qpu_xla_amd.errors import DependencyError
+from qpu_xla_amd.kernels import mxfp4
+from qpu_xla_amd.kernels.add_rms_norm import add_rms_norm_mxfp4, add_rms_norm_mxfp8
 from qpu_xla_amd.kernels.gemm_int8 import w8a8_gemm_dequantize
 from qpu_xla_amd.kernels.quantize import quantize_rows_int8
 from qpu_xla_amd.placement import Placement
@@ -586,3 +592,82 @@ class CalibratedW8A8Linear:
         return self._gpu.execute_hybrid(
             destination, source, qpu_queue=queue, cpu_queue=cpu_queue, qpu_outputs=dispatch.units, wait_for=wait_for,
         )
+
+
+# ------------------------------------------------------ microscaling 4-bit weights
+
+
+@dataclass(frozen=True)
+class QuantizedMatrixMxfp4:
+    """Matrix [N, K] in microscaling 4-bit blocks along K: packed values uint8 [N, K/2], scales uint8 [N, K/32]."""
+
+    values: torch.Tensor
+    scales: torch.Tensor
+
+    def __post_init__(self) -> None:
+        if self.values.dim() != 2 or self.scales.dim() != 2 or self.values.shape[0] != self.scales.shape[0]:
+            raise ValueError("microscaling matrix values and scales must be rank-2 with the same rows")
+        if self.values.dtype != torch.uint8 or self.scales.dtype != torch.uint8:
+            raise ValueError("microscaling matrix values and scales must be uint8")
+        if self.values.shape[1] != 16 * self.scales.shape[1] or not self.scales.shape[1]:
+            raise ValueError("microscaling matrix must have a scale for every 32 columns")
+        if not self.values.is_contiguous() or not self.scales.is_contiguous():
+            raise ValueError("microscaling matrix values and scales must be contiguous")
+
+    @property
+    def shape(self) -> tuple[int, int]:
+        return (int(self.values.shape[0]), 2 * int(self.values.shape[1]))
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        return mxfp4.dequantize_mxfp4(self.values, self.scales, dtype=dtype)
+
+
+def quantize_matrix_mxfp4(weight: torch.Tensor, *, stream: Any = None) -> QuantizedMatrixMxfp4:
+    """Quantise float ``(output, input)`` weights to microscaling 4-bit blocks on the GPU."""
+    return QuantizedMatrixMxfp4(*mxfp4.quantize_mxfp4(weight, stream=stream))
+
+
+def mxfp4_linear(
+    x: torch.Tensor,
+    weight: QuantizedMatrixMxfp4,
+    bias: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    *,
+    activations: str = "mxfp8",
+    dtype: torch.dtype | None = None,
+    stream: Any = None,
+) -> torch.Tensor:
+    """``x @ weight.T (+ bias)`` of float rows [M, K], quantised to ``activations`` blocks; x's type unless said otherwise."""
+    return mxfp4.mxfp4_linear(x, weight.values, weight.scales, bias, out, activations=activations, dtype=dtype, stream=stream)
+
+
+def mxfp4_feed_forward(
+    x: torch.Tensor,
+    residual: torch.Tensor | None,
+    norm_weight: torch.Tensor,
+    gate: QuantizedMatrixMxfp4,
+    up: QuantizedMatrixMxfp4,
+    down: QuantizedMatrixMxfp4,
+    *,
+    epsilon: float = 1e-6,
+    activations: str = "mxfp8",
+    function: str = "silu",
+    residual_out: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    dtype: torch.dtype | None = None,
+    stream: Any = None,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """A decoder layer's feed-forward block: (y [M, D], the stream x + residual).
+
+    Three operators whose rows stay in blocks of ``activations`` between them: the stream's norm, ``f(gate) * up`` with
+    f ``function``, and the linear down, in x's type unless ``out`` or ``dtype`` says otherwise.  y is not added to the
+    stream: the next norm does that.
+    """
+    mxfp4.mx_format("mxfp4_feed_forward", activations)
+    norm = add_rms_norm_mxfp8 if activations == "mxfp8" else add_rms_norm_mxfp4
+    values, scales, total = norm(x, norm_weight, residual, epsilon=epsilon, residual_out=residual_out, stream=stream)
+    inner = mxfp4.mxfp4_gated_gemm(values, scales, gate.values, gate.scales, up.values, up.scales, gate=function,
+                                   output=activations, stream=stream)
+    if dtype is None:
+        dtype = x.dtype if out is None else out.dtype
+    return mxfp4.mxfp4_gemm(*inner, down.values, down.scales, None, out, dtype=dtype, stream=stream), total
