@@ -165,7 +165,8 @@ __global__ __launch_bounds__(kMostThreads) void add_rms_norm_kernel(NormArgs a) 
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             h[i].v[e] = h[i].v[e] * factor * by[e];
-            if (OUT == QXT_ROWS_INT8) largest = fmaxf(largest, fabsf(h[i].v[e]));
+            // (Only the row's own: what a thread past it re-read may be a sum stored in place by then.)
+            if (OUT == QXT_ROWS_INT8 && threadIdx.x + i * threads < pieces) largest = fmaxf(largest, fabsf(h[i].v[e]));
         }
     }
     float scale = 0.0f;

@@ -197,3 +197,19 @@ def test_queue_kernel_and_captured() -> None:
         torch.cuda.synchronize()
         eager = add_rms_norm(x, weight, residual, epsilon=EPSILON)
         assert torch.equal(captured[0], eager[0]) and torch.equal(captured[1], eager[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("columns", [520, 1096, 4104, 8200, 9000])
+def test_quantised_rows_with_the_sum_in_place(columns, dtype) -> None:
+    """Widths that leave threads past the row: they re-read a place whose sum may be stored by then."""
+    x, weight, residual = _inputs(2048, columns, dtype, dtype)
+    xs, ws, rs = _cuda(x, weight, residual)
+    want = add_rms_norm_int8(xs, ws, rs, epsilon=EPSILON)
+    got = add_rms_norm_int8(xs, ws, rs, epsilon=EPSILON, residual_out=rs)
+    assert got[2] is rs
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    _, rounded, total = reference.norm(x[:64], weight, residual[:64], EPSILON)
+    codes, scale = reference.int8_rows(rounded)
+    assert torch.equal(want[0][:64].cpu(), codes) and torch.equal(want[1][:64].cpu(), scale) and torch.equal(want[2][:64].cpu(), total)
