@@ -321,6 +321,22 @@ int run_norm(NormArgs &a, uint32_t out_kind, uint32_t rows, hipStream_t stream) 
     if (a.residual != nullptr && (!strides(a.residual, a.residual_stride, r_size, width * r_size) ||
                                   !strides(a.sum, a.sum_stride, r_size, width * r_size)))
         return fail(QXT_INVALID_ARGUMENT, "%s: bad strides or alignment", name);
+    // A thread writes floats only where it has read the element of that place itself: they may lie exactly over x or the
+    // residual.
+    const RowSpan inputs[2] = {{a.x, a.x_stride, rows, width * x_size}, {a.residual, a.residual_stride, rows, width * r_size}};
+    const RowSpan sum{a.residual != nullptr ? a.sum : nullptr, a.sum_stride, rows, width * r_size}, weight{a.weight, 0, 1, width * sizeof(float)};
+    const RowSpan out{a.out, a.out_stride, rows, out_row};
+    const RowSpan scales{planes ? a.scales : nullptr, out_kind == QXT_ROWS_INT8 ? 4 : a.scales_stride, rows,
+                         out_kind == QXT_ROWS_INT8 ? 4 : width / 32};
+    auto clash = [&](const RowSpan &to, bool may_replace) {
+        for (const RowSpan &from : inputs)
+            if (overlap(to, from) && !(may_replace && to.at == from.at && to.bytes == from.bytes && (rows == 1 || to.stride == from.stride)))
+                return true;
+        return overlap(to, weight);
+    };
+    if (clash(sum, true) || clash(out, out_kind <= QXT_TYPE_F16) || clash(scales, false) || overlap(sum, out) || overlap(sum, scales) ||
+        overlap(out, scales))
+        return fail(QXT_INVALID_ARGUMENT, "%s: an output shares memory with another operand", name);
     if (int rc = injected(QXT_FAIL_SUBMISSION)) return rc;
     auto sixteen = [](const void *p, int64_t stride) { return aligned(p, 16) && stride % 16 == 0; };
     const size_t store = out_kind <= QXT_TYPE_F16 ? 16 : out_kind == QXT_ROWS_Q8_0 ? 2 : out_kind == QXT_ROWS_MXFP4 ? 4 : 8;

@@ -16,6 +16,24 @@ constexpr int kMxBlock = 32;
 inline bool known_mx(uint32_t format) { return format == QXT_MX_FP4 || format == QXT_MX_FP8; }
 inline size_t mx_row_bytes(uint32_t format, uint32_t columns) { return format == QXT_MX_FP4 ? columns / 2 : columns; }
 
+// Rows in memory, `bytes` each.
+struct RowSpan {
+    const void *at;
+    int64_t stride;
+    uint64_t rows, bytes;
+};
+// Whether two sets of rows share memory.  (Sets of one stride may lie between each other's rows; sets of different strides
+// are taken to meet where their ranges do.)
+inline bool overlap(const RowSpan &x, const RowSpan &y) {
+    if (x.at == nullptr || y.at == nullptr || x.rows == 0 || y.rows == 0) return false;
+    const uint64_t x0 = reinterpret_cast<uintptr_t>(x.at), y0 = reinterpret_cast<uintptr_t>(y.at);
+    const uint64_t x_skip = x.rows > 1 ? x.stride : y.rows > 1 ? y.stride : 0, y_skip = y.rows > 1 ? y.stride : x_skip;
+    if (x0 + (x.rows - 1) * x_skip + x.bytes <= y0 || y0 + (y.rows - 1) * y_skip + y.bytes <= x0) return false;
+    if (x_skip != y_skip || x_skip == 0) return true;
+    const uint64_t ahead = y0 >= x0 ? (y0 - x0) % x_skip : x_skip - 1 - (x0 - y0 - 1) % x_skip;
+    return ahead < x.bytes || ahead + y.bytes > x_skip;
+}
+
 // Eight neighbouring elements of a row as fp32.
 struct Eight {
     float v[8];

@@ -61,6 +61,10 @@ int run_mx(bool quantize, MxRows &a, uint32_t rows, uint32_t columns, uint32_t f
     if (rows > 1 && (x_stride < columns * element || v_stride < mx_row_bytes(format, columns) ||
                      static_cast<size_t>(a.scales_stride) < columns / kMxBlock))
         return fail(QXT_INVALID_ARGUMENT, "%s: a row stride is below the row", name);
+    const RowSpan floats{a.x, a.x_stride, rows, columns * element}, scales{a.scales, a.scales_stride, rows, columns / kMxBlock};
+    const RowSpan values{a.values, a.values_stride, rows, mx_row_bytes(format, columns)};
+    if (overlap(floats, values) || overlap(floats, scales) || overlap(values, scales))
+        return fail(QXT_INVALID_ARGUMENT, "%s: an output shares memory with another operand", name);
     if (int rc = injected(QXT_FAIL_SUBMISSION)) return rc;
     a.pieces = static_cast<uint32_t>(pieces);
     a.row = fast_div(columns / 8);

@@ -59,7 +59,7 @@ __device__ __forceinline__ i8 both_halves(u4 a, u4 b) {
 
 // Activation operands of one instruction, and acc += W A over 128 elements of K: 16 weight rows (4-bit) by 16 activation
 // rows.  Lane l holds weight row l % 16 and activation row l % 16; of 4-bit rows the 32 elements of block l / 16, of 8-bit
-// ones bytes 16 (l / 16) + [0, 16) and 64 + the same; and of both rows byte J of a word of scales: that of block l / 16.
+// ones bytes 16 (l / 16) + [0, 16) and 64 + the same; and of both rows the scale of block l / 16.
 // It receives weight rows 4 (l / 16) + [0, 4) of activation row l % 16.
 template <int ACT>
 struct ActPiece {
@@ -82,12 +82,12 @@ struct ActPiece {
     }
 };
 
-template <int ACT, int J>
+template <int ACT>
 __device__ __forceinline__ f4 mx_mfma(u4 w, const ActPiece<ACT> &a, f4 acc, uint32_t w_scales, uint32_t a_scales) {
     constexpr int form = ACT == kAct4 ? 4 : 0;
-    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(low_half(w), a.v, acc, 4, form, J, w_scales, J, a_scales);
+    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(low_half(w), a.v, acc, 4, form, 0, w_scales, 0, a_scales);
     if constexpr (ACT == kAct8Parts)
-        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(low_half(w), a.rest, acc, 4, form, J, w_scales, J, a_scales);
+        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(low_half(w), a.rest, acc, 4, form, 0, w_scales, 0, a_scales);
     return acc;
 }
 

@@ -195,7 +195,7 @@ __global__ __launch_bounds__(64 * WAVES) void mxfp4_stream_kernel(MxLinearArgs a
         for (int u = 0; u < 2; ++u) {
             const ActPiece<ACT> act(lo[u], hi[u]);
 #pragma unroll
-            for (int t = 0; t < TILES; ++t) acc[t] = mx_mfma<ACT, 0>(w[t][u], act, acc[t], wscale[t][u], ascale[u]);
+            for (int t = 0; t < TILES; ++t) acc[t] = mx_mfma<ACT>(w[t][u], act, acc[t], wscale[t][u], ascale[u]);
         }
         slot = slot + 1 == SLOTS ? 0 : slot + 1;
     }
@@ -385,6 +385,15 @@ int run_linear(MxLinearArgs &a, const Floats *x, uint32_t format, bool is_gated,
         (a.m > 1 && (static_cast<size_t>(a.y_stride) < out_row ||
                      (blocks_out && static_cast<size_t>(a.y_scale_stride) < a.n / kMxBlock))))
         return fail(QXT_INVALID_ARGUMENT, "%s: bad strides or alignment", name);
+    const RowSpan y{a.y, a.y_stride, a.m, out_row}, y_scales{blocks_out ? a.y_scales : nullptr, a.y_scale_stride, a.m, a.n / kMxBlock};
+    auto clash = [&](const RowSpan &from) { return overlap(y, from) || overlap(y_scales, from); };
+    auto clashes = [&](const MxOperand &o, uint32_t kind, uint32_t rows) {
+        return clash({o.values, o.stride, rows, mx_row_bytes(kind, k)}) || clash({o.scales, o.scale_stride, rows, a.blocks});
+    };
+    if (overlap(y, y_scales) || clash({a.bias, 0, 1, a.n * sizeof(float)}) || clashes(a.w[0], QXT_MX_FP4, a.n) ||
+        (is_gated && clashes(a.w[1], QXT_MX_FP4, a.n)) ||
+        (x != nullptr ? clash({x->x, x->stride, a.m, k * type_bytes(x->type)}) : clashes(a.a, format, a.m)))
+        return fail(QXT_INVALID_ARGUMENT, "%s: an output shares memory with another operand", name);
     if (int rc = injected(QXT_FAIL_SUBMISSION)) return rc;
     a.vec_out = aligned(a.y, 16) && a.y_stride % 16 == 0;
     if (x != nullptr && !fused) {

@@ -179,7 +179,7 @@ __global__ __launch_bounds__(64 * WN * WM) void mxfp4_tile_kernel(MxLinearArgs a
         for (int j = 0; j < TA; ++j) {
             const ActPiece<ACT> act(lo[j], hi[j]);
 #pragma unroll
-            for (int i = 0; i < TW; ++i) acc[i][j] = mx_mfma<ACT, 0>(w[i], act, acc[i][j], wscale[i], ascale[j]);
+            for (int i = 0; i < TW; ++i) acc[i][j] = mx_mfma<ACT>(w[i], act, acc[i][j], wscale[i], ascale[j]);
         }
     };
     // All but the youngest `younger` stages in flight have landed.  (A group's scales are fetched before a stage's rows,

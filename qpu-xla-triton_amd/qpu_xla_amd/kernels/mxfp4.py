@@ -12,7 +12,7 @@ uint8 [R, K/32] (bytes of ``torch.float8_e8m0fnu``).
 * ``mxfp4_gated_gemm``, ``mxfp4_gated_linear`` -- ``f(a @ gate.T) * (a @ up.T)``, the inner product of a feed-forward
   block, as floats or as the blocks that the next linear takes.
 
-Sums are fp32, each result is rounded once.  There are no gradients: the weights are quantised ones, for serving.  No
+Sums are fp32, each result is rounded once.  An output shares no memory with the operands.  There are no gradients: the weights are quantised ones, for serving.  No
 counterpart in the reference, whose block formats are ggml's.
 """
 
@@ -216,17 +216,20 @@ def mxfp4_gated_gemm(
     out: Any = None,
     *,
     gate: str = "silu",
-    output: Any = torch.float32,
+    output: Any = None,
     stream: Any = None,
 ) -> Any:
     """``f(a @ gate.T) * (a @ up.T)`` [M, N] of blocks, f ``gate`` ("silu", or "gelu" by erf) of the fp32 sums.
 
-    ``output``: a float type, or "mxfp8" / "mxfp4" for (values, scales), N a multiple of 32; ``out`` likewise.
+    ``output``: a float type (float32, or ``out``'s, where it is not given), or "mxfp8" / "mxfp4" for (values, scales), N a
+    multiple of 32, and then ``out`` is such a pair.
     """
     name = "mxfp4_gated_gemm"
     m, k, fmt, a = mx_rows(name, "a", a_values, a_scales)
     n, gate_at, up_at = _gate_weights(name, k, gate_values, gate_scales, up_values, up_scales)
     function = _gate_function(name, gate)
+    if output is None:
+        output = out.dtype if isinstance(out, torch.Tensor) else torch.float32
     result, tensors, kind, places = _gated_out(name, a_values, output, out, m, n, stream)
     require_current_gpu(name, a_values, a_scales, gate_values, gate_scales, up_values, up_scales, *tensors)
     workspace, at, size = _workspace(m, n, k, 2, fmt, 0, kind, stream, a_values.device)

@@ -258,3 +258,37 @@ def test_other_device_is_refused() -> None:
         quantize_mxfp4(x, w[0][:2].cpu())
     with pytest.raises(ValueError, match="HIP device"):
         dequantize_mxfp4(w[0], w[1].cpu())
+
+
+@pytest.mark.parametrize("m", [2, 40])
+def test_types_of_blocks_that_torch_names(m) -> None:
+    """Packed pairs as float4_e2m1fn_x2 and scales as float8_e8m0fnu are the same bytes."""
+    gen = torch.Generator().manual_seed(m)
+    x, w = torch.randn((m, 128), generator=gen).cuda(), quantize_mxfp4(torch.randn((64, 128), generator=gen).cuda())
+    named = (w[0].view(torch.float4_e2m1fn_x2), w[1].view(torch.float8_e8m0fnu))
+    a = quantize_mxfp4(x)
+    named_a = (a[0].view(torch.float4_e2m1fn_x2), a[1].view(torch.float8_e8m0fnu))
+    assert torch.equal(mxfp4_linear(x, *named), mxfp4_linear(x, *w))
+    assert torch.equal(mxfp4_gemm(*named_a, *named), mxfp4_gemm(*a, *w))
+    assert torch.equal(mxfp4_gated_gemm(*named_a, *named, *named), mxfp4_gated_gemm(*a, *w, *w))
+    assert torch.equal(dequantize_mxfp4(*named), dequantize_mxfp4(*w))
+    values, scales = quantize_mxfp4(x, torch.empty_like(a[0]).view(torch.float4_e2m1fn_x2), torch.empty_like(a[1]).view(torch.float8_e8m0fnu))
+    assert torch.equal(values.view(torch.uint8), a[0]) and torch.equal(scales.view(torch.uint8), a[1])
+
+
+def test_outputs_in_given_tensors() -> None:
+    a, w = quantize_mxfp8(torch.randn((3, 128), device="cuda")), quantize_mxfp4(torch.randn((64, 128), device="cuda"))
+    out = torch.empty((3, 64), dtype=torch.float16, device="cuda")
+    assert mxfp4_gated_gemm(*a, *w, *w, out) is out
+    assert torch.equal(out, mxfp4_gated_gemm(*a, *w, *w, output=torch.float16))
+    pair = (torch.empty((3, 64), dtype=torch.float8_e4m3fn, device="cuda"), torch.empty((3, 2), dtype=torch.uint8, device="cuda"))
+    got = mxfp4_gated_gemm(*a, *w, *w, pair, output="mxfp8")
+    assert got[0] is pair[0] and got[1] is pair[1]
+    x = torch.randn((64, 64), device="cuda")
+    with pytest.raises(Exception, match="shares memory"):
+        mxfp4_linear(x, *quantize_mxfp4(x), out=x)
+    wide = torch.randn((5, 256), device="cuda")
+    left, right = wide[:, :128], wide[:, 128:192]
+    want = mxfp4_linear(left, *w)
+    mxfp4_linear(left, *w, out=right)  # columns of one tensor share none
+    assert torch.equal(right, want)

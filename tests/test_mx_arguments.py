@@ -14,7 +14,7 @@ from qpu_xla_amd import KernelError, LaunchConfig, _lib
 from qpu_xla_amd import kernels as k
 from qpu_xla_amd.quantization import QuantizedMatrixMxfp4
 
-FAKE = 1 << 20  # 16-byte aligned, never dereferenced
+FAKE, FAR = 1 << 20, 1 << 28  # 16-byte aligned, never dereferenced; operands of one call lie FAR apart
 BF16 = torch.bfloat16
 
 
@@ -206,8 +206,9 @@ def _c(name, *args):
     return getattr(_lib.load(), name)(*args)
 
 
-def _norm_call(x=FAKE, x_stride=256, x_type=0, residual=FAKE, residual_stride=256, residual_type=0, total=FAKE, sum_stride=256,
-               weight=FAKE, epsilon=1e-6, out=FAKE, out_stride=256, scales=FAKE, scales_stride=2, kind=0, rows=2, columns=64):
+def _norm_call(x=FAKE, x_stride=256, x_type=0, residual=FAKE + FAR, residual_stride=256, residual_type=0, total=FAKE + 2 * FAR, sum_stride=256,
+               weight=FAKE + 3 * FAR, epsilon=1e-6, out=FAKE + 4 * FAR, out_stride=256, scales=FAKE + 5 * FAR, scales_stride=2, kind=0,
+               rows=2, columns=64):
     return _c("qxt_add_rms_norm", x, x_stride, x_type, residual, residual_stride, residual_type, total, sum_stride, weight,
               epsilon, out, out_stride, scales, scales_stride, kind, rows, columns, None)
 
@@ -232,11 +233,11 @@ def test_entries_return_at_once_without_rows() -> None:
 @pytest.mark.parametrize("changes", [
     {"x": None}, {"values": None}, {"scales": None}, {"type": 3}, {"format": 2}, {"columns": 48}, {"columns": 0}, {"x": FAKE + 1},
     {"x_stride": 100}, {"v_stride": 28}, {"values": FAKE + 2}, {"s_stride": 1}, {"format": 1, "values": FAKE + 4},
-    {"rows": 2**31 - 1, "columns": 2**20},
+    {"rows": 2**31 - 1, "columns": 2**20}, {"values": FAKE}, {"values": FAKE + 700}, {"scales": FAKE + 256}, {"scales": FAKE + FAR + 20},
 ])
 def test_quantise_entries_refuse(name, changes) -> None:
-    a = {"x": FAKE, "x_stride": 256, "type": 0, "values": FAKE, "v_stride": 64, "scales": FAKE, "s_stride": 2, "rows": 3, "columns": 64, "format": 0,
-         **changes}
+    a = {"x": FAKE, "x_stride": 256, "type": 0, "values": FAKE + FAR, "v_stride": 64, "scales": FAKE + 2 * FAR, "s_stride": 2, "rows": 3,
+         "columns": 64, "format": 0, **changes}
     x, values = (a["x"], a["x_stride"], a["type"]), (a["values"], a["v_stride"], a["scales"], a["s_stride"])
     args = (*x, *values) if name == "qxt_quantize_mx" else (*values, *x)
     assert _c(name, *args, a["rows"], a["columns"], a["format"], None) == _lib.INVALID_ARGUMENT
@@ -246,8 +247,8 @@ def _matrix(values=FAKE, stride=32, scales=FAKE, scale_stride=2):
     return _lib.MX_MATRIX.pack(values or 0, stride, scales or 0, scale_stride)
 
 
-def _linear_call(floats=False, gated=False, a=None, w=None, up=None, fmt=0, gate=0, bias=None, y=FAKE, ldy=256, scales=FAKE, lds=2, kind=0,
-                 m=3, n=64, k=64, x=FAKE, ldx=256, x_type=0, workspace=FAKE, size=1 << 30):
+def _linear_call(floats=False, gated=False, a=None, w=None, up=None, fmt=0, gate=0, bias=None, y=FAKE + 2 * FAR, ldy=256, scales=FAKE + 3 * FAR,
+                 lds=2, kind=0, m=3, n=64, k=64, x=FAKE + FAR, ldx=256, x_type=0, workspace=FAKE + 4 * FAR, size=1 << 30):
     first = (x, ldx, x_type, fmt) if floats else (a or _matrix(), fmt)
     tail = (m, n, k, workspace, size, None)
     if gated:
@@ -293,6 +294,47 @@ def test_gated_entry_refuses(changes) -> None:
     assert _linear_call(gated=True, **changes) == _lib.INVALID_ARGUMENT
 
 
+@pytest.mark.parametrize("changes", [
+    {"out": FAKE + 4, "out_stride": 256}, {"out": FAKE, "out_stride": 512}, {"out": FAKE, "kind": 1}, {"total": FAKE + FAR + 4},
+    {"total": FAKE, "sum_stride": 512}, {"total": FAKE + 4 * FAR}, {"out": FAKE + 3 * FAR}, {"kind": 3, "scales": FAKE + 4 * FAR + 60},
+    {"kind": 5, "scales": FAKE + FAR + 2}, {"kind": 5, "out": FAKE}, {"kind": 3, "scales": FAKE + 2 * FAR + 4},
+])
+def test_norm_entry_refuses_shared_memory(changes) -> None:
+    assert _norm_call(**changes) == _lib.INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("floats", [False, True])
+@pytest.mark.parametrize("changes", [
+    {"y": FAKE}, {"y": FAKE + FAR, "w": _matrix(FAKE + FAR)}, {"y": FAKE + 1024, "w": _matrix(scales=FAKE + 1536)},
+    {"y": FAKE + 64, "ldy": 512}, {"y": FAKE + FAR + 256, "x": FAKE + FAR, "a": _matrix(FAKE + FAR + 512)},
+])
+def test_linear_entries_refuse_shared_memory(gated, floats, changes) -> None:
+    assert _linear_call(floats, gated, **changes) == _lib.INVALID_ARGUMENT
+
+
+def test_linear_outputs_refuse_shared_memory() -> None:
+    assert _linear_call(bias=FAKE + 2 * FAR) == _lib.INVALID_ARGUMENT
+    assert _linear_call(gated=True, up=_matrix(FAKE + 2 * FAR)) == _lib.INVALID_ARGUMENT
+    assert _linear_call(gated=True, kind=5, scales=FAKE + 2 * FAR + 32) == _lib.INVALID_ARGUMENT
+    assert _linear_call(gated=True, kind=5, scales=FAKE) == _lib.INVALID_ARGUMENT
+
+
+def test_rows_between_rows_of_one_buffer_are_taken() -> None:
+    """Columns of one wide tensor: the injected failure tells that the checks are passed."""
+    _lib.set_failure_mask(_lib.FAIL_SUBMISSION)
+    try:
+        for changes in ({"out": FAKE, "residual": None}, {"total": FAKE + FAR}, {"total": FAKE}, {"out": FAKE}, {"out": FAKE + FAR},
+                        {"x_stride": 512, "out": FAKE + 256, "out_stride": 512}, {"x_stride": 768, "out": FAKE + 256, "out_stride": 768, "total": FAKE + 512, "sum_stride": 768},
+                        {"kind": 5, "out_stride": 66, "scales": FAKE + 4 * FAR + 64, "scales_stride": 66}, {"kind": 3, "out": FAKE + 8 * FAR}):
+            assert _norm_call(**changes) == _lib.SUBMISSION_FAILED, changes
+        assert _linear_call(True, ldx=512, y=FAKE + FAR + 256, ldy=512) == _lib.SUBMISSION_FAILED
+        assert _linear_call(True, ldx=512, x=FAKE + FAR + 256, y=FAKE + FAR, ldy=512) == _lib.SUBMISSION_FAILED
+        assert _linear_call(True, ldx=512, y=FAKE + FAR + 252, ldy=512) == _lib.INVALID_ARGUMENT
+    finally:
+        _lib.set_failure_mask(_lib.FAIL_NONE)
+
+
 def test_null_matrices() -> None:
     assert _c("qxt_mxfp4_gemm", None, 0, _matrix(), None, FAKE, 256, 0, 3, 64, 64, None, 0, None) == _lib.INVALID_ARGUMENT
     assert _c("qxt_mxfp4_linear", FAKE, 256, 0, 0, None, None, FAKE, 256, 0, 3, 64, 64, None, 0, None) == _lib.INVALID_ARGUMENT
@@ -303,7 +345,7 @@ def test_failure_injection_comes_before_any_launch() -> None:
     _lib.set_failure_mask(_lib.FAIL_SUBMISSION)
     try:
         assert _norm_call() == _lib.SUBMISSION_FAILED
-        assert _c("qxt_quantize_mx", FAKE, 256, 0, FAKE, 64, FAKE, 2, 3, 64, 0, None) == _lib.SUBMISSION_FAILED
+        assert _c("qxt_quantize_mx", FAKE, 256, 0, FAKE + FAR, 64, FAKE + 2 * FAR, 2, 3, 64, 0, None) == _lib.SUBMISSION_FAILED
         for floats in (False, True):
             for gated in (False, True):
                 assert _linear_call(floats, gated) == _lib.SUBMISSION_FAILED
