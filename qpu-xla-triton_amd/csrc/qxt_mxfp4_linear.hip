@@ -11,9 +11,11 @@ namespace {
 
 // Few activation rows: bound by the weights' bytes.  A workgroup owns 16 RT rows of each weight and all of the (at most 16)
 // activation rows, which lie in LDS for the whole of K, and its waves take every WAVES-th unit of 256 elements of K: 128
-// bytes of each weight row, a cache line, fetched by DMA into one of the wave's SLOTS own LDS buffers, where it lies so
-// that the reads of a piece (16 bytes) over 16 rows touch all banks.  Nothing but its own loads is waited for by a wave
-// until the sums of all are added up.  Float activations come into LDS as they are and are quantised there, by every
+// bytes of each weight row, a cache line, fetched by DMA into the wave's own LDS buffer, where it lies so that the reads of
+// a piece (16 bytes) over 16 rows touch all banks.  A wave requests its next unit once it has read one into registers, and
+// waits for nothing but its own loads until the sums of all are added up: what is in flight meanwhile are the other waves'
+// units (two buffers a wave leave room for fewer workgroups: one row, K = 14336, N = 4096 8.6 -> 8.9 us, gated K = 4096,
+// N = 14336 14.1 -> 14.7 us).  Float activations come into LDS as they are and are quantised there, by every
 // workgroup for itself: less than a launch where they are few.  Activations too are fetched by DMA, ahead of the first
 // weights: waiting for a load into registers would wait for every weight requested after it.
 struct Floats {
@@ -40,7 +42,7 @@ __host__ __device__ inline ActRows act_rows(uint32_t m, uint32_t blocks) {
 // Bytes of a float row in LDS.
 __host__ __device__ inline uint32_t float_row(uint32_t type, uint32_t blocks) { return blocks * (type == QXT_TYPE_F32 ? 128 : 64); }
 
-template <int ACT, bool GATED, bool FLOATS, bool WORDS, int RT, int WAVES, int SLOTS>
+template <int ACT, bool GATED, bool FLOATS, bool WORDS, int RT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void mxfp4_stream_kernel(MxLinearArgs a, Floats f) {
     constexpr int W = GATED ? 2 : 1, TILES = W * RT, THREADS = 64 * WAVES;
     constexpr int DATA = 2 * TILES, SCALES = WORDS ? (TILES + 1) / 2 : 0, LOADS = DATA + SCALES;  // loads of a unit
@@ -50,7 +52,7 @@ __global__ __launch_bounds__(64 * WAVES) void mxfp4_stream_kernel(MxLinearArgs a
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t n0 = blockIdx.x * 16 * RT, blocks = a.blocks, units = (blocks + 7) / 8;
     const ActRows rows = act_rows<ACT>(a.m, blocks);
-    const uint32_t slots = rows.bytes + wave * SLOTS * kSlot;
+    const uint32_t slot = rows.bytes + wave * kSlot;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds)));
 
     // Rows of `bytes` (a multiple of 16) to LDS, `pitch` apart: the waves take 1024 bytes in turn.
@@ -65,7 +67,7 @@ __global__ __launch_bounds__(64 * WAVES) void mxfp4_stream_kernel(MxLinearArgs a
             while (at >= loads && row < a.m) at -= loads, ++row;
         }
     };
-    const uint32_t raw = rows.bytes + WAVES * SLOTS * kSlot, raw_row = FLOATS ? float_row(f.type, blocks) : 0;
+    const uint32_t raw = rows.bytes + WAVES * kSlot, raw_row = FLOATS ? float_row(f.type, blocks) : 0;
     if constexpr (FLOATS) {
         fetch_rows(f.x, f.stride, raw_row, raw, raw_row);
     } else {
@@ -102,13 +104,12 @@ __global__ __launch_bounds__(64 * WAVES) void mxfp4_stream_kernel(MxLinearArgs a
         s_from[i] = a.w[0].scales + at * a.w[0].scale_stride;
         if (W == 2 && t % 2 == 1) s_from[i] = a.w[1].scales + at * a.w[1].scale_stride;
     }
-    auto fetch = [&](uint32_t unit, uint32_t slot) {
-        const uint32_t to = slots + slot * kSlot;
+    auto fetch = [&](uint32_t unit) {
         const bool whole = 8 * unit + 8 <= blocks;
         const char *zero = reinterpret_cast<const char *>(&kZeroPiece);
 #pragma unroll
         for (int i = 0; i < (TILES + 1) / 2; ++i) {
-            const uint32_t block = 8 * unit + lane % 2 * 4, at = to + TILES * 2048 + i * 256;
+            const uint32_t block = 8 * unit + lane % 2 * 4, at = slot + TILES * 2048 + i * 256;
             if constexpr (WORDS) {
                 const char *src = reinterpret_cast<const char *>(s_from[i] + block);
                 dma4_from(block < blocks ? src : zero, lds0 + at);
@@ -125,18 +126,15 @@ __global__ __launch_bounds__(64 * WAVES) void mxfp4_stream_kernel(MxLinearArgs a
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const char *src = w_from[t][h] + unit * 128ull;
-                dma16_from(whole || 8 * unit + wpiece < blocks ? src : zero, lds0 + to + t * 2048 + h * 1024);
+                dma16_from(whole || 8 * unit + wpiece < blocks ? src : zero, lds0 + slot + t * 2048 + h * 1024);
             }
     };
-#pragma unroll
-    for (int s = 0; s < SLOTS; ++s)
-        if (wave + s * WAVES < units) fetch(wave + s * WAVES, s);
-
-    // The activations have landed when only the weights are left in flight.
-    const uint32_t mine = wave < units ? min((units - 1 - wave) / WAVES + 1, static_cast<uint32_t>(SLOTS)) : 0u;
-    if (SLOTS > 1 && mine == 2) landed<2 * LOADS>();
-    else if (mine == 1) landed<LOADS>();
-    else landed<0>();
+    if (wave < units) {
+        fetch(wave);
+        landed<LOADS>();  // the activations: only the weights are left in flight
+    } else {
+        landed<0>();
+    }
     if constexpr (FLOATS) {
         meet();
         for (uint32_t row = 0; row < a.m; ++row) {
@@ -168,13 +166,9 @@ __global__ __launch_bounds__(64 * WAVES) void mxfp4_stream_kernel(MxLinearArgs a
     const char *a_at = lds + arow * rows.row + c * 16;
     const char *as_at = lds + rows.scales + arow * rows.scale_row + c;
     f4 acc[TILES] = {};
-    uint32_t slot = 0;
     for (uint32_t unit = wave; unit < units; unit += WAVES) {
-        // Units behind this one that are in flight.
-        const uint32_t younger = min((units - 1 - unit) / WAVES, static_cast<uint32_t>(SLOTS - 1));
-        if (SLOTS > 1 && younger == 1) landed<LOADS>();
-        else landed<0>();
-        const char *from = lds + slots + slot * kSlot;
+        landed<0>();
+        const char *from = lds + slot;
         u4 w[TILES][2], lo[2], hi[2];
         uint32_t wscale[TILES][2], ascale[2];
 #pragma unroll
@@ -190,14 +184,13 @@ __global__ __launch_bounds__(64 * WAVES) void mxfp4_stream_kernel(MxLinearArgs a
             }
         }
         reads_done();
-        if (unit + SLOTS * WAVES < units) fetch(unit + SLOTS * WAVES, slot);
+        if (unit + WAVES < units) fetch(unit + WAVES);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             const ActPiece<ACT> act(lo[u], hi[u]);
 #pragma unroll
             for (int t = 0; t < TILES; ++t) acc[t] = mx_mfma<ACT>(w[t][u], act, acc[t], wscale[t][u], ascale[u]);
         }
-        slot = slot + 1 == SLOTS ? 0 : slot + 1;
     }
 
     // The waves' sums lie where the units were.
@@ -248,36 +241,32 @@ __global__ __launch_bounds__(256) void pad_scales_kernel(const uint8_t *from, in
     to[at] = word;
 }
 
-template <int ACT, bool GATED, int RT, int WAVES, int SLOTS>
+template <int ACT, bool GATED, int RT, int WAVES>
 constexpr size_t stream_lds(const MxLinearArgs &a, const Floats *f) {
     constexpr uint32_t tiles = RT * (GATED ? 2 : 1), slot = tiles * 2048 + (tiles + 1) / 2 * 256;
-    static_assert(SLOTS >= 1 && SLOTS <= 2 && slot >= tiles * 1024, "the sums lie where the units were");
-    return act_rows<ACT>(a.m, a.blocks).bytes + WAVES * SLOTS * slot + (f != nullptr ? a.m * float_row(f->type, a.blocks) : 0);
+    static_assert(slot >= tiles * 1024, "the sums lie where the units were");
+    return act_rows<ACT>(a.m, a.blocks).bytes + WAVES * slot + (f != nullptr ? a.m * float_row(f->type, a.blocks) : 0);
 }
 
-template <int ACT, bool GATED, int RT, int WAVES, int SLOTS>
+template <int ACT, bool GATED, int RT, int WAVES>
 int launch_stream(const MxLinearArgs &a, const Floats *f, bool words, hipStream_t stream) {
-    auto kernel = f != nullptr ? (words ? mxfp4_stream_kernel<ACT, GATED, true, true, RT, WAVES, SLOTS>
-                                        : mxfp4_stream_kernel<ACT, GATED, true, false, RT, WAVES, SLOTS>)
-                               : (words ? mxfp4_stream_kernel<ACT, GATED, false, true, RT, WAVES, SLOTS>
-                                        : mxfp4_stream_kernel<ACT, GATED, false, false, RT, WAVES, SLOTS>);
+    auto kernel = f != nullptr ? (words ? mxfp4_stream_kernel<ACT, GATED, true, true, RT, WAVES>
+                                        : mxfp4_stream_kernel<ACT, GATED, true, false, RT, WAVES>)
+                               : (words ? mxfp4_stream_kernel<ACT, GATED, false, true, RT, WAVES>
+                                        : mxfp4_stream_kernel<ACT, GATED, false, false, RT, WAVES>);
     return launch("mxfp4_stream_kernel", kernel, dim3((a.n + 16 * RT - 1) / (16 * RT)), dim3(64 * WAVES),
-                  stream_lds<ACT, GATED, RT, WAVES, SLOTS>(a, f), stream, a, f != nullptr ? *f : Floats{});
+                  stream_lds<ACT, GATED, RT, WAVES>(a, f), stream, a, f != nullptr ? *f : Floats{});
 }
 
-// Which rows, waves and buffers.  Gated products hold 32 rows of each weight, for whole blocks of results; two buffers a
-// wave where two workgroups fit a CU all the same (one row, K = 4096, N = 14336, 8-bit rows: 14.0 -> 13.7 us; with them
-// where only one fits, as with bf16 rows: 13.6 -> 16.8 us).  A single weight of many columns, or of a short K, in 32 rows
-// by four waves (one row, K = 4096, N = 14336: 8.1 us, with 16 rows by eight waves 8.9; K = 2048, N = 5632 4.8, 5.2), else
-// in 16 rows by eight waves (K = 14336, N = 4096: 8.2 us, with 32 rows by four 8.9; K = 4096 4.4, 5.1).
+// Which rows and waves.  Gated products hold 32 rows of each weight, for whole blocks of results.  A single weight of many
+// columns, or of a short K, in 32 rows by four waves (one row, K = 4096, N = 14336 8.4 us, with 16 rows by eight waves 9.8;
+// K = 2048, N = 5632 4.3, 4.6), else in 16 rows by eight waves (K = 14336, N = 4096 8.5 us, with 32 rows by four 11.6; K =
+// 4096 4.8, 5.8).
 template <int ACT>
 int launch_act(const MxLinearArgs &a, const Floats *f, bool is_gated, bool words, hipStream_t stream) {
-    if (is_gated) {
-        if (stream_lds<ACT, true, 2, 4, 2>(a, f) <= 80 * 1024) return launch_stream<ACT, true, 2, 4, 2>(a, f, words, stream);
-        return launch_stream<ACT, true, 2, 4, 1>(a, f, words, stream);
-    }
-    if (a.n >= 12288 || a.blocks <= 64) return launch_stream<ACT, false, 2, 4, 2>(a, f, words, stream);
-    return launch_stream<ACT, false, 1, 8, 2>(a, f, words, stream);
+    if (is_gated) return launch_stream<ACT, true, 2, 4>(a, f, words, stream);
+    if (a.n >= 12288 || a.blocks <= 64) return launch_stream<ACT, false, 2, 4>(a, f, words, stream);
+    return launch_stream<ACT, false, 1, 8>(a, f, words, stream);
 }
 
 constexpr uint32_t kMostK = 1u << 22;
