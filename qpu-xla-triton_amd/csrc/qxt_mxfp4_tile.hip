@@ -44,7 +44,7 @@ struct Tiles {
     static constexpr int LDS = OPERANDS > RESULTS ? OPERANDS : RESULTS;
     static_assert(W_LOADS % WAVES == 0 && A_LOADS % WAVES == 0 && LDS <= 160 * 1024, "tile shape");
     static_assert(OUT % 32 == 0 && OUT <= 128, "a wave's results hold whole blocks, and 64 lanes at most 16 rows of them");
-    static_assert(RING <= GROUP, "a group's scales are fetched with the last stage of the group before");
+    static_assert(RING >= 2 && RING <= 3 && RING <= GROUP, "a group's scales are fetched with the last stage of the group before");
 };
 
 // Where piece p (16 bytes) of row r of a stage lies, in pieces from the row's start.
@@ -185,8 +185,7 @@ __global__ __launch_bounds__(64 * WN * WM) void mxfp4_tile_kernel(MxLinearArgs a
     // All but the youngest `younger` stages in flight have landed.  (A group's scales are fetched before a stage's rows,
     // so they have landed with them, or before.)
     auto landed_but = [&](uint32_t younger) {
-        if (RING > 3 && younger == 2) landed<2 * T::LOADS>();
-        else if (RING > 2 && younger == 1) landed<T::LOADS>();
+        if (RING > 2 && younger == 1) landed<T::LOADS>();
         else landed<0>();
     };
 
@@ -301,7 +300,8 @@ __global__ __launch_bounds__(64 * WN * WM) void mxfp4_tile_kernel(MxLinearArgs a
     });
 }
 
-// Joins the parts of K: a thread adds up eight columns of a row, in the order of the parts.
+// Joins the parts of K: a thread adds up eight columns of a row, in the order of the parts, whose loads it issues several
+// parts at a time (77 x 4096 results of eight parts: 4.1 us, one part at a time 5.1).
 template <int ACT, bool GATED>
 __global__ __launch_bounds__(256) void mxfp4_join_kernel(MxLinearArgs a, FastDiv row) {
     const uint32_t at = blockIdx.x * 256 + threadIdx.x, m = fast_quotient(at, row), n = (at - m * row.divisor) * 8;
@@ -309,11 +309,26 @@ __global__ __launch_bounds__(256) void mxfp4_join_kernel(MxLinearArgs a, FastDiv
     const uint64_t plane = static_cast<uint64_t>(a.m) * a.part_row;
     const float *from = a.parts + static_cast<uint64_t>(m) * a.part_row + n;
     f4 sum[GATED ? 2 : 1][2] = {};
-    for (uint32_t s = 0; s < a.splits; ++s)
+    constexpr uint32_t kWeights = GATED ? 2 : 1, kParts = 8 / kWeights;
+    for (uint32_t first = 0; first < a.splits; first += kParts) {
+        f4 part[kParts][kWeights][2];
 #pragma unroll
-        for (int w = 0; w < (GATED ? 2 : 1); ++w, from += plane)
+        for (uint32_t s = 0; s < kParts; ++s)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) sum[w][h] += *reinterpret_cast<const f4 *>(from + 4 * h);
+            for (uint32_t w = 0; w < kWeights; ++w)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    part[s][w][h] = *reinterpret_cast<const f4 *>(from + (min(first + s, a.splits - 1) * kWeights + w) * plane + 4 * h);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (uint32_t s = 0; s < kParts; ++s) {
+            if (first + s >= a.splits) break;
+#pragma unroll
+            for (uint32_t w = 0; w < kWeights; ++w)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) sum[w][h] += part[s][w][h];
+        }
+    }
     Eight e;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -352,31 +367,34 @@ constexpr uint32_t kTileRows[kTiles][2] = {{256, 256}, {128, 128}, {128, 64}, {6
 
 template <int ACT, bool GATED>
 int launch_tiles(MxLinearArgs &a, const TilePlan &plan, hipStream_t stream) {
-    // 4-bit rows take two steps of K a stage, for whole cache lines.
-    constexpr int SUB = ACT == kAct4 ? 2 : 1, RING = ACT == kAct4 ? 2 : 3, DEEP = ACT == kAct4 ? 2 : 4;
+    // 4-bit rows take two steps of K a stage, for whole cache lines.  Eight waves alone on a CU take the stages that fit.
+    // Where several workgroups share a CU two stages are better than three (8-bit, 333 x 4096 x 14336, 128 x 128: 34.4 ->
+    // 32.3 us; 1024 x 2048 x 5632, 128 x 64: 22.4 -> 18.5), or as good, but for the small tiles, whose products of one part
+    // are short (64 x 64, 128 x 4096 x 11008: two stages 21.6, three 19.9, four 20.4 us).
+    constexpr int SUB = ACT == kAct4 ? 2 : 1, RING = ACT == kAct4 ? 2 : 3, SMALL = ACT == kAct8 ? 3 : 2;
     switch (plan.tile) {
         case 0: return launch_tile<ACT, GATED, 8, 4, 2, 4, SUB, RING>(a, plan.splits, stream);
-        case 1: return launch_tile<ACT, GATED, 4, 4, 2, 2, SUB, RING>(a, plan.splits, stream);
-        case 2: return launch_tile<ACT, GATED, 4, 2, 2, 2, SUB, RING>(a, plan.splits, stream);
-        case 3: return launch_tile<ACT, GATED, 4, 1, 1, 4, SUB, DEEP>(a, plan.splits, stream);
-        default: return launch_tile<ACT, GATED, 4, 1, 2, 2, SUB, DEEP>(a, plan.splits, stream);
+        case 1: return launch_tile<ACT, GATED, 4, 4, 2, 2, SUB, 2>(a, plan.splits, stream);
+        case 2: return launch_tile<ACT, GATED, 4, 2, 2, 2, SUB, 2>(a, plan.splits, stream);
+        case 3: return launch_tile<ACT, GATED, 4, 1, 1, 4, SUB, SMALL>(a, plan.splits, stream);
+        default: return launch_tile<ACT, GATED, 4, 1, 2, 2, SUB, SMALL>(a, plan.splits, stream);
     }
 }
 
 // Estimated microseconds of a launch: a step of 128 elements of K takes `step` where few workgroups run and half of that
 // plus `share` for each 256 workgroups where many do; `edge`: filling the ring and storing the results, for each 256
 // workgroups.  Fitted to 4093 measured calls (17 to 4096 rows, K 512 to 14336, 1024 to 14336 columns, every tile and up to
-// 16 parts; rms error 8 %); the least estimate is on average 2 % slower than the fastest of them, at most 24 %.
+// 16 parts; rms error 9 %); the least estimate is on average 2.5 % slower than the fastest of them, at most 25 %.
 struct TileCost {
     float step, share, edge;
 };
 constexpr TileCost kCosts[3][kTiles] = {
-    {{0.92f, 0.65f, 5.4f}, {0.37f, 0.26f, 2.3f}, {0.29f, 0.18f, 1.5f}, {0.25f, 0.11f, 0.7f}, {0.27f, 0.15f, 0.8f}},  // kAct4
-    {{1.10f, 0.87f, 5.5f}, {0.61f, 0.36f, 2.2f}, {0.36f, 0.25f, 1.6f}, {0.30f, 0.17f, 0.8f}, {0.29f, 0.21f, 1.1f}},  // kAct8
-    {{2.36f, 1.53f, 6.1f}, {1.01f, 0.61f, 2.9f}, {0.58f, 0.34f, 2.1f}, {0.44f, 0.25f, 1.3f}, {0.44f, 0.26f, 1.6f}},  // kAct8Parts
+    {{0.94f, 0.62f, 4.9f}, {0.37f, 0.26f, 2.2f}, {0.29f, 0.18f, 1.4f}, {0.25f, 0.11f, 0.7f}, {0.27f, 0.15f, 0.8f}},  // kAct4
+    {{1.11f, 0.83f, 4.8f}, {0.59f, 0.36f, 1.6f}, {0.51f, 0.24f, 0.9f}, {0.32f, 0.17f, 0.6f}, {0.30f, 0.21f, 0.7f}},  // kAct8
+    {{2.38f, 1.42f, 5.5f}, {0.98f, 0.59f, 2.5f}, {0.57f, 0.32f, 1.8f}, {0.46f, 0.19f, 1.1f}, {0.49f, 0.22f, 1.1f}},  // kAct8Parts
 };
 // The second kernel that parts of K need, and a megabyte of their sums.
-constexpr float kJoin = 2.7f, kJoinMegabyte = 0.09f;
+constexpr float kJoin = 2.2f, kJoinMegabyte = 0.1f;
 constexpr uint32_t kMostSplits = 16;
 
 }  // namespace
