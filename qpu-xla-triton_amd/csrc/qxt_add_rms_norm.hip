@@ -13,8 +13,8 @@
 // Bound by its bytes: a workgroup holds a row in registers between the load, the
 // sum over the row and the store, so every input is read once.  Measured, with a residual: 4096 rows of 4096, bf16 to
 // 8-bit blocks 26.8 us (4.4 TB/s), to bf16 27.6 (4.9), to int8 rows 32 (3.7: the maximum is a second wait for all waves),
-// fp32 to 4-bit blocks 46.3 (4.5); 4096 of 8192, bf16 53.6 (5.0); 777 of 11008, fp16 22.5 (3.0: three rows a CU, all at
-// once, so loads, sums and stores of few rows overlap); one row of 2048 3.5.
+// fp32 to 4-bit blocks 46.3 (4.5); 4096 of 8192, bf16 53.6 (5.0); 777 of 11008, fp16 22.5 (3.0: three rows a CU, all in
+// one go, so that little of one's stores overlaps another's loads); one row of 2048 3.5.
 #include "qxt_mx.h"
 
 namespace qxt {

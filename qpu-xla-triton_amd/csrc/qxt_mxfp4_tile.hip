@@ -10,6 +10,14 @@
 // so that the reads of one piece over 16 rows touch all banks.  A gated product
 // takes the tiles of gate and up in turn, so that a wave holds both sums of a
 // result.
+//
+// Measured: 4096 x 4096 x 14336 with 4-bit activations 166 us (2.9 PFLOP/s; matrix
+// units 38 % busy), gated with 8-bit ones 366 us (2.6 PFLOP/s, 60 %).  With the rest
+// taken out, at 8192 x 8192 x 8192, the products alone take 59 % of the time (8-bit
+// 69 %) and the fetches alone 52 % (60 %: 33 clocks a KB on each CU); the two
+// overlap in part only, since a fetch's writes and the waves' reads share LDS.
+// 77 x 11008 x 4096: 11.6 us and 4.0 for joining eight parts of K, against 4.8 for
+// its bytes: a CU has six stages of one tile, too few to hide the first and last.
 #include "qxt_mxfp4.h"
 
 namespace qxt {
