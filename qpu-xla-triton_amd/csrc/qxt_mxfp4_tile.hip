@@ -389,21 +389,27 @@ int launch_tiles(MxLinearArgs &a, const TilePlan &plan, hipStream_t stream) {
     }
 }
 
-// Estimated microseconds of a launch: a step of 128 elements of K takes `step` where few workgroups run and half of that
-// plus `share` for each 256 workgroups where many do; `edge`: filling the ring and storing the results, for each 256
-// workgroups.  Fitted to 4093 measured calls (17 to 4096 rows, K 512 to 14336, 1024 to 14336 columns, every tile and up to
-// 16 parts; rms error 9 %); the least estimate is on average 2.5 % slower than the fastest of them, at most 25 %.
+// Estimated microseconds of a launch: a step of 128 elements of K takes `least`, or `base` plus `share` for each workgroup
+// a CU; `edge`: filling the ring and storing the results, for each workgroup a CU.  (Workgroups a CU: a third of their mean
+// over 256 CUs and two thirds of the fullest CU's.)  Fitted to 10182 measured calls (606 products of 17 to 4096 rows, K 512
+// to 14336, 1024 to 14336 columns, every tile and number of parts below; rms error 9 %); the least estimate is on average
+// 1 % slower than the fastest of them, in five products more than 10 %, at most 21 %.
 struct TileCost {
-    float step, share, edge;
+    float least, base, share, edge;
 };
 constexpr TileCost kCosts[3][kTiles] = {
-    {{0.94f, 0.62f, 4.9f}, {0.37f, 0.26f, 2.2f}, {0.29f, 0.18f, 1.4f}, {0.25f, 0.11f, 0.7f}, {0.27f, 0.15f, 0.8f}},  // kAct4
-    {{1.11f, 0.83f, 4.8f}, {0.59f, 0.36f, 1.6f}, {0.51f, 0.24f, 0.9f}, {0.32f, 0.17f, 0.6f}, {0.30f, 0.21f, 0.7f}},  // kAct8
-    {{2.38f, 1.42f, 5.5f}, {0.98f, 0.59f, 2.5f}, {0.57f, 0.32f, 1.8f}, {0.46f, 0.19f, 1.1f}, {0.49f, 0.22f, 1.1f}},  // kAct8Parts
+    // kAct4
+    {{0.96f, 0.03f, 0.90f, 7.3f}, {0.41f, 0.03f, 0.26f, 2.4f}, {0.30f, 0.01f, 0.20f, 1.6f}, {0.25f, 0.08f, 0.11f, 0.6f}, {0.30f, 0.07f, 0.15f, 1.2f}},
+    // kAct8
+    {{0.51f, 0.37f, 0.78f, 8.2f}, {0.46f, 0.40f, 0.24f, 2.4f}, {0.52f, 0.10f, 0.27f, 1.0f}, {0.28f, 0.20f, 0.14f, 0.6f}, {0.29f, 0.14f, 0.19f, 0.6f}},
+    // kAct8Parts
+    {{0.21f, 1.39f, 1.36f, 8.4f}, {0.95f, 0.64f, 0.42f, 3.7f}, {0.00f, 0.44f, 0.18f, 2.1f}, {0.47f, 0.12f, 0.22f, 1.1f}, {0.48f, 0.10f, 0.25f, 1.3f}},
 };
-// The second kernel that parts of K need, and a megabyte of their sums.
-constexpr float kJoin = 2.2f, kJoinMegabyte = 0.1f;
-constexpr uint32_t kMostSplits = 16;
+// The second kernel that parts of K need, and a megabyte of their sums, written and read.
+constexpr float kJoin = 2.3f, kJoinMegabyte = 0.175f;
+// Numbers of parts, and the most workgroups that K is split for.
+constexpr uint32_t kParts[] = {1, 2, 3, 4, 6, 8, 12, 16};
+constexpr float kMostSplitTiles = 600.0f;
 
 }  // namespace
 
@@ -415,12 +421,14 @@ TilePlan plan_tiles(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, int ac
     for (uint32_t t = 0; t < kTiles; ++t) {
         const float tiles = static_cast<float>((m + kTileRows[t][1] - 1) / kTileRows[t][1]) *
                             static_cast<float>((static_cast<uint64_t>(n) * weights + kTileRows[t][0] - 1) / kTileRows[t][0]);
-        for (uint32_t wanted = 1; wanted <= kMostSplits && wanted <= groups; ++wanted) {
+        for (const uint32_t wanted : kParts) {
+            if (wanted > groups || (wanted > 1 && tiles * static_cast<float>(wanted) > kMostSplitTiles)) break;
             const uint32_t each = (groups + wanted - 1) / wanted, splits = (groups + each - 1) / each;
             if (splits < wanted) continue;  // the same as fewer
             const TileCost &c = kCosts[act][t];
-            const float load = tiles * static_cast<float>(splits) / 256.0f, depth = static_cast<float>(min(4 * each, steps));
-            float cost = depth * fmaxf(c.step, 0.5f * c.step + c.share * load) + c.edge * fmaxf(load, 1.0f);
+            const float mean = tiles * static_cast<float>(splits) / 256.0f, load = (mean + 2.0f * ceilf(mean)) / 3.0f;
+            const float depth = static_cast<float>(min(4 * each, steps));
+            float cost = depth * fmaxf(c.least, c.base + c.share * load) + c.edge * load;
             if (splits > 1) cost += kJoin + kJoinMegabyte * 2.0f * static_cast<float>(splits) * sums;
             if (least == 0.0f || cost < least) {
                 least = cost;
