@@ -16,8 +16,9 @@
 // taken out, at 8192 x 8192 x 8192, the products alone take 59 % of the time (8-bit
 // 69 %) and the fetches alone 52 % (60 %: 33 clocks a KB on each CU); the two
 // overlap in part only, since a fetch's writes and the waves' reads share LDS.
-// 77 x 11008 x 4096: 11.6 us and 4.0 for joining eight parts of K, against 4.8 for
-// its bytes: a CU has six stages of one tile, too few to hide the first and last.
+// 77 x 11008 x 4096: 12.4 us and 4.1 for joining four parts of K, against 4.8 for
+// its bytes: two workgroups a CU of eleven stages each, which more parts, larger
+// tiles or deeper rings do not make faster (16.3 to 17.5 us together).
 #include "qxt_mxfp4.h"
 
 namespace qxt {
