@@ -292,21 +292,27 @@ MxOperand operand(const qxt_mx_matrix *m) {
 size_t up16(size_t bytes) { return (bytes + 15) / 16 * 16; }
 uint32_t padded(uint32_t blocks) { return (blocks + 3) / 4 * 4; }
 
-// Activation rows that the streaming kernel takes: up to 16, as long as they leave room in LDS for the weights.
-constexpr size_t kStreamBytes = 48 * 1024;
+// Activation rows that the streaming kernel takes: up to 16, as long as they leave room in LDS for the weights of two
+// workgroups, or of one where there are no more than CUs (a single weight in 16 rows a workgroup).  Four rows, K = 14336, N =
+// 4096: 9.2 us, on tiles 13.2; eight 10.2, 13.2; sixteen of K = 4096 7.3, 8.2.  (With more workgroups than CUs, or few
+// columns that parts of K spread over the CUs, tiles are faster: 16 rows, K = 4096, N = 14336 12.3 us, 16.3 here; K = 8192,
+// N = 1024 8.1, 8.6.)
+constexpr size_t kStreamBytes = 48 * 1024, kAloneBytes = 136 * 1024;
+bool alone(uint32_t n, uint32_t weights) { return weights == 1 && n > 64 * 16 && n <= 256 * 16; }
 // Bytes of float activations that every workgroup of it quantises for itself.
 constexpr size_t kFusedBytes = 32 * 1024;
-bool streams(uint32_t m, uint32_t k, uint32_t format) {
+bool streams(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, uint32_t format) {
     const uint32_t blocks = k / kMxBlock;
-    return m <= 16 && (format == QXT_MX_FP4 ? act_rows<kAct4>(m, blocks) : act_rows<kAct8>(m, blocks)).bytes <= kStreamBytes;
+    return m <= 16 && (format == QXT_MX_FP4 ? act_rows<kAct4>(m, blocks) : act_rows<kAct8>(m, blocks)).bytes <=
+                          (alone(n, weights) ? kAloneBytes : kStreamBytes);
 }
 // x_kind: 0 for blocks, else 1 + the floats' type, with QXT_ROWS_ALIGNED where rows start at multiples of 16 bytes.
 uint32_t kind_of(const Floats *x, uint32_t m) {
     if (x == nullptr) return 0;
     return 1 + x->type + (aligned(x->x, 16) && (m == 1 || x->stride % 16 == 0) ? QXT_ROWS_ALIGNED : 0);
 }
-bool fuses(uint32_t x_kind, uint32_t m, uint32_t k, uint32_t format) {
-    return (x_kind & QXT_ROWS_ALIGNED) != 0 && streams(m, k, format) &&
+bool fuses(uint32_t x_kind, uint32_t m, uint32_t n, uint32_t k, uint32_t weights, uint32_t format) {
+    return (x_kind & QXT_ROWS_ALIGNED) != 0 && streams(m, n, k, weights, format) &&
            m * static_cast<size_t>(float_row((x_kind & ~QXT_ROWS_ALIGNED) - 1, k / kMxBlock)) <= kFusedBytes;
 }
 
@@ -317,11 +323,11 @@ struct Workspace {
     Workspace(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, uint32_t format, uint32_t x_kind, uint32_t out_kind) {
         const size_t pad = padded(k / kMxBlock);
         const bool floats = x_kind != 0;
-        if (floats && !fuses(x_kind, m, k, format)) {
+        if (floats && !fuses(x_kind, m, n, k, weights, format)) {
             scales = up16(m * mx_row_bytes(format, k));
             bytes = scales + up16(m * pad);
         }
-        if (streams(m, k, format)) return;
+        if (streams(m, n, k, weights, format)) return;
         a_scales = bytes;
         if (!floats) bytes += up16(m * pad);
         w_scales = bytes;
@@ -349,8 +355,8 @@ int run_linear(MxLinearArgs &a, const Floats *x, uint32_t format, bool is_gated,
     a.blocks = k / kMxBlock;
     if (a.m == 0 || a.n == 0) return QXT_OK;
     if (a.y == nullptr || (blocks_out && a.y_scales == nullptr)) return fail(QXT_INVALID_ARGUMENT, "%s: null pointer", name);
-    const uint32_t x_kind = kind_of(x, a.m);
-    const Workspace room(a.m, a.n, k, is_gated ? 2 : 1, format, x_kind, a.out_kind);
+    const uint32_t x_kind = kind_of(x, a.m), weights = is_gated ? 2 : 1;
+    const Workspace room(a.m, a.n, k, weights, format, x_kind, a.out_kind);
     if (x != nullptr) {
         const size_t element = type_bytes(x->type);
         if (x->x == nullptr) return fail(QXT_INVALID_ARGUMENT, "%s: null pointer", name);
@@ -358,7 +364,7 @@ int run_linear(MxLinearArgs &a, const Floats *x, uint32_t format, bool is_gated,
             (a.m > 1 && static_cast<size_t>(x->stride) < k * element))
             return fail(QXT_INVALID_ARGUMENT, "%s: bad strides or alignment", name);
     }
-    const bool fused = fuses(x_kind, a.m, k, format);
+    const bool fused = fuses(x_kind, a.m, a.n, k, weights, format);
     if (x != nullptr && !fused) {
         a.a.values = static_cast<const char *>(workspace);
         a.a.stride = static_cast<int64_t>(mx_row_bytes(format, k));
@@ -369,7 +375,7 @@ int run_linear(MxLinearArgs &a, const Floats *x, uint32_t format, bool is_gated,
         return fail(QXT_INVALID_ARGUMENT, "%s: workspace too small or not aligned to 16 bytes", name);
     if (!fused)
         if (int rc = check_operand(name, a.a, format, a.m, a.blocks)) return rc;
-    for (int w = 0; w < (is_gated ? 2 : 1); ++w)
+    for (uint32_t w = 0; w < weights; ++w)
         if (int rc = check_operand(name, a.w[w], QXT_MX_FP4, a.n, a.blocks)) return rc;
     const size_t out_align = blocks_out ? (a.out_kind == QXT_ROWS_MXFP8 ? 8 : 4) : type_bytes(a.out_kind);
     const size_t out_row = a.out_kind == QXT_ROWS_MXFP8 ? a.n : a.out_kind == QXT_ROWS_MXFP4 ? a.n / 2 : a.n * type_bytes(a.out_kind);
@@ -401,9 +407,9 @@ int run_linear(MxLinearArgs &a, const Floats *x, uint32_t format, bool is_gated,
         if (int rc = run_mx(true, rows, a.m, k, format, stream)) return rc;
     }
     const hipStream_t s = as_stream(stream);
-    const bool tiles = !streams(a.m, k, format);
+    const bool tiles = !streams(a.m, a.n, k, weights, format);
     bool words = true;  // the weights' rows of scales are in words
-    for (int o = 0; o < (is_gated ? 3 : 2); ++o) {
+    for (uint32_t o = 0; o <= weights; ++o) {
         MxOperand &operand = o == 0 ? a.a : a.w[o - 1];
         if (o == 0 && (x != nullptr || !tiles)) continue;  // written so, or read byte by byte
         if (a.blocks % 4 == 0 && aligned(operand.scales, 4) && operand.scale_stride % 4 == 0) continue;
@@ -422,7 +428,7 @@ int run_linear(MxLinearArgs &a, const Floats *x, uint32_t format, bool is_gated,
     if (tiles) {
         a.parts = reinterpret_cast<float *>(static_cast<char *>(workspace) + room.parts);
         const int act = act_of(format, a.out_kind);
-        return mxfp4_tiles(a, act, is_gated, plan_tiles(a.m, a.n, k, is_gated ? 2 : 1, act), s);
+        return mxfp4_tiles(a, act, is_gated, plan_tiles(a.m, a.n, k, weights, act), s);
     }
     Floats f{};
     if (fused) f = *x;

@@ -61,6 +61,19 @@ def test_fullest_lds(m, k, fmt) -> None:
         assert torch.equal(mxfp4_linear(rows, *g, activations=fmt, dtype=torch.float32), mxfp4_gemm(*QUANTIZE[fmt](rows), *g))
 
 
+@pytest.mark.parametrize("fmt,m,k", [("mxfp8", 16, 8192), ("mxfp8", 9, 14336), ("mxfp8", 10, 14336), ("mxfp4", 16, 16384), ("mxfp8", 12, 4128)])
+@pytest.mark.parametrize("n", [1030, 4096])
+def test_rows_that_fill_the_lds_of_a_lone_workgroup(n, m, k, fmt) -> None:
+    gen = torch.Generator(device="cuda").manual_seed(k + m)
+    x = torch.randn((m, k), generator=gen, device="cuda")
+    w = quantize_mxfp4(torch.randn((n, k), generator=gen, device="cuda"))
+    a = QUANTIZE[fmt](x)
+    want, size = reference.product(READ[fmt](*a).cpu().double(), dequantize_mxfp4(*w).cpu().double())
+    got = mxfp4_gemm(*a, *w)
+    reference.check(got, want, reference.rounded(want, reference.sum_error(size, k, fmt, True), torch.float32))
+    assert torch.equal(got, mxfp4_linear(x, *w, activations=fmt))
+
+
 @pytest.mark.parametrize("m", [3, 40])
 def test_rows_gigabytes_apart(m) -> None:
     """Offsets past 32 bits, in elements' and in bytes."""

@@ -364,6 +364,8 @@ def test_workspace() -> None:
     assert _workspace(1, 4096, 4096, x_kind=2 + _lib.ROWS_ALIGNED) == 0
     assert _workspace(1, 4096, 4096, x_kind=2) == 4096 + 128
     assert _workspace(8, 4096, 4096, x_kind=1 + _lib.ROWS_ALIGNED) == 8 * (4096 + 128)
+    assert _workspace(4, 4096, 14336) == _workspace(8, 4096, 14336) == 0 and _workspace(4, 4097, 14336) > 0 and _workspace(4, 1024, 14336) > 0
+    assert _workspace(8, 4096, 14336, weights=2) > 0 and _workspace(16, 4096, 14336) > 0
     # Many rows: quantised rows, scales in words, and the sums of the parts of K.
     plain = _workspace(4096, 4096, 4096)
     assert plain == 4096 * 128 * 2
