@@ -9,8 +9,10 @@ import mx_reference as reference
 from qpu_xla_amd import quantization
 from qpu_xla_amd.kernels import (
     add_rms_norm,
+    add_rms_norm_int8,
     add_rms_norm_mxfp4,
     add_rms_norm_mxfp8,
+    add_rms_norm_q8_0,
     dequantize_mxfp4,
     mxfp4_gated_gemm,
     mxfp4_gated_linear,
@@ -18,7 +20,12 @@ from qpu_xla_amd.kernels import (
     mxfp4_linear,
     quantize_mxfp4,
     quantize_mxfp8,
+    quantize_q4_0,
+    quantize_q8_0,
 )
+from qpu_xla_amd.kernels.gemm_int8 import w8a8_gemm_dequantize
+from qpu_xla_amd.kernels.ggml_q4_0 import ggml_q4_0_q8_0_linear
+from qpu_xla_amd.kernels.ggml_q8_0 import ggml_q8_0_q8_0_linear
 
 pytestmark = pytest.mark.gpu
 
@@ -292,3 +299,21 @@ def test_outputs_in_given_tensors() -> None:
     want = mxfp4_linear(left, *w)
     mxfp4_linear(left, *w, out=right)  # columns of one tensor share none
     assert torch.equal(right, want)
+
+
+@pytest.mark.parametrize("m", [1, 5, 40])
+def test_norms_before_the_other_linears(m) -> None:
+    """Rows that the norm quantised give what the W8A8, Q4_0 and Q8_0 linears make of the norm in floats."""
+    gen = torch.Generator().manual_seed(m)
+    weight, w = (1 + 0.1 * torch.randn(256, generator=gen)).cuda(), (torch.randn((64, 256), generator=gen) / 16).cuda()
+    x, residual = torch.randn((m, 256), generator=gen).cuda(), torch.randn((m, 256), generator=gen).cuda()
+    y, total = add_rms_norm(x, weight, residual)
+    matrix = quantization.quantize_per_output_channel_int8(w)
+    codes, scales, again = add_rms_norm_int8(x, weight, residual)
+    assert torch.equal(again, total)
+    assert torch.equal(w8a8_gemm_dequantize(codes, matrix.values, scales, matrix.scales), quantization.w8a8_linear(y, matrix))
+    blocks, again = add_rms_norm_q8_0(x, weight, residual)
+    assert torch.equal(again, total)
+    q4, q8 = quantize_q4_0(w), quantize_q8_0(w)
+    assert torch.equal(ggml_q4_0_q8_0_linear(blocks, q4), ggml_q4_0_q8_0_linear(quantize_q8_0(y), q4))
+    assert torch.equal(ggml_q8_0_q8_0_linear(blocks, q8), ggml_q8_0_q8_0_linear(quantize_q8_0(y), q8))
