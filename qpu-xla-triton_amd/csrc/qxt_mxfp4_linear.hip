@@ -203,7 +203,7 @@ __global__ __launch_bounds__(64 * WAVES) void mxfp4_stream_kernel(MxLinearArgs a
     for (int t = 0; t < TILES; ++t) *reinterpret_cast<f4 *>(sums + ((wave * TILES + t) * 16 + r) * 16 + 4 * c) = acc[t];
     __syncthreads();
     // 2 RT threads an activation row, eight columns each.
-    with_kind<ACT, GATED, true>(a.out_kind, [&](auto kind) {
+    with_kind<GATED>(a.out_kind, [&](auto kind) {
         for (uint32_t i = threadIdx.x; i < a.m * 2 * RT; i += THREADS) {
             const uint32_t m = i / (2 * RT), at = i % (2 * RT), n = n0 + 8 * at;
             Eight e[W];
@@ -320,7 +320,7 @@ bool fuses(uint32_t x_kind, uint32_t m, uint32_t n, uint32_t k, uint32_t weights
 // operand's scales in rows of words, and the sums of the parts of K.
 struct Workspace {
     size_t scales = 0, a_scales = 0, w_scales = 0, w_each = 0, parts = 0, bytes = 0;
-    Workspace(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, uint32_t format, uint32_t x_kind, uint32_t out_kind) {
+    Workspace(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, uint32_t format, uint32_t x_kind) {
         const size_t pad = padded(k / kMxBlock);
         const bool floats = x_kind != 0;
         if (floats && !fuses(x_kind, m, n, k, weights, format)) {
@@ -334,7 +334,7 @@ struct Workspace {
         w_each = up16(n * pad);
         bytes += weights * w_each;
         parts = bytes;
-        const TilePlan plan = plan_tiles(m, n, k, weights, act_of(format, out_kind));
+        const TilePlan plan = plan_tiles(m, n, k, weights, act_of(format));
         if (plan.splits > 1) bytes += static_cast<size_t>(plan.splits) * weights * m * part_row(n) * sizeof(float);
     }
 };
@@ -356,7 +356,7 @@ int run_linear(MxLinearArgs &a, const Floats *x, uint32_t format, bool is_gated,
     if (a.m == 0 || a.n == 0) return QXT_OK;
     if (a.y == nullptr || (blocks_out && a.y_scales == nullptr)) return fail(QXT_INVALID_ARGUMENT, "%s: null pointer", name);
     const uint32_t x_kind = kind_of(x, a.m), weights = is_gated ? 2 : 1;
-    const Workspace room(a.m, a.n, k, weights, format, x_kind, a.out_kind);
+    const Workspace room(a.m, a.n, k, weights, format, x_kind);
     if (x != nullptr) {
         const size_t element = type_bytes(x->type);
         if (x->x == nullptr) return fail(QXT_INVALID_ARGUMENT, "%s: null pointer", name);
@@ -427,13 +427,13 @@ int run_linear(MxLinearArgs &a, const Floats *x, uint32_t format, bool is_gated,
     a.a_words = a.blocks % 4 == 0 && aligned(a.a.scales, 4) && a.a.scale_stride % 4 == 0;
     if (tiles) {
         a.parts = reinterpret_cast<float *>(static_cast<char *>(workspace) + room.parts);
-        const int act = act_of(format, a.out_kind);
+        const int act = act_of(format);
         return mxfp4_tiles(a, act, is_gated, plan_tiles(a.m, a.n, k, weights, act), s);
     }
     Floats f{};
     if (fused) f = *x;
     if (format == QXT_MX_FP4) return launch_act<kAct4>(a, fused ? &f : nullptr, is_gated, words, s);
-    return launch_act<kAct8Parts>(a, fused ? &f : nullptr, is_gated, words, s);
+    return launch_act<kAct8>(a, fused ? &f : nullptr, is_gated, words, s);
 }
 
 MxLinearArgs linear_args(const qxt_mx_matrix *w, const qxt_mx_matrix *up, void *y, size_t ldy, uint32_t kind, uint32_t m, uint32_t n) {
@@ -456,11 +456,11 @@ using namespace qxt;
 extern "C" {
 
 size_t qxt_mxfp4_linear_workspace(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, uint32_t format, uint32_t x_kind,
-                                  uint32_t out_kind) {
+                                  uint32_t /* out_kind: every one takes the same */) {
     if (!known_mx(format) || k == 0 || k % kMxBlock || k >= kMostK || weights == 0 || weights > 2 || m == 0 || n == 0 ||
         (x_kind & ~QXT_ROWS_ALIGNED) > 1 + QXT_TYPE_F16)
         return 0;
-    return Workspace(m, n, k, weights, format, x_kind, out_kind).bytes;
+    return Workspace(m, n, k, weights, format, x_kind).bytes;
 }
 
 int qxt_mxfp4_gemm(const qxt_mx_matrix *a, uint32_t format, const qxt_mx_matrix *w, const float *bias, void *y, size_t ldy,

@@ -12,10 +12,11 @@
 // result.
 //
 // Measured: 4096 x 4096 x 14336 with 4-bit activations 166 us (2.9 PFLOP/s; matrix
-// units 38 % busy), gated with 8-bit ones 366 us (2.6 PFLOP/s, 60 %).  With the rest
-// taken out, at 8192 x 8192 x 8192, the products alone take 59 % of the time (8-bit
-// 69 %) and the fetches alone 52 % (60 %: 33 clocks a KB on each CU); the two
-// overlap in part only, since a fetch's writes and the waves' reads share LDS.
+// units 38 % busy), gated with 8-bit ones 627 us (1.5 PFLOP/s of results, each product
+// in two parts).  With the rest taken out, at 8192 x 8192 x 8192 in 4 bits, the
+// products alone take 59 % of the time and the fetches alone 52 % (33 clocks a KB on
+// each CU); the two overlap in part only, since a fetch's writes and the waves' reads
+// share LDS.
 // 77 x 11008 x 4096: 12.4 us and 4.1 for joining four parts of K, against 4.8 for
 // its bytes: two workgroups a CU of eleven stages each, which more parts, larger
 // tiles or deeper rings do not make faster (16.3 to 17.5 us together).
@@ -275,7 +276,7 @@ __global__ __launch_bounds__(64 * WN * WM) void mxfp4_tile_kernel(MxLinearArgs a
         for (int e = 0; e < 8; ++e) bias[e] = a.bias != nullptr && out_n + e < a.n ? a.bias[out_n + e] : 0.0f;
     }
     const bool whole = a.vec_out && out_n + 8 <= a.n;
-    with_kind<ACT, GATED, false>(a.out_kind, [&](auto kind) {
+    with_kind<GATED>(a.out_kind, [&](auto kind) {
 #pragma unroll
         for (int j = 0; j < TA; ++j) {
 #pragma unroll
@@ -311,7 +312,7 @@ __global__ __launch_bounds__(64 * WN * WM) void mxfp4_tile_kernel(MxLinearArgs a
 
 // Joins the parts of K: a thread adds up eight columns of a row, in the order of the parts, whose loads it issues several
 // parts at a time (77 x 4096 results of eight parts: 4.1 us, one part at a time 5.1).
-template <int ACT, bool GATED>
+template <bool GATED>
 __global__ __launch_bounds__(256) void mxfp4_join_kernel(MxLinearArgs a, FastDiv row) {
     const uint32_t at = blockIdx.x * 256 + threadIdx.x, m = fast_quotient(at, row), n = (at - m * row.divisor) * 8;
     if (m >= a.m) return;  // (rows of four lanes leave together where blocks are stored)
@@ -345,7 +346,7 @@ __global__ __launch_bounds__(256) void mxfp4_join_kernel(MxLinearArgs a, FastDiv
         if constexpr (GATED) e.v[i] = gated(a.gate, e.v[i], sum[1][i / 4][i % 4]);
         else if (a.bias != nullptr && n + i < a.n) e.v[i] += a.bias[n + i];
     }
-    with_kind<ACT, GATED, false>(a.out_kind, [&](auto kind) {
+    with_kind<GATED>(a.out_kind, [&](auto kind) {
         store_results<decltype(kind)::value>(a, m, n, a.vec_out && n + 8 <= a.n, e);
     });
 }
@@ -365,7 +366,7 @@ int launch_tile(MxLinearArgs &a, uint32_t splits, hipStream_t stream) {
     const int rc = launch("mxfp4_tile_kernel", mxfp4_tile_kernel<ACT, GATED, TW, TA, WN, WM, SUB, RING>,
                           dim3(static_cast<uint32_t>(grid)), dim3(T::THREADS), 0, stream, a);
     if (rc != QXT_OK || a.splits == 1) return rc;
-    return launch("mxfp4_join_kernel", mxfp4_join_kernel<ACT, GATED>, dim3(static_cast<uint32_t>(joins)), dim3(256), 0, stream, a,
+    return launch("mxfp4_join_kernel", mxfp4_join_kernel<GATED>, dim3(static_cast<uint32_t>(joins)), dim3(256), 0, stream, a,
                   fast_div(row));
 }
 
@@ -377,33 +378,30 @@ constexpr uint32_t kTileRows[kTiles][2] = {{256, 256}, {128, 128}, {128, 64}, {6
 template <int ACT, bool GATED>
 int launch_tiles(MxLinearArgs &a, const TilePlan &plan, hipStream_t stream) {
     // 4-bit rows take two steps of K a stage, for whole cache lines.  Eight waves alone on a CU take the stages that fit.
-    // Where several workgroups share a CU two stages are better than three (8-bit, 333 x 4096 x 14336, 128 x 128: 34.4 ->
-    // 32.3 us; 1024 x 2048 x 5632, 128 x 64: 22.4 -> 18.5), or as good, but for the small tiles, whose products of one part
-    // are short (64 x 64, 128 x 4096 x 11008: two stages 21.6, three 19.9, four 20.4 us).
-    constexpr int SUB = ACT == kAct4 ? 2 : 1, RING = ACT == kAct4 ? 2 : 3, SMALL = ACT == kAct8 ? 3 : 2;
+    // Where several workgroups share a CU two stages are better than three, or as good (8-bit, 333 x 4096 x 14336 56.3 ->
+    // 48.1 us).
+    constexpr int SUB = ACT == kAct4 ? 2 : 1, RING = ACT == kAct4 ? 2 : 3;
     switch (plan.tile) {
         case 0: return launch_tile<ACT, GATED, 8, 4, 2, 4, SUB, RING>(a, plan.splits, stream);
         case 1: return launch_tile<ACT, GATED, 4, 4, 2, 2, SUB, 2>(a, plan.splits, stream);
         case 2: return launch_tile<ACT, GATED, 4, 2, 2, 2, SUB, 2>(a, plan.splits, stream);
-        case 3: return launch_tile<ACT, GATED, 4, 1, 1, 4, SUB, SMALL>(a, plan.splits, stream);
-        default: return launch_tile<ACT, GATED, 4, 1, 2, 2, SUB, SMALL>(a, plan.splits, stream);
+        case 3: return launch_tile<ACT, GATED, 4, 1, 1, 4, SUB, 2>(a, plan.splits, stream);
+        default: return launch_tile<ACT, GATED, 4, 1, 2, 2, SUB, 2>(a, plan.splits, stream);
     }
 }
 
 // Estimated microseconds of a launch: a step of 128 elements of K takes `least`, or `base` plus `share` for each workgroup
 // a CU; `edge`: filling the ring and storing the results, for each workgroup a CU.  (Workgroups a CU: a third of their mean
-// over 256 CUs and two thirds of the fullest CU's.)  Fitted to 10182 measured calls (606 products of 17 to 4096 rows, K 512
-// to 14336, 1024 to 14336 columns, every tile and number of parts below; rms error 9 %); the least estimate is on average
-// 1 % slower than the fastest of them, in five products more than 10 %, at most 21 %.
+// over 256 CUs and two thirds of the fullest CU's.)  Fitted to 3459 measured calls (198 products of 24 to 4096 rows, 8-bit
+// ones to 1024, K 512 to 14336, 1024 to 14336 columns, every tile and number of parts below; rms error 9 % and 6 %); the
+// least estimate is on average 1 % slower than the fastest of them, in one product more than 10 % (10.8 %).
 struct TileCost {
     float least, base, share, edge;
 };
-constexpr TileCost kCosts[3][kTiles] = {
+constexpr TileCost kCosts[2][kTiles] = {
     // kAct4
     {{0.96f, 0.03f, 0.90f, 7.3f}, {0.41f, 0.03f, 0.26f, 2.4f}, {0.30f, 0.01f, 0.20f, 1.6f}, {0.25f, 0.08f, 0.11f, 0.6f}, {0.30f, 0.07f, 0.15f, 1.2f}},
     // kAct8
-    {{0.51f, 0.37f, 0.78f, 8.2f}, {0.46f, 0.40f, 0.24f, 2.4f}, {0.52f, 0.10f, 0.27f, 1.0f}, {0.28f, 0.20f, 0.14f, 0.6f}, {0.29f, 0.14f, 0.19f, 0.6f}},
-    // kAct8Parts
     {{0.21f, 1.39f, 1.36f, 8.4f}, {0.95f, 0.64f, 0.42f, 3.7f}, {0.00f, 0.44f, 0.18f, 2.1f}, {0.47f, 0.12f, 0.22f, 1.1f}, {0.48f, 0.10f, 0.25f, 1.3f}},
 };
 // The second kernel that parts of K need, and a megabyte of their sums, written and read.
@@ -443,8 +441,7 @@ TilePlan plan_tiles(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, int ac
 int mxfp4_tiles(MxLinearArgs &a, int act, bool gated, const TilePlan &plan, hipStream_t stream) {
     switch (act) {
         case kAct4: return gated ? launch_tiles<kAct4, true>(a, plan, stream) : launch_tiles<kAct4, false>(a, plan, stream);
-        case kAct8: return gated ? launch_tiles<kAct8, true>(a, plan, stream) : launch_tiles<kAct8, false>(a, plan, stream);
-        default: return gated ? launch_tiles<kAct8Parts, true>(a, plan, stream) : launch_tiles<kAct8Parts, false>(a, plan, stream);
+        default: return gated ? launch_tiles<kAct8, true>(a, plan, stream) : launch_tiles<kAct8, false>(a, plan, stream);
     }
 }
 
