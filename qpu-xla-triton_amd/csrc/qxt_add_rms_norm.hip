@@ -294,7 +294,21 @@ int launch_norm(const NormArgs &a, uint32_t rows, bool vec, hipStream_t stream) 
         threads = ((pieces + each - 1) / each + 63) / 64 * 64;
         kernel = each == 1 ? add_rms_norm_kernel<OUT, 1> : add_rms_norm_kernel<OUT, 4>;
     }
-    return launch(name, kernel, dim3(rows), dim3(threads), 0, stream, a);
+    // A launch has fewer than 2^32 threads (the runtime takes a larger one and runs what is left of it modulo that): more rows
+    // take several.
+    const uint32_t most = UINT32_MAX / threads;
+    NormArgs part = a;
+    for (uint32_t first = 0; first < rows; first += most) {
+        part.x = a.x + first * a.x_stride;
+        if (a.residual != nullptr) {
+            part.residual = a.residual + first * a.residual_stride;
+            part.sum = a.sum + first * a.sum_stride;
+        }
+        part.out = a.out + first * a.out_stride;
+        if (a.scales != nullptr) part.scales = a.scales + first * (OUT == QXT_ROWS_INT8 ? 4 : a.scales_stride);
+        if (int rc = launch(name, kernel, dim3(min(rows - first, most)), dim3(threads), 0, stream, part)) return rc;
+    }
+    return QXT_OK;
 }
 
 int run_norm(NormArgs &a, uint32_t out_kind, uint32_t rows, hipStream_t stream) {
