@@ -55,6 +55,10 @@ void timing_record(const char *kernel_name, hipEvent_t start, hipEvent_t stop);
 template <typename... KArgs, typename... Args>
 int launch(const char *name, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t lds, hipStream_t stream,
            Args... args) {
+    // The threads of each dimension have to be below 2^32: the runtime takes more and runs what is left of them modulo that.
+    if (static_cast<uint64_t>(grid.x) * block.x > UINT32_MAX || static_cast<uint64_t>(grid.y) * block.y > UINT32_MAX ||
+        static_cast<uint64_t>(grid.z) * block.z > UINT32_MAX)
+        return fail(QXT_INVALID_ARGUMENT, "%s: a launch of 2^32 threads or more", name);
     if (timing_enabled()) {
         hipEvent_t start = nullptr, stop = nullptr;
         timing_events(&start, &stop);
