@@ -97,7 +97,8 @@ __device__ __forceinline__ float gated(uint32_t gate, float g, float up) {
         const float e = __builtin_amdgcn_exp2f(t) * (1.0f + 0.6931471806f * (fabsf(g) < 87.0f ? rest : 0.0f));
         return g * __builtin_amdgcn_rcpf(1.0f + e) * up;
     }
-    return 0.5f * g * (1.0f + erff(g * 0.7071067812f)) * up;
+    // (1 + erf would cancel for negative g.  What is left is the rounding of the argument, which erfc takes times g^2 + 1.)
+    return 0.5f * g * erfcf(g * -0.7071067812f) * up;
 }
 
 // Source of what lies past a row's last block.
