@@ -87,15 +87,18 @@ __device__ __forceinline__ f4 mx_mfma(u4 w, const ActPiece<ACT> &a, f4 acc, uint
     return acc;
 }
 
-// exp(-g) through the hardware's power of two: the part of g log2(e) that its
-// rounding loses is put back to first order, so the error is a few units of fp32
-// for every g (without it, |g| units).
+// SiLU from e = exp(-|g|), which cannot overflow: g / (1 + e), and g e / (1 + e) for negative g.  e comes through the
+// hardware's power of two: the part of g log2(e) that its rounding loses is put back to first order, so the result is good
+// to 11 units of 2^-24 for every g (without it, |g| units).  Below 2^-100 e is taken 2^64 times as large, since neither the
+// power nor the product with g may fall below the normal numbers before the result does; beyond -200 it is zero.
 __device__ __forceinline__ float gated(uint32_t gate, float g, float up) {
     if (gate == QXT_GATE_SILU) {
-        const float t = fminf(fmaxf(g * -1.442695041f, -126.0f), 200.0f);
-        const float rest = fmaf(g, -1.442695041f, -t) + g * -1.925963033e-8f;
-        const float e = __builtin_amdgcn_exp2f(t) * (1.0f + 0.6931471806f * (fabsf(g) < 87.0f ? rest : 0.0f));
-        return g * __builtin_amdgcn_rcpf(1.0f + e) * up;
+        const float a = fmaxf(-fabsf(g), -200.0f), t = a * 1.442695041f;
+        const float rest = fmaf(a, 1.442695041f, -t) + a * 1.925963033e-8f;
+        const bool far = t < -100.0f;
+        const float e = __builtin_amdgcn_exp2f(far ? t + 64.0f : t) * (1.0f + 0.6931471806f * rest);
+        const float f = (g < 0.0f ? g * e : g) * __builtin_amdgcn_rcpf(1.0f + e) * up;
+        return far && g < 0.0f ? f * 0x1p-64f : f;
     }
     // (1 + erf would cancel for negative g.  What is left is the rounding of the argument, which erfc takes times g^2 + 1.)
     return 0.5f * g * erfcf(g * -0.7071067812f) * up;

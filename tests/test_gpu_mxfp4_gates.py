@@ -2,7 +2,8 @@
 
 Gates are sums of two elements, ups are one element each, so that both are exact in float32.
 
-GELU: the argument is off by 1.5 units (its product and its constant), which erfc takes
+SiLU: a power of two and a reciprocal (2 units of 2^-24 each), the power's correction (2), the sum in the denominator (1) and
+four products at most: 11 units.  GELU: the argument is off by 1.5 units (its product and its constant), which erfc takes
 times 2 x^2 + 1 at most, x^2 = g^2 / 2; erfc itself is good for 16 units in the last place (32), and there are two products.
 Below float32's normal numbers a result is off by one of its least steps.
 """
@@ -46,13 +47,13 @@ def _gates(low, high):
 
 @pytest.mark.parametrize("m", [8, 400])
 @pytest.mark.parametrize("up_power", [0, 90])
-@pytest.mark.parametrize("gate,low,high", [("gelu", 0.05, 12.8)])
+@pytest.mark.parametrize("gate,low,high", [("silu", 0.05, 104.0), ("gelu", 0.05, 12.8)])
 def test_gate_functions_to_a_few_units(gate, low, high, up_power, m) -> None:
     g_high, g_low = _gates(low, high)
     g = g_high + g_low
     assert torch.equal(g, g.float().double()) and float(g.min()) < -0.9 * high
     want = reference.gate_of(gate, g) * 2.0**up_power
-    units = 1.5 * (g.square() + 1) + 34
+    units = 11.0 if gate == "silu" else 1.5 * (g.square() + 1) + 34
     bound = units * UNIT * want.abs() + 2.0**-149
     for start in range(0, len(g), m):  # few rows a call, and many
         part = slice(start, start + m)
