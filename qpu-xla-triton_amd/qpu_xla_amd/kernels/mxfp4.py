@@ -25,7 +25,17 @@ import torch
 
 from qpu_xla_amd import _lib
 from qpu_xla_amd._paged import TYPES, workspace_for
-from qpu_xla_amd._rows import FP8, MX_BLOCK, float_rows, mx_format, mx_outputs, mx_rows, new_rows, require_current_gpu, vector
+from qpu_xla_amd._rows import (
+    FP8,
+    MX_BLOCK,
+    float_rows,
+    mx_format,
+    mx_outputs,
+    mx_rows,
+    new_rows,
+    require_current_gpu,
+    vector,
+)
 from qpu_xla_amd._tensors import stream_handle
 from qpu_xla_amd.errors import KernelError
 from qpu_xla_amd.kernel import Kernel
@@ -265,6 +275,38 @@ def mxfp4_gated_linear(
     _lib.call("qxt_mxfp4_gated_linear", x.data_ptr(), x_stride, x_code, fmt, gate_at, up_at, function, *places, kind, m, n, k, at, size,
               stream_handle(stream))
     return result
+
+
+# What the C entries take: rows or columns, and K.
+_MOST_ROWS, _MOST_K = (2**31 - 1) // 32, 2**22
+
+
+def feed_forward_outputs(
+    name: str, x: torch.Tensor, gate: Any, up: Any, down: Any, activations: str, function: str, out: torch.Tensor | None,
+    dtype: torch.dtype | None, stream: Any,
+) -> tuple[tuple[torch.Tensor, torch.Tensor], torch.Tensor]:
+    """The checks of a feed-forward block's products, and their outputs: (the inner blocks, y).
+
+    They come before the block's norm, which may write the sum over the residual: nothing may be refused after that.
+    """
+    m, k, _, _ = float_rows(name, "x", x)
+    fmt = mx_format(name, activations)
+    _gate_function(name, function)
+    n, _, _ = _gate_weights(name, k, gate.values, gate.scales, up.values, up.scales)
+    columns, down_k, _, _ = mx_rows(name, "down", down.values, down.scales, (_lib.MX_FP4,))
+    if down_k != n:
+        raise ValueError(f"{name}: the gated rows and down differ in K")
+    if max(m, n, columns) > _MOST_ROWS or max(k, n) >= _MOST_K:
+        raise ValueError(f"{name}: too many rows or columns")
+    weights = (gate.values, up.values, down.values, gate.scales, up.scales, down.scales)
+    if any(w.data_ptr() % 16 for w in weights[:3]):
+        raise ValueError(f"{name}: weights must be in rows aligned to 16 bytes")
+    if dtype is None:
+        dtype = x.dtype if out is None else out.dtype
+    out, _, _ = _float_out(name, x, out, dtype, m, columns, stream)
+    values, _, scales, _ = mx_outputs(name, x, m, n, fmt == _lib.MX_FP8, None, None, stream)
+    require_current_gpu(name, x, *weights, out)
+    return (values, scales), out
 
 
 # -------------------------------------------------------------- queue kernels

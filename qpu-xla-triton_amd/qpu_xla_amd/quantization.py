@@ -661,13 +661,12 @@ def mxfp4_feed_forward(
 
     Three operators whose rows stay in blocks of ``activations`` between them: the stream's norm, ``f(gate) * up`` with
     f ``function``, and the linear down, in x's type unless ``out`` or ``dtype`` says otherwise.  y is not added to the
-    stream: the next norm does that.
+    stream: the next norm does that.  A refused call leaves ``residual_out`` as it was.
     """
-    mxfp4.mx_format("mxfp4_feed_forward", activations)
+    inner, out = mxfp4.feed_forward_outputs("mxfp4_feed_forward", x, gate, up, down, activations, function, out, dtype,
+                                            stream)
     norm = add_rms_norm_mxfp8 if activations == "mxfp8" else add_rms_norm_mxfp4
     values, scales, total = norm(x, norm_weight, residual, epsilon=epsilon, residual_out=residual_out, stream=stream)
-    inner = mxfp4.mxfp4_gated_gemm(values, scales, gate.values, gate.scales, up.values, up.scales, gate=function,
-                                   output=activations, stream=stream)
-    if dtype is None:
-        dtype = x.dtype if out is None else out.dtype
-    return mxfp4.mxfp4_gemm(*inner, down.values, down.scales, None, out, dtype=dtype, stream=stream), total
+    mxfp4.mxfp4_gated_gemm(values, scales, gate.values, gate.scales, up.values, up.scales, inner, gate=function,
+                           output=activations, stream=stream)
+    return mxfp4.mxfp4_gemm(*inner, down.values, down.scales, None, out, stream=stream), total
