@@ -118,3 +118,25 @@ def mx_outputs(name: str, like: torch.Tensor, rows: int, columns: int, fp8: bool
     else:
         scale_stride = _byte_rows(name, "scales", scales, _SCALES, (rows, columns // MX_BLOCK))
     return values, stride, scales, scale_stride
+
+
+def share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether rows of two tensors (or vectors) with dense rows share memory, as the C entries tell it.
+
+    Tensors of one row stride may lie between each other's rows; those of different strides are taken to meet where their
+    ranges do.
+    """
+    spans = []
+    for t in (a, b):
+        rows, size = (t.shape[0], t.element_size()) if t.dim() > 1 else (1, t.element_size())
+        spans.append((t.data_ptr(), rows, t.stride(0) * size if rows > 1 else 0, t.shape[-1] * size))
+    (at, rows, skip, size), (to, to_rows, to_skip, to_size) = spans
+    if not (rows and size and to_rows and to_size) or a.get_device() != b.get_device():
+        return False
+    skip, to_skip = skip or to_skip, to_skip or skip
+    if at + (rows - 1) * skip + size <= to or to + (to_rows - 1) * to_skip + to_size <= at:
+        return False
+    if skip != to_skip or not skip:
+        return True
+    ahead = (to - at) % skip
+    return ahead < size or ahead + to_size > skip

@@ -34,6 +34,7 @@ from qpu_xla_amd._rows import (
     mx_rows,
     new_rows,
     require_current_gpu,
+    share_memory,
     vector,
 )
 from qpu_xla_amd._tensors import stream_handle
@@ -282,8 +283,8 @@ _MOST_ROWS, _MOST_K = (2**31 - 1) // 32, 2**22
 
 
 def feed_forward_outputs(
-    name: str, x: torch.Tensor, gate: Any, up: Any, down: Any, activations: str, function: str, out: torch.Tensor | None,
-    dtype: torch.dtype | None, stream: Any,
+    name: str, x: torch.Tensor, norm_weight: torch.Tensor, residual_out: torch.Tensor | None, gate: Any, up: Any, down: Any,
+    activations: str, function: str, out: torch.Tensor | None, dtype: torch.dtype | None, stream: Any,
 ) -> tuple[tuple[torch.Tensor, torch.Tensor], torch.Tensor]:
     """The checks of a feed-forward block's products, and their outputs: (the inner blocks, y).
 
@@ -303,9 +304,15 @@ def feed_forward_outputs(
         raise ValueError(f"{name}: weights must be in rows aligned to 16 bytes")
     if dtype is None:
         dtype = x.dtype if out is None else out.dtype
+    given = out
     out, _, _ = _float_out(name, x, out, dtype, m, columns, stream)
     values, _, scales, _ = mx_outputs(name, x, m, n, fmt == _lib.MX_FP8, None, None, stream)
     require_current_gpu(name, x, *weights, out)
+    for written, others in ((given, (norm_weight, residual_out, *weights)), (residual_out, weights)):
+        # (What is not rows is refused by the norm, before its launch.)
+        if written is not None and written.dim() == 2 and any(
+                t is not None and t.dim() in (1, 2) and share_memory(written, t) for t in others):
+            raise ValueError(f"{name}: an output shares memory with another operand")
     return (values, scales), out
 
 

@@ -661,10 +661,11 @@ def mxfp4_feed_forward(
 
     Three operators whose rows stay in blocks of ``activations`` between them: the stream's norm, ``f(gate) * up`` with
     f ``function``, and the linear down, in x's type unless ``out`` or ``dtype`` says otherwise.  y is not added to the
-    stream: the next norm does that.  A refused call leaves ``residual_out`` as it was.
+    stream: the next norm does that.  A refused call leaves ``residual_out`` as it was; ``out`` may be x, or
+    the residual where the sum goes elsewhere.
     """
-    inner, out = mxfp4.feed_forward_outputs("mxfp4_feed_forward", x, gate, up, down, activations, function, out, dtype,
-                                            stream)
+    inner, out = mxfp4.feed_forward_outputs("mxfp4_feed_forward", x, norm_weight, residual_out, gate, up, down, activations,
+                                            function, out, dtype, stream)
     norm = add_rms_norm_mxfp8 if activations == "mxfp8" else add_rms_norm_mxfp4
     values, scales, total = norm(x, norm_weight, residual, epsilon=epsilon, residual_out=residual_out, stream=stream)
     mxfp4.mxfp4_gated_gemm(values, scales, gate.values, gate.scales, up.values, up.scales, inner, gate=function,

@@ -1,10 +1,11 @@
-"""A refused feed-forward block leaves the stream as it was."""
+"""A refused feed-forward block leaves the stream as it was, and no output of one is written over another operand."""
 
 from __future__ import annotations
 
 import pytest
 import torch
 
+from qpu_xla_amd import quantization
 from qpu_xla_amd.errors import DependencyError
 from qpu_xla_amd.quantization import QuantizedMatrixMxfp4, mxfp4_feed_forward, quantize_matrix_mxfp4
 
@@ -62,3 +63,29 @@ def test_refused_calls_leave_the_stream(changes) -> None:
     assert total is residual and torch.equal(residual, x + kept)
     want, _ = mxfp4_feed_forward(x, kept, weight, gate, up, down)
     assert torch.equal(y, want)
+
+
+def test_outputs_over_other_operands_are_refused() -> None:
+    x, residual, weight, gate, up, down = _layer()
+    kept = [t.clone() for t in (x, residual, weight, gate.values, up.values, down.values, gate.scales, up.scales, down.scales)]
+    over = lambda t, rows, columns: t.view(torch.float32).flatten()[: rows * columns].view(rows, columns)  # noqa: E731
+    for options in ({"out": residual, "residual_out": residual}, {"out": x, "residual_out": x},
+                    {"out": over(gate.values, M, D)}, {"out": over(up.values, M, D)}, {"out": over(down.values, M, D)},
+                    {"residual_out": over(gate.values, M, D)}, {"residual_out": over(down.values, M, D)}):
+        with pytest.raises(ValueError, match="shares memory"):
+            mxfp4_feed_forward(x, residual, weight, gate, up, down, **options)
+    for t, was in zip((x, residual, weight, gate.values, up.values, down.values, gate.scales, up.scales, down.scales), kept):
+        assert torch.equal(t, was)
+
+
+def test_outputs_over_what_is_no_longer_read() -> None:
+    x, residual, weight, gate, up, down = _layer()
+    want, total = mxfp4_feed_forward(x, residual, weight, gate, up, down)
+    for place in (0, 1):  # over x, over the residual
+        rows = [x.clone(), residual.clone()]
+        y, again = mxfp4_feed_forward(*rows, weight, gate, up, down, out=rows[place])
+        assert y is rows[place] and torch.equal(y, want) and torch.equal(again, total)
+    wide = torch.zeros((M, 2 * D), device="cuda")  # y and the sum side by side
+    y, again = mxfp4_feed_forward(x, residual, weight, gate, up, down, out=wide[:, :D], residual_out=wide[:, D:])
+    assert torch.equal(y, want) and torch.equal(again, total)
+    assert quantization.mxfp4_feed_forward(x[:0], residual[:0], weight, gate, up, down)[0].shape == (0, D)
