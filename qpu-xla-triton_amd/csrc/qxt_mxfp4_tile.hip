@@ -352,7 +352,7 @@ __global__ __launch_bounds__(256) void mxfp4_join_kernel(MxLinearArgs a, FastDiv
 }
 
 template <int ACT, bool GATED, int TW, int TA, int WN, int WM, int SUB, int RING>
-int launch_tile(MxLinearArgs &a, uint32_t splits, hipStream_t stream) {
+int launch_tile(MxLinearArgs &a, const char *name, uint32_t splits, hipStream_t stream) {
     typedef Tiles<ACT, GATED, TW, TA, WN, WM, SUB, RING> T;
     constexpr uint32_t columns = T::BN / (GATED ? 2 : 1);
     const uint32_t groups = (a.blocks + 15) / 16;
@@ -363,7 +363,7 @@ int launch_tile(MxLinearArgs &a, uint32_t splits, hipStream_t stream) {
     const uint32_t row = a.part_row / 8;
     const uint64_t joins = (static_cast<uint64_t>(a.m) * row + 255) / 256;
     if (grid > INT32_MAX || (a.splits > 1 && joins * 256 > INT32_MAX)) return fail(QXT_INVALID_ARGUMENT, "mxfp4 linear: too many outputs");
-    const int rc = launch("mxfp4_tile_kernel", mxfp4_tile_kernel<ACT, GATED, TW, TA, WN, WM, SUB, RING>,
+    const int rc = launch(name, mxfp4_tile_kernel<ACT, GATED, TW, TA, WN, WM, SUB, RING>,
                           dim3(static_cast<uint32_t>(grid)), dim3(T::THREADS), 0, stream, a);
     if (rc != QXT_OK || a.splits == 1) return rc;
     return launch("mxfp4_join_kernel", mxfp4_join_kernel<GATED>, dim3(static_cast<uint32_t>(joins)), dim3(256), 0, stream, a,
@@ -374,6 +374,8 @@ int launch_tile(MxLinearArgs &a, uint32_t splits, hipStream_t stream) {
 // two to four workgroups a CU.
 constexpr uint32_t kTiles = 5;
 constexpr uint32_t kTileRows[kTiles][2] = {{256, 256}, {128, 128}, {128, 64}, {64, 64}, {128, 32}};
+constexpr const char *kTileNames[kTiles] = {"mxfp4_tile_kernel 256x256", "mxfp4_tile_kernel 128x128", "mxfp4_tile_kernel 128x64",
+                                            "mxfp4_tile_kernel 64x64", "mxfp4_tile_kernel 128x32"};
 
 template <int ACT, bool GATED>
 int launch_tiles(MxLinearArgs &a, const TilePlan &plan, hipStream_t stream) {
@@ -381,12 +383,13 @@ int launch_tiles(MxLinearArgs &a, const TilePlan &plan, hipStream_t stream) {
     // Where several workgroups share a CU two stages are better than three, or as good (8-bit, 333 x 4096 x 14336 56.3 ->
     // 48.1 us).
     constexpr int SUB = ACT == kAct4 ? 2 : 1, RING = ACT == kAct4 ? 2 : 3;
+    const char *name = kTileNames[plan.tile];
     switch (plan.tile) {
-        case 0: return launch_tile<ACT, GATED, 8, 4, 2, 4, SUB, RING>(a, plan.splits, stream);
-        case 1: return launch_tile<ACT, GATED, 4, 4, 2, 2, SUB, 2>(a, plan.splits, stream);
-        case 2: return launch_tile<ACT, GATED, 4, 2, 2, 2, SUB, 2>(a, plan.splits, stream);
-        case 3: return launch_tile<ACT, GATED, 4, 1, 1, 4, SUB, 2>(a, plan.splits, stream);
-        default: return launch_tile<ACT, GATED, 4, 1, 2, 2, SUB, 2>(a, plan.splits, stream);
+        case 0: return launch_tile<ACT, GATED, 8, 4, 2, 4, SUB, RING>(a, name, plan.splits, stream);
+        case 1: return launch_tile<ACT, GATED, 4, 4, 2, 2, SUB, 2>(a, name, plan.splits, stream);
+        case 2: return launch_tile<ACT, GATED, 4, 2, 2, 2, SUB, 2>(a, name, plan.splits, stream);
+        case 3: return launch_tile<ACT, GATED, 4, 1, 1, 4, SUB, 2>(a, name, plan.splits, stream);
+        default: return launch_tile<ACT, GATED, 4, 1, 2, 2, SUB, 2>(a, name, plan.splits, stream);
     }
 }
 
