@@ -277,7 +277,7 @@ constexpr uint32_t kMostK = 1u << 22;
 int check_operand(const char *name, const MxOperand &o, uint32_t format, uint32_t rows, uint32_t blocks) {
     if (o.values == nullptr || o.scales == nullptr) return fail(QXT_INVALID_ARGUMENT, "%s: null pointer", name);
     if (!aligned(o.values, 16) || o.stride % 16) return fail(QXT_INVALID_ARGUMENT, "%s: values must be in rows aligned to 16 bytes", name);
-    if (rows > 1 && o.stride >= 1 << 23) return fail(QXT_INVALID_ARGUMENT, "%s: rows of values must lie less than 8 MiB apart", name);
+    if (rows > 1 && static_cast<size_t>(o.stride) >= 1u << 23) return fail(QXT_INVALID_ARGUMENT, "%s: rows of values must lie less than 8 MiB apart", name);
     if (rows > 1 && (static_cast<size_t>(o.stride) < mx_row_bytes(format, blocks * kMxBlock) ||
                      static_cast<size_t>(o.scale_stride) < blocks))
         return fail(QXT_INVALID_ARGUMENT, "%s: a row stride is below the row", name);

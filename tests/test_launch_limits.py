@@ -28,3 +28,17 @@ def test_results_of_more_tiles_than_a_launch_takes(fmt, kind) -> None:
     blocks = lambda at, row: _lib.MX_MATRIX.pack(at, row, at + FAR // 2, 4)  # noqa: E731
     _refused("qxt_mxfp4_gemm", blocks(FAKE, 128 if fmt else 64), fmt, blocks(FAKE + FAR, 64), None, FAKE + 4 * FAR, 4 * n, kind, m, n, k,
              FAKE + 2 * FAR, 2**62, None)
+
+
+@pytest.mark.parametrize("stride", [1 << 23, 1 << 40, 1 << 63, 2**64 - 16])
+@pytest.mark.parametrize("rows", [3, 40])
+def test_weights_that_lie_far_apart(rows, stride) -> None:
+    """Strides are unsigned: those past 2^63 are as far apart as any."""
+    blocks = lambda at, row: _lib.MX_MATRIX.pack(at, row, at + FAR // 2, 4)  # noqa: E731
+    _lib.set_failure_mask(_lib.FAIL_SUBMISSION)
+    try:
+        for a_stride, w_stride in ((stride, 64), (64, stride)):
+            assert _lib.load().qxt_mxfp4_gemm(blocks(FAKE, a_stride), _lib.MX_FP4, blocks(FAKE + FAR, w_stride), None, FAKE + 4 * FAR,
+                                              256, 0, rows, 64, 128, FAKE + 2 * FAR, 2**40, None) == _lib.INVALID_ARGUMENT
+    finally:
+        _lib.set_failure_mask(_lib.FAIL_NONE)
