@@ -87,9 +87,9 @@ __device__ __forceinline__ u2 int8_of(const Eight &e, float s) {
 
 // Eight elements of a 34-byte block at piece `at` of a row (four neighbouring lanes hold the block).
 __device__ __forceinline__ void store_q8_0(char *row, uint32_t at, const Eight &e, bool in_row) {
-    float largest = 0.0f;
+    float largest = fabsf(e.v[0]);  // not from zero: a block that is all NaN has a scale of NaN
 #pragma unroll
-    for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fabsf(e.v[i]));
+    for (int i = 1; i < 8; ++i) largest = fmaxf(largest, fabsf(e.v[i]));
     largest = fmaxf(largest, __shfl_xor(largest, 1, 4));
     largest = fmaxf(largest, __shfl_xor(largest, 2, 4));
     if (!in_row) return;
