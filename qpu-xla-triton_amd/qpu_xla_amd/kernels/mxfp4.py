@@ -40,6 +40,7 @@ from qpu_xla_amd._rows import (
 from qpu_xla_amd._tensors import stream_handle
 from qpu_xla_amd.errors import KernelError
 from qpu_xla_amd.kernel import Kernel
+from qpu_xla_amd.kernels.add_rms_norm import add_rms_norm_mxfp4, add_rms_norm_mxfp8
 
 _GATES = {"silu": _lib.GATE_SILU, "gelu": _lib.GATE_GELU}
 _BLOCK_KINDS = {"mxfp8": _lib.ROWS_MXFP8, "mxfp4": _lib.ROWS_MXFP4}
@@ -282,38 +283,59 @@ def mxfp4_gated_linear(
 _MOST_ROWS, _MOST_K = (2**31 - 1) // 32, 2**22
 
 
-def feed_forward_outputs(
-    name: str, x: torch.Tensor, norm_weight: torch.Tensor, residual_out: torch.Tensor | None, gate: Any, up: Any, down: Any,
-    activations: str, function: str, out: torch.Tensor | None, dtype: torch.dtype | None, stream: Any,
-) -> tuple[tuple[torch.Tensor, torch.Tensor], torch.Tensor]:
-    """The checks of a feed-forward block's products, and their outputs: (the inner blocks, y).
+def feed_forward(
+    x: torch.Tensor, residual: torch.Tensor | None, norm_weight: torch.Tensor, gate: Any, up: Any, down: Any, epsilon: float,
+    activations: str, function: str, residual_out: torch.Tensor | None, out: torch.Tensor | None, dtype: torch.dtype | None,
+    stream: Any,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """``quantization.mxfp4_feed_forward``: the norm, ``mxfp4_gated_gemm`` and ``mxfp4_gemm`` in a row.
 
-    They come before the block's norm, which may write the sum over the residual: nothing may be refused after that.
+    The norm may write the sum over the residual, so that nothing may be refused after it: the checks of all three come
+    first, and so do the outputs and the workspace.
     """
+    name = "mxfp4_feed_forward"
     m, k, _, _ = float_rows(name, "x", x)
-    fmt = mx_format(name, activations)
-    _gate_function(name, function)
-    n, _, _ = _gate_weights(name, k, gate.values, gate.scales, up.values, up.scales)
-    columns, down_k, _, _ = mx_rows(name, "down", down.values, down.scales, (_lib.MX_FP4,))
+    fmt, kind = mx_format(name, activations), _BLOCK_KINDS[activations]
+    gate_function = _gate_function(name, function)
+    n, gate_at, up_at = _gate_weights(name, k, gate.values, gate.scales, up.values, up.scales)
+    columns, down_k, _, down_at = mx_rows(name, "down", down.values, down.scales, (_lib.MX_FP4,))
     if down_k != n:
         raise ValueError(f"{name}: the gated rows and down differ in K")
     if max(m, n, columns) > _MOST_ROWS or max(k, n) >= _MOST_K:
         raise ValueError(f"{name}: too many rows or columns")
     weights = (gate.values, up.values, down.values, gate.scales, up.scales, down.scales)
-    if any(w.data_ptr() % 16 for w in weights[:3]):
+    ranges = [(w.data_ptr(), w.numel()) for w in weights]
+    if any(at % 16 for at, _ in ranges[:3]):
         raise ValueError(f"{name}: weights must be in rows aligned to 16 bytes")
     if dtype is None:
         dtype = x.dtype if out is None else out.dtype
     given = out
-    out, _, _ = _float_out(name, x, out, dtype, m, columns, stream)
-    values, _, scales, _ = mx_outputs(name, x, m, n, fmt == _lib.MX_FP8, None, None, stream)
+    out, code, stride = _float_out(name, x, out, dtype, m, columns, stream)
+    h, h_stride, h_scales, h_scale_stride = mx_outputs(name, x, m, n, fmt == _lib.MX_FP8, None, None, stream)
     require_current_gpu(name, x, *weights, out)
-    for written, others in ((given, (norm_weight, residual_out, *weights)), (residual_out, weights)):
-        # (What is not rows is refused by the norm, before its launch.)
-        if written is not None and written.dim() == 2 and any(
-                t is not None and t.dim() in (1, 2) and share_memory(written, t) for t in others):
-            raise ValueError(f"{name}: an output shares memory with another operand")
-    return (values, scales), out
+    for written in (given, residual_out):
+        # (A residual_out that is not rows is refused by the norm, before its launch.)
+        if written is not None and m and written.dim() == 2:
+            first = written.data_ptr()
+            last = first + ((m - 1) * written.stride(0) + written.shape[1]) * written.element_size()
+            if any(first < at + size and at < last for at, size in ranges):
+                raise ValueError(f"{name}: an output shares memory with another operand")
+    if given is not None and any(t is not None and t.dim() == d and share_memory(out, t) for t, d in ((norm_weight, 1), (residual_out, 2))):
+        raise ValueError(f"{name}: an output shares memory with another operand")
+    query = (_lib._lib or _lib.load()).qxt_mxfp4_linear_workspace
+    size = max(query(m, n, k, 2, fmt, 0, kind), query(m, columns, n, 1, fmt, 0, code))
+    workspace = workspace_for(stream, size, x.device)
+    at = None if workspace is None else workspace.data_ptr()
+
+    norm = add_rms_norm_mxfp8 if fmt == _lib.MX_FP8 else add_rms_norm_mxfp4
+    values, scales, total = norm(x, norm_weight, residual, epsilon=epsilon, residual_out=residual_out, stream=stream)
+    handle = stream_handle(stream)
+    rows = _lib.MX_MATRIX.pack(values.data_ptr(), values.shape[1], scales.data_ptr(), scales.shape[1])
+    _lib.call("qxt_mxfp4_gated_gemm", rows, fmt, gate_at, up_at, gate_function, h.data_ptr(), h_stride, h_scales.data_ptr(),
+              h_scale_stride, kind, m, n, k, at, size, handle)
+    rows = _lib.MX_MATRIX.pack(h.data_ptr(), h_stride, h_scales.data_ptr(), h_scale_stride)
+    _lib.call("qxt_mxfp4_gemm", rows, fmt, down_at, None, out.data_ptr(), stride, code, m, columns, n, at, size, handle)
+    return out, total
 
 
 # -------------------------------------------------------------- queue kernels

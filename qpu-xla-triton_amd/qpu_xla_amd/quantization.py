@@ -37,7 +37,6 @@ from qpu_xla_amd._tensors import ptr, require_gpu, row_stride, rows_are_dense, s
 from qpu_xla_amd.candidates import CandidateRecord, CandidateRegistry
 from qpu_xla_amd.errors import DependencyError
 from qpu_xla_amd.kernels import mxfp4
-from qpu_xla_amd.kernels.add_rms_norm import add_rms_norm_mxfp4, add_rms_norm_mxfp8
 from qpu_xla_amd.kernels.gemm_int8 import w8a8_gemm_dequantize
 from qpu_xla_amd.kernels.quantize import quantize_rows_int8
 from qpu_xla_amd.placement import Placement
@@ -661,13 +660,8 @@ def mxfp4_feed_forward(
 
     Three operators whose rows stay in blocks of ``activations`` between them: the stream's norm, ``f(gate) * up`` with
     f ``function``, and the linear down, in x's type unless ``out`` or ``dtype`` says otherwise.  y is not added to the
-    stream: the next norm does that.  A refused call leaves ``residual_out`` as it was; ``out`` may be x, or
-    the residual where the sum goes elsewhere.
+    stream: the next norm does that.  A refused call leaves ``residual_out`` as it was; ``out`` may be x, or the
+    residual where the sum goes elsewhere.
     """
-    inner, out = mxfp4.feed_forward_outputs("mxfp4_feed_forward", x, norm_weight, residual_out, gate, up, down, activations,
-                                            function, out, dtype, stream)
-    norm = add_rms_norm_mxfp8 if activations == "mxfp8" else add_rms_norm_mxfp4
-    values, scales, total = norm(x, norm_weight, residual, epsilon=epsilon, residual_out=residual_out, stream=stream)
-    mxfp4.mxfp4_gated_gemm(values, scales, gate.values, gate.scales, up.values, up.scales, inner, gate=function,
-                           output=activations, stream=stream)
-    return mxfp4.mxfp4_gemm(*inner, down.values, down.scales, None, out, stream=stream), total
+    return mxfp4.feed_forward(x, residual, norm_weight, gate, up, down, epsilon, activations, function, residual_out, out, dtype,
+                              stream)
