@@ -13,8 +13,10 @@
 // Bound by its bytes: a workgroup holds a row in registers between the load, the
 // sum over the row and the store, so every input is read once.  Measured, with a residual: 4096 rows of 4096, bf16 to
 // 8-bit blocks 26.8 us (4.4 TB/s), to bf16 27.6 (4.9), to int8 rows 32 (3.7: the maximum is a second wait for all waves),
-// fp32 to 4-bit blocks 46.3 (4.5); 4096 of 8192, bf16 53.6 (5.0); 777 of 11008, fp16 22.5 (3.0: three rows a CU, all in
-// one go, so that little of one's stores overlaps another's loads); one row of 2048 3.5.
+// fp32 to 4-bit blocks 46.3 (4.5); 4096 of 8192, bf16 53.6 (5.0); 777 of 11008, fp16 21.7 (3.1); one row of 2048 2.8.
+// Rows of more than 8192 take four pieces a thread, and of those the last load of x and of the residual passes through
+// scratch (80 bytes a thread), because the branches on the type join behind it: x, the residual and the weights are waited
+// for in turn.
 #include "qxt_mx.h"
 
 namespace qxt {
@@ -115,7 +117,7 @@ __global__ __launch_bounds__(kMostThreads) void add_rms_norm_kernel(NormArgs a) 
     __shared__ float maxima[kMostThreads / 64], shared_factor;
     const uint32_t row = blockIdx.x, pieces = a.width / 8, threads = blockDim.x;
     u4 xa[CH], xb[CH], ra[CH], rb[CH];
-    // Every load is issued before any is used; a thread past the row re-reads its last piece.  Inputs are read once: past
+    // With one piece a thread every load is issued before any is used; a thread past the row re-reads its last piece.  Inputs are read once: past
     // the caches (4096 rows of 4096, bf16 to 8-bit blocks: 34 -> 31 us).
     auto load_row = [&](uint32_t type, const char *from, u4 (&lo)[CH], u4 (&hi)[CH]) {
         if (type == QXT_TYPE_F32) {

@@ -292,14 +292,18 @@ MxOperand operand(const qxt_mx_matrix *m) {
 size_t up16(size_t bytes) { return (bytes + 15) / 16 * 16; }
 uint32_t padded(uint32_t blocks) { return (blocks + 3) / 4 * 4; }
 
-// Activation rows that the streaming kernel takes: up to 16, as long as they leave room in LDS for the weights of two
-// workgroups, or of one where there are no more than CUs (a single weight in 16 rows a workgroup).  Four rows, K = 14336, N =
+// Activation rows that the streaming kernel takes: up to 16 of 48 KB, so that two workgroups of a single weight share a CU
+// (of a gated product, whose weights take 34 KB, up to 46 KB), or as many as leave room for the weights of one where there
+// are no more workgroups than CUs (a single weight in 16 rows a workgroup).  Four rows, K = 14336, N =
 // 4096: 9.2 us, on tiles 13.2; eight 10.2, 13.2; sixteen of K = 4096 7.3, 8.2.  (With more workgroups than CUs, or few
 // columns that parts of K spread over the CUs, tiles are faster: 16 rows, K = 4096, N = 14336 12.3 us, 16.3 here; K = 8192,
 // N = 1024 8.1, 8.6.)
 constexpr size_t kStreamBytes = 48 * 1024, kAloneBytes = 136 * 1024;
 bool alone(uint32_t n, uint32_t weights) { return weights == 1 && n > 64 * 16 && n <= 256 * 16; }
-// Bytes of float activations that every workgroup of it quantises for itself.
+// Bytes of float activations that every workgroup of it quantises for itself (in LDS, beside their blocks).  With a launch
+// before it instead, K = 4096, N = 14336, bf16: one row 7.9 us, 9.8 with the launch, gated 13.6, 15.9; three rows 9.4, 10.1,
+// gated 14.4, 16.0; four rows, at the limit, 10.5, 10.2, gated 21.3, 16.1 (one workgroup a CU); K = 2048, N = 5632, four
+// rows 5.7, 6.5, eight 7.4, 7.1.
 constexpr size_t kFusedBytes = 32 * 1024;
 bool streams(uint32_t m, uint32_t n, uint32_t k, uint32_t weights, uint32_t format) {
     const uint32_t blocks = k / kMxBlock;

@@ -7,13 +7,14 @@
 // 16-byte pieces land in lane order, so which piece a lane fetches decides the
 // layout.  Rows of 64 bytes (4-bit) or 128 (8-bit) are fetched whole by
 // neighbouring lanes, and piece p of row r lies at p ^ (r / 2 % 4) or p ^ (r % 8),
-// so that the reads of one piece over 16 rows touch all banks.  A gated product
-// takes the tiles of gate and up in turn, so that a wave holds both sums of a
-// result.
+// so that the reads of one piece over 16 rows spread over the banks (0.9 conflicts
+// are counted for each LDS instruction, of which about half read one byte of scales).
+// A gated product takes the tiles of gate and up in turn, so that a wave holds both
+// sums of a result.
 //
 // Measured: 4096 x 4096 x 14336 with 4-bit activations 166 us (2.9 PFLOP/s; matrix
-// units 38 % busy), gated with 8-bit ones 627 us (1.5 PFLOP/s of results, each product
-// in two parts).  With the rest taken out, at 8192 x 8192 x 8192 in 4 bits, the
+// units 38 % busy), gated with 8-bit ones 627 us (1.5 PFLOP/s, each product in two
+// parts; matrix units 62 % busy, vector units, which part them, 47 %).  With the rest taken out, at 8192 x 8192 x 8192 in 4 bits, the
 // products alone take 59 % of the time and the fetches alone 52 % (33 clocks a KB on
 // each CU); the two overlap in part only, since a fetch's writes and the waves' reads
 // share LDS.
